@@ -337,6 +337,168 @@ nut_status nut_peer_all_reduce(const float *x, float *out, int64_t n, float *con
                                unsigned *const *flags, int rank, int world, unsigned *epochs,
                                int *error, int64_t limit_ns, void *stream);
 
+/* ---- Paged KV cache ------------------------------------------------------ */
+
+/* Keys and values of many sequences of unequal length in one pool of
+ * fixed-size pages, in the CALLER's device memory, and the operators on it.
+ * The reference keeps one contiguous fp32 cache per sequence (include/
+ * kvcache.hpp:8-31); KVCache::store, the rotation and attention_step
+ * (src/quant_model.cpp:26-105) are what nut_paged_append and
+ * nut_paged_attention do for a batch of such caches. */
+
+/* Element types of caches and rows. */
+enum { NUT_F32 = 0, NUT_F16 = 1, NUT_BF16 = 2 };
+
+/* The pool and its tables (device pointers).  Slot t of sequence s lies in
+ * page table[s][t / page_size] at place t % page_size; element d of kv head
+ * h of that slot at
+ *   page * page_stride + h * head_stride + place * slot_stride + d
+ * of `keys` and of `values`.  All three strides 0 means contiguous
+ * [n_pages][kv_heads][page_size][head_dim].  head_dim is a multiple of 8 up
+ * to 256; keys, values and the strides are multiples of 16 bytes.  Pages of
+ * different sequences must differ.  Table entries behind a sequence's last
+ * page are never read.
+ *   lengths  slots in use of each sequence, read on the device by every call
+ *            (0 is an idle place); the caller advances it before it appends.
+ *   bounds, bound_scales  (both or neither) the key bounds of every page and
+ *            kv head, for nut_paged_select: greatest and least key of each
+ *            dimension over the page's used slots, as int8 in units of
+ *            bound_scales (a power of two, the least under which all fit
+ *            127), the greatest rounded up and the least down.  Kept by
+ *            nut_paged_append and nut_paged_summarise.  NaN keys count as 0
+ *            and infinite ones as the largest finite float.
+ *   max_rows  most rows of one attention or select call (0: sequences).
+ *   track_weights  nut_paged_attention may be asked for attention weights
+ *            (costs [sequences][heads][max_pages * page_size] floats). */
+typedef struct nut_paged_view {
+    void *keys, *values;
+    const int32_t *table;   /* [sequences][max_pages] */
+    const int32_t *lengths; /* [sequences] */
+    int8_t *bounds;         /* [n_pages][kv_heads][2][head_dim], or NULL */
+    float *bound_scales;    /* [n_pages][kv_heads], or NULL */
+    int64_t page_stride, head_stride, slot_stride; /* in elements */
+    int64_t sequences, max_pages, n_pages, page_size;
+    int64_t heads, kv_heads, head_dim, max_rows;
+    int32_t type; /* of keys and values */
+    int32_t track_weights;
+} nut_paged_view;
+
+/* A handle on a pool: the view and this library's workspace for it.  The
+ * operators enqueue on `stream` (a cudaStream_t, NULL = the legacy default
+ * stream) and return without synchronising; none allocates.  Calls of one
+ * handle share its workspace: issue them on one stream or order the streams
+ * with events. */
+typedef struct nut_paged nut_paged;
+
+nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **out);
+nut_status nut_paged_destroy(nut_paged *paged);
+/* Synchronises `stream` and reports what the device saw wrong in earlier
+ * calls' device-resident arguments (NUT_OUT_OF_RANGE: a page number outside
+ * the pool, a length outside the table, a row's sequence, a position beyond
+ * the rotation table, inconsistent `starts`), clearing it.  The work that
+ * met it was skipped: nothing outside the caller's buffers is touched. */
+nut_status nut_paged_error(nut_paged *paged, void *stream);
+
+/* Appends new tokens.  The rows of sequence s are starts[s] ..
+ * starts[s + 1] - 1, its newest ones: with n of them they take slots
+ * lengths[s] - n .. lengths[s] - 1 and positions seen[s] - n .. seen[s] - 1.
+ * Row r of k and v is [kv_heads][head_dim] at r * k_stride / v_stride
+ * elements (0: contiguous), likewise q, q_out [heads][head_dim].  Queries
+ * and keys are rotated in neighbouring pairs in fp32 with unfused products,
+ * as the token loop does (src/quant_model.cpp:26-37), then rounded to the
+ * type of q_out / the cache (fp16 saturates at +-65504). */
+typedef struct nut_paged_append_args {
+    const void *q; /* NULL: keys and values only */
+    const void *k, *v;
+    void *q_out; /* may be q */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *starts; /* [sequences + 1], ascending from 0 */
+    int64_t rows;    /* starts[sequences] */
+    int64_t max_new; /* most rows of one sequence */
+    const float *rope_cos, *rope_sin; /* [rope_rows][head_dim / 2]; NULL: no rotation */
+    int64_t rope_rows;
+    const int32_t *seen; /* [sequences] tokens so far, these included; NULL: lengths */
+    /* [sequences][kv_heads][max_pages * page_size], each or NULL: the new
+     * slots' positions are recorded, their weights set to 0 */
+    int32_t *positions;
+    float *weights;
+    int32_t type; /* of q, k, v and q_out */
+} nut_paged_append_args;
+nut_status nut_paged_append(nut_paged *paged, const nut_paged_append_args *args, void *stream);
+/* Recomputes the key bounds of every used page of every sequence (after
+ * keys were written or moved by other means than nut_paged_append). */
+nut_status nut_paged_summarise(nut_paged *paged, void *stream);
+
+/* out[r][h] = sum_t w_t v_t with w = softmax_t(scale q[r][h] . k_t) over the
+ * first row_length[r] slots of sequence row_sequence[r], kv head
+ * h / (heads / kv_heads).  A row that sees nothing gives zeros and
+ * lse = -infinity.  Sums, the softmax and its statistics are fp32 and the
+ * operands enter unrounded (16-bit caches: queries and weights are split
+ * into two or three 16-bit terms).
+ * `selected` restricts row r, kv head g to the pages whose numbers within the
+ * sequence are listed, in any order, -1 for none; a page listed twice counts
+ * twice.  With weights / weights_out (one row per sequence, no `selected`)
+ *   weights_out[s][g][t] = weights[s][g][t] + sum of w_t over the group's heads
+ * for the slots in use; the two may be the same buffer. */
+typedef struct nut_paged_attention_args {
+    const void *q; /* [rows][heads][head_dim] */
+    void *out;
+    int64_t q_stride, out_stride; /* elements between rows; 0: contiguous */
+    float *lse; /* [rows][heads] natural log of the softmax sum, or NULL */
+    const int32_t *row_sequence; /* [rows]; NULL: row r is sequence r */
+    const int32_t *row_length;   /* [rows]; NULL: the sequence's length */
+    const int32_t *selected;     /* [rows][kv_heads][n_selected], or NULL */
+    int64_t n_selected;
+    const float *weights; /* [sequences][kv_heads][max_pages * page_size], or NULL */
+    float *weights_out;
+    int64_t rows;
+    float scale;  /* 0: 1 / sqrt(head_dim) */
+    int32_t type; /* of q and out: NUT_F32 or the cache's */
+} nut_paged_attention_args;
+nut_status nut_paged_attention(nut_paged *paged, const nut_paged_attention_args *args,
+                               void *stream);
+
+/* Chooses pages for each row and kv head by a score that bounds the logits:
+ * with each query head in 8 bits, x = rint(q / u), u the least power of two
+ * under which |x| <= 127,
+ *   score(page) = max over the group's heads of
+ *                 u * bound_scale * sum_d max(x_d greatest_d, x_d least_d).
+ * Every term is an integer times a power of two, so the score is exact and
+ * the choice does not depend on the order of any sum.  The first sink_pages
+ * and the last recent_pages pages of the row's length come before all
+ * others; then the highest scores, ties to the lowest page.  selected[r][g]
+ * receives the min(n_selected, pages) chosen ones ascending, then -1. */
+typedef struct nut_paged_select_args {
+    const void *q;
+    int64_t q_stride;
+    const int32_t *row_sequence, *row_length; /* as for the attention */
+    int32_t *selected; /* [rows][kv_heads][n_selected] */
+    int64_t n_selected, sink_pages, recent_pages, rows;
+    int32_t type;
+} nut_paged_select_args;
+nut_status nut_paged_select(nut_paged *paged, const nut_paged_select_args *args, void *stream);
+
+/* Trims each sequence to `budget` slots, for each kv head on its own: kept
+ * are the tokens with position < sinks or >= seen - recent, then those with
+ * most weight (ties: the lowest slot; a NaN weight is the least).  The kept
+ * tokens in slots from the new length on move into the freed slots below
+ * it, both taken in ascending order; keys were rotated when stored, so the
+ * order of slots does not matter to the attention.  weights_out and
+ * positions_out (which may be weights / positions) receive the moved
+ * entries, 0 and -1 in the slots given up, and new_lengths (which may be
+ * the view's lengths) min(length, budget).  Key bounds are not recomputed
+ * (nut_paged_summarise). */
+typedef struct nut_paged_evict_args {
+    const float *weights;     /* [sequences][kv_heads][max_pages * page_size] */
+    const int32_t *positions; /* same shape; NULL (with positions_out) if sinks == recent == 0 */
+    const int32_t *seen;      /* [sequences]; NULL if recent == 0 */
+    int64_t budget, sinks, recent;
+    int32_t *new_lengths; /* [sequences] */
+    float *weights_out;
+    int32_t *positions_out;
+} nut_paged_evict_args;
+nut_status nut_paged_evict(nut_paged *paged, const nut_paged_evict_args *args, void *stream);
+
 /* ---- Greedy head without allocation ------------------------------------ */
 
 /* Largest batch of nut_greedy_head_static. */

@@ -33,6 +33,11 @@ INT4 = 1
 # (load_llama2c_model and the ModelWeights overload of generation)
 FP32 = 2
 
+# element types of the paged cache and its rows
+F32 = 0
+F16 = 1
+BF16 = 2
+
 NUT_OK = 0
 NUT_INVALID_ARGUMENT = 1
 NUT_OUT_OF_RANGE = 2
@@ -126,6 +131,45 @@ class GenerationStats(C.Structure):
                 ("prefill_seconds", C.c_double), ("decode_seconds", C.c_double)]
 
 
+class PagedView(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in (
+        "keys", "values", "table", "lengths", "bounds", "bound_scales")] + [
+        (n, C.c_int64) for n in (
+            "page_stride", "head_stride", "slot_stride", "sequences", "max_pages", "n_pages",
+            "page_size", "heads", "kv_heads", "head_dim", "max_rows")] + [
+        ("type", C.c_int32), ("track_weights", C.c_int32)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        (n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [
+        ("starts", C.c_void_p), ("rows", C.c_int64), ("max_new", C.c_int64),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_rows", C.c_int64),
+        ("seen", C.c_void_p), ("positions", C.c_void_p), ("weights", C.c_void_p),
+        ("type", C.c_int32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("lse", C.c_void_p), ("row_sequence", C.c_void_p),
+                ("row_length", C.c_void_p), ("selected", C.c_void_p), ("n_selected", C.c_int64),
+                ("weights", C.c_void_p), ("weights_out", C.c_void_p), ("rows", C.c_int64),
+                ("scale", C.c_float), ("type", C.c_int32)]
+
+
+class PagedSelectArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("row_sequence", C.c_void_p),
+                ("row_length", C.c_void_p), ("selected", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("n_selected", "sink_pages", "recent_pages", "rows")] + [
+        ("type", C.c_int32)]
+
+
+class PagedEvictArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("weights", "positions", "seen")] + [
+        (n, C.c_int64) for n in ("budget", "sinks", "recent")] + [
+        (n, C.c_void_p) for n in ("new_lengths", "weights_out", "positions_out")]
+
+
 # --------------------------------------------------------------------------
 # library loading
 
@@ -204,6 +248,13 @@ def cuda_lib() -> C.CDLL:
                                               _I64, _P])
         _declare(lib, "nut_batch_generate", [_P, _P, _I64, _I64, _P, _P,
                                              C.POINTER(GenerationStats)])
+        _declare(lib, "nut_paged_create", [C.POINTER(PagedView), C.c_int, C.POINTER(_P)])
+        _declare(lib, "nut_paged_destroy", [_P])
+        _declare(lib, "nut_paged_error", [_P, _P])
+        _declare(lib, "nut_paged_summarise", [_P, _P])
+        for op, kind in (("append", PagedAppendArgs), ("attention", PagedAttentionArgs),
+                         ("select", PagedSelectArgs), ("evict", PagedEvictArgs)):
+            _declare(lib, f"nut_paged_{op}", [_P, C.POINTER(kind), _P])
         _cuda = lib
     return _cuda
 
@@ -900,3 +951,113 @@ def generate_greedy(model: DeviceModel, cache: KVCache, prompt: Sequence[int],
         max_tokens, int(stop_at_eos), _ptr(ids), C.byref(n), _ptr(lg),
         C.byref(stats)))
     return ids[:n.value].copy(), (lg[:n.value] if lg is not None else None), stats
+
+
+# --------------------------------------------------------------------------
+# paged KV cache
+
+
+class PagedCache:
+    """Keys and values of many sequences of unequal length in fixed-size pages
+    (nut_paged), in device memory of the caller.  Every pointer is a device
+    address (an int, such as a tensor's data_ptr()) and has to stay valid
+    while the object is used.
+
+    keys, values   pool [n_pages][kv_heads][page_size][head_dim] of `dtype`
+                   (F32, F16, BF16), or any layout with the three strides
+                   (in elements) and contiguous head_dim
+    table          int32 [sequences][max_pages], page numbers
+    lengths        int32 [sequences], slots in use
+    bounds, bound_scales  int8 [n_pages][kv_heads][2][head_dim] and fp32
+                   [n_pages][kv_heads]: the key bounds select() reads
+    max_rows       most rows of one attention() or select() (0: sequences)
+    track_weights  attention() may be asked for attention weights
+
+    The operators enqueue on `stream` (0: the legacy default stream) and do
+    not synchronise; calls of one object must be ordered as on one stream."""
+
+    def __init__(self, keys: int, values: int, table: int, lengths: int, *, sequences: int,
+                 max_pages: int, n_pages: int, page_size: int, heads: int, kv_heads: int,
+                 head_dim: int, dtype: int = F32, page_stride: int = 0, head_stride: int = 0,
+                 slot_stride: int = 0, bounds: int = 0, bound_scales: int = 0, max_rows: int = 0,
+                 track_weights: bool = False, device: int = 0):
+        self.handle = None
+        view = PagedView(keys, values, table, lengths, bounds, bound_scales, page_stride,
+                         head_stride, slot_stride, sequences, max_pages, n_pages, page_size,
+                         heads, kv_heads, head_dim, max_rows, dtype, int(track_weights))
+        h = C.c_void_p()
+        lib = cuda_lib()
+        _check(lib.nut_paged_create(C.byref(view), device, C.byref(h)))
+        self.handle = h
+        self._append, self._attention = lib.nut_paged_append, lib.nut_paged_attention
+        self._select, self._evict = lib.nut_paged_select, lib.nut_paged_evict
+
+    def append(self, q: int, k: int, v: int, starts: int, rows: int, max_new: int, *,
+               dtype: int = F32, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0,
+               q_out: int = 0, q_out_stride: int = 0, cos: int = 0, sin: int = 0,
+               rope_rows: int = 0, seen: int = 0, positions: int = 0, weights: int = 0,
+               stream: int = 0) -> None:
+        """Rotates the new rows' queries (into q_out; q may be 0) and keys and
+        stores keys and values in each sequence's newest slots
+        (nut_paged_append).  Rows of sequence s: starts[s] .. starts[s+1]-1;
+        `lengths` already counts them."""
+        args = PagedAppendArgs(q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, starts,
+                               rows, max_new, cos, sin, rope_rows, seen, positions, weights, dtype)
+        status = self._append(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def attention(self, q: int, out: int, rows: int, *, dtype: int = F32, scale: float = 0.0,
+                  q_stride: int = 0, out_stride: int = 0, lse: int = 0, row_sequence: int = 0,
+                  row_length: int = 0, selected: int = 0, n_selected: int = 0, weights: int = 0,
+                  weights_out: int = 0, stream: int = 0) -> None:
+        """Attention of each row over its sequence's slots, or over the pages
+        listed in `selected` (nut_paged_attention); with weights, adds the
+        attention weight each slot received into weights_out."""
+        args = PagedAttentionArgs(q, out, q_stride, out_stride, lse, row_sequence, row_length,
+                                  selected, n_selected, weights, weights_out, rows, scale, dtype)
+        status = self._attention(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def select(self, q: int, selected: int, rows: int, n_selected: int, *, dtype: int = F32,
+               q_stride: int = 0, sink_pages: int = 0, recent_pages: int = 1,
+               row_sequence: int = 0, row_length: int = 0, stream: int = 0) -> None:
+        """Writes the numbers of the n_selected pages whose keys can match
+        each row's queries best, ascending, -1 behind (nut_paged_select)."""
+        args = PagedSelectArgs(q, q_stride, row_sequence, row_length, selected, n_selected,
+                               sink_pages, recent_pages, rows, dtype)
+        status = self._select(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def evict(self, weights: int, positions: int, seen: int, budget: int, *, new_lengths: int,
+              weights_out: int, positions_out: int = 0, sinks: int = 0, recent: int = 0,
+              stream: int = 0) -> None:
+        """Trims every sequence and kv head to the `budget` slots with most
+        accumulated weight (nut_paged_evict)."""
+        args = PagedEvictArgs(weights, positions, seen, budget, sinks, recent, new_lengths,
+                              weights_out, positions_out)
+        status = self._evict(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def summarise(self, stream: int = 0) -> None:
+        """Recomputes the key bounds of every used page (nut_paged_summarise)."""
+        _check(cuda_lib().nut_paged_summarise(self.handle, stream))
+
+    def check(self, stream: int = 0) -> None:
+        """Synchronises `stream`; raises IndexError if the device met a page
+        number, length, sequence or position out of range (nut_paged_error)."""
+        _check(cuda_lib().nut_paged_error(self.handle, stream))
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            cuda_lib().nut_paged_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

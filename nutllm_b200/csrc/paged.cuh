@@ -1,0 +1,149 @@
+#pragma once
+/* Device helpers of the paged KV cache operators (paged_*.cu). */
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace nut {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+/* Rounds to nearest; fp16 saturates at +-65504 and keeps NaN. */
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) {
+    return __float2half_rn(v > 65504.0f ? 65504.0f : v < -65504.0f ? -65504.0f : v);
+}
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ void paged_fail(const PagedPool &p, int bit) { atomicOr(p.error, bit); }
+
+/* Slots in use of sequence s; 0, with the error recorded, when the length
+ * is not one the table can hold. */
+__device__ __forceinline__ int checked_length(const PagedPool &p, int length) {
+    if (length < 0 || length > p.capacity) {
+        paged_fail(p, kPagedBadLength);
+        return 0;
+    }
+    return length;
+}
+
+/* Page number of logical page j of sequence s, or -1 (recorded). */
+__device__ __forceinline__ int checked_page(const PagedPool &p, int s, int j) {
+    const int page = p.table[int64_t(s) * p.max_pages + j];
+    if (unsigned(page) >= unsigned(p.n_pages)) {
+        paged_fail(p, kPagedBadPage);
+        return -1;
+    }
+    return page;
+}
+
+/* Sequence of attention row r and the slots it sees (0 for a bad row). */
+__device__ __forceinline__ int row_span(const PagedPool &p, const int32_t *row_sequence,
+                                        const int32_t *row_length, int r, int &length) {
+    int s = row_sequence ? row_sequence[r] : r;
+    if (unsigned(s) >= unsigned(p.sequences)) {
+        paged_fail(p, kPagedBadSequence);
+        length = 0;
+        return 0;
+    }
+    length = checked_length(p, row_length ? row_length[r] : p.lengths[s]);
+    return s;
+}
+
+/* Power of two u, at least 2^-126, least with top <= 127 u (0 for top = 0):
+ * top = m 2^e with 1 <= m < 2 needs u = 2^(e - 6), or twice that when
+ * m > 127 / 64. */
+__device__ __forceinline__ float unit_of(float top) {
+    if (!(top > 0.0f))
+        return 0.0f;
+    const uint32_t b = __float_as_uint(top);
+    int e = int(b >> 23) - 127 - 6;
+    if ((b & 0x7fffffu) > 0x7e0000u) /* mantissa of 127 / 64 */
+        e++;
+    if (e < -126)
+        e = -126;
+    return __uint_as_float(uint32_t(e + 127) << 23);
+}
+
+/* NaN counts as 0, infinities as the largest finite float. */
+__device__ __forceinline__ float finite_key(float v) {
+    return v != v ? 0.0f : fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f);
+}
+
+/* ---- choosing the largest of many keys ------------------------------- */
+
+constexpr int kChooseThreads = 1024;
+
+struct ChooseScratch {
+    int hist[256];
+    int warp[3][kChooseThreads / 32];
+    uint32_t prefix;
+    int left;
+};
+
+/* The `want` largest of key(0) .. key(n - 1), ties to the lowest index, by
+ * four 8-bit histogram passes from the top: key(i) is chosen when it is
+ * above `threshold`, or equal to it and one of the first `quota` such. */
+template <typename Key>
+__device__ void choose_largest(Key key, int n, int want, ChooseScratch &s, uint32_t &threshold,
+                               int &quota) {
+    if (want <= 0 || want >= n) {
+        threshold = want <= 0 ? 0xffffffffu : 0u;
+        quota = want <= 0 ? 0 : n;
+        return;
+    }
+    uint32_t prefix = 0;
+    int left = want;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = threadIdx.x; i < 256; i += blockDim.x)
+            s.hist[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            const uint32_t k = key(i);
+            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&s.hist[(k >> shift) & 255], 1);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int b = 255, c = left;
+            while (b > 0 && s.hist[b] < c)
+                c -= s.hist[b--];
+            s.prefix = prefix | (uint32_t(b) << shift);
+            s.left = c;
+        }
+        __syncthreads();
+        prefix = s.prefix;
+        left = s.left;
+    }
+    threshold = prefix;
+    quota = left;
+}
+
+/* Exclusive rank of each thread's flag among the block's, and the total. */
+__device__ __forceinline__ int block_rank(bool flag, int *warp_totals, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const uint32_t m = __ballot_sync(0xffffffffu, flag);
+    if (lane == 0)
+        warp_totals[warp] = __popc(m);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < warps; w++) {
+        const int c = warp_totals[w];
+        before += w < warp ? c : 0;
+        all += c;
+    }
+    __syncthreads();
+    total = all;
+    return before + __popc(m & ((1u << lane) - 1u));
+}
+
+} // namespace nut

@@ -1,0 +1,86 @@
+#pragma once
+/* Paged KV cache operators (nut_paged_* in nutllm_cuda.h): what the kernels
+ * see of a pool, and their host-side launchers. */
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace nut {
+
+/* Bits of a handle's error word. */
+enum PagedError {
+    kPagedBadPage = 1,     /* page number outside the pool */
+    kPagedBadLength = 2,   /* length outside [0, capacity] */
+    kPagedBadSequence = 4, /* row's sequence outside the table */
+    kPagedBadStarts = 8,   /* starts not ascending, or more new rows than slots */
+    kPagedBadPosition = 16 /* position outside the rotation table */
+};
+
+struct PagedPool {
+    void *keys, *values;
+    const int32_t *table, *lengths;
+    int8_t *bounds;
+    float *bound_scales;
+    int64_t page_stride, head_stride, slot_stride;
+    int sequences, max_pages, n_pages, page_size;
+    int heads, kv_heads, head_dim, group; /* group = heads / kv_heads */
+    int capacity;                         /* max_pages * page_size */
+    int type;
+    int *error;
+};
+
+struct PagedAppend {
+    PagedPool p;
+    const void *q, *k, *v;
+    void *q_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *starts, *seen;
+    const float *cos, *sin;
+    int rows, max_new, rope_rows, type;
+    int32_t *positions;
+    float *weights;
+};
+
+struct PagedAttention {
+    PagedPool p;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    float *lse;
+    const int32_t *row_sequence, *row_length, *selected;
+    int n_selected;
+    const float *weights;
+    float *weights_out;
+    int rows, type;
+    float scale;
+    float *logits; /* [sequences][heads][capacity] with weights */
+};
+
+struct PagedSelect {
+    PagedPool p;
+    const void *q;
+    int64_t q_stride;
+    const int32_t *row_sequence, *row_length;
+    int32_t *selected;
+    int n_selected, sink_pages, recent_pages, rows, type;
+    float *scores; /* [rows][kv_heads][max_pages] */
+};
+
+struct PagedEvict {
+    PagedPool p;
+    const float *weights;
+    const int32_t *positions, *seen;
+    int budget, sinks, recent;
+    int32_t *new_lengths;
+    float *weights_out;
+    int32_t *positions_out;
+    int32_t *pairs;  /* [sequences][kv_heads][capacity]: holes, then sources from the far end */
+    int32_t *counts; /* [sequences][kv_heads][2]: pairs, old length */
+};
+
+cudaError_t paged_append(const PagedAppend &a, cudaStream_t s);
+cudaError_t paged_summarise(const PagedPool &p, cudaStream_t s);
+cudaError_t paged_attention(const PagedAttention &a, cudaStream_t s);
+cudaError_t paged_select(const PagedSelect &a, cudaStream_t s);
+cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s);
+
+} // namespace nut

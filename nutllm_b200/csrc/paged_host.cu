@@ -1,0 +1,412 @@
+/* C ABI of the paged KV cache (nut_paged_* in nutllm_cuda.h): argument
+ * checks, the handle's workspace, and the calls into paged_*.cu. */
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <memory>
+#include <stdexcept>
+#include <string>
+
+#include <cuda_runtime.h>
+
+#include "../../include/nutllm_cuda.h"
+#include "kernels.h"
+#include "paged.h"
+
+namespace {
+
+struct Failure {
+    nut_status status;
+    std::string message;
+};
+
+[[noreturn]] void raise(nut_status s, const std::string &m) { throw Failure{s, "paged: " + m}; }
+
+void cuda_check(cudaError_t e, const char *what) {
+    if (e != cudaSuccess)
+        throw Failure{NUT_RUNTIME_ERROR,
+                      std::string("cuda: ") + what + ": " + cudaGetErrorString(e)};
+}
+
+template <typename F> nut_status guarded(F &&body) {
+    try {
+        body();
+        return NUT_OK;
+    } catch (const Failure &f) {
+        nut::set_last_error(f.message);
+        return f.status;
+    } catch (const std::bad_alloc &) {
+        nut::set_last_error("nutllm: host allocation failed");
+        return NUT_RUNTIME_ERROR;
+    } catch (const std::exception &e) {
+        nut::set_last_error(e.what());
+        return NUT_RUNTIME_ERROR;
+    }
+}
+
+/* Makes the handle's device current where it is not, and restores it. */
+struct DeviceScope {
+    int previous = 0, device;
+    explicit DeviceScope(int d) : device(d) {
+        cuda_check(cudaGetDevice(&previous), "get device");
+        if (previous != device)
+            cuda_check(cudaSetDevice(device), "set device");
+    }
+    ~DeviceScope() {
+        if (previous != device)
+            cudaSetDevice(previous);
+    }
+};
+
+template <typename T> T *dev_alloc(size_t count, const char *what) {
+    void *p = nullptr;
+    cuda_check(cudaMalloc(&p, (count == 0 ? 1 : count) * sizeof(T)), what);
+    return static_cast<T *>(p);
+}
+
+constexpr int64_t kMaxGrid = 65535; /* sequences and rows are grid dimensions */
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+void check_view(const nut_paged_view &v) {
+    if (!v.keys || !v.values || !v.table || !v.lengths)
+        raise(NUT_INVALID_ARGUMENT, "null pool, table or lengths");
+    if ((v.bounds == nullptr) != (v.bound_scales == nullptr))
+        raise(NUT_INVALID_ARGUMENT, "bounds and bound_scales go together");
+    if (v.type != NUT_F32 && v.type != NUT_F16 && v.type != NUT_BF16)
+        raise(NUT_INVALID_ARGUMENT, "unknown cache type");
+    if (v.sequences <= 0 || v.max_pages <= 0 || v.n_pages <= 0 || v.page_size <= 0 ||
+        v.heads <= 0 || v.kv_heads <= 0 || v.head_dim <= 0 || v.max_rows < 0)
+        raise(NUT_INVALID_ARGUMENT, "invalid dimensions");
+    if (v.heads % v.kv_heads != 0)
+        raise(NUT_INVALID_ARGUMENT, "heads must divide by kv_heads");
+    if (v.head_dim % 8 != 0 || v.head_dim > 256)
+        raise(NUT_INVALID_ARGUMENT, "head_dim must be a multiple of 8 up to 256");
+    if (v.sequences > kMaxGrid || v.max_rows > kMaxGrid || v.kv_heads > 4096 || v.heads > 65536)
+        raise(NUT_LENGTH_ERROR, "dimensions exceed device limits");
+    if (v.n_pages > INT_MAX || v.page_size > (1 << 24) || v.max_pages > (1 << 24) ||
+        v.max_pages * v.page_size > (int64_t(1) << 30))
+        raise(NUT_LENGTH_ERROR, "dimensions exceed device limits");
+    const int64_t unit = v.type == NUT_F32 ? 4 : 8; /* elements of 16 bytes */
+    if (!aligned16(v.keys) || !aligned16(v.values) || v.page_stride % unit != 0 ||
+        v.head_stride % unit != 0 || v.slot_stride % unit != 0)
+        raise(NUT_INVALID_ARGUMENT, "keys, values and strides must be multiples of 16 bytes");
+    if (v.page_stride < 0 || v.head_stride < 0 || v.slot_stride < 0)
+        raise(NUT_INVALID_ARGUMENT, "negative stride");
+    if ((v.page_stride || v.head_stride || v.slot_stride) &&
+        !(v.page_stride && v.head_stride && v.slot_stride))
+        raise(NUT_INVALID_ARGUMENT, "give all three strides or none");
+}
+
+/* Row stride in elements: 0 stands for the contiguous width. */
+int64_t stride_of(int64_t given, int64_t width, const char *name) {
+    if (given == 0)
+        return width;
+    if (given < width)
+        raise(NUT_INVALID_ARGUMENT, std::string(name) + " is less than a row");
+    return given;
+}
+
+} // namespace
+
+struct nut_paged {
+    int device = 0;
+    nut::PagedPool pool{};
+    int max_rows = 0;
+    bool track = false;
+    int *error = nullptr;
+    float *logits = nullptr, *scores = nullptr;
+    int32_t *pairs = nullptr, *counts = nullptr;
+    ~nut_paged() {
+        for (void *p : {static_cast<void *>(error), static_cast<void *>(logits),
+                        static_cast<void *>(scores), static_cast<void *>(pairs),
+                        static_cast<void *>(counts)})
+            if (p)
+                cudaFree(p);
+    }
+};
+
+namespace {
+
+void check_row_type(const nut_paged &h, int32_t type) {
+    if (type != NUT_F32 && type != h.pool.type)
+        raise(NUT_INVALID_ARGUMENT, "rows must be fp32 or of the cache's type");
+}
+
+void check_rows(const nut_paged &h, int64_t rows, const int32_t *row_sequence) {
+    if (rows < 0)
+        raise(NUT_INVALID_ARGUMENT, "negative row count");
+    if (rows > h.max_rows)
+        raise(NUT_LENGTH_ERROR, "more rows than max_rows");
+    if (!row_sequence && rows > h.pool.sequences)
+        raise(NUT_INVALID_ARGUMENT, "more rows than sequences need row_sequence");
+}
+
+} // namespace
+
+extern "C" {
+
+nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **out) {
+    return guarded([&] {
+        if (!view || !out)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        *out = nullptr;
+        check_view(*view);
+        const nut_paged_view &v = *view;
+        DeviceScope scope(device);
+        auto h = std::make_unique<nut_paged>();
+        h->device = device;
+        h->max_rows = int(v.max_rows ? v.max_rows : v.sequences);
+        h->track = v.track_weights != 0;
+        nut::PagedPool &p = h->pool;
+        p.keys = v.keys;
+        p.values = v.values;
+        p.table = v.table;
+        p.lengths = v.lengths;
+        p.bounds = v.bounds;
+        p.bound_scales = v.bound_scales;
+        const bool strided = v.page_stride != 0;
+        p.slot_stride = strided ? v.slot_stride : v.head_dim;
+        p.head_stride = strided ? v.head_stride : v.page_size * v.head_dim;
+        p.page_stride = strided ? v.page_stride : v.kv_heads * v.page_size * v.head_dim;
+        p.sequences = int(v.sequences);
+        p.max_pages = int(v.max_pages);
+        p.n_pages = int(v.n_pages);
+        p.page_size = int(v.page_size);
+        p.heads = int(v.heads);
+        p.kv_heads = int(v.kv_heads);
+        p.head_dim = int(v.head_dim);
+        p.group = int(v.heads / v.kv_heads);
+        p.capacity = int(v.max_pages * v.page_size);
+        p.type = v.type;
+        h->error = dev_alloc<int>(1, "alloc error word");
+        p.error = h->error;
+        cuda_check(cudaMemset(h->error, 0, sizeof(int)), "clear error word");
+        const size_t items = size_t(p.sequences) * p.kv_heads;
+        h->pairs = dev_alloc<int32_t>(items * p.capacity, "alloc slot pairs");
+        h->counts = dev_alloc<int32_t>(items * 2, "alloc pair counts");
+        if (h->track)
+            h->logits = dev_alloc<float>(size_t(p.sequences) * p.heads * p.capacity,
+                                         "alloc attention logits");
+        if (p.bounds)
+            h->scores = dev_alloc<float>(size_t(h->max_rows) * p.kv_heads * p.max_pages,
+                                         "alloc page scores");
+        cuda_check(cudaStreamSynchronize(nullptr), "finish workspace");
+        *out = h.release();
+    });
+}
+
+nut_status nut_paged_destroy(nut_paged *h) {
+    return guarded([&] {
+        if (!h)
+            return;
+        DeviceScope scope(h->device);
+        delete h;
+    });
+}
+
+nut_status nut_paged_error(nut_paged *h, void *stream) {
+    return guarded([&] {
+        if (!h)
+            raise(NUT_INVALID_ARGUMENT, "null handle");
+        DeviceScope scope(h->device);
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int code = 0;
+        cuda_check(cudaMemcpyAsync(&code, h->error, sizeof code, cudaMemcpyDeviceToHost, s),
+                   "read error word");
+        cuda_check(cudaStreamSynchronize(s), "synchronize");
+        if (code == 0)
+            return;
+        cuda_check(cudaMemsetAsync(h->error, 0, sizeof code, s), "clear error word");
+        cuda_check(cudaStreamSynchronize(s), "synchronize");
+        std::string m;
+        const auto add = [&](int bit, const char *what) {
+            if (code & bit)
+                m += (m.empty() ? "" : ", ") + std::string(what);
+        };
+        add(nut::kPagedBadPage, "page number outside the pool");
+        add(nut::kPagedBadLength, "length outside the table");
+        add(nut::kPagedBadSequence, "row sequence out of range");
+        add(nut::kPagedBadStarts, "inconsistent starts");
+        add(nut::kPagedBadPosition, "position outside the rotation table");
+        raise(NUT_OUT_OF_RANGE, m);
+    });
+}
+
+nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_append_args &g = *args;
+        const nut::PagedPool &p = h->pool;
+        if (!g.k || !g.v || !g.starts)
+            raise(NUT_INVALID_ARGUMENT, "null keys, values or starts");
+        if ((g.q == nullptr) != (g.q_out == nullptr))
+            raise(NUT_INVALID_ARGUMENT, "q and q_out go together");
+        if ((g.rope_cos == nullptr) != (g.rope_sin == nullptr))
+            raise(NUT_INVALID_ARGUMENT, "rope_cos and rope_sin go together");
+        if (g.rope_cos && g.rope_rows <= 0)
+            raise(NUT_INVALID_ARGUMENT, "empty rotation table");
+        if (g.rows < 0 || g.max_new < 0)
+            raise(NUT_INVALID_ARGUMENT, "negative row count");
+        check_row_type(*h, g.type);
+        nut::PagedAppend a{};
+        a.p = p;
+        const int64_t D = p.head_dim;
+        a.q_stride = stride_of(g.q_stride, p.heads * D, "q_stride");
+        a.k_stride = stride_of(g.k_stride, p.kv_heads * D, "k_stride");
+        a.v_stride = stride_of(g.v_stride, p.kv_heads * D, "v_stride");
+        a.q_out_stride = stride_of(g.q_out_stride, p.heads * D, "q_out_stride");
+        if (g.rows > INT_MAX)
+            raise(NUT_LENGTH_ERROR, "too many rows");
+        if (g.max_new > p.capacity)
+            raise(NUT_LENGTH_ERROR, "more new tokens than a sequence can hold");
+        if (g.rows == 0 || g.max_new == 0)
+            return;
+        a.q = g.q;
+        a.k = g.k;
+        a.v = g.v;
+        a.q_out = g.q_out;
+        a.starts = g.starts;
+        a.seen = g.seen;
+        a.cos = g.rope_cos;
+        a.sin = g.rope_sin;
+        a.rows = int(g.rows);
+        a.max_new = int(g.max_new);
+        a.rope_rows = int(std::min<int64_t>(g.rope_rows, INT_MAX));
+        a.type = g.type;
+        a.positions = g.positions;
+        a.weights = g.weights;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_append(a, static_cast<cudaStream_t>(stream)), "paged append");
+    });
+}
+
+nut_status nut_paged_summarise(nut_paged *h, void *stream) {
+    return guarded([&] {
+        if (!h)
+            raise(NUT_INVALID_ARGUMENT, "null handle");
+        if (!h->pool.bounds)
+            raise(NUT_INVALID_ARGUMENT, "the pool has no bounds");
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_summarise(h->pool, static_cast<cudaStream_t>(stream)),
+                   "paged summarise");
+    });
+}
+
+nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_attention_args &g = *args;
+        const nut::PagedPool &p = h->pool;
+        if (!g.q || !g.out)
+            raise(NUT_INVALID_ARGUMENT, "null q or out");
+        check_row_type(*h, g.type);
+        check_rows(*h, g.rows, g.row_sequence);
+        if (g.selected && g.n_selected <= 0)
+            raise(NUT_INVALID_ARGUMENT, "n_selected must be positive");
+        if (g.selected && g.n_selected * p.page_size > (int64_t(1) << 30))
+            raise(NUT_LENGTH_ERROR, "too many selected pages");
+        if ((g.weights == nullptr) != (g.weights_out == nullptr))
+            raise(NUT_INVALID_ARGUMENT, "weights and weights_out go together");
+        if (g.weights && !h->track)
+            raise(NUT_INVALID_ARGUMENT, "the handle does not track weights");
+        if (g.weights && (g.selected || g.row_sequence))
+            raise(NUT_INVALID_ARGUMENT, "weights need one row per sequence over all of its pages");
+        if (!std::isfinite(g.scale))
+            raise(NUT_INVALID_ARGUMENT, "scale must be finite");
+        nut::PagedAttention a{};
+        a.p = p;
+        a.q_stride = stride_of(g.q_stride, int64_t(p.heads) * p.head_dim, "q_stride");
+        a.out_stride = stride_of(g.out_stride, int64_t(p.heads) * p.head_dim, "out_stride");
+        if (g.rows == 0)
+            return;
+        a.q = g.q;
+        a.out = g.out;
+        a.lse = g.lse;
+        a.row_sequence = g.row_sequence;
+        a.row_length = g.row_length;
+        a.selected = g.selected;
+        a.n_selected = g.selected ? int(g.n_selected) : 0;
+        a.weights = g.weights;
+        a.weights_out = g.weights_out;
+        a.rows = int(g.rows);
+        a.type = g.type;
+        a.scale = g.scale != 0.0f ? g.scale : float(1.0 / std::sqrt(double(p.head_dim)));
+        a.logits = h->logits;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_attention(a, static_cast<cudaStream_t>(stream)), "paged attention");
+    });
+}
+
+nut_status nut_paged_select(nut_paged *h, const nut_paged_select_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_select_args &g = *args;
+        const nut::PagedPool &p = h->pool;
+        if (!p.bounds)
+            raise(NUT_INVALID_ARGUMENT, "the pool has no bounds");
+        if (!g.q || !g.selected)
+            raise(NUT_INVALID_ARGUMENT, "null q or selected");
+        check_row_type(*h, g.type);
+        check_rows(*h, g.rows, g.row_sequence);
+        if (g.n_selected <= 0 || g.sink_pages < 0 || g.recent_pages < 0)
+            raise(NUT_INVALID_ARGUMENT, "invalid page counts");
+        if (g.n_selected > INT_MAX)
+            raise(NUT_LENGTH_ERROR, "too many selected pages");
+        nut::PagedSelect a{};
+        a.p = p;
+        a.q_stride = stride_of(g.q_stride, int64_t(p.heads) * p.head_dim, "q_stride");
+        if (g.rows == 0)
+            return;
+        a.q = g.q;
+        a.row_sequence = g.row_sequence;
+        a.row_length = g.row_length;
+        a.selected = g.selected;
+        a.n_selected = int(g.n_selected);
+        a.sink_pages = int(std::min<int64_t>(g.sink_pages, INT_MAX));
+        a.recent_pages = int(std::min<int64_t>(g.recent_pages, INT_MAX));
+        a.rows = int(g.rows);
+        a.type = g.type;
+        a.scores = h->scores;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_select(a, static_cast<cudaStream_t>(stream)), "paged select");
+    });
+}
+
+nut_status nut_paged_evict(nut_paged *h, const nut_paged_evict_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_evict_args &g = *args;
+        if (!g.weights || !g.weights_out || !g.new_lengths)
+            raise(NUT_INVALID_ARGUMENT, "null weights, weights_out or new_lengths");
+        if ((g.positions == nullptr) != (g.positions_out == nullptr))
+            raise(NUT_INVALID_ARGUMENT, "positions and positions_out go together");
+        if (g.budget < 0 || g.sinks < 0 || g.recent < 0)
+            raise(NUT_INVALID_ARGUMENT, "negative budget, sinks or recent");
+        if ((g.sinks || g.recent) && !g.positions)
+            raise(NUT_INVALID_ARGUMENT, "sinks and recent need positions");
+        if (g.recent && !g.seen)
+            raise(NUT_INVALID_ARGUMENT, "recent needs seen");
+        nut::PagedEvict a{};
+        a.p = h->pool;
+        a.weights = g.weights;
+        a.positions = g.positions;
+        a.seen = g.seen;
+        a.budget = int(std::min<int64_t>(g.budget, INT_MAX));
+        a.sinks = int(std::min<int64_t>(g.sinks, INT_MAX));
+        a.recent = int(std::min<int64_t>(g.recent, INT_MAX));
+        a.new_lengths = g.new_lengths;
+        a.weights_out = g.weights_out;
+        a.positions_out = g.positions_out;
+        a.pairs = h->pairs;
+        a.counts = h->counts;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_evict(a, static_cast<cudaStream_t>(stream)), "paged evict");
+    });
+}
+
+} // extern "C"
