@@ -52,8 +52,18 @@ struct PagedAttention {
     float *weights_out;
     int rows, type;
     float scale;
-    float *logits; /* [sequences][heads][capacity] with weights */
+    float *logits; /* [sequences][heads][capacity] with weights, in log2 */
+    float *lse2;   /* [sequences][heads] with weights, in log2 */
+    float *partial; /* [CTAs][2][kPartialFloats]: items shared between CTAs */
+    int *counters;  /* [max_rows][items of a row], 0 between calls */
+    int sms;
 };
+
+/* A CTA's part of an attention item: maxima [8], sums [8], outputs [8][256]. */
+constexpr int kMaxDim = 256;
+constexpr int kPartialFloats = 8 * 2 + 8 * kMaxDim;
+constexpr int kMaxCtasPerSm = 4;
+constexpr int kMaxDevices = 64;
 
 struct PagedSelect {
     PagedPool p;

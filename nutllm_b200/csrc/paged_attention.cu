@@ -4,9 +4,16 @@
  *   z_t = scale q . k_t,  m = max z,  l = sum exp(z_t - m),
  *   out = sum exp(z_t - m) v_t / l,   lse = m + log l
  * in one pass over the keys and values with a running maximum and sum.
- * A CTA takes one row and kv head, its warps every fourth slot.
+ *
+ * Work.  A row, a kv head and up to 8 of its query heads are an item; an
+ * item's slots are cut into tiles, and all tiles of all items form one line
+ * that is cut evenly among the CTAs whatever the lengths.  An item that lies
+ * in one CTA is finished there.  Of one that spans several, each leaves its
+ * unnormalised output, maximum and sum, and the last to arrive joins them
+ * in order of their slots, so results do not depend on timing.
  */
 #include <cstdint>
+#include <type_traits>
 #include <cuda_runtime.h>
 
 #include "kernels.h"
@@ -15,108 +22,817 @@
 namespace nut {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMaxDim = 256;
+constexpr int kChunk = 16; /* slots a warp takes at a time */
+constexpr int kRows = 8;   /* query heads of an item */
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <typename R, typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-    attention_simple_kernel(const __grid_constant__ PagedAttention a) {
-    __shared__ float part[kWarps][kMaxDim], maxima[kWarps], sums[kWarps];
-    const PagedPool &p = a.p;
-    const int head = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int D = p.head_dim, ps = p.page_size;
-    int length;
-    const int s = row_span(p, a.row_sequence, a.row_length, r, length);
-    const int span = a.selected ? a.n_selected * ps : length;
-    const int32_t *list =
-        a.selected ? a.selected + (int64_t(r) * p.kv_heads + head) * a.n_selected : nullptr;
-    for (int g = 0; g < p.group; g++) {
-        const int h = head * p.group + g;
-        const R *q = static_cast<const R *>(a.q) + r * a.q_stride + int64_t(h) * D;
-        float x[8], acc[8], m = -INFINITY, l = 0.0f;
-        for (int i = 0; i < 8; i++) {
-            x[i] = lane + 32 * i < D ? to_float(q[lane + 32 * i]) : 0.0f;
-            acc[i] = 0.0f;
-        }
-        for (int v = warp; v < span; v += kWarps) {
-            const int j = list ? list[v / ps] : v / ps, t = j * ps + v % ps;
-            if (j < 0 || j >= p.max_pages || t >= length)
-                continue;
-            const int page = checked_page(p, s, j);
-            if (page < 0)
-                continue;
-            const int64_t at = int64_t(page) * p.page_stride + int64_t(head) * p.head_stride +
-                               int64_t(v % ps) * p.slot_stride;
-            const T *k = static_cast<const T *>(p.keys) + at,
-                    *val = static_cast<const T *>(p.values) + at;
-            float dot = 0.0f;
-            for (int i = 0; i < 8; i++)
-                if (lane + 32 * i < D)
-                    dot = fmaf(x[i], to_float(k[lane + 32 * i]), dot);
-            const float z = warp_sum(dot) * a.scale;
-            if (a.weights && lane == 0)
-                a.logits[(int64_t(r) * p.heads + h) * p.capacity + t] = z;
-            const float top = fmaxf(m, z), keep = m == top ? 1.0f : expf(m - top);
-            const float w = z == -INFINITY ? 0.0f : expf(z - top);
-            l = l * keep + w;
-            for (int i = 0; i < 8; i++)
-                if (lane + 32 * i < D)
-                    acc[i] = fmaf(acc[i], keep, w * to_float(val[lane + 32 * i]));
-            m = top;
-        }
-        for (int i = 0; i < 8; i++)
-            if (lane + 32 * i < D)
-                part[warp][lane + 32 * i] = acc[i];
-        if (lane == 0) {
-            maxima[warp] = m;
-            sums[warp] = l;
-        }
-        __syncthreads();
-        float top = -INFINITY, total = 0.0f;
-        for (int w = 0; w < kWarps; w++)
-            top = fmaxf(top, maxima[w]);
-        for (int w = 0; w < kWarps; w++)
-            total += maxima[w] == -INFINITY ? 0.0f : sums[w] * expf(maxima[w] - top);
-        const float lse = top + logf(total);
-        for (int d = threadIdx.x; d < D; d += blockDim.x) {
-            float o = 0.0f;
-            for (int w = 0; w < kWarps; w++)
-                if (maxima[w] != -INFINITY)
-                    o = fmaf(part[w][d], expf(maxima[w] - top), o);
-            static_cast<R *>(a.out)[r * a.out_stride + int64_t(h) * D + d] =
-                from_float<R>(total == 0.0f ? 0.0f : o / total);
-        }
-        if (a.lse && threadIdx.x == 0)
-            a.lse[int64_t(r) * p.heads + h] = total == 0.0f ? -INFINITY : lse;
-        if (a.weights) {
-            const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity;
-            const float *z = a.logits + (int64_t(r) * p.heads + h) * p.capacity;
-            const float *from = g == 0 ? a.weights : a.weights_out;
-            for (int t = threadIdx.x; t < length; t += blockDim.x)
-                a.weights_out[to + t] = from[to + t] + expf(z[t] - lse);
-        }
-        __syncthreads();
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+/* 16 bytes to shared memory, zeros where !valid (nothing is read then). */
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from),
+                 "r"(valid ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    }
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+                     "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+    }
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+                     "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+};
+
+/* What is left of x, y after the 16-bit pair `taken` is taken away. */
+template <typename T> __device__ __forceinline__ float2 left_of(float x, float y, uint32_t taken) {
+    const float2 f = Pair<T>::unpack(taken);
+    return make_float2(x - f.x, y - f.y);
+}
+
+/* hi + rest, but an infinite hi as it is: the lower terms of a product with
+ * an infinity are infinities of any sign. */
+__device__ __forceinline__ float plus_terms(float hi, float rest) {
+    return fabsf(hi) == INFINITY ? hi : hi + rest;
+}
+
+/* ---- 16-bit caches: mma.sync m16n8k16 ------------------------------- *
+ *
+ * Of the 16 rows of an A operand only 8 can be different query heads that
+ * share the keys (8 is Llama's largest group), so rows 8-15 carry what the
+ * 16-bit rounding of rows 0-7 left out: a query is hi + lo, and c of row g
+ * plus c of row g + 8, which lie in the same thread, is the fp32 logit at no
+ * further cost.  The weights of the second product are split the same way.
+ * fp16's two terms hold 22 bits (fp32 queries are first scaled by a power
+ * of two into its range), bf16's two hold 16; with fp32 rows a third bf16
+ * term goes through a second mma. */
+template <typename T, typename R, int DP_> struct Halves {
+    static constexpr int DP = DP_, kWarps = 4;
+    static constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value && std::is_same<R, float>::value;
+    static constexpr bool kScaled = std::is_same<T, __half>::value && std::is_same<R, float>::value;
+    static constexpr bool kSplitQ = std::is_same<R, float>::value;
+    static constexpr int kRow = DP * 2 + 16; /* an odd number of 16-byte units: ldmatrix without conflicts */
+    static constexpr int kStageBytes = 2 * kChunk * kRow;
+    static constexpr int kSteps = DP / 16;
+    using Cache = T;
+
+    uint32_t q[kSteps][kSplitQ ? 4 : 2], q3[kThird ? kSteps : 1][2];
+    float o[DP / 8][4];
+    float m, l, unit; /* running maximum (log2), this lane's share of the sum, logit unit */
+
+    __device__ __forceinline__ void begin(const PagedAttention &a, const void *query, int heads,
+                                          float *) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, D = a.p.head_dim;
+        const R *x = static_cast<const R *>(query) + int64_t(g) * D;
+        float top = 0.0f;
+        if (kScaled && g < heads)
+            for (int d = 2 * t; d < D; d += 8)
+                top = fmaxf(top, fmaxf(fabsf(to_float(x[d])), fabsf(to_float(x[d + 1]))));
+        float gain = 1.0f;
+        unit = a.scale * kLog2e;
+        if (kScaled) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            /* greatest |q| to [2^10, 2^11) */
+            const int e = int(__float_as_uint(top) >> 23);
+            if (e > 0 && e < 255) {
+                const int field = min(264 - e, 253);
+                gain = __uint_as_float(uint32_t(field) << 23);
+                unit *= __uint_as_float(uint32_t(254 - field) << 23);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; s++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int d = s * 16 + half * 8 + 2 * t;
+                float v0 = 0.0f, v1 = 0.0f;
+                if (g < heads && d < D) {
+                    v0 = to_float(x[d]) * gain;
+                    v1 = to_float(x[d + 1]) * gain;
+                }
+                const uint32_t hi = Pair<T>::pack(v0, v1);
+                if constexpr (kSplitQ) {
+                    const float2 r = left_of<T>(v0, v1, hi);
+                    const uint32_t lo = Pair<T>::pack(r.x, r.y);
+                    q[s][2 * half] = hi;
+                    q[s][2 * half + 1] = lo;
+                    if constexpr (kThird) {
+                        const float2 r3 = left_of<T>(r.x, r.y, lo);
+                        q3[s][half] = Pair<T>::pack(r3.x, r3.y);
+                    }
+                } else {
+                    q[s][half] = hi;
+                }
+            }
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++)
+            o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    }
+
+    /* 16 slots from the stage at `at`; bit t of `valid` says whether slot t
+     * counts.  z (if not NULL) receives their log2 logits, [heads][stride]. */
+    __device__ __forceinline__ void step(uint32_t at, uint32_t valid, float *, float *z, int stride,
+                                         int heads) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float c[2][2][4], c3[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                c[0][i][j] = c[1][i][j] = c3[i][j] = 0.0f;
+        const uint32_t krow = at + ((lane >> 4) * 8 + (lane & 7)) * kRow + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            uint32_t b[4];
+            load_matrices(b, krow + s * 32);
+            if constexpr (kSplitQ) {
+                Pair<T>::mma(c[s & 1][0], q[s][0], q[s][1], q[s][2], q[s][3], b[0], b[1]);
+                Pair<T>::mma(c[s & 1][1], q[s][0], q[s][1], q[s][2], q[s][3], b[2], b[3]);
+                if constexpr (kThird) {
+                    Pair<T>::mma(c3[0], q3[s][0], 0u, q3[s][1], 0u, b[0], b[1]);
+                    Pair<T>::mma(c3[1], q3[s][0], 0u, q3[s][1], 0u, b[2], b[3]);
+                }
+            } else {
+                Pair<T>::mma(c[s & 1][0], q[s][0], 0u, q[s][1], 0u, b[0], b[1]);
+                Pair<T>::mma(c[s & 1][1], q[s][0], 0u, q[s][1], 0u, b[2], b[3]);
+            }
+        }
+        /* logits of head g, slots 8 i + 2 t + j, in units of log 2 */
+        float s2[2][2], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float v = c[0][i][j] + c[1][i][j];
+                if constexpr (kSplitQ)
+                    v = plus_terms(v, c[0][i][2 + j] + c[1][i][2 + j] + c3[i][j]);
+                v *= unit;
+                if (valid != 0xffffu && !((valid >> (8 * i + 2 * t + j)) & 1))
+                    v = -INFINITY;
+                s2[i][j] = v;
+                top = fmaxf(top, v);
+            }
+        if (z != nullptr && g < heads)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    if ((valid >> (8 * i + 2 * t + j)) & 1)
+                        z[int64_t(g) * stride + 8 * i + 2 * t + j] = s2[i][j];
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float next = fmaxf(m, top);
+        if (__any_sync(0xffffffffu, next != m)) {
+            const float keep = m == next ? 1.0f : exp2f(m - next);
+            l *= keep;
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) {
+                o[n][0] *= keep;
+                o[n][1] *= keep;
+                o[n][2] *= keep;
+                o[n][3] *= keep;
+            }
+            m = next;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        uint32_t hi[2], lo[2], p3[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float w0 = exp2f(s2[i][0] - base), w1 = exp2f(s2[i][1] - base);
+            l += w0 + w1;
+            hi[i] = Pair<T>::pack(w0, w1);
+            const float2 r = left_of<T>(w0, w1, hi[i]);
+            lo[i] = Pair<T>::pack(r.x, r.y);
+            if constexpr (kThird) {
+                const float2 r3 = left_of<T>(r.x, r.y, lo[i]);
+                p3[i] = Pair<T>::pack(r3.x, r3.y);
+            }
+        }
+        const uint32_t vrow = at + kChunk * kRow + (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow +
+                              (lane >> 4) * 16;
+#pragma unroll
+        for (int n = 0; n < DP / 16; n++) {
+            uint32_t b[4];
+            load_matrices_t(b, vrow + n * 32);
+            Pair<T>::mma(o[2 * n], hi[0], lo[0], hi[1], lo[1], b[0], b[1]);
+            Pair<T>::mma(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b[2], b[3]);
+            if constexpr (kThird) {
+                /* into the rows of the second terms */
+                Pair<T>::mma(o[2 * n], 0u, p3[0], 0u, p3[1], b[0], b[1]);
+                Pair<T>::mma(o[2 * n + 1], 0u, p3[0], 0u, p3[1], b[2], b[3]);
+            }
+        }
+    }
+
+    /* This warp's state to out [8][DP], maxima [8], sums [8]. */
+    __device__ __forceinline__ void end(float *out, float *maxima, float *sums) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++)
+            *reinterpret_cast<float2 *>(out + g * DP + n * 8 + 2 * t) =
+                make_float2(plus_terms(o[n][0], o[n][2]), plus_terms(o[n][1], o[n][3]));
+        if (t == 0) {
+            maxima[g] = m;
+            sums[g] = l;
+        }
+    }
+};
+
+/* ---- fp32 caches: FFMA ---------------------------------------------- *
+ *
+ * Logits: lane (slot, half) takes half of the dims of one of 16 slots for
+ * all query heads (queries broadcast from shared memory); the halves meet
+ * with one exchange, after which half h keeps heads h NQ/2 ...  Context: a
+ * lane owns 4 dims, or with fewer than 128 dims 4 dims of a share of the
+ * slots, for all heads. */
+template <int NQ, int DP_> struct Wide {
+    static constexpr int DP = DP_, kWarps = DP > 128 ? 2 : 4;
+    static constexpr int kRow = DP * 4 + 16;
+    static constexpr int kStageBytes = 2 * kChunk * kRow;
+    static constexpr int kOwn = NQ >= 2 ? NQ / 2 : 1; /* heads a lane does the softmax of */
+    static constexpr int kQuads = DP / 4;             /* 4-dim pieces of a row */
+    static constexpr int kLanes = kQuads < 32 ? (kQuads >= 16 ? 16 : 8) : 32; /* lanes across a row */
+    static constexpr int kPieces = (kQuads + kLanes - 1) / kLanes;
+    static constexpr int kShares = 32 / kLanes; /* lanes that share a piece, over slots */
+    using Cache = float;
+
+    float o[NQ][kPieces][4];
+    float m[kOwn], l[kOwn], unit;
+
+    /* scratch: queries [NQ][DP], then per slot weights [16][NQ], then keep [NQ] */
+    static constexpr int kScratch = NQ * DP + kChunk * NQ + NQ + 3;
+
+    __device__ __forceinline__ void begin(const PagedAttention &a, const void *query, int heads,
+                                          float *scratch) {
+        const int lane = threadIdx.x & 31, D = a.p.head_dim;
+        const float *x = static_cast<const float *>(query);
+        __syncwarp();
+        for (int i = lane; i < NQ * DP; i += 32) {
+            const int g = i / DP, d = i % DP;
+            scratch[i] = g < heads && d < D ? x[int64_t(g) * D + d] : 0.0f;
+        }
+        __syncwarp();
+        unit = a.scale * kLog2e;
+#pragma unroll
+        for (int g = 0; g < kOwn; g++) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+        }
+#pragma unroll
+        for (int g = 0; g < NQ; g++)
+#pragma unroll
+            for (int n = 0; n < kPieces; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[g][n][j] = 0.0f;
+    }
+
+    __device__ __forceinline__ void step(uint32_t at, uint32_t valid, float *scratch, float *z,
+                                         int stride, int heads) {
+        const int lane = threadIdx.x & 31, slot = lane & 15, half = lane >> 4;
+        const char *stage = static_cast<const char *>(__cvta_shared_to_generic(at));
+        float s[NQ];
+#pragma unroll
+        for (int g = 0; g < NQ; g++)
+            s[g] = 0.0f;
+        const char *krow = stage + slot * kRow + half * (DP * 2);
+#pragma unroll 4
+        for (int d = 0; d < DP / 2; d += 4) {
+            const float4 k = *reinterpret_cast<const float4 *>(krow + d * 4);
+#pragma unroll
+            for (int g = 0; g < NQ; g++) {
+                const float4 x = *reinterpret_cast<const float4 *>(scratch + g * DP + half * (DP / 2) + d);
+                s[g] = fmaf(x.x, k.x, s[g]);
+                s[g] = fmaf(x.y, k.y, s[g]);
+                s[g] = fmaf(x.z, k.z, s[g]);
+                s[g] = fmaf(x.w, k.w, s[g]);
+            }
+        }
+        float own[kOwn];
+        if constexpr (NQ == 1) {
+            own[0] = s[0] + __shfl_xor_sync(0xffffffffu, s[0], 16);
+        } else {
+#pragma unroll
+            for (int g = 0; g < kOwn; g++) {
+                const float give = half ? s[g] : s[g + kOwn], mine = half ? s[g + kOwn] : s[g];
+                own[g] = mine + __shfl_xor_sync(0xffffffffu, give, 16);
+            }
+        }
+        const bool live = (valid >> slot) & 1;
+        float *weights = scratch + NQ * DP, *keeps = weights + kChunk * NQ;
+        const int h0 = NQ == 1 ? 0 : half * kOwn;
+#pragma unroll
+        for (int g = 0; g < kOwn; g++) {
+            const float v = live ? own[g] * unit : -INFINITY;
+            if (z != nullptr && live && h0 + g < heads && (NQ > 1 || half == 0))
+                z[int64_t(h0 + g) * stride + slot] = v;
+            float top = v;
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float next = fmaxf(m[g], top);
+            const float keep = m[g] == next ? 1.0f : exp2f(m[g] - next);
+            m[g] = next;
+            const float w = exp2f(v - (next == -INFINITY ? 0.0f : next));
+            l[g] = l[g] * keep + w;
+            weights[slot * NQ + h0 + g] = w;
+            if (slot == 0)
+                keeps[h0 + g] = keep;
+        }
+        __syncwarp();
+        const int piece = lane % kLanes, share = lane / kLanes;
+        float keep[NQ];
+#pragma unroll
+        for (int g = 0; g < NQ; g++)
+            keep[g] = keeps[g];
+#pragma unroll
+        for (int g = 0; g < NQ; g++)
+#pragma unroll
+            for (int n = 0; n < kPieces; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[g][n][j] *= keep[g];
+#pragma unroll 4
+        for (int t = share; t < kChunk; t += kShares) {
+            float w[NQ];
+#pragma unroll
+            for (int g = 0; g < NQ; g++)
+                w[g] = weights[t * NQ + g];
+#pragma unroll
+            for (int n = 0; n < kPieces; n++) {
+                if (piece + n * kLanes >= kQuads)
+                    break;
+                const float4 v = *reinterpret_cast<const float4 *>(stage + (kChunk + t) * kRow +
+                                                                   (piece + n * kLanes) * 16);
+#pragma unroll
+                for (int g = 0; g < NQ; g++) {
+                    o[g][n][0] = fmaf(w[g], v.x, o[g][n][0]);
+                    o[g][n][1] = fmaf(w[g], v.y, o[g][n][1]);
+                    o[g][n][2] = fmaf(w[g], v.z, o[g][n][2]);
+                    o[g][n][3] = fmaf(w[g], v.w, o[g][n][3]);
+                }
+            }
+        }
+        __syncwarp(); /* weights are overwritten by the next step */
+    }
+
+    __device__ __forceinline__ void end(float *out, float *maxima, float *sums) {
+        const int lane = threadIdx.x & 31, half = lane >> 4;
+        const int piece = lane % kLanes, share = lane / kLanes;
+#pragma unroll
+        for (int g = 0; g < NQ; g++)
+#pragma unroll
+            for (int n = 0; n < kPieces; n++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int x = kLanes; x < 32; x <<= 1)
+                        o[g][n][j] += __shfl_xor_sync(0xffffffffu, o[g][n][j], x);
+                if (share == 0 && piece + n * kLanes < kQuads)
+                    *reinterpret_cast<float4 *>(out + g * DP + (piece + n * kLanes) * 4) =
+                        make_float4(o[g][n][0], o[g][n][1], o[g][n][2], o[g][n][3]);
+            }
+#pragma unroll
+        for (int g = 0; g < kOwn; g++) {
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1)
+                l[g] += __shfl_xor_sync(0xffffffffu, l[g], x);
+            const int h = (NQ == 1 ? 0 : half * kOwn) + g;
+            if ((lane & 15) == 0 && (NQ > 1 || half == 0)) {
+                maxima[h] = m[g];
+                sums[h] = l[g];
+            }
+        }
+    }
+};
+
+template <typename Op> struct Scratch {
+    static constexpr int value = 0;
+};
+template <int NQ, int DP> struct Scratch<Wide<NQ, DP>> {
+    static constexpr int value = (Wide<NQ, DP>::kScratch + 3) / 4 * 4;
+};
+
+template <int DP> constexpr int stages_of(int stage_bytes) {
+    return stage_bytes <= 5000 ? 4 : stage_bytes <= 13000 ? 3 : 2;
+}
+
+/* Shared memory: each warp's ring of stages and scratch; the warps' states
+ * at an item's end lie over the rings. */
+template <typename Op> struct Plan {
+    static constexpr int kStages = stages_of<Op::DP>(Op::kStageBytes);
+    static constexpr int kRing = kStages * Op::kStageBytes;
+    static constexpr int kScratchBytes = Scratch<Op>::value * 4;
+    static constexpr int kState = (kRows * Op::DP + 2 * kRows) * 4;
+    static constexpr int kWarps = Op::kWarps, kThreads = kWarps * 32;
+    static constexpr int kTile = kWarps * kChunk; /* slots of a tile */
+    static constexpr int kBody = kWarps * (kRing + kScratchBytes);
+    static constexpr int kBytes = kBody > kWarps * kState ? kBody : kWarps * kState;
+};
+
+/* Slots of a row that the kernel walks: its length, or the listed pages. */
+__device__ __forceinline__ int walked(const PagedAttention &a, int length) {
+    return length == 0 ? 0 : a.selected ? a.n_selected * a.p.page_size : length;
+}
+
+template <typename Op, typename R>
+__global__ void __launch_bounds__(Plan<Op>::kThreads)
+    attention_kernel(const __grid_constant__ PagedAttention a) {
+    using T = typename Op::Cache;
+    constexpr int DP = Op::DP, kStages = Plan<Op>::kStages, kWarps = Plan<Op>::kWarps,
+                  kThreads = Plan<Op>::kThreads, kTile = Plan<Op>::kTile;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ uint32_t masks[kWarps][kStages];
+    __shared__ int64_t warp_sum64[kWarps];
+    __shared__ int found_row, is_last;
+    __shared__ int64_t found_tile;
+    const PagedPool &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int groups = (p.group + kRows - 1) / kRows, items_per_row = p.kv_heads * groups;
+
+    /* rows that see nothing */
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        int length;
+        row_span(p, a.row_sequence, a.row_length, r, length);
+        if (length != 0)
+            continue;
+        for (int i = tid; i < p.heads * p.head_dim; i += kThreads)
+            static_cast<R *>(a.out)[r * a.out_stride + i] = from_float<R>(0.0f);
+        for (int h = tid; h < p.heads; h += kThreads)
+            if (a.lse)
+                a.lse[int64_t(r) * p.heads + h] = -INFINITY;
+    }
+
+    /* this CTA's share of the line of tiles: thread i sums a run of rows */
+    const int run = (a.rows + kThreads - 1) / kThreads;
+    const int r0 = min(tid * run, a.rows), r1 = min(r0 + run, a.rows);
+    int64_t mine = 0;
+    for (int r = r0; r < r1; r++) {
+        int length;
+        row_span(p, a.row_sequence, a.row_length, r, length);
+        mine += (walked(a, length) + kTile - 1) / kTile;
+    }
+    int64_t upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
+        upto += lane >= x ? v : 0;
+    }
+    if (lane == 31)
+        warp_sum64[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        upto += w < warp ? warp_sum64[w] : 0;
+        total += warp_sum64[w];
+    }
+    total *= items_per_row;
+    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    int64_t pos = int64_t(blockIdx.x) * share;
+    const int64_t last = min(pos + share, total);
+    if (pos >= last)
+        return;
+    const int64_t before = upto - mine;
+    if (pos >= before * items_per_row && pos < upto * items_per_row) {
+        int64_t at = before * items_per_row;
+        for (int r = r0; r < r1; r++) {
+            int length;
+            row_span(p, a.row_sequence, a.row_length, r, length);
+            const int64_t n = int64_t((walked(a, length) + kTile - 1) / kTile) * items_per_row;
+            if (pos < at + n) {
+                found_row = r;
+                found_tile = pos - at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    int r = found_row;
+    int64_t in_row = found_tile; /* tile within the row's items */
+
+    char *ring = smem + warp * Plan<Op>::kRing;
+    const uint32_t ring_at = smem_addr(ring);
+    float *scratch = reinterpret_cast<float *>(smem + kWarps * Plan<Op>::kRing +
+                                               warp * Plan<Op>::kScratchBytes);
+    const int D = p.head_dim;
+    constexpr int kUnit = 16 / sizeof(T);    /* elements of a 16-byte piece */
+    constexpr int kPieces = DP / kUnit;      /* of a padded row */
+    const int pieces = D / kUnit;            /* of a row */
+
+    while (pos < last) {
+        int length;
+        const int s = row_span(p, a.row_sequence, a.row_length, r, length);
+        const int span = walked(a, length), tiles = (span + kTile - 1) / kTile;
+        if (tiles == 0) {
+            r++;
+            continue;
+        }
+        const int item = int(in_row / tiles), tile0 = int(in_row % tiles);
+        const int tile1 = int(min(int64_t(tiles), tile0 + (last - pos)));
+        const int head = item / groups, first_head = head * p.group + (item % groups) * kRows;
+        const int heads = min(kRows, p.group - (item % groups) * kRows);
+        const int32_t *list =
+            a.selected ? a.selected + (int64_t(r) * p.kv_heads + head) * a.n_selected : nullptr;
+        const T *keys = static_cast<const T *>(p.keys) + int64_t(head) * p.head_stride;
+        const T *values = static_cast<const T *>(p.values) + int64_t(head) * p.head_stride;
+
+        /* where slot `lane` (of 16) of this warp's chunk in a tile lies, or -1 */
+        auto locate = [&](int tile) -> int64_t {
+            const int v = tile * kTile + warp * kChunk + (lane & 15);
+            if (tile >= tile1 || v >= span)
+                return -1;
+            int j = v / p.page_size;
+            const int place = v - j * p.page_size;
+            if (list) {
+                j = list[j];
+                if (j < 0 || j >= p.max_pages || j * p.page_size + place >= length)
+                    return -1;
+            }
+            const int page = checked_page(p, s, j);
+            return page < 0 ? -1 : int64_t(page) * p.page_stride + int64_t(place) * p.slot_stride;
+        };
+        auto issue = [&](int stage, int64_t offset) {
+            const uint32_t to = ring_at + stage * Op::kStageBytes;
+            const uint32_t valid = __ballot_sync(0xffffffffu, offset >= 0) & 0xffffu;
+            if (lane == 0)
+                masks[warp][stage] = valid;
+            if (valid != 0) {
+#pragma unroll
+                for (int i = 0; i < kPieces * kChunk / 32; i++) {
+                    const int e = i * 32 + lane, row = e / kPieces, piece = e % kPieces;
+                    const int64_t off = __shfl_sync(0xffffffffu, offset, row);
+                    const bool ok = off >= 0 && piece < pieces;
+                    const int64_t from = ok ? off + piece * kUnit : 0;
+                    copy16(to + row * Op::kRow + piece * 16, keys + from, ok);
+                    copy16(to + (kChunk + row) * Op::kRow + piece * 16, values + from, ok);
+                }
+            }
+            copies_commit();
+        };
+
+        Op op;
+        int64_t next = locate(tile0);
+        for (int i = 0; i < kStages - 1; i++) {
+            issue(i, next);
+            next = locate(tile0 + i + 1);
+        }
+        op.begin(a, static_cast<const R *>(a.q) + r * a.q_stride + int64_t(first_head) * D, heads,
+                 scratch);
+        int stage = 0;
+        for (int tile = tile0; tile < tile1; tile++) {
+            issue(stage == 0 ? kStages - 1 : stage - 1, next);
+            next = locate(tile + kStages);
+            copies_wait<kStages - 1>();
+            __syncwarp();
+            const uint32_t valid = masks[warp][stage];
+            if (valid != 0) {
+                float *z = a.weights ? a.logits + (int64_t(r) * p.heads + first_head) * p.capacity +
+                                           tile * kTile + warp * kChunk
+                                     : nullptr;
+                op.step(ring_at + stage * Op::kStageBytes, valid, scratch, z, p.capacity, heads);
+            }
+            __syncwarp();
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        copies_wait<0>();
+        __syncthreads(); /* every warp is done with its ring */
+
+        /* the warps' states, joined: o at [row][d], statistics per row */
+        float *state = reinterpret_cast<float *>(smem);
+        constexpr int kStateFloats = Plan<Op>::kState / 4;
+        {
+            float *own = state + warp * kStateFloats;
+            op.end(own, own + kRows * DP, own + kRows * DP + kRows);
+        }
+        __syncthreads();
+        const bool whole = tile0 == 0 && tile1 == tiles;
+        const int64_t item_start = pos - tile0; /* of this item on the line */
+        float *part = a.partial + (int64_t(blockIdx.x) * 2 + (item_start <= int64_t(blockIdx.x) * share ? 0 : 1)) *
+                                      kPartialFloats;
+        for (int i = tid; i < heads * DP; i += kThreads) {
+            const int g = i / DP, d = i % DP;
+            float top = -INFINITY, sum = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++)
+                top = fmaxf(top, state[w * kStateFloats + kRows * DP + g]);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float *st = state + w * kStateFloats;
+                const float f = exp2f(st[kRows * DP + g] - base);
+                sum = fmaf(st[kRows * DP + kRows + g], f, sum);
+                if (f > 0.0f || f != f)
+                    o = fmaf(st[i], f, o);
+            }
+            if (!whole) {
+                part[2 * kRows + g * kMaxDim + d] = o;
+                if (d == 0) {
+                    part[g] = top;
+                    part[kRows + g] = sum;
+                }
+                continue;
+            }
+            if (d < D)
+                static_cast<R *>(a.out)[r * a.out_stride + int64_t(first_head + g) * D + d] =
+                    from_float<R>(sum == 0.0f ? 0.0f : o / sum);
+            if (d == 0) {
+                const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
+                if (a.lse)
+                    a.lse[int64_t(r) * p.heads + first_head + g] = lse2 * kLn2;
+                if (a.weights)
+                    a.lse2[int64_t(r) * p.heads + first_head + g] = lse2;
+            }
+        }
+        if (!whole) {
+            const int64_t c0 = item_start / share, c1 = (item_start + tiles - 1) / share;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                int *counter = a.counters + int64_t(r) * items_per_row + item;
+                is_last = atomicAdd(counter, 1) == int(c1 - c0);
+                if (is_last)
+                    *counter = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (is_last) {
+                for (int i = tid; i < heads * DP; i += kThreads) {
+                    const int g = i / DP, d = i % DP;
+                    float top = -INFINITY, sum = 0.0f, o = 0.0f;
+                    for (int64_t c = c0; c <= c1; c++) {
+                        const float *x = a.partial + (c * 2 + (item_start <= c * share ? 0 : 1)) * kPartialFloats;
+                        const float mc = __ldcg(x + g), lc = __ldcg(x + kRows + g);
+                        if (lc == 0.0f) /* nothing seen there */
+                            continue;
+                        const float oc = __ldcg(x + 2 * kRows + g * kMaxDim + d);
+                        const float nt = fmaxf(top, mc), f0 = top == nt ? 1.0f : exp2f(top - nt),
+                                    f1 = mc == nt ? 1.0f : exp2f(mc - nt);
+                        sum = sum * f0 + lc * f1;
+                        o = o * f0 + oc * f1;
+                        top = nt;
+                    }
+                    if (d < D)
+                        static_cast<R *>(a.out)[r * a.out_stride + int64_t(first_head + g) * D + d] =
+                            from_float<R>(sum == 0.0f ? 0.0f : o / sum);
+                    if (d == 0) {
+                        const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
+                        if (a.lse)
+                            a.lse[int64_t(r) * p.heads + first_head + g] = lse2 * kLn2;
+                        if (a.weights)
+                            a.lse2[int64_t(r) * p.heads + first_head + g] = lse2;
+                    }
+                }
+            }
+        }
+        __syncthreads(); /* the state is overwritten by the next item's stages */
+        pos += tile1 - tile0;
+        in_row += tile1 - tile0;
+        if (in_row >= int64_t(tiles) * items_per_row) {
+            in_row = 0;
+            r++;
+        }
+    }
+}
+
+/* weights_out[t] = weights[t] + sum over the group of exp(z_t - lse): every
+ * slot has one writer, so the order of the sum is fixed. */
+__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ PagedAttention a) {
+    const PagedPool &p = a.p;
+    const int head = blockIdx.y, r = blockIdx.z;
+    int length;
+    row_span(p, a.row_sequence, a.row_length, r, length);
+    const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity;
+    const int64_t h0 = int64_t(r) * p.heads + head * p.group;
+    for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < length; t += gridDim.x * blockDim.x) {
+        float w = 0.0f;
+        for (int g = 0; g < p.group; g++)
+            w += exp2f(a.logits[(h0 + g) * p.capacity + t] - a.lse2[h0 + g]);
+        a.weights_out[to + t] = a.weights[to + t] + w;
+    }
+}
+
+template <typename Op, typename R>
+cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
+    constexpr int bytes = Plan<Op>::kBytes, threads = Plan<Op>::kThreads, tile = Plan<Op>::kTile;
+    static_assert(bytes <= 227 * 1024, "stages exceed the SM's shared memory");
+    static int fit[kMaxDevices] = {};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    int &per_sm = fit[device % kMaxDevices];
+    if (per_sm == 0) {
+        e = cudaFuncSetAttribute(attention_kernel<Op, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess)
+            return e;
+        int n = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_kernel<Op, R>, threads, bytes);
+        if (e != cudaSuccess)
+            return e;
+        per_sm = n < 1 ? 1 : n > kMaxCtasPerSm ? kMaxCtasPerSm : n;
+    }
+    const PagedPool &p = a.p;
+    const int64_t items = int64_t(a.rows) * p.kv_heads * ((p.group + kRows - 1) / kRows);
+    const int64_t slots = a.selected ? int64_t(a.n_selected) * p.page_size : p.capacity;
+    const int64_t tiles = items * ((slots + tile - 1) / tile);
+    const int64_t ctas = int64_t(a.sms) * per_sm;
+    attention_kernel<Op, R><<<unsigned(tiles < ctas ? tiles : ctas), threads, bytes, s>>>(a);
+    count_launches(1);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !a.weights)
+        return e;
+    const unsigned blocks = unsigned((p.capacity + 1023) / 1024);
+    weights_kernel<<<dim3(blocks, p.kv_heads, a.rows), 256, 0, s>>>(a);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+template <typename T, typename R> cudaError_t launch_halves(const PagedAttention &a, cudaStream_t s) {
+    const int D = a.p.head_dim;
+    if (D <= 32)
+        return launch<Halves<T, R, 32>, R>(a, s);
+    if (D <= 64)
+        return launch<Halves<T, R, 64>, R>(a, s);
+    if (D <= 96)
+        return launch<Halves<T, R, 96>, R>(a, s);
+    if (D <= 128)
+        return launch<Halves<T, R, 128>, R>(a, s);
+    if (D <= 192)
+        return launch<Halves<T, R, 192>, R>(a, s);
+    return launch<Halves<T, R, 256>, R>(a, s);
+}
+
+template <int NQ> cudaError_t launch_wide(const PagedAttention &a, cudaStream_t s) {
+    const int D = a.p.head_dim;
+    if (D <= 32)
+        return launch<Wide<NQ, 32>, float>(a, s);
+    if (D <= 64)
+        return launch<Wide<NQ, 64>, float>(a, s);
+    if (D <= 128)
+        return launch<Wide<NQ, 128>, float>(a, s);
+    return launch<Wide<NQ, 256>, float>(a, s);
 }
 
 } // namespace
 
 cudaError_t paged_attention(const PagedAttention &a, cudaStream_t s) {
-    const PagedPool &p = a.p;
-    const dim3 grid(p.kv_heads, a.rows);
-    const int n = kWarps * 32;
-    if (p.type == 0)
-        attention_simple_kernel<float, float><<<grid, n, 0, s>>>(a);
-    else if (p.type == 1 && a.type == 0)
-        attention_simple_kernel<float, __half><<<grid, n, 0, s>>>(a);
-    else if (p.type == 1)
-        attention_simple_kernel<__half, __half><<<grid, n, 0, s>>>(a);
-    else if (a.type == 0)
-        attention_simple_kernel<float, __nv_bfloat16><<<grid, n, 0, s>>>(a);
-    else
-        attention_simple_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, n, 0, s>>>(a);
-    count_launches(1);
-    return cudaGetLastError();
+    if (a.p.type == 0)
+        return a.p.group == 1 ? launch_wide<1>(a, s) : a.p.group <= 4 ? launch_wide<4>(a, s) : launch_wide<8>(a, s);
+    if (a.p.type == 1)
+        return a.type == 0 ? launch_halves<__half, float>(a, s) : launch_halves<__half, __half>(a, s);
+    return a.type == 0 ? launch_halves<__nv_bfloat16, float>(a, s)
+                       : launch_halves<__nv_bfloat16, __nv_bfloat16>(a, s);
 }
 
 } // namespace nut

@@ -114,15 +114,14 @@ struct nut_paged {
     nut::PagedPool pool{};
     int max_rows = 0;
     bool track = false;
-    int *error = nullptr;
-    float *logits = nullptr, *scores = nullptr;
+    int sms = 0;
+    char *block = nullptr; /* one allocation, cut into the parts below */
+    int *error = nullptr, *counters = nullptr;
+    float *partial = nullptr, *logits = nullptr, *lse2 = nullptr, *scores = nullptr;
     int32_t *pairs = nullptr, *counts = nullptr;
     ~nut_paged() {
-        for (void *p : {static_cast<void *>(error), static_cast<void *>(logits),
-                        static_cast<void *>(scores), static_cast<void *>(pairs),
-                        static_cast<void *>(counts)})
-            if (p)
-                cudaFree(p);
+        if (block)
+            cudaFree(block);
     }
 };
 
@@ -179,18 +178,36 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         p.group = int(v.heads / v.kv_heads);
         p.capacity = int(v.max_pages * v.page_size);
         p.type = v.type;
-        h->error = dev_alloc<int>(1, "alloc error word");
-        p.error = h->error;
-        cuda_check(cudaMemset(h->error, 0, sizeof(int)), "clear error word");
+        cuda_check(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device),
+                   "count SMs");
         const size_t items = size_t(p.sequences) * p.kv_heads;
-        h->pairs = dev_alloc<int32_t>(items * p.capacity, "alloc slot pairs");
-        h->counts = dev_alloc<int32_t>(items * 2, "alloc pair counts");
-        if (h->track)
-            h->logits = dev_alloc<float>(size_t(p.sequences) * p.heads * p.capacity,
-                                         "alloc attention logits");
-        if (p.bounds)
-            h->scores = dev_alloc<float>(size_t(h->max_rows) * p.kv_heads * p.max_pages,
-                                         "alloc page scores");
+        size_t bytes = 0;
+        const auto part = [&](size_t count, size_t size) {
+            const size_t at = bytes;
+            bytes += (count * size + 255) / 256 * 256;
+            return at;
+        };
+        /* zeroed at first: the error word and the counters */
+        const size_t error = part(1, 4);
+        const size_t counters = part(size_t(h->max_rows) * p.kv_heads * ((p.group + 7) / 8), 4);
+        const size_t zeroed = bytes;
+        const size_t partial = part(size_t(h->sms) * nut::kMaxCtasPerSm * 2 * nut::kPartialFloats, 4);
+        const size_t pairs = part(items * p.capacity, 4), counts = part(items * 2, 4);
+        const size_t logits = part(h->track ? size_t(p.sequences) * p.heads * p.capacity : 0, 4);
+        const size_t lse2 = part(h->track ? size_t(p.sequences) * p.heads : 0, 4);
+        const size_t scores = part(p.bounds ? size_t(h->max_rows) * p.kv_heads * p.max_pages : 0, 4);
+        h->block = dev_alloc<char>(bytes, "alloc workspace");
+        const auto floats = [&](size_t at) { return reinterpret_cast<float *>(h->block + at); };
+        const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(h->block + at); };
+        p.error = h->error = ints(error);
+        h->counters = ints(counters);
+        h->partial = floats(partial);
+        h->pairs = ints(pairs);
+        h->counts = ints(counts);
+        h->logits = floats(logits);
+        h->lse2 = floats(lse2);
+        h->scores = floats(scores);
+        cuda_check(cudaMemset(h->block, 0, zeroed), "clear workspace");
         cuda_check(cudaStreamSynchronize(nullptr), "finish workspace");
         *out = h.release();
     });
@@ -335,6 +352,10 @@ nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *arg
         a.type = g.type;
         a.scale = g.scale != 0.0f ? g.scale : float(1.0 / std::sqrt(double(p.head_dim)));
         a.logits = h->logits;
+        a.lse2 = h->lse2;
+        a.partial = h->partial;
+        a.counters = h->counters;
+        a.sms = h->sms;
         DeviceScope scope(h->device);
         cuda_check(nut::paged_attention(a, static_cast<cudaStream_t>(stream)), "paged attention");
     });
