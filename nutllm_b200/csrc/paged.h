@@ -63,6 +63,7 @@ struct PagedAttention {
 constexpr int kMaxDim = 256;
 constexpr int kPartialFloats = 8 * 2 + 8 * kMaxDim;
 constexpr int kMaxCtasPerSm = 4;
+constexpr int kMaxSms = 160;
 constexpr int kMaxDevices = 64;
 
 struct PagedSelect {

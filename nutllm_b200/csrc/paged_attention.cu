@@ -477,11 +477,75 @@ template <typename Op> struct Plan {
     static constexpr int kTile = kWarps * kChunk; /* slots of a tile */
     static constexpr int kBody = kWarps * (kRing + kScratchBytes);
     static constexpr int kBytes = kBody > kWarps * kState ? kBody : kWarps * kState;
+    static_assert(kBytes >= kMaxSms * kMaxCtasPerSm * kRows * 4, "an item's parts have their factors there");
 };
 
 /* Slots of a row that the kernel walks: its length, or the listed pages. */
 __device__ __forceinline__ int walked(const PagedAttention &a, int length) {
     return length == 0 ? 0 : a.selected ? a.n_selected * a.p.page_size : length;
+}
+
+/* Joins the `parts` parts of an item left by CTAs c0, c0 + 1, ...; run by
+ * the whole CTA that arrived last.  Warps first turn the parts' maxima and
+ * sums into one factor exp(m_c - m) / l per part and head, in shared memory;
+ * then a thread adds 4 dims of the parts' outputs with many loads in flight
+ * (one after another, 37 parts cost 200 us; this way 6). */
+template <typename R, int DP, int kWarps>
+__device__ void join_parts(const PagedAttention &a, int64_t item_start, int64_t share, int c0, int parts,
+                           int r, int first_head, int heads, float *factor) {
+    const PagedPool &p = a.p;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    /* an item that starts inside its first CTA's share lies in that one's second slot */
+    const float *first = a.partial + (int64_t(c0) * 2 + (item_start <= c0 * share ? 0 : 1)) * kPartialFloats;
+    const float *rest = a.partial + (int64_t(c0) * 2 + 2) * kPartialFloats;
+    auto part = [&](int c) { return c == 0 ? first : rest + int64_t(c - 1) * 2 * kPartialFloats; };
+    for (int g = warp; g < heads; g += kWarps) {
+        float top = -INFINITY;
+        for (int c = lane; c < parts; c += 32) {
+            const float m = __ldcg(part(c) + g);
+            factor[c * kRows + g] = m;
+            top = fmaxf(top, m);
+        }
+        top = warp_max(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        for (int c = lane; c < parts; c += 32) {
+            const float f = exp2f(factor[c * kRows + g] - base), l = __ldcg(part(c) + kRows + g);
+            factor[c * kRows + g] = f;
+            sum = l != 0.0f ? fmaf(l, f, sum) : sum;
+        }
+        sum = warp_sum(sum);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int c = lane; c < parts; c += 32)
+            factor[c * kRows + g] *= inv;
+        if (lane == 0) {
+            const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
+            if (a.lse)
+                a.lse[int64_t(r) * p.heads + first_head + g] = lse2 * kLn2;
+            if (a.weights)
+                a.lse2[int64_t(r) * p.heads + first_head + g] = lse2;
+        }
+    }
+    __syncthreads();
+    const int quads = p.head_dim / 4;
+    for (int i = threadIdx.x; i < heads * quads; i += kWarps * 32) {
+        const int g = i / quads, d = i % quads * 4, at = 2 * kRows + g * kMaxDim + d;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int c = 0; c < parts; c++) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(c) + at));
+            const float f = factor[c * kRows + g];
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
+            o.z = fmaf(x.z, f, o.z);
+            o.w = fmaf(x.w, f, o.w);
+        }
+        R *to = static_cast<R *>(a.out) + r * a.out_stride + int64_t(first_head + g) * p.head_dim + d;
+        to[0] = from_float<R>(o.x);
+        to[1] = from_float<R>(o.y);
+        to[2] = from_float<R>(o.z);
+        to[3] = from_float<R>(o.w);
+    }
 }
 
 template <typename Op, typename R>
@@ -706,34 +770,9 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
                 __threadfence();
             }
             __syncthreads();
-            if (is_last) {
-                for (int i = tid; i < heads * DP; i += kThreads) {
-                    const int g = i / DP, d = i % DP;
-                    float top = -INFINITY, sum = 0.0f, o = 0.0f;
-                    for (int64_t c = c0; c <= c1; c++) {
-                        const float *x = a.partial + (c * 2 + (item_start <= c * share ? 0 : 1)) * kPartialFloats;
-                        const float mc = __ldcg(x + g), lc = __ldcg(x + kRows + g);
-                        if (lc == 0.0f) /* nothing seen there */
-                            continue;
-                        const float oc = __ldcg(x + 2 * kRows + g * kMaxDim + d);
-                        const float nt = fmaxf(top, mc), f0 = top == nt ? 1.0f : exp2f(top - nt),
-                                    f1 = mc == nt ? 1.0f : exp2f(mc - nt);
-                        sum = sum * f0 + lc * f1;
-                        o = o * f0 + oc * f1;
-                        top = nt;
-                    }
-                    if (d < D)
-                        static_cast<R *>(a.out)[r * a.out_stride + int64_t(first_head + g) * D + d] =
-                            from_float<R>(sum == 0.0f ? 0.0f : o / sum);
-                    if (d == 0) {
-                        const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
-                        if (a.lse)
-                            a.lse[int64_t(r) * p.heads + first_head + g] = lse2 * kLn2;
-                        if (a.weights)
-                            a.lse2[int64_t(r) * p.heads + first_head + g] = lse2;
-                    }
-                }
-            }
+            if (is_last)
+                join_parts<R, DP, kWarps>(a, item_start, share, int(c0), int(c1 - c0) + 1, r, first_head,
+                                          heads, reinterpret_cast<float *>(smem));
         }
         __syncthreads(); /* the state is overwritten by the next item's stages */
         pos += tile1 - tile0;

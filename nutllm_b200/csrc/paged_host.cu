@@ -180,6 +180,7 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         p.type = v.type;
         cuda_check(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device),
                    "count SMs");
+        h->sms = std::min(h->sms, nut::kMaxSms);
         const size_t items = size_t(p.sequences) * p.kv_heads;
         size_t bytes = 0;
         const auto part = [&](size_t count, size_t size) {
