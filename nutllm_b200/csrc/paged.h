@@ -2,6 +2,7 @@
 /* Paged KV cache operators (nut_paged_* in nutllm_cuda.h): what the kernels
  * see of a pool, and their host-side launchers. */
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace nut {
@@ -12,7 +13,8 @@ enum PagedError {
     kPagedBadLength = 2,   /* length outside [0, capacity] */
     kPagedBadSequence = 4, /* row's sequence outside the table */
     kPagedBadStarts = 8,   /* starts not ascending, or more new rows than slots */
-    kPagedBadPosition = 16 /* position outside the rotation table */
+    kPagedBadPosition = 16, /* position outside the rotation table */
+    kPagedTimeout = 32      /* a copy did not arrive in time */
 };
 
 struct PagedPool {
@@ -41,7 +43,9 @@ struct PagedAppend {
 };
 
 struct PagedAttention {
+    CUtensorMap key_map, value_map; /* (dim, slot, kv head, page), boxes of 128 bytes x `box` slots */
     PagedPool p;
+    int box; /* the greatest power of two up to 16 that divides page_size */
     const void *q;
     void *out;
     int64_t q_stride, out_stride;

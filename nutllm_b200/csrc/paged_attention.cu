@@ -18,27 +18,43 @@
 
 #include "kernels.h"
 #include "paged.cuh"
+#include "stream.cuh"
 
 namespace nut {
 namespace {
 
 constexpr int kChunk = 16; /* slots a warp takes at a time */
 constexpr int kRows = 8;   /* query heads of an item */
+constexpr int kBlock = kChunk * 128; /* a chunk's 128-byte columns, in the 128-byte swizzle */
+constexpr int kItemCost = 2; /* what an item costs besides its tiles, in tiles */
+constexpr uint64_t kPagedWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-/* 16 bytes to shared memory, zeros where !valid (nothing is read then). */
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from),
-                 "r"(valid ? 16 : 0)
+/* One box of the pool to shared memory: columns x .. x + 128 bytes, the map's
+ * rows from slot y, of kv head h and page w; arrives on `bar`. */
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, int x, int y, int h, int w,
+                                         uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(to),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(h), "r"(w)
                  : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+
+/* Waits for a stage without sleeping; false after kPagedWaitNs. */
+__device__ __forceinline__ bool stage_wait(uint64_t *bar, uint32_t parity) {
+    uint64_t start = 0;
+    for (int i = 0;; i++) {
+        if (mbar_try_wait(bar, parity))
+            return true;
+        if ((i & 63) == 63) {
+            const uint64_t now = global_ns();
+            if (start == 0)
+                start = now;
+            else if (now - start > kPagedWaitNs)
+                return false;
+        }
+    }
 }
 
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
@@ -115,8 +131,8 @@ template <typename T, typename R, int DP_> struct Halves {
     static constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value && std::is_same<R, float>::value;
     static constexpr bool kScaled = std::is_same<T, __half>::value && std::is_same<R, float>::value;
     static constexpr bool kSplitQ = std::is_same<R, float>::value;
-    static constexpr int kRow = DP * 2 + 16; /* an odd number of 16-byte units: ldmatrix without conflicts */
-    static constexpr int kStageBytes = 2 * kChunk * kRow;
+    static constexpr int kBlocks = (DP * 2 + 127) / 128; /* 128-byte columns of a row */
+    static constexpr int kStageBytes = 2 * kBlocks * kBlock;
     static constexpr int kSteps = DP / 16;
     using Cache = T;
 
@@ -187,11 +203,12 @@ template <typename T, typename R, int DP_> struct Halves {
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 c[0][i][j] = c[1][i][j] = c3[i][j] = 0.0f;
-        const uint32_t krow = at + ((lane >> 4) * 8 + (lane & 7)) * kRow + ((lane >> 3) & 1) * 16;
+        /* 16-byte piece c of row r lies at piece c ^ (r & 7) of its 128 bytes */
+        const uint32_t krow = at + ((lane >> 4) * 8 + (lane & 7)) * 128, kx = (((lane >> 3) & 1) ^ (lane & 7)) * 16;
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
             uint32_t b[4];
-            load_matrices(b, krow + s * 32);
+            load_matrices(b, krow + (s / 4) * kBlock + (kx ^ ((s & 3) * 32)));
             if constexpr (kSplitQ) {
                 Pair<T>::mma(c[s & 1][0], q[s][0], q[s][1], q[s][2], q[s][3], b[0], b[1]);
                 Pair<T>::mma(c[s & 1][1], q[s][0], q[s][1], q[s][2], q[s][3], b[2], b[3]);
@@ -255,12 +272,11 @@ template <typename T, typename R, int DP_> struct Halves {
                 p3[i] = Pair<T>::pack(r3.x, r3.y);
             }
         }
-        const uint32_t vrow = at + kChunk * kRow + (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow +
-                              (lane >> 4) * 16;
+        const uint32_t vrow = at + kBlocks * kBlock + (lane & 15) * 128, vx = ((lane >> 4) ^ (lane & 7)) * 16;
 #pragma unroll
         for (int n = 0; n < DP / 16; n++) {
             uint32_t b[4];
-            load_matrices_t(b, vrow + n * 32);
+            load_matrices_t(b, vrow + (n / 4) * kBlock + (vx ^ ((n & 3) * 32)));
             Pair<T>::mma(o[2 * n], hi[0], lo[0], hi[1], lo[1], b[0], b[1]);
             Pair<T>::mma(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b[2], b[3]);
             if constexpr (kThird) {
@@ -296,8 +312,8 @@ template <typename T, typename R, int DP_> struct Halves {
  * slots, for all heads. */
 template <int NQ, int DP_> struct Wide {
     static constexpr int DP = DP_, kWarps = DP > 128 ? 2 : 4;
-    static constexpr int kRow = DP * 4 + 16;
-    static constexpr int kStageBytes = 2 * kChunk * kRow;
+    static constexpr int kBlocks = DP / 32; /* 128-byte columns of a row */
+    static constexpr int kStageBytes = 2 * kBlocks * kBlock;
     static constexpr int kOwn = NQ >= 2 ? NQ / 2 : 1; /* heads a lane does the softmax of */
     static constexpr int kQuads = DP / 4;             /* 4-dim pieces of a row */
     static constexpr int kLanes = kQuads < 32 ? (kQuads >= 16 ? 16 : 8) : 32; /* lanes across a row */
@@ -344,10 +360,13 @@ template <int NQ, int DP_> struct Wide {
 #pragma unroll
         for (int g = 0; g < NQ; g++)
             s[g] = 0.0f;
-        const char *krow = stage + slot * kRow + half * (DP * 2);
+        /* 16-byte piece c of row r lies at piece c ^ (r & 7) of its 128 bytes */
+        const char *krow = stage + slot * 128;
 #pragma unroll 4
         for (int d = 0; d < DP / 2; d += 4) {
-            const float4 k = *reinterpret_cast<const float4 *>(krow + d * 4);
+            const int piece = half * (DP / 8) + d / 4;
+            const float4 k = *reinterpret_cast<const float4 *>(krow + (piece >> 3) * kBlock +
+                                                               (((piece & 7) ^ (slot & 7)) << 4));
 #pragma unroll
             for (int g = 0; g < NQ; g++) {
                 const float4 x = *reinterpret_cast<const float4 *>(scratch + g * DP + half * (DP / 2) + d);
@@ -411,8 +430,9 @@ template <int NQ, int DP_> struct Wide {
             for (int n = 0; n < kPieces; n++) {
                 if (piece + n * kLanes >= kQuads)
                     break;
-                const float4 v = *reinterpret_cast<const float4 *>(stage + (kChunk + t) * kRow +
-                                                                   (piece + n * kLanes) * 16);
+                const int c = piece + n * kLanes;
+                const float4 v = *reinterpret_cast<const float4 *>(stage + (kBlocks + (c >> 3)) * kBlock + t * 128 +
+                                                                   (((c & 7) ^ (t & 7)) << 4));
 #pragma unroll
                 for (int g = 0; g < NQ; g++) {
                     o[g][n][0] = fmaf(w[g], v.x, o[g][n][0]);
@@ -463,7 +483,7 @@ template <int NQ, int DP> struct Scratch<Wide<NQ, DP>> {
 };
 
 template <int DP> constexpr int stages_of(int stage_bytes) {
-    return stage_bytes <= 5000 ? 4 : stage_bytes <= 13000 ? 3 : 2;
+    return stage_bytes <= 4096 ? 4 : stage_bytes <= 12288 ? 3 : 2;
 }
 
 /* Shared memory: each warp's ring of stages and scratch; the warps' states
@@ -476,7 +496,7 @@ template <typename Op> struct Plan {
     static constexpr int kWarps = Op::kWarps, kThreads = kWarps * 32;
     static constexpr int kTile = kWarps * kChunk; /* slots of a tile */
     static constexpr int kBody = kWarps * (kRing + kScratchBytes);
-    static constexpr int kBytes = kBody > kWarps * kState ? kBody : kWarps * kState;
+    static constexpr int kBytes = (kBody > kWarps * kState ? kBody : kWarps * kState) + 1024; /* to align */
     static_assert(kBytes >= kMaxSms * kMaxCtasPerSm * kRows * 4, "an item's parts have their factors there");
 };
 
@@ -548,20 +568,32 @@ __device__ void join_parts(const PagedAttention &a, int64_t item_start, int64_t 
     }
 }
 
+/* An item of so many tiles takes up this much of the line: its tiles come
+ * behind kItemCost places without one. */
+__device__ __forceinline__ int line_of(int tiles) { return tiles == 0 ? 0 : tiles + kItemCost; }
+
 template <typename Op, typename R>
 __global__ void __launch_bounds__(Plan<Op>::kThreads)
     attention_kernel(const __grid_constant__ PagedAttention a) {
     using T = typename Op::Cache;
     constexpr int DP = Op::DP, kStages = Plan<Op>::kStages, kWarps = Plan<Op>::kWarps,
                   kThreads = Plan<Op>::kThreads, kTile = Plan<Op>::kTile;
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ char smem_raw[];
+    char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint32_t masks[kWarps][kStages];
+    __shared__ uint64_t full[kWarps][kStages];
     __shared__ int64_t warp_sum64[kWarps];
     __shared__ int found_row, is_last;
     __shared__ int64_t found_tile;
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int groups = (p.group + kRows - 1) / kRows, items_per_row = p.kv_heads * groups;
+
+    if (tid == 0) {
+        for (int i = 0; i < kWarps * kStages; i++)
+            mbar_init(&full[0][0] + i, 1);
+        fence_barrier_init();
+    }
 
     /* rows that see nothing */
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -583,7 +615,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
     for (int r = r0; r < r1; r++) {
         int length;
         row_span(p, a.row_sequence, a.row_length, r, length);
-        mine += (walked(a, length) + kTile - 1) / kTile;
+        mine += line_of((walked(a, length) + kTile - 1) / kTile);
     }
     int64_t upto = mine;
 #pragma unroll
@@ -612,7 +644,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
         for (int r = r0; r < r1; r++) {
             int length;
             row_span(p, a.row_sequence, a.row_length, r, length);
-            const int64_t n = int64_t((walked(a, length) + kTile - 1) / kTile) * items_per_row;
+            const int64_t n = int64_t(line_of((walked(a, length) + kTile - 1) / kTile)) * items_per_row;
             if (pos < at + n) {
                 found_row = r;
                 found_tile = pos - at;
@@ -623,16 +655,16 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
     }
     __syncthreads();
     int r = found_row;
-    int64_t in_row = found_tile; /* tile within the row's items */
+    int64_t in_row = found_tile; /* place within the row's items */
 
     char *ring = smem + warp * Plan<Op>::kRing;
-    const uint32_t ring_at = smem_addr(ring);
+    const uint32_t ring_at = smem_u32(ring);
     float *scratch = reinterpret_cast<float *>(smem + kWarps * Plan<Op>::kRing +
                                                warp * Plan<Op>::kScratchBytes);
-    const int D = p.head_dim;
-    constexpr int kUnit = 16 / sizeof(T);    /* elements of a 16-byte piece */
-    constexpr int kPieces = DP / kUnit;      /* of a padded row */
-    const int pieces = D / kUnit;            /* of a row */
+    const int D = p.head_dim, box = a.box, boxes = kChunk / box;
+    constexpr int kBoxWidth = 128 / sizeof(T);
+    uint32_t phases = 0;
+    bool dead = false; /* a wait gave up: nothing more is read */
 
     while (pos < last) {
         int length;
@@ -642,74 +674,112 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
             r++;
             continue;
         }
-        const int item = int(in_row / tiles), tile0 = int(in_row % tiles);
-        const int tile1 = int(min(int64_t(tiles), tile0 + (last - pos)));
+        const int item = int(in_row / line_of(tiles)), place = int(in_row % line_of(tiles));
+        const int taken = int(min(int64_t(line_of(tiles) - place), last - pos));
+        const int tile0 = max(place - kItemCost, 0), tile1 = place + taken - kItemCost;
+        const int64_t item_start = pos - place + kItemCost; /* where its first tile lies */
+        pos += taken;
+        in_row += taken;
+        const int row = r;
+        if (in_row >= int64_t(line_of(tiles)) * items_per_row) {
+            in_row = 0;
+            r++;
+        }
+        if (tile1 <= tile0)
+            continue;
         const int head = item / groups, first_head = head * p.group + (item % groups) * kRows;
         const int heads = min(kRows, p.group - (item % groups) * kRows);
         const int32_t *list =
-            a.selected ? a.selected + (int64_t(r) * p.kv_heads + head) * a.n_selected : nullptr;
-        const T *keys = static_cast<const T *>(p.keys) + int64_t(head) * p.head_stride;
-        const T *values = static_cast<const T *>(p.values) + int64_t(head) * p.head_stride;
+            a.selected ? a.selected + (int64_t(row) * p.kv_heads + head) * a.n_selected : nullptr;
 
-        /* where slot `lane` (of 16) of this warp's chunk in a tile lies, or -1 */
-        auto locate = [&](int tile) -> int64_t {
-            const int v = tile * kTile + warp * kChunk + (lane & 15);
-            if (tile >= tile1 || v >= span)
-                return -1;
+        /* lane i < boxes: where box i of this warp's chunk in a tile lies, and
+         * how many of its slots count */
+        struct Place {
+            int page, slot, count;
+        };
+        auto locate = [&](int tile) -> Place {
+            const int v = tile * kTile + warp * kChunk + lane * box;
+            Place x{0, 0, 0};
+            if (lane >= boxes || tile >= tile1 || v >= span)
+                return x;
             int j = v / p.page_size;
-            const int place = v - j * p.page_size;
+            x.slot = v - j * p.page_size;
             if (list) {
                 j = list[j];
-                if (j < 0 || j >= p.max_pages || j * p.page_size + place >= length)
-                    return -1;
+                if (j < 0 || j >= p.max_pages || j * p.page_size + x.slot >= length)
+                    return x;
             }
-            const int page = checked_page(p, s, j);
-            return page < 0 ? -1 : int64_t(page) * p.page_stride + int64_t(place) * p.slot_stride;
+            x.page = checked_page(p, s, j);
+            if (x.page >= 0)
+                x.count = min(box, length - j * p.page_size - x.slot);
+            return x;
         };
-        auto issue = [&](int stage, int64_t offset) {
-            const uint32_t to = ring_at + stage * Op::kStageBytes;
-            const uint32_t valid = __ballot_sync(0xffffffffu, offset >= 0) & 0xffffu;
-            if (lane == 0)
+        auto issue = [&](int stage, const Place &x) {
+            const uint32_t to = ring_at + stage * Op::kStageBytes + lane * box * 128;
+            const bool mine = x.count > 0 && !dead;
+            const uint32_t valid =
+                __reduce_or_sync(0xffffffffu, mine ? ((1u << x.count) - 1u) << (lane * box) : 0u);
+            const int n = __popc(__ballot_sync(0xffffffffu, mine));
+            uint64_t *bar = &full[warp][stage];
+            if (lane == 0) {
                 masks[warp][stage] = valid;
-            if (valid != 0) {
-#pragma unroll
-                for (int i = 0; i < kPieces * kChunk / 32; i++) {
-                    const int e = i * 32 + lane, row = e / kPieces, piece = e % kPieces;
-                    const int64_t off = __shfl_sync(0xffffffffu, offset, row);
-                    const bool ok = off >= 0 && piece < pieces;
-                    const int64_t from = ok ? off + piece * kUnit : 0;
-                    copy16(to + row * Op::kRow + piece * 16, keys + from, ok);
-                    copy16(to + (kChunk + row) * Op::kRow + piece * 16, values + from, ok);
-                }
+                if (n > 0)
+                    mbar_expect_tx(bar, n * box * 128 * 2 * Op::kBlocks);
             }
-            copies_commit();
+            __syncwarp();
+            if (mine)
+#pragma unroll
+                for (int b = 0; b < Op::kBlocks; b++) {
+                    copy_box(to + b * kBlock, &a.key_map, b * kBoxWidth, x.slot, head, x.page, smem_u32(bar));
+                    copy_box(to + (Op::kBlocks + b) * kBlock, &a.value_map, b * kBoxWidth, x.slot, head, x.page,
+                             smem_u32(bar));
+                }
         };
 
         Op op;
-        int64_t next = locate(tile0);
+        Place next = locate(tile0);
         for (int i = 0; i < kStages - 1; i++) {
             issue(i, next);
             next = locate(tile0 + i + 1);
         }
-        op.begin(a, static_cast<const R *>(a.q) + r * a.q_stride + int64_t(first_head) * D, heads,
+        op.begin(a, static_cast<const R *>(a.q) + row * a.q_stride + int64_t(first_head) * D, heads,
                  scratch);
         int stage = 0;
         for (int tile = tile0; tile < tile1; tile++) {
             issue(stage == 0 ? kStages - 1 : stage - 1, next);
             next = locate(tile + kStages);
-            copies_wait<kStages - 1>();
-            __syncwarp();
             const uint32_t valid = masks[warp][stage];
-            if (valid != 0) {
-                float *z = a.weights ? a.logits + (int64_t(r) * p.heads + first_head) * p.capacity +
+            bool arrived = valid != 0;
+            if (arrived) {
+                arrived = stage_wait(&full[warp][stage], (phases >> stage) & 1);
+                phases ^= 1u << stage;
+                if (!arrived) {
+                    paged_fail(p, kPagedTimeout);
+                    dead = true;
+                }
+            }
+            if (arrived) {
+                const uint32_t at = ring_at + stage * Op::kStageBytes;
+                if (valid != 0xffffu) {
+                    /* values that do not count meet weights of 0: they must be finite */
+                    for (int i = lane; i < kChunk * 8 * Op::kBlocks; i += 32)
+                        if (!((valid >> (i / 8 % kChunk)) & 1))
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(
+                                             at + Op::kBlocks * kBlock + i * 16),
+                                         "r"(0)
+                                         : "memory");
+                    __syncwarp();
+                }
+                float *z = a.weights ? a.logits + (int64_t(row) * p.heads + first_head) * p.capacity +
                                            tile * kTile + warp * kChunk
                                      : nullptr;
-                op.step(ring_at + stage * Op::kStageBytes, valid, scratch, z, p.capacity, heads);
+                op.step(at, valid, scratch, z, p.capacity, heads);
+                if (valid != 0xffffu)
+                    fence_async(); /* the zeros, before the stage is filled again */
             }
             __syncwarp();
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
-        copies_wait<0>();
         __syncthreads(); /* every warp is done with its ring */
 
         /* the warps' states, joined: o at [row][d], statistics per row */
@@ -721,7 +791,6 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
         }
         __syncthreads();
         const bool whole = tile0 == 0 && tile1 == tiles;
-        const int64_t item_start = pos - tile0; /* of this item on the line */
         float *part = a.partial + (int64_t(blockIdx.x) * 2 + (item_start <= int64_t(blockIdx.x) * share ? 0 : 1)) *
                                       kPartialFloats;
         for (int i = tid; i < heads * DP; i += kThreads) {
@@ -748,14 +817,14 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
                 continue;
             }
             if (d < D)
-                static_cast<R *>(a.out)[r * a.out_stride + int64_t(first_head + g) * D + d] =
+                static_cast<R *>(a.out)[row * a.out_stride + int64_t(first_head + g) * D + d] =
                     from_float<R>(sum == 0.0f ? 0.0f : o / sum);
             if (d == 0) {
                 const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
                 if (a.lse)
-                    a.lse[int64_t(r) * p.heads + first_head + g] = lse2 * kLn2;
+                    a.lse[int64_t(row) * p.heads + first_head + g] = lse2 * kLn2;
                 if (a.weights)
-                    a.lse2[int64_t(r) * p.heads + first_head + g] = lse2;
+                    a.lse2[int64_t(row) * p.heads + first_head + g] = lse2;
             }
         }
         if (!whole) {
@@ -763,7 +832,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                int *counter = a.counters + int64_t(r) * items_per_row + item;
+                int *counter = a.counters + int64_t(row) * items_per_row + item;
                 is_last = atomicAdd(counter, 1) == int(c1 - c0);
                 if (is_last)
                     *counter = 0;
@@ -771,16 +840,11 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
             }
             __syncthreads();
             if (is_last)
-                join_parts<R, DP, kWarps>(a, item_start, share, int(c0), int(c1 - c0) + 1, r, first_head,
+                join_parts<R, DP, kWarps>(a, item_start, share, int(c0), int(c1 - c0) + 1, row, first_head,
                                           heads, reinterpret_cast<float *>(smem));
         }
-        __syncthreads(); /* the state is overwritten by the next item's stages */
-        pos += tile1 - tile0;
-        in_row += tile1 - tile0;
-        if (in_row >= int64_t(tiles) * items_per_row) {
-            in_row = 0;
-            r++;
-        }
+        fence_async(); /* the state is overwritten by the next item's stages */
+        __syncthreads();
     }
 }
 
@@ -839,8 +903,6 @@ cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
 
 template <typename T, typename R> cudaError_t launch_halves(const PagedAttention &a, cudaStream_t s) {
     const int D = a.p.head_dim;
-    if (D <= 32)
-        return launch<Halves<T, R, 32>, R>(a, s);
     if (D <= 64)
         return launch<Halves<T, R, 64>, R>(a, s);
     if (D <= 96)

@@ -84,6 +84,10 @@ void check_view(const nut_paged_view &v) {
         raise(NUT_INVALID_ARGUMENT, "head_dim must be a multiple of 8 up to 256");
     if (v.sequences > kMaxGrid || v.max_rows > kMaxGrid || v.kv_heads > 4096 || v.heads > 65536)
         raise(NUT_LENGTH_ERROR, "dimensions exceed device limits");
+    /* strides of 2^36 elements stay within a tensor map's 2^40 bytes */
+    if (std::max({v.page_stride, v.head_stride, v.slot_stride}) >= (int64_t(1) << 36) ||
+        v.kv_heads * v.page_size * v.head_dim >= (int64_t(1) << 36))
+        raise(NUT_LENGTH_ERROR, "strides exceed device limits");
     if (v.n_pages > INT_MAX || v.page_size > (1 << 24) || v.max_pages > (1 << 24) ||
         v.max_pages * v.page_size > (int64_t(1) << 30))
         raise(NUT_LENGTH_ERROR, "dimensions exceed device limits");
@@ -96,6 +100,43 @@ void check_view(const nut_paged_view &v) {
     if ((v.page_stride || v.head_stride || v.slot_stride) &&
         !(v.page_stride && v.head_stride && v.slot_stride))
         raise(NUT_INVALID_ARGUMENT, "give all three strides or none");
+}
+
+/* cuTensorMapEncodeTiled through the runtime: the library does not link the
+ * driver library. */
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+/* The pool as (dim, slot, kv head, page), read in boxes of 128 bytes by
+ * `box` slots; dims behind head_dim read as zeros. */
+CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box) {
+    static const EncodeTiled encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    if (!encode)
+        raise(NUT_RUNTIME_ERROR, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t size = p.type == NUT_F32 ? 4 : 2;
+    const CUtensorMapDataType type = p.type == NUT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : p.type == NUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.page_size), cuuint64_t(p.kv_heads),
+                                cuuint64_t(p.n_pages)};
+    const cuuint64_t strides[3] = {cuuint64_t(p.slot_stride) * size, cuuint64_t(p.head_stride) * size,
+                                   cuuint64_t(p.page_stride) * size};
+    const cuuint32_t boxes[4] = {cuuint32_t(128 / size), cuuint32_t(box), 1, 1}, steps[4] = {1, 1, 1, 1};
+    CUtensorMap map;
+    if (encode(&map, type, 4, base, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        raise(NUT_INVALID_ARGUMENT, "the pool's strides cannot be mapped");
+    return map;
 }
 
 /* Row stride in elements: 0 stands for the contiguous width. */
@@ -112,6 +153,8 @@ int64_t stride_of(int64_t given, int64_t width, const char *name) {
 struct nut_paged {
     int device = 0;
     nut::PagedPool pool{};
+    CUtensorMap key_map{}, value_map{};
+    int box = 16;
     int max_rows = 0;
     bool track = false;
     int sms = 0;
@@ -181,6 +224,10 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         cuda_check(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device),
                    "count SMs");
         h->sms = std::min(h->sms, nut::kMaxSms);
+        while (p.page_size % h->box != 0)
+            h->box /= 2;
+        h->key_map = pool_map(p, p.keys, h->box);
+        h->value_map = pool_map(p, p.values, h->box);
         const size_t items = size_t(p.sequences) * p.kv_heads;
         size_t bytes = 0;
         const auto part = [&](size_t count, size_t size) {
@@ -237,6 +284,8 @@ nut_status nut_paged_error(nut_paged *h, void *stream) {
             return;
         cuda_check(cudaMemsetAsync(h->error, 0, sizeof code, s), "clear error word");
         cuda_check(cudaStreamSynchronize(s), "synchronize");
+        if (code & nut::kPagedTimeout)
+            raise(NUT_DEVICE_TIMEOUT, "a copy from the pool did not arrive");
         std::string m;
         const auto add = [&](int bit, const char *what) {
             if (code & bit)
@@ -357,6 +406,9 @@ nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *arg
         a.partial = h->partial;
         a.counters = h->counters;
         a.sms = h->sms;
+        a.key_map = h->key_map;
+        a.value_map = h->value_map;
+        a.box = h->box;
         DeviceScope scope(h->device);
         cuda_check(nut::paged_attention(a, static_cast<cudaStream_t>(stream)), "paged attention");
     });
