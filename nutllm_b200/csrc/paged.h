@@ -66,7 +66,7 @@ struct PagedAttention {
 /* A CTA's part of an attention item: maxima [8], sums [8], outputs [8][256]. */
 constexpr int kMaxDim = 256;
 constexpr int kPartialFloats = 8 * 2 + 8 * kMaxDim;
-constexpr int kMaxCtasPerSm = 4;
+constexpr int kMaxCtasPerSm = 3;
 constexpr int kMaxSms = 160;
 constexpr int kMaxDevices = 64;
 

@@ -26,7 +26,10 @@ namespace {
 constexpr int kChunk = 16; /* slots a warp takes at a time */
 constexpr int kRows = 8;   /* query heads of an item */
 constexpr int kBlock = kChunk * 128; /* a chunk's 128-byte columns, in the 128-byte swizzle */
-constexpr int kItemCost = 2; /* what an item costs besides its tiles, in tiles */
+/* What an item costs besides its tiles, in tiles: with 0, 1, 2 and 3 a batch
+ * whose shares hold 1 to 20 items took 147, 108, 101 and 100 us. */
+constexpr int kItemCost = 3;
+constexpr float kSlack = 8.0f; /* log2 by which a logit may pass the maximum in use */
 constexpr uint64_t kPagedWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -131,6 +134,7 @@ template <typename T, typename R, int DP_> struct Halves {
     static constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value && std::is_same<R, float>::value;
     static constexpr bool kScaled = std::is_same<T, __half>::value && std::is_same<R, float>::value;
     static constexpr bool kSplitQ = std::is_same<R, float>::value;
+    static constexpr int kMaxPerSm = DP >= 128 && kThird ? 2 : 3; /* by registers */
     static constexpr int kBlocks = (DP * 2 + 127) / 128; /* 128-byte columns of a row */
     static constexpr int kStageBytes = 2 * kBlocks * kBlock;
     static constexpr int kSteps = DP / 16;
@@ -245,7 +249,9 @@ template <typename T, typename R, int DP_> struct Halves {
                         z[int64_t(g) * stride + 8 * i + 2 * t + j] = s2[i][j];
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float next = fmaxf(m, top);
+        /* the maximum in use may lag behind by kSlack: weights then reach 2^8,
+         * which costs no precision, and outputs are rarely rescaled */
+        const float next = top > m + kSlack || m == -INFINITY ? fmaxf(m, top) : m;
         if (__any_sync(0xffffffffu, next != m)) {
             const float keep = m == next ? 1.0f : exp2f(m - next);
             l *= keep;
@@ -287,18 +293,29 @@ template <typename T, typename R, int DP_> struct Halves {
         }
     }
 
-    /* This warp's state to out [8][DP], maxima [8], sums [8]. */
-    __device__ __forceinline__ void end(float *out, float *maxima, float *sums) {
+    /* This warp's maxima and sums of the 8 heads. */
+    __device__ __forceinline__ void statistics(float *maxima, float *sums) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-#pragma unroll
-        for (int n = 0; n < DP / 8; n++)
-            *reinterpret_cast<float2 *>(out + g * DP + n * 8 + 2 * t) =
-                make_float2(plus_terms(o[n][0], o[n][2]), plus_terms(o[n][1], o[n][3]));
         if (t == 0) {
             maxima[g] = m;
             sums[g] = l;
+        }
+    }
+    /* Its output, times factor[head], to out [8][DP], or added there. */
+    template <bool kAdd> __device__ __forceinline__ void output(float *out, const float *factor) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const float f = factor[g];
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) {
+            float2 *to = reinterpret_cast<float2 *>(out + g * DP + n * 8 + 2 * t);
+            float2 v = make_float2(0.0f, 0.0f);
+            if (f != 0.0f)
+                v = make_float2(plus_terms(o[n][0], o[n][2]) * f, plus_terms(o[n][1], o[n][3]) * f);
+            if (kAdd)
+                v = make_float2(v.x + to->x, v.y + to->y);
+            *to = v;
         }
     }
 };
@@ -311,7 +328,7 @@ template <typename T, typename R, int DP_> struct Halves {
  * lane owns 4 dims, or with fewer than 128 dims 4 dims of a share of the
  * slots, for all heads. */
 template <int NQ, int DP_> struct Wide {
-    static constexpr int DP = DP_, kWarps = DP > 128 ? 2 : 4;
+    static constexpr int DP = DP_, kWarps = DP > 128 ? 2 : 4, kMaxPerSm = 3;
     static constexpr int kBlocks = DP / 32; /* 128-byte columns of a row */
     static constexpr int kStageBytes = 2 * kBlocks * kBlock;
     static constexpr int kOwn = NQ >= 2 ? NQ / 2 : 1; /* heads a lane does the softmax of */
@@ -445,22 +462,8 @@ template <int NQ, int DP_> struct Wide {
         __syncwarp(); /* weights are overwritten by the next step */
     }
 
-    __device__ __forceinline__ void end(float *out, float *maxima, float *sums) {
+    __device__ __forceinline__ void statistics(float *maxima, float *sums) {
         const int lane = threadIdx.x & 31, half = lane >> 4;
-        const int piece = lane % kLanes, share = lane / kLanes;
-#pragma unroll
-        for (int g = 0; g < NQ; g++)
-#pragma unroll
-            for (int n = 0; n < kPieces; n++) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int x = kLanes; x < 32; x <<= 1)
-                        o[g][n][j] += __shfl_xor_sync(0xffffffffu, o[g][n][j], x);
-                if (share == 0 && piece + n * kLanes < kQuads)
-                    *reinterpret_cast<float4 *>(out + g * DP + (piece + n * kLanes) * 4) =
-                        make_float4(o[g][n][0], o[g][n][1], o[g][n][2], o[g][n][3]);
-            }
 #pragma unroll
         for (int g = 0; g < kOwn; g++) {
 #pragma unroll
@@ -473,6 +476,32 @@ template <int NQ, int DP_> struct Wide {
             }
         }
     }
+    template <bool kAdd> __device__ __forceinline__ void output(float *out, const float *factor) {
+        const int lane = threadIdx.x & 31, piece = lane % kLanes, share = lane / kLanes;
+#pragma unroll
+        for (int g = 0; g < NQ; g++) {
+            const float f = factor[g];
+#pragma unroll
+            for (int n = 0; n < kPieces; n++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int x = kLanes; x < 32; x <<= 1)
+                        o[g][n][j] += __shfl_xor_sync(0xffffffffu, o[g][n][j], x);
+                if (share == 0 && piece + n * kLanes < kQuads) {
+                    float4 *to = reinterpret_cast<float4 *>(out + g * DP + (piece + n * kLanes) * 4);
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (f != 0.0f)
+                        v = make_float4(o[g][n][0] * f, o[g][n][1] * f, o[g][n][2] * f, o[g][n][3] * f);
+                    if (kAdd) {
+                        const float4 u = *to;
+                        v = make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+                    }
+                    *to = v;
+                }
+            }
+        }
+    }
 };
 
 template <typename Op> struct Scratch {
@@ -482,22 +511,24 @@ template <int NQ, int DP> struct Scratch<Wide<NQ, DP>> {
     static constexpr int value = (Wide<NQ, DP>::kScratch + 3) / 4 * 4;
 };
 
-template <int DP> constexpr int stages_of(int stage_bytes) {
-    return stage_bytes <= 4096 ? 4 : stage_bytes <= 12288 ? 3 : 2;
-}
+/* Stages of a warp's ring.  With 8 KB stages, three and two CTAs an SM stream
+ * from HBM faster than two and three CTAs (100 against 110 us for 545 MB); out
+ * of L2 it is the other way round (203 against 183 us for 2.1 GB). */
+constexpr int stages_of(int stage_bytes) { return stage_bytes <= 4096 ? 4 : stage_bytes <= 12288 ? 3 : 2; }
 
-/* Shared memory: each warp's ring of stages and scratch; the warps' states
- * at an item's end lie over the rings. */
+/* Shared memory: each warp's ring of stages and scratch, and two outputs of
+ * [8][DP] in which the warps' states meet. */
 template <typename Op> struct Plan {
-    static constexpr int kStages = stages_of<Op::DP>(Op::kStageBytes);
+    static constexpr int kStages = stages_of(Op::kStageBytes);
     static constexpr int kRing = kStages * Op::kStageBytes;
     static constexpr int kScratchBytes = Scratch<Op>::value * 4;
-    static constexpr int kState = (kRows * Op::DP + 2 * kRows) * 4;
     static constexpr int kWarps = Op::kWarps, kThreads = kWarps * 32;
     static constexpr int kTile = kWarps * kChunk; /* slots of a tile */
-    static constexpr int kBody = kWarps * (kRing + kScratchBytes);
-    static constexpr int kBytes = (kBody > kWarps * kState ? kBody : kWarps * kState) + 1024; /* to align */
-    static_assert(kBytes >= kMaxSms * kMaxCtasPerSm * kRows * 4, "an item's parts have their factors there");
+    static constexpr int kOutputBytes = kRows * Op::DP * 4;
+    static constexpr int kBytes = kWarps * (kRing + kScratchBytes) + 2 * kOutputBytes + 1024; /* to align */
+    static constexpr int kFit = 228 * 1024 / (kBytes + 2048);
+    static constexpr int kPerSm = kFit < Op::kMaxPerSm ? (kFit > 1 ? kFit : 1) : Op::kMaxPerSm;
+    static_assert(kWarps * kRing >= kMaxSms * kPerSm * kRows * 4, "an item's parts have their factors there");
 };
 
 /* Slots of a row that the kernel walks: its length, or the listed pages. */
@@ -505,38 +536,72 @@ __device__ __forceinline__ int walked(const PagedAttention &a, int length) {
     return length == 0 ? 0 : a.selected ? a.n_selected * a.p.page_size : length;
 }
 
+template <typename R> __device__ __forceinline__ void store4(R *to, float4 v) {
+    to[0] = from_float<R>(v.x);
+    to[1] = from_float<R>(v.y);
+    to[2] = from_float<R>(v.z);
+    to[3] = from_float<R>(v.w);
+}
+
 /* Joins the `parts` parts of an item left by CTAs c0, c0 + 1, ...; run by
  * the whole CTA that arrived last.  Warps first turn the parts' maxima and
  * sums into one factor exp(m_c - m) / l per part and head, in shared memory;
  * then a thread adds 4 dims of the parts' outputs with many loads in flight
  * (one after another, 37 parts cost 200 us; this way 6). */
-template <typename R, int DP, int kWarps>
-__device__ void join_parts(const PagedAttention &a, int64_t item_start, int64_t share, int c0, int parts,
-                           int r, int first_head, int heads, float *factor) {
+template <typename R, int kWarps>
+__device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, int c0, int parts, int r, int first_head,
+                           int heads, float *factor) {
     const PagedPool &p = a.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     /* an item that starts inside its first CTA's share lies in that one's second slot */
-    const float *first = a.partial + (int64_t(c0) * 2 + (item_start <= c0 * share ? 0 : 1)) * kPartialFloats;
+    const float *first = a.partial + (int64_t(c0) * 2 + (inside ? 1 : 0)) * kPartialFloats;
     const float *rest = a.partial + (int64_t(c0) * 2 + 2) * kPartialFloats;
     auto part = [&](int c) { return c == 0 ? first : rest + int64_t(c - 1) * 2 * kPartialFloats; };
+    /* outputs of the first parts are on their way while the factors are made */
+    constexpr int kFlight = 16;
+    const int quads = p.head_dim / 4;
+    float4 x[kFlight];
+    auto fetch = [&](int i, int c0) {
+        const int at = 2 * kRows + i / quads * kMaxDim + i % quads * 4;
+#pragma unroll
+        for (int k = 0; k < kFlight; k++)
+            x[k] = c0 + k < parts ? __ldcg(reinterpret_cast<const float4 *>(part(c0 + k) + at))
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    if (threadIdx.x < heads * quads)
+        fetch(threadIdx.x, 0);
     for (int g = warp; g < heads; g += kWarps) {
-        float top = -INFINITY;
-        for (int c = lane; c < parts; c += 32) {
-            const float m = __ldcg(part(c) + g);
-            factor[c * kRows + g] = m;
-            top = fmaxf(top, m);
+        /* the first 64 parts' statistics in registers, both loads together */
+        float m0[2], l0[2], top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int c = lane + 32 * k;
+            m0[k] = c < parts ? __ldcg(part(c) + g) : -INFINITY;
+            l0[k] = c < parts ? __ldcg(part(c) + kRows + g) : 0.0f;
+            top = fmaxf(top, m0[k]);
         }
+        for (int c = lane + 64; c < parts; c += 32)
+            top = fmaxf(top, __ldcg(part(c) + g));
         top = warp_max(top);
         const float base = top == -INFINITY ? 0.0f : top;
         float sum = 0.0f;
-        for (int c = lane; c < parts; c += 32) {
-            const float f = exp2f(factor[c * kRows + g] - base), l = __ldcg(part(c) + kRows + g);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            m0[k] = exp2f(m0[k] - base);
+            sum = l0[k] != 0.0f ? fmaf(l0[k], m0[k], sum) : sum;
+        }
+        for (int c = lane + 64; c < parts; c += 32) {
+            const float f = exp2f(__ldcg(part(c) + g) - base), l = __ldcg(part(c) + kRows + g);
             factor[c * kRows + g] = f;
             sum = l != 0.0f ? fmaf(l, f, sum) : sum;
         }
         sum = warp_sum(sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        for (int c = lane; c < parts; c += 32)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (lane + 32 * k < parts)
+                factor[(lane + 32 * k) * kRows + g] = m0[k] * inv;
+        for (int c = lane + 64; c < parts; c += 32)
             factor[c * kRows + g] *= inv;
         if (lane == 0) {
             const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
@@ -547,24 +612,23 @@ __device__ void join_parts(const PagedAttention &a, int64_t item_start, int64_t 
         }
     }
     __syncthreads();
-    const int quads = p.head_dim / 4;
     for (int i = threadIdx.x; i < heads * quads; i += kWarps * 32) {
-        const int g = i / quads, d = i % quads * 4, at = 2 * kRows + g * kMaxDim + d;
+        const int g = i / quads;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int c = 0; c < parts; c++) {
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(part(c) + at));
-            const float f = factor[c * kRows + g];
-            o.x = fmaf(x.x, f, o.x);
-            o.y = fmaf(x.y, f, o.y);
-            o.z = fmaf(x.z, f, o.z);
-            o.w = fmaf(x.w, f, o.w);
+        for (int c = 0; c < parts; c += kFlight) {
+            if (c > 0 || i >= kWarps * 32)
+                fetch(i, c);
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+                const float f = c + k < parts ? factor[(c + k) * kRows + g] : 0.0f;
+                o.x = fmaf(x[k].x, f, o.x);
+                o.y = fmaf(x[k].y, f, o.y);
+                o.z = fmaf(x[k].z, f, o.z);
+                o.w = fmaf(x[k].w, f, o.w);
+            }
         }
-        R *to = static_cast<R *>(a.out) + r * a.out_stride + int64_t(first_head + g) * p.head_dim + d;
-        to[0] = from_float<R>(o.x);
-        to[1] = from_float<R>(o.y);
-        to[2] = from_float<R>(o.z);
-        to[3] = from_float<R>(o.w);
+        store4<R>(static_cast<R *>(a.out) + r * a.out_stride + int64_t(first_head + g) * p.head_dim +
+                      i % quads * 4, o);
     }
 }
 
@@ -572,8 +636,50 @@ __device__ void join_parts(const PagedAttention &a, int64_t item_start, int64_t 
  * behind kItemCost places without one. */
 __device__ __forceinline__ int line_of(int tiles) { return tiles == 0 ? 0 : tiles + kItemCost; }
 
+/* One item, or the part of it that lies in a CTA's share. */
+struct Item {
+    int row, sequence, length, span, tiles, index; /* index within the row */
+    int tile, tile0, tile1;
+    int64_t first; /* where its first tile lies on the line */
+};
+
+/* Walks the items of a share. */
+struct Cursor {
+    int64_t pos, last, in_row; /* place on the line, end, place within the row's items */
+    int r;
+
+    __device__ __forceinline__ bool next(const PagedAttention &a, int items_per_row, int tile_slots, Item &x) {
+        while (pos < last) {
+            x.sequence = row_span(a.p, a.row_sequence, a.row_length, r, x.length);
+            x.span = walked(a, x.length);
+            x.tiles = (x.span + tile_slots - 1) / tile_slots;
+            if (x.tiles == 0) {
+                r++;
+                continue;
+            }
+            const int len = line_of(x.tiles);
+            x.index = int(in_row / len);
+            const int place = int(in_row - int64_t(x.index) * len);
+            const int taken = int(min(int64_t(len - place), last - pos));
+            x.row = r;
+            x.tile = x.tile0 = max(place - kItemCost, 0);
+            x.tile1 = place + taken - kItemCost;
+            x.first = pos - place + kItemCost;
+            pos += taken;
+            in_row += taken;
+            if (in_row >= int64_t(len) * items_per_row) {
+                in_row = 0;
+                r++;
+            }
+            if (x.tile1 > x.tile0)
+                return true;
+        }
+        return false;
+    }
+};
+
 template <typename Op, typename R>
-__global__ void __launch_bounds__(Plan<Op>::kThreads)
+__global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     attention_kernel(const __grid_constant__ PagedAttention a) {
     using T = typename Op::Cache;
     constexpr int DP = Op::DP, kStages = Plan<Op>::kStages, kWarps = Plan<Op>::kWarps,
@@ -582,9 +688,10 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
     char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint32_t masks[kWarps][kStages];
     __shared__ uint64_t full[kWarps][kStages];
-    __shared__ int64_t warp_sum64[kWarps];
-    __shared__ int found_row, is_last;
-    __shared__ int64_t found_tile;
+    __shared__ float maxima[2][kWarps][kRows], sums[2][kWarps][kRows], factors[kWarps][kRows];
+    __shared__ int64_t warp_sum64[kWarps], found_place;
+    __shared__ int found_row, arrived_last[2];
+    __shared__ Item shared[2]; /* items that other CTAs have parts of: the first and the last at most */
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int groups = (p.group + kRows - 1) / kRows, items_per_row = p.kv_heads * groups;
@@ -593,19 +700,6 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
         for (int i = 0; i < kWarps * kStages; i++)
             mbar_init(&full[0][0] + i, 1);
         fence_barrier_init();
-    }
-
-    /* rows that see nothing */
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        int length;
-        row_span(p, a.row_sequence, a.row_length, r, length);
-        if (length != 0)
-            continue;
-        for (int i = tid; i < p.heads * p.head_dim; i += kThreads)
-            static_cast<R *>(a.out)[r * a.out_stride + i] = from_float<R>(0.0f);
-        for (int h = tid; h < p.heads; h += kThreads)
-            if (a.lse)
-                a.lse[int64_t(r) * p.heads + h] = -INFINITY;
     }
 
     /* this CTA's share of the line of tiles: thread i sums a run of rows */
@@ -633,121 +727,117 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
         total += warp_sum64[w];
     }
     total *= items_per_row;
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    int64_t pos = int64_t(blockIdx.x) * share;
-    const int64_t last = min(pos + share, total);
-    if (pos >= last)
-        return;
+    const int64_t share = (total + gridDim.x - 1) / gridDim.x, start = int64_t(blockIdx.x) * share;
     const int64_t before = upto - mine;
-    if (pos >= before * items_per_row && pos < upto * items_per_row) {
+    if (start < total && start >= before * items_per_row && start < upto * items_per_row) {
         int64_t at = before * items_per_row;
         for (int r = r0; r < r1; r++) {
             int length;
             row_span(p, a.row_sequence, a.row_length, r, length);
             const int64_t n = int64_t(line_of((walked(a, length) + kTile - 1) / kTile)) * items_per_row;
-            if (pos < at + n) {
+            if (start < at + n) {
                 found_row = r;
-                found_tile = pos - at;
+                found_place = start - at;
                 break;
             }
             at += n;
         }
     }
     __syncthreads();
-    int r = found_row;
-    int64_t in_row = found_tile; /* place within the row's items */
 
     char *ring = smem + warp * Plan<Op>::kRing;
     const uint32_t ring_at = smem_u32(ring);
-    float *scratch = reinterpret_cast<float *>(smem + kWarps * Plan<Op>::kRing +
-                                               warp * Plan<Op>::kScratchBytes);
+    float *scratch = reinterpret_cast<float *>(smem + kWarps * Plan<Op>::kRing + warp * Plan<Op>::kScratchBytes);
+    float *outputs = reinterpret_cast<float *>(smem + kWarps * (Plan<Op>::kRing + Plan<Op>::kScratchBytes));
     const int D = p.head_dim, box = a.box, boxes = kChunk / box;
     constexpr int kBoxWidth = 128 / sizeof(T);
     uint32_t phases = 0;
     bool dead = false; /* a wait gave up: nothing more is read */
 
-    while (pos < last) {
-        int length;
-        const int s = row_span(p, a.row_sequence, a.row_length, r, length);
-        const int span = walked(a, length), tiles = (span + kTile - 1) / kTile;
-        if (tiles == 0) {
-            r++;
-            continue;
-        }
-        const int item = int(in_row / line_of(tiles)), place = int(in_row % line_of(tiles));
-        const int taken = int(min(int64_t(line_of(tiles) - place), last - pos));
-        const int tile0 = max(place - kItemCost, 0), tile1 = place + taken - kItemCost;
-        const int64_t item_start = pos - place + kItemCost; /* where its first tile lies */
-        pos += taken;
-        in_row += taken;
-        const int row = r;
-        if (in_row >= int64_t(line_of(tiles)) * items_per_row) {
-            in_row = 0;
-            r++;
-        }
-        if (tile1 <= tile0)
-            continue;
-        const int head = item / groups, first_head = head * p.group + (item % groups) * kRows;
-        const int heads = min(kRows, p.group - (item % groups) * kRows);
-        const int32_t *list =
-            a.selected ? a.selected + (int64_t(row) * p.kv_heads + head) * a.n_selected : nullptr;
+    /* The copies run ahead of the arithmetic by kStages - 1 chunks, through
+     * the ends of items: under load a round trip to memory takes 3 us, and an
+     * item that began with empty stages cost 10 to 20. */
+    Cursor feed{start, min(start + share, total), found_place, found_row}, eat = feed;
+    Item in, x;
+    bool more = feed.next(a, items_per_row, kTile, in);
 
-        /* lane i < boxes: where box i of this warp's chunk in a tile lies, and
-         * how many of its slots count */
-        struct Place {
-            int page, slot, count;
-        };
-        auto locate = [&](int tile) -> Place {
-            const int v = tile * kTile + warp * kChunk + lane * box;
-            Place x{0, 0, 0};
-            if (lane >= boxes || tile >= tile1 || v >= span)
-                return x;
-            int j = v / p.page_size;
-            x.slot = v - j * p.page_size;
-            if (list) {
-                j = list[j];
-                if (j < 0 || j >= p.max_pages || j * p.page_size + x.slot >= length)
-                    return x;
-            }
-            x.page = checked_page(p, s, j);
-            if (x.page >= 0)
-                x.count = min(box, length - j * p.page_size - x.slot);
-            return x;
-        };
-        auto issue = [&](int stage, const Place &x) {
-            const uint32_t to = ring_at + stage * Op::kStageBytes + lane * box * 128;
-            const bool mine = x.count > 0 && !dead;
-            const uint32_t valid =
-                __reduce_or_sync(0xffffffffu, mine ? ((1u << x.count) - 1u) << (lane * box) : 0u);
-            const int n = __popc(__ballot_sync(0xffffffffu, mine));
-            uint64_t *bar = &full[warp][stage];
-            if (lane == 0) {
-                masks[warp][stage] = valid;
-                if (n > 0)
-                    mbar_expect_tx(bar, n * box * 128 * 2 * Op::kBlocks);
-            }
-            __syncwarp();
-            if (mine)
+    /* lane i < boxes: where box i of this warp's chunk of in.tile lies, and how
+     * many of its slots count */
+    int next_page = 0, next_slot = 0, next_count = 0;
+    auto locate = [&] {
+        const int v = in.tile * kTile + warp * kChunk + lane * box;
+        next_count = 0;
+        if (!more || lane >= boxes || v >= in.span)
+            return;
+        int j = v / p.page_size;
+        next_slot = v - j * p.page_size;
+        if (a.selected) {
+            j = a.selected[(int64_t(in.row) * p.kv_heads + in.index / groups) * a.n_selected + j];
+            if (j < 0 || j >= p.max_pages || j * p.page_size + next_slot >= in.length)
+                return;
+        }
+        next_page = checked_page(p, in.sequence, j);
+        if (next_page >= 0)
+            next_count = min(box, in.length - j * p.page_size - next_slot);
+    };
+    auto issue = [&](int stage) {
+        const uint32_t to = ring_at + stage * Op::kStageBytes + lane * box * 128;
+        const bool mine = next_count > 0 && !dead;
+        const uint32_t valid =
+            __reduce_or_sync(0xffffffffu, mine ? ((1u << next_count) - 1u) << (lane * box) : 0u);
+        const int n = __popc(__ballot_sync(0xffffffffu, mine));
+        uint64_t *bar = &full[warp][stage];
+        if (lane == 0) {
+            masks[warp][stage] = valid;
+            if (n > 0)
+                mbar_expect_tx(bar, n * box * 128 * 2 * Op::kBlocks);
+        }
+        __syncwarp();
+        const int head = in.index / groups;
+        if (mine)
 #pragma unroll
-                for (int b = 0; b < Op::kBlocks; b++) {
-                    copy_box(to + b * kBlock, &a.key_map, b * kBoxWidth, x.slot, head, x.page, smem_u32(bar));
-                    copy_box(to + (Op::kBlocks + b) * kBlock, &a.value_map, b * kBoxWidth, x.slot, head, x.page,
-                             smem_u32(bar));
-                }
-        };
-
-        Op op;
-        Place next = locate(tile0);
-        for (int i = 0; i < kStages - 1; i++) {
-            issue(i, next);
-            next = locate(tile0 + i + 1);
+            for (int b = 0; b < Op::kBlocks; b++) {
+                copy_box(to + b * kBlock, &a.key_map, b * kBoxWidth, next_slot, head, next_page, smem_u32(bar));
+                copy_box(to + (Op::kBlocks + b) * kBlock, &a.value_map, b * kBoxWidth, next_slot, head, next_page,
+                         smem_u32(bar));
+            }
+        if (more && ++in.tile == in.tile1) {
+            more = feed.next(a, items_per_row, kTile, in);
+            if (more && warp == 0) { /* its queries, on their way to L2 */
+                const char *q = reinterpret_cast<const char *>(
+                    static_cast<const R *>(a.q) + in.row * a.q_stride +
+                    int64_t(in.index / groups * p.group + in.index % groups * kRows) * D);
+                if (lane * 128 < min(kRows, p.group - in.index % groups * kRows) * D * int(sizeof(R)))
+                    asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + lane * 128));
+            }
         }
-        op.begin(a, static_cast<const R *>(a.q) + row * a.q_stride + int64_t(first_head) * D, heads,
-                 scratch);
-        int stage = 0;
-        for (int tile = tile0; tile < tile1; tile++) {
-            issue(stage == 0 ? kStages - 1 : stage - 1, next);
-            next = locate(tile + kStages);
+        locate();
+    };
+
+    locate();
+    for (int i = 0; i < kStages - 1; i++)
+        issue(i);
+    /* rows that see nothing */
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        int length;
+        row_span(p, a.row_sequence, a.row_length, r, length);
+        if (length != 0)
+            continue;
+        for (int i = tid; i < p.heads * p.head_dim; i += kThreads)
+            static_cast<R *>(a.out)[r * a.out_stride + i] = from_float<R>(0.0f);
+        for (int h = tid; h < p.heads; h += kThreads)
+            if (a.lse)
+                a.lse[int64_t(r) * p.heads + h] = -INFINITY;
+    }
+
+    int stage = 0, turn = 0, parts = 0;
+    while (eat.next(a, items_per_row, kTile, x)) {
+        const int first_head = x.index / groups * p.group + x.index % groups * kRows;
+        const int heads = min(kRows, p.group - x.index % groups * kRows);
+        Op op;
+        op.begin(a, static_cast<const R *>(a.q) + x.row * a.q_stride + int64_t(first_head) * D, heads, scratch);
+        for (; x.tile < x.tile1; x.tile++) {
+            issue(stage == 0 ? kStages - 1 : stage - 1);
             const uint32_t valid = masks[warp][stage];
             bool arrived = valid != 0;
             if (arrived) {
@@ -770,8 +860,8 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
                                          : "memory");
                     __syncwarp();
                 }
-                float *z = a.weights ? a.logits + (int64_t(row) * p.heads + first_head) * p.capacity +
-                                           tile * kTile + warp * kChunk
+                float *z = a.weights ? a.logits + (int64_t(x.row) * p.heads + first_head) * p.capacity +
+                                           x.tile * kTile + warp * kChunk
                                      : nullptr;
                 op.step(at, valid, scratch, z, p.capacity, heads);
                 if (valid != 0xffffu)
@@ -780,72 +870,95 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads)
             __syncwarp();
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
-        __syncthreads(); /* every warp is done with its ring */
 
-        /* the warps' states, joined: o at [row][d], statistics per row */
-        float *state = reinterpret_cast<float *>(smem);
-        constexpr int kStateFloats = Plan<Op>::kState / 4;
-        {
-            float *own = state + warp * kStateFloats;
-            op.end(own, own + kRows * DP, own + kRows * DP + kRows);
-        }
+        /* the warps' states meet: a common maximum, then outputs in a fixed
+         * order, warps 0 and 1 first, 2 and 3 on top */
+        float(&top)[kWarps][kRows] = maxima[turn], (&sum)[kWarps][kRows] = sums[turn];
+        turn ^= 1;
+        op.statistics(top[warp], sum[warp]);
         __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == tiles;
-        float *part = a.partial + (int64_t(blockIdx.x) * 2 + (item_start <= int64_t(blockIdx.x) * share ? 0 : 1)) *
-                                      kPartialFloats;
-        for (int i = tid; i < heads * DP; i += kThreads) {
-            const int g = i / DP, d = i % DP;
-            float top = -INFINITY, sum = 0.0f, o = 0.0f;
+        float(&factor)[kRows] = factors[warp];
+        const bool whole = x.tile0 == 0 && x.tile1 == x.tiles;
+        float *part = a.partial + (int64_t(blockIdx.x) * 2 + (x.first <= start ? 0 : 1)) * kPartialFloats;
+        if (lane < kRows) {
+            float m = -INFINITY, l = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; w++)
-                top = fmaxf(top, state[w * kStateFloats + kRows * DP + g]);
-            const float base = top == -INFINITY ? 0.0f : top;
+                m = fmaxf(m, top[w][lane]);
+            const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                const float *st = state + w * kStateFloats;
-                const float f = exp2f(st[kRows * DP + g] - base);
-                sum = fmaf(st[kRows * DP + kRows + g], f, sum);
-                if (f > 0.0f || f != f)
-                    o = fmaf(st[i], f, o);
-            }
-            if (!whole) {
-                part[2 * kRows + g * kMaxDim + d] = o;
-                if (d == 0) {
-                    part[g] = top;
-                    part[kRows + g] = sum;
+            for (int w = 0; w < kWarps; w++)
+                l = fmaf(sum[w][lane], exp2f(top[w][lane] - base), l);
+            /* a whole item's outputs are divided by the sum here */
+            const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            factor[lane] = exp2f(top[warp][lane] - base) * inv;
+            if (warp == 0 && lane < heads) {
+                if (whole) {
+                    const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+                    const int64_t at = int64_t(x.row) * p.heads + first_head + lane;
+                    if (a.lse)
+                        a.lse[at] = lse2 * kLn2;
+                    if (a.weights)
+                        a.lse2[at] = lse2;
+                } else {
+                    part[lane] = m;
+                    part[kRows + lane] = l;
                 }
-                continue;
             }
-            if (d < D)
-                static_cast<R *>(a.out)[row * a.out_stride + int64_t(first_head + g) * D + d] =
-                    from_float<R>(sum == 0.0f ? 0.0f : o / sum);
-            if (d == 0) {
-                const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
-                if (a.lse)
-                    a.lse[int64_t(row) * p.heads + first_head + g] = lse2 * kLn2;
-                if (a.weights)
-                    a.lse2[int64_t(row) * p.heads + first_head + g] = lse2;
-            }
+        }
+        __syncwarp();
+        if (warp < 2)
+            op.template output<false>(outputs + warp * kRows * DP, factor);
+        __syncthreads();
+        if (kWarps > 2) {
+            if (warp >= 2)
+                op.template output<true>(outputs + (warp - 2) * kRows * DP, factor);
+            __syncthreads();
+        }
+        for (int i = tid; i < heads * (DP / 4); i += kThreads) {
+            const int g = i / (DP / 4), d = i % (DP / 4) * 4;
+            const float4 u = *reinterpret_cast<const float4 *>(outputs + g * DP + d);
+            const float4 v = *reinterpret_cast<const float4 *>(outputs + (kRows + g) * DP + d);
+            const float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+            if (!whole)
+                *reinterpret_cast<float4 *>(part + 2 * kRows + g * kMaxDim + d) = o;
+            else if (d < D)
+                store4<R>(static_cast<R *>(a.out) + x.row * a.out_stride + int64_t(first_head + g) * D + d, o);
         }
         if (!whole) {
-            const int64_t c0 = item_start / share, c1 = (item_start + tiles - 1) / share;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                int *counter = a.counters + int64_t(row) * items_per_row + item;
-                is_last = atomicAdd(counter, 1) == int(c1 - c0);
-                if (is_last)
-                    *counter = 0;
-                __threadfence();
-            }
-            __syncthreads();
-            if (is_last)
-                join_parts<R, DP, kWarps>(a, item_start, share, int(c0), int(c1 - c0) + 1, row, first_head,
-                                          heads, reinterpret_cast<float *>(smem));
+            if (tid == 0)
+                shared[parts] = x;
+            parts++;
         }
-        fence_async(); /* the state is overwritten by the next item's stages */
-        __syncthreads();
+        __syncthreads(); /* outputs and factors are free again */
     }
+    if (parts == 0)
+        return;
+
+    /* of items shared with other CTAs, the last to arrive joins the parts */
+    __syncthreads();
+    if (tid < parts) {
+        const Item &y = shared[tid];
+        int *counter = a.counters + int64_t(y.row) * items_per_row + y.index, before_me;
+        const int others = int((y.first + y.tiles - 1) / share - y.first / share);
+        /* releases the block's parts (ordered before by the barrier) and
+         * acquires the others' */
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;\n" : "=r"(before_me) : "l"(counter) : "memory");
+        arrived_last[tid] = before_me == others;
+        if (before_me == others)
+            *counter = 0;
+    }
+    __syncthreads();
+    for (int i = 0; i < parts; i++)
+        if (arrived_last[i]) {
+            const Item &y = shared[i];
+            const int64_t c0 = y.first / share, c1 = (y.first + y.tiles - 1) / share;
+            join_parts<R, kWarps>(a, y.first > c0 * share, int(c0), int(c1 - c0) + 1, y.row,
+                                      y.index / groups * p.group + y.index % groups * kRows,
+                                      min(kRows, p.group - y.index % groups * kRows),
+                                      reinterpret_cast<float *>(smem));
+            __syncthreads();
+        }
 }
 
 /* weights_out[t] = weights[t] + sum over the group of exp(z_t - lse): every
@@ -883,7 +996,7 @@ cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
         e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_kernel<Op, R>, threads, bytes);
         if (e != cudaSuccess)
             return e;
-        per_sm = n < 1 ? 1 : n > kMaxCtasPerSm ? kMaxCtasPerSm : n;
+        per_sm = n < 1 ? 1 : n > Plan<Op>::kPerSm ? Plan<Op>::kPerSm : n;
     }
     const PagedPool &p = a.p;
     const int64_t items = int64_t(a.rows) * p.kv_heads * ((p.group + kRows - 1) / kRows);
