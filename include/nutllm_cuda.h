@@ -360,7 +360,7 @@ enum { NUT_F32 = 0, NUT_F16 = 1, NUT_BF16 = 2 };
  * page are never read.
  *   lengths  slots in use of each sequence, read on the device by every call
  *            (0 is an idle place); the caller advances it before it appends.
- *   bounds, bound_scales  (both or neither) the key bounds of every page and
+ *   bounds, bound_scales  (both or neither; bounds a multiple of 16 bytes) the key bounds of every page and
  *            kv head, for nut_paged_select: greatest and least key of each
  *            dimension over the page's used slots, as int8 in units of
  *            bound_scales (a power of two, the least under which all fit

@@ -79,71 +79,4 @@ __device__ __forceinline__ float finite_key(float v) {
     return v != v ? 0.0f : fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f);
 }
 
-/* ---- choosing the largest of many keys ------------------------------- */
-
-constexpr int kChooseThreads = 1024;
-
-struct ChooseScratch {
-    int hist[256];
-    int warp[3][kChooseThreads / 32];
-    uint32_t prefix;
-    int left;
-};
-
-/* The `want` largest of key(0) .. key(n - 1), ties to the lowest index, by
- * four 8-bit histogram passes from the top: key(i) is chosen when it is
- * above `threshold`, or equal to it and one of the first `quota` such. */
-template <typename Key>
-__device__ void choose_largest(Key key, int n, int want, ChooseScratch &s, uint32_t &threshold,
-                               int &quota) {
-    if (want <= 0 || want >= n) {
-        threshold = want <= 0 ? 0xffffffffu : 0u;
-        quota = want <= 0 ? 0 : n;
-        return;
-    }
-    uint32_t prefix = 0;
-    int left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += blockDim.x)
-            s.hist[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            const uint32_t k = key(i);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&s.hist[(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int b = 255, c = left;
-            while (b > 0 && s.hist[b] < c)
-                c -= s.hist[b--];
-            s.prefix = prefix | (uint32_t(b) << shift);
-            s.left = c;
-        }
-        __syncthreads();
-        prefix = s.prefix;
-        left = s.left;
-    }
-    threshold = prefix;
-    quota = left;
-}
-
-/* Exclusive rank of each thread's flag among the block's, and the total. */
-__device__ __forceinline__ int block_rank(bool flag, int *warp_totals, int &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const uint32_t m = __ballot_sync(0xffffffffu, flag);
-    if (lane == 0)
-        warp_totals[warp] = __popc(m);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < warps; w++) {
-        const int c = warp_totals[w];
-        before += w < warp ? c : 0;
-        all += c;
-    }
-    __syncthreads();
-    total = all;
-    return before + __popc(m & ((1u << lane) - 1u));
-}
-
 } // namespace nut

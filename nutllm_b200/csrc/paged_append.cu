@@ -18,49 +18,131 @@
 namespace nut {
 namespace {
 
+constexpr int kThreads = 256;
+
+/* 8 neighbouring elements as floats; kVec: 16-byte aligned. */
+template <bool kVec> __device__ __forceinline__ void load8(const float *x, float (&v)[8]) {
+    if constexpr (kVec) {
+        const float4 a = reinterpret_cast<const float4 *>(x)[0], b = reinterpret_cast<const float4 *>(x)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = x[i];
+    }
+}
+template <bool kVec, typename T> __device__ __forceinline__ void load8(const T *x, float (&v)[8]) {
+    if constexpr (kVec) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(x);
+        const T *e = reinterpret_cast<const T *>(&a);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = to_float(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = to_float(x[i]);
+    }
+}
+template <bool kVec> __device__ __forceinline__ void store8(float *x, const float (&v)[8]) {
+    if constexpr (kVec) {
+        reinterpret_cast<float4 *>(x)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(x)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = v[i];
+    }
+}
+template <bool kVec, typename T> __device__ __forceinline__ void store8(T *x, const float (&v)[8]) {
+    if constexpr (kVec) {
+        uint4 a;
+        T *e = reinterpret_cast<T *>(&a);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            e[i] = from_float<T>(v[i]);
+        *reinterpret_cast<uint4 *>(x) = a;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = from_float<T>(v[i]);
+    }
+}
+
 /* Greatest and least key of each dimension over `used` slots, in 8 bits
- * (the bounds of nut_paged_view); every thread of the block takes part. */
+ * (the bounds of nut_paged_view); every thread of the block takes part.  A
+ * thread takes 8 dims of every `groups`-th slot, then the groups meet in
+ * shared memory. */
 template <typename T>
 __device__ void page_bounds(const PagedPool &p, int page, int head, int used) {
-    __shared__ float tops[8];
+    __shared__ float most_of[kThreads * 8], least_of[kThreads * 8], tops[kThreads / 32];
     const T *keys = static_cast<const T *>(p.keys) + int64_t(page) * p.page_stride +
                     int64_t(head) * p.head_stride;
-    const int D = p.head_dim, d = threadIdx.x;
-    float most = 0.0f, least = 0.0f;
-    if (d < D) {
-        most = -INFINITY;
-        least = INFINITY;
-        for (int t = 0; t < used; t++) {
-            const float k = finite_key(to_float(keys[int64_t(t) * p.slot_stride + d]));
-            most = fmaxf(most, k);
-            least = fminf(least, k);
+    const int D = p.head_dim, octets = D / 8, groups = kThreads / octets;
+    const int o = threadIdx.x % octets, group = threadIdx.x / octets;
+    float most[8], least[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        most[i] = -INFINITY;
+        least[i] = INFINITY;
+    }
+    if (group < groups) {
+        for (int t = group; t < used; t += groups) {
+            float k[8];
+            load8<true>(keys + int64_t(t) * p.slot_stride + o * 8, k);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float v = finite_key(k[i]);
+                most[i] = fmaxf(most[i], v);
+                least[i] = fminf(least[i], v);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            most_of[group * D + o * 8 + i] = most[i];
+            least_of[group * D + o * 8 + i] = least[i];
         }
     }
-    const float top = warp_max(fmaxf(fabsf(most), fabsf(least)));
+    __syncthreads();
+    const int d = threadIdx.x, filled = min(groups, used);
+    float hi = 0.0f, lo = 0.0f;
+    if (d < D) {
+        hi = -INFINITY;
+        lo = INFINITY;
+        for (int i = 0; i < filled; i++) {
+            hi = fmaxf(hi, most_of[i * D + d]);
+            lo = fminf(lo, least_of[i * D + d]);
+        }
+    }
+    const float top = warp_max(fmaxf(fabsf(hi), fabsf(lo)));
     if ((threadIdx.x & 31) == 0)
         tops[threadIdx.x >> 5] = top;
     __syncthreads();
     float all = 0.0f;
-    for (int w = 0; w < int(blockDim.x >> 5); w++)
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; w++)
         all = fmaxf(all, tops[w]);
     const float u = unit_of(all);
     const int64_t at = int64_t(page) * p.kv_heads + head;
     if (d < D) {
         const float inv = u > 0.0f ? 1.0f / u : 0.0f; /* exact: u is a power of two */
-        p.bounds[at * 2 * D + d] = int8_t(ceilf(most * inv));
-        p.bounds[at * 2 * D + D + d] = int8_t(floorf(least * inv));
+        p.bounds[at * 2 * D + d] = int8_t(ceilf(hi * inv));
+        p.bounds[at * 2 * D + D + d] = int8_t(floorf(lo * inv));
     }
     if (threadIdx.x == 0)
         p.bound_scales[at] = u;
-    __syncthreads();
 }
 
-template <typename R, typename T>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ PagedAppend a) {
+/* A thread keeps one of the octets of a row and walks the page's new
+ * (token, unit) rows, a unit being one of the group's query heads, the key or
+ * the value. */
+template <typename R, typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ PagedAppend a) {
     const PagedPool &p = a.p;
     const int head = blockIdx.y, s = blockIdx.z;
-    const int row0 = a.starts[s], row1 = a.starts[s + 1];
-    const int n = row1 - row0, length = checked_length(p, p.lengths[s]);
+    const int row0 = a.starts[s], row1 = a.starts[s + 1], stored = p.lengths[s];
+    const int n = row1 - row0, length = checked_length(p, stored);
     if (n == 0)
         return;
     if (row0 < 0 || n < 0 || row1 > a.rows || n > a.max_new || n > length) {
@@ -75,54 +157,61 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Pag
     const int page = checked_page(p, s, j);
     if (page < 0)
         return;
-    const int seen = a.seen ? a.seen[s] : length;
-    const int D = p.head_dim, half = D / 2;
-    const int64_t base = int64_t(page) * p.page_stride + int64_t(head) * p.head_stride;
+    const int ahead = a.seen ? a.seen[s] - length : 0; /* position less slot */
+    const int D = p.head_dim, half = D / 2, octets = D / 8, groups = kThreads / octets;
+    const int o = threadIdx.x % octets * 8, group = threadIdx.x / octets;
+    const int64_t base = int64_t(page) * p.page_stride + int64_t(head) * p.head_stride + o;
     T *keys = static_cast<T *>(p.keys) + base, *values = static_cast<T *>(p.values) + base;
-    const int units = (a.q ? p.group : 0) + 2; /* query heads, key, value */
-    for (int e = threadIdx.x; e < (t1 - t0) * units * half; e += blockDim.x) {
-        const int t = t0 + e / (units * half), rest = e % (units * half);
-        const int unit = rest / half, i = rest % half;
-        const int row = row0 + (t - first);
-        if (unit == units - 1) {
-            const R *v = static_cast<const R *>(a.v) + row * a.v_stride + head * D + 2 * i;
-            T *to = values + int64_t(t - j * ps) * p.slot_stride + 2 * i;
-            to[0] = from_float<T>(to_float(v[0]));
-            to[1] = from_float<T>(to_float(v[1]));
-            continue;
-        }
-        const bool is_key = unit == units - 2;
-        const R *x = is_key ? static_cast<const R *>(a.k) + row * a.k_stride + head * D
-                            : static_cast<const R *>(a.q) + row * a.q_stride +
-                                  (head * p.group + unit) * D;
-        float x0 = to_float(x[2 * i]), x1 = to_float(x[2 * i + 1]);
-        if (a.cos) {
-            const int64_t pos = int64_t(t) + (seen - length);
-            if (pos < 0 || pos >= a.rope_rows) {
-                paged_fail(p, kPagedBadPosition);
-            } else {
-                const float c = a.cos[pos * half + i], z = a.sin[pos * half + i];
-                const float y0 = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, z));
-                x1 = __fadd_rn(__fmul_rn(x0, z), __fmul_rn(x1, c));
-                x0 = y0;
+    const int heads = a.q ? p.group : 0, units = heads + 2;
+    if (group < groups)
+        for (int e = group; e < (t1 - t0) * units; e += groups) {
+            const int t = t0 + e / units, unit = e % units;
+            const int64_t row = row0 + (t - first);
+            float v[8];
+            if (unit == heads + 1) {
+                load8<kVec>(static_cast<const R *>(a.v) + row * a.v_stride + head * D + o, v);
+                store8<true>(values + int64_t(t - j * ps) * p.slot_stride, v);
+                continue;
             }
+            const bool is_key = unit == heads;
+            const int64_t column = (head * p.group + unit) * D + o;
+            load8<kVec>(is_key ? static_cast<const R *>(a.k) + row * a.k_stride + head * D + o
+                               : static_cast<const R *>(a.q) + row * a.q_stride + column,
+                        v);
+            if (a.cos) {
+                const int64_t pos = int64_t(t) + ahead;
+                if (pos < 0 || pos >= a.rope_rows) {
+                    paged_fail(p, kPagedBadPosition);
+                } else {
+                    float c[4], z[4];
+                    if constexpr (kVec) {
+                        *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(a.cos + pos * half + o / 2);
+                        *reinterpret_cast<float4 *>(z) = *reinterpret_cast<const float4 *>(a.sin + pos * half + o / 2);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            c[i] = a.cos[pos * half + o / 2 + i];
+                            z[i] = a.sin[pos * half + o / 2 + i];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                        v[2 * i] = __fsub_rn(__fmul_rn(x0, c[i]), __fmul_rn(x1, z[i]));
+                        v[2 * i + 1] = __fadd_rn(__fmul_rn(x0, z[i]), __fmul_rn(x1, c[i]));
+                    }
+                }
+            }
+            if (is_key)
+                store8<true>(keys + int64_t(t - j * ps) * p.slot_stride, v);
+            else
+                store8<kVec>(static_cast<R *>(a.q_out) + row * a.q_out_stride + column, v);
         }
-        if (is_key) {
-            T *to = keys + int64_t(t - j * ps) * p.slot_stride + 2 * i;
-            to[0] = from_float<T>(x0);
-            to[1] = from_float<T>(x1);
-        } else {
-            R *to = static_cast<R *>(a.q_out) + row * a.q_out_stride +
-                    (head * p.group + unit) * D + 2 * i;
-            to[0] = from_float<R>(x0);
-            to[1] = from_float<R>(x1);
-        }
-    }
     if (a.positions || a.weights) {
         const int64_t at = (int64_t(s) * p.kv_heads + head) * p.capacity;
-        for (int t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
+        for (int t = t0 + threadIdx.x; t < t1; t += kThreads) {
             if (a.positions)
-                a.positions[at + t] = t + (seen - length);
+                a.positions[at + t] = t + ahead;
             if (a.weights)
                 a.weights[at + t] = 0.0f;
         }
@@ -134,7 +223,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Pag
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) summarise_kernel(const __grid_constant__ PagedPool p) {
+__global__ void __launch_bounds__(kThreads) summarise_kernel(const __grid_constant__ PagedPool p) {
     const int j = blockIdx.x, head = blockIdx.y, s = blockIdx.z;
     const int used = min(checked_length(p, p.lengths[s]) - j * p.page_size, p.page_size);
     if (used <= 0)
@@ -144,23 +233,36 @@ __global__ void __launch_bounds__(256) summarise_kernel(const __grid_constant__ 
         page_bounds<T>(p, page, head, used);
 }
 
-} // namespace
-
-cudaError_t paged_append(const PagedAppend &a, cudaStream_t s) {
+template <typename R, typename T> void launch_append(const PagedAppend &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     /* pages that max_new consecutive slots can touch */
     const dim3 grid((a.max_new + p.page_size - 2) / p.page_size + 1, p.kv_heads, p.sequences);
-    const bool wide = a.type == 0;
-    if (p.type == 0)
-        append_kernel<float, float><<<grid, 256, 0, s>>>(a);
-    else if (p.type == 1 && wide)
-        append_kernel<float, __half><<<grid, 256, 0, s>>>(a);
-    else if (p.type == 1)
-        append_kernel<__half, __half><<<grid, 256, 0, s>>>(a);
-    else if (wide)
-        append_kernel<float, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    uintptr_t bits = 0;
+    for (const void *x : {a.q, a.k, a.v, static_cast<const void *>(a.q_out), static_cast<const void *>(a.cos),
+                          static_cast<const void *>(a.sin)})
+        bits |= reinterpret_cast<uintptr_t>(x);
+    for (int64_t stride : {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride})
+        bits |= uintptr_t(stride) * sizeof(R);
+    if ((bits & 15) == 0)
+        append_kernel<R, T, true><<<grid, kThreads, 0, s>>>(a);
     else
-        append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
+        append_kernel<R, T, false><<<grid, kThreads, 0, s>>>(a);
+}
+
+} // namespace
+
+cudaError_t paged_append(const PagedAppend &a, cudaStream_t s) {
+    const bool wide = a.type == 0;
+    if (a.p.type == 0)
+        launch_append<float, float>(a, s);
+    else if (a.p.type == 1 && wide)
+        launch_append<float, __half>(a, s);
+    else if (a.p.type == 1)
+        launch_append<__half, __half>(a, s);
+    else if (wide)
+        launch_append<float, __nv_bfloat16>(a, s);
+    else
+        launch_append<__nv_bfloat16, __nv_bfloat16>(a, s);
     count_launches(1);
     return cudaGetLastError();
 }
@@ -168,11 +270,11 @@ cudaError_t paged_append(const PagedAppend &a, cudaStream_t s) {
 cudaError_t paged_summarise(const PagedPool &p, cudaStream_t s) {
     const dim3 grid(p.max_pages, p.kv_heads, p.sequences);
     if (p.type == 0)
-        summarise_kernel<float><<<grid, 256, 0, s>>>(p);
+        summarise_kernel<float><<<grid, kThreads, 0, s>>>(p);
     else if (p.type == 1)
-        summarise_kernel<__half><<<grid, 256, 0, s>>>(p);
+        summarise_kernel<__half><<<grid, kThreads, 0, s>>>(p);
     else
-        summarise_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+        summarise_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
     count_launches(1);
     return cudaGetLastError();
 }

@@ -1,0 +1,183 @@
+#pragma once
+/* Choosing the largest of many 32-bit keys, ties to the lowest index: page
+ * selection and slot eviction of the paged KV cache.
+ *
+ * A radix select by 11, 11 and 10 bits from the top.  One block, or the
+ * blocks of a cluster that each hold a run of the keys and add their
+ * histograms over distributed shared memory.  A thread owns kOwn
+ * neighbouring keys of every chunk of kOwn * threads, and while the block's
+ * run is a single chunk keeps them in registers over all passes. */
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace nut {
+
+constexpr int kChooseThreads = 512;
+constexpr int kChooseWarps = kChooseThreads / 32;
+constexpr int kOwn = 8;
+constexpr int kChooseChunk = kOwn * kChooseThreads;
+constexpr int kBins = 2048;
+
+struct ChooseScratch {
+    int hist[kBins], sums[kBins];
+    int warp[2][kChooseWarps];
+    uint32_t prefix;
+    int left, all;
+    int shared[4]; /* read by the cluster's other blocks */
+};
+
+/* Exclusive rank of each thread's count within the block, and the total.
+ * Two of these in a row need different `turn`s. */
+__device__ __forceinline__ int block_before(int count, ChooseScratch &s, int turn, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int upto = count;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, x);
+        upto += lane >= x ? v : 0;
+    }
+    if (lane == 31)
+        s.warp[turn][warp] = upto;
+    __syncthreads();
+    int t = lane < kChooseWarps ? s.warp[turn][lane] : 0;
+    total = __reduce_add_sync(0xffffffffu, t);
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? t : 0);
+    return before + upto - count;
+}
+
+/* 8 neighbouring words from x; aligned: 16-byte loads. */
+template <typename T> __device__ __forceinline__ void load_own(const T *x, int there, T (&v)[kOwn]) {
+    static_assert(sizeof(T) == 4 && kOwn == 8, "two 16-byte loads");
+    if (there >= kOwn && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(x);
+        *reinterpret_cast<uint4 *>(v + 4) = *reinterpret_cast<const uint4 *>(x + 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            v[e] = e < there ? x[e] : T(0);
+    }
+}
+
+/* The keys of this thread in the chunk that starts at `base`; 0 beyond n.
+ * key.own(i, there, k) makes the first `there` of keys i .. i + 7. */
+template <typename Key>
+__device__ __forceinline__ void own_keys(const Key &key, int base, int n, uint32_t (&k)[kOwn]) {
+    const int i0 = base + int(threadIdx.x) * kOwn;
+    key.own(i0, max(0, min(kOwn, n - i0)), k);
+}
+
+/* Adds `value` of every block of the cluster, for blocks of lower rank only
+ * (before) and for all. */
+template <int kBlocks>
+__device__ __forceinline__ void cluster_before(int value, ChooseScratch &s, int place, int &before, int &all) {
+    if constexpr (kBlocks == 1) {
+        before = 0;
+        all = value;
+    } else {
+        auto cluster = cooperative_groups::this_cluster();
+        if (threadIdx.x == 0)
+            s.shared[place] = value;
+        cluster.sync();
+        const int rank = int(cluster.block_rank());
+        before = all = 0;
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+            const int v = *cluster.map_shared_rank(&s.shared[place], b);
+            all += v;
+            before += b < rank ? v : 0;
+        }
+    }
+}
+
+/* The `want` largest of all keys of the cluster (key(0) .. key(n - 1) in
+ * this block, `all` in the cluster): a key is chosen when it is above
+ * `threshold`, or equal to it and one of the first `quota` such.  k holds
+ * the block's first chunk. */
+template <int kBlocks, typename Key>
+__device__ void choose_largest(const Key &key, int n, int all, int want, const uint32_t (&first)[kOwn],
+                               ChooseScratch &s, uint32_t &threshold, int &quota) {
+    if (want <= 0 || want >= all) {
+        threshold = want <= 0 ? 0xffffffffu : 0u;
+        quota = want <= 0 ? 0 : all;
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 31;
+    uint32_t prefix = 0;
+    int left = want;
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        for (int i = tid; i < kBins; i += kChooseThreads)
+            s.hist[i] = 0;
+        __syncthreads();
+        for (int base = 0; base < n; base += kChooseChunk) {
+            uint32_t k[kOwn];
+            if (base == 0) {
+#pragma unroll
+                for (int e = 0; e < kOwn; e++)
+                    k[e] = first[e];
+            } else {
+                own_keys(key, base, n, k);
+            }
+            if (base + (tid & ~31) * kOwn >= n)
+                continue; /* nothing in this warp */
+#pragma unroll
+            for (int e = 0; e < kOwn; e++) {
+                /* one addition for each bin among the warp's keys: scores
+                 * crowd into few bins */
+                const bool in = base + tid * kOwn + e < n &&
+                                (pass == 0 || (k[e] >> (shift + bits)) == (prefix >> (shift + bits)));
+                const uint32_t bin = in ? (k[e] >> shift) & ((1u << bits) - 1u) : 0xffffffffu;
+                const uint32_t same = __match_any_sync(0xffffffffu, bin);
+                if (in && lane == __ffs(same) - 1)
+                    atomicAdd(&s.hist[bin], __popc(same));
+            }
+        }
+        __syncthreads();
+        const int *hist = s.hist;
+        if constexpr (kBlocks > 1) {
+            auto cluster = cooperative_groups::this_cluster();
+            cluster.sync();
+            for (int i = tid; i < kBins; i += kChooseThreads) {
+                int v = 0;
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++)
+                    v += *cluster.map_shared_rank(&s.hist[i], b);
+                s.sums[i] = v;
+            }
+            cluster.sync(); /* the others' histograms have been read */
+            hist = s.sums;
+        }
+        /* bins from the top: thread t has four of them */
+        constexpr int kEach = kBins / kChooseThreads;
+        int c[kEach], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; i++)
+            sum += c[i] = hist[kBins - 1 - (tid * kEach + i)];
+        int total;
+        int before = block_before(sum, s, pass & 1, total);
+        if (before < left && left <= before + sum) {
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                if (left > before && left <= before + c[i]) {
+                    s.prefix = prefix | (uint32_t(kBins - 1 - (tid * kEach + i)) << shift);
+                    s.left = left - before;
+                    s.all = c[i];
+                }
+                before += c[i];
+            }
+        }
+        __syncthreads();
+        prefix = s.prefix;
+        left = s.left;
+        if (left == s.all && prefix != 0u) { /* the whole bin: no key is left to tell apart */
+            threshold = prefix - 1u;
+            quota = 0;
+            return;
+        }
+    }
+    threshold = prefix;
+    quota = left;
+}
+
+} // namespace nut

@@ -10,82 +10,196 @@
  * choose_slots_kernel finds the threshold, lists the pairs and moves the
  * weights and positions; move_kernel moves keys and values.
  */
+#include <algorithm>
 #include <cstdint>
 #include <cuda_runtime.h>
 
 #include "kernels.h"
 #include "paged.cuh"
+#include "paged_choose.cuh"
 
 namespace nut {
 namespace {
 
+struct SlotKeys {
+    const float *weights;
+    const int32_t *positions;
+    int sinks;
+    int64_t recent_from;
+    __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[kOwn]) const {
+        float w[kOwn];
+        int32_t at[kOwn];
+        load_own(weights + i, there, w);
+        if (positions)
+            load_own(positions + i, there, at);
+#pragma unroll
+        for (int e = 0; e < kOwn; e++) {
+            k[e] = w[e] != w[e] ? 0u : ordered_bits(w[e]);
+            if (positions && (at[e] < sinks || at[e] >= recent_from))
+                k[e] = ordered_bits(INFINITY);
+            if (e >= there)
+                k[e] = 0u;
+        }
+    }
+};
+
+/* kBlocks blocks (a cluster) for each sequence and kv head, each with a run
+ * of the slots. */
+template <int kBlocks>
 __global__ void __launch_bounds__(kChooseThreads)
     choose_slots_kernel(const __grid_constant__ PagedEvict a) {
     __shared__ ChooseScratch scratch;
     const PagedPool &p = a.p;
-    const int head = blockIdx.x, s = blockIdx.y;
-    const int n = checked_length(p, p.lengths[s]), m = min(n, a.budget);
+    const int rank = int(blockIdx.x) % kBlocks, head = int(blockIdx.x) / kBlocks, s = blockIdx.y;
+    const int tid = threadIdx.x;
+    const int length = checked_length(p, p.lengths[s]), m = min(length, a.budget);
+    /* runs of whole groups of kOwn slots */
+    const int run = (length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn;
+    const int from = min(rank * run, length), n = min(run, length - from);
     const int64_t item = int64_t(s) * p.kv_heads + head, at = item * p.capacity;
-    const float *w = a.weights + at;
-    const int32_t *pos = a.positions ? a.positions + at : nullptr;
+    const float *w = a.weights + at + from;
+    const int32_t *pos = a.positions ? a.positions + at + from : nullptr;
     const int64_t recent_from = a.recent ? int64_t(a.seen[s]) - a.recent : INT64_MAX;
-    const int sinks = a.sinks;
-    auto key = [=](int i) -> uint32_t {
-        if (pos && (pos[i] < sinks || pos[i] >= recent_from))
-            return ordered_bits(INFINITY);
-        const float v = w[i];
-        return v != v ? 0u : ordered_bits(v);
-    };
-    uint32_t threshold;
+    const SlotKeys key{w, pos, a.sinks, recent_from};
+    uint32_t first[kOwn], threshold;
     int quota;
-    choose_largest(key, n, m, scratch, threshold, quota);
+    own_keys(key, 0, n, first);
+    choose_largest<kBlocks>(key, n, length, m, first, scratch, threshold, quota);
+
+    /* ties, holes and sources of the blocks before this one */
+    int ties = 0, holes_n = 0, sources_n = 0;
     int32_t *holes = a.pairs + at, *sources = holes + p.capacity / 2;
-    int ties = 0, hole_n = 0, source_n = 0;
-    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
-        const int i = i0 + threadIdx.x;
-        const uint32_t k = i < n ? key(i) : 0u;
-        const bool tie = i < n && k == threshold;
-        int total;
-        const int rank = ties + block_rank(tie, scratch.warp[0], total);
-        ties += total;
-        const bool kept = i < n && (k > threshold || (tie && rank < quota));
-        const bool hole = i < m && !kept, source = i >= m && kept;
-        const int to = hole_n + block_rank(hole, scratch.warp[1], total);
-        hole_n += total;
-        if (hole)
-            holes[to] = i;
-        const int from = source_n + block_rank(source, scratch.warp[2], total);
-        source_n += total;
-        if (source)
-            sources[from] = i;
+    if constexpr (kBlocks > 1) {
+        int mine = 0, total, all;
+        for (int base = 0; base < n; base += kChooseChunk) {
+            uint32_t k[kOwn];
+            own_keys(key, base, n, k);
+#pragma unroll
+            for (int e = 0; e < kOwn; e++)
+                mine += base + tid * kOwn + e < n && k[e] == threshold;
+        }
+        block_before(mine, scratch, 0, total);
+        cluster_before<kBlocks>(total, scratch, 0, ties, all);
+        /* kept slots below m and from m on, up to this block's run, follow
+         * from the counts of kept ones */
     }
-    if (threadIdx.x == 0) {
-        a.counts[item * 2] = hole_n;
+    auto flags = [&](int base, int rank0, const uint32_t (&k)[kOwn], uint32_t &kept) {
+        const int i0 = base + tid * kOwn;
+        kept = 0;
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            if (i0 + e < n && (k[e] > threshold || (k[e] == threshold && rank0++ < quota)))
+                kept |= 1u << e;
+    };
+    auto own_mask = [&](int base) { /* this thread's slots of the chunk, and those of them below m */
+        const int i0 = base + tid * kOwn;
+        const int there = max(0, min(kOwn, n - i0)), low = max(0, min(there, m - from - i0));
+        return make_uint2((1u << there) - 1u, (1u << low) - 1u);
+    };
+    if constexpr (kBlocks > 1) {
+        int h = 0, q = 0, t0 = ties, total, all;
+        for (int base = 0; base < n; base += kChooseChunk) {
+            uint32_t k[kOwn], kept;
+            own_keys(key, base, n, k);
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < kOwn; e++)
+                mine += base + tid * kOwn + e < n && k[e] == threshold;
+            const int rank0 = t0 + block_before(mine, scratch, 0, total);
+            t0 += total;
+            flags(base, rank0, k, kept);
+            const uint2 own = own_mask(base);
+            h += __popc(own.y & ~kept);
+            q += __popc(kept & ~own.y);
+            __syncthreads(); /* before the scan's scratch is used again */
+        }
+        block_before(h, scratch, 1, total);
+        cluster_before<kBlocks>(total, scratch, 1, holes_n, all);
+        __syncthreads();
+        block_before(q, scratch, 1, total);
+        cluster_before<kBlocks>(total, scratch, 2, sources_n, all);
+        __syncthreads();
+    }
+    int ties_seen = ties;
+    for (int base = 0; base < n; base += kChooseChunk) {
+        uint32_t k[kOwn], kept;
+        if (base == 0) {
+#pragma unroll
+            for (int e = 0; e < kOwn; e++)
+                k[e] = first[e];
+        } else {
+            own_keys(key, base, n, k);
+        }
+        int mine = 0, total;
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            mine += base + tid * kOwn + e < n && k[e] == threshold;
+        const int rank0 = ties_seen + block_before(mine, scratch, 0, total);
+        ties_seen += total;
+        flags(base, rank0, k, kept);
+        const uint2 own = own_mask(base);
+        uint32_t hole = own.y & ~kept, source = kept & ~own.y;
+        /* both counts in one scan */
+        const int both = __popc(hole) | (__popc(source) << 16);
+        const int before = block_before(both, scratch, 1, total);
+        int to = holes_n + (before & 0xffff), of = sources_n + (before >> 16);
+        holes_n += total & 0xffff;
+        sources_n += total >> 16;
+        const int i0 = from + base + tid * kOwn;
+        for (; hole; hole &= hole - 1)
+            holes[to++] = i0 + __ffs(hole) - 1;
+        for (; source; source &= source - 1)
+            sources[of++] = i0 + __ffs(source) - 1;
+    }
+    /* the last block of the run has seen them all */
+    if (rank == kBlocks - 1 && tid == 0) {
+        a.counts[item * 2] = holes_n;
         a.counts[item * 2 + 1] = m;
+        scratch.shared[3] = holes_n;
     }
-    __syncthreads();
+    const float *w0 = a.weights + at;
+    const int32_t *pos0 = a.positions ? a.positions + at : nullptr;
     /* kept slots first: a hole's own entry is overwritten after */
+    const int low = max(0, min(n, m - from));
     if (a.weights_out != a.weights)
-        for (int i = threadIdx.x; i < m; i += blockDim.x)
-            a.weights_out[at + i] = w[i];
+        for (int i = tid; i < low; i += kChooseThreads)
+            a.weights_out[at + from + i] = w[i];
     if (pos && a.positions_out != a.positions)
-        for (int i = threadIdx.x; i < m; i += blockDim.x)
-            a.positions_out[at + i] = pos[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < hole_n; i += blockDim.x) {
-        a.weights_out[at + holes[i]] = w[sources[i]];
-        if (pos)
-            a.positions_out[at + holes[i]] = pos[sources[i]];
+        for (int i = tid; i < low; i += kChooseThreads)
+            a.positions_out[at + from + i] = pos[i];
+    int pairs;
+    if constexpr (kBlocks > 1) {
+        auto cluster = cooperative_groups::this_cluster();
+        __threadfence();
+        cluster.sync();
+        pairs = *cluster.map_shared_rank(&scratch.shared[3], kBlocks - 1);
+    } else {
+        __syncthreads();
+        pairs = holes_n;
     }
-    __syncthreads();
-    for (int i = m + threadIdx.x; i < n; i += blockDim.x) {
-        a.weights_out[at + i] = 0.0f;
+    for (int i = rank * kChooseThreads + tid; i < pairs; i += kBlocks * kChooseThreads) {
+        const int to = holes[i], of = sources[i];
+        a.weights_out[at + to] = w0[of];
         if (pos)
-            a.positions_out[at + i] = -1;
+            a.positions_out[at + to] = pos0[of];
+    }
+    if constexpr (kBlocks > 1)
+        cooperative_groups::this_cluster().sync(); /* sources read, and shared memory done with */
+    else
+        __syncthreads();
+    for (int i = low + tid; i < n; i += kChooseThreads) {
+        a.weights_out[at + from + i] = 0.0f;
+        if (pos)
+            a.positions_out[at + from + i] = -1;
     }
 }
 
-__global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ PagedEvict a, int row16) {
+/* Keys and values of the pairs: a group of row16 threads moves a row of
+ * row16 16-byte pieces, kFlight pairs at a time so that the look-ups and the
+ * rows of several are on their way together. */
+constexpr int kMoveThreads = 256, kFlight = 4;
+
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ PagedEvict a, int row16) {
     const PagedPool &p = a.p;
     const int head = blockIdx.y, s = blockIdx.z;
     const int64_t item = int64_t(s) * p.kv_heads + head;
@@ -93,21 +207,41 @@ __global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ Paged
     if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0)
         a.new_lengths[s] = a.counts[item * 2 + 1];
     const int32_t *holes = a.pairs + item * p.capacity, *sources = holes + p.capacity / 2;
-    const int size = p.type == 0 ? 4 : 2, ps = p.page_size;
-    for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < int64_t(n) * row16;
-         e += int64_t(gridDim.x) * blockDim.x) {
-        const int i = int(e / row16), c = int(e % row16);
-        const int to = holes[i], from = sources[i];
-        const int pt = checked_page(p, s, to / ps), pf = checked_page(p, s, from / ps);
-        if (pt < 0 || pf < 0)
-            continue;
-        const int64_t dst = (int64_t(pt) * p.page_stride + int64_t(head) * p.head_stride +
-                             int64_t(to % ps) * p.slot_stride) * size + c * 16;
-        const int64_t src = (int64_t(pf) * p.page_stride + int64_t(head) * p.head_stride +
-                             int64_t(from % ps) * p.slot_stride) * size + c * 16;
-        char *k = static_cast<char *>(p.keys), *v = static_cast<char *>(p.values);
-        *reinterpret_cast<uint4 *>(k + dst) = *reinterpret_cast<const uint4 *>(k + src);
-        *reinterpret_cast<uint4 *>(v + dst) = *reinterpret_cast<const uint4 *>(v + src);
+    const int groups = kMoveThreads / row16, group = threadIdx.x / row16, piece = threadIdx.x % row16;
+    if (group >= groups)
+        return;
+    const int ps = p.page_size, all = gridDim.x * groups;
+    const int64_t unit = p.type == 0 ? 4 : 2;
+    char *keys = static_cast<char *>(p.keys) + int64_t(head) * p.head_stride * unit + piece * 16;
+    char *values = static_cast<char *>(p.values) + int64_t(head) * p.head_stride * unit + piece * 16;
+    for (int i0 = blockIdx.x * groups + group; i0 < n; i0 += all * kFlight) {
+        int slot[2][kFlight], page[2][kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; k++) {
+            const int i = i0 + k * all;
+            slot[0][k] = i < n ? holes[i] : -1;
+            slot[1][k] = i < n ? sources[i] : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; k++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+                page[x][k] = slot[x][k] >= 0 ? checked_page(p, s, slot[x][k] / ps) : -1;
+        uint4 key[kFlight], value[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; k++)
+            if (page[0][k] >= 0 && page[1][k] >= 0) {
+                const int64_t at = (page[1][k] * p.page_stride + slot[1][k] % ps * p.slot_stride) * unit;
+                key[k] = *reinterpret_cast<const uint4 *>(keys + at);
+                value[k] = *reinterpret_cast<const uint4 *>(values + at);
+            }
+#pragma unroll
+        for (int k = 0; k < kFlight; k++)
+            if (page[0][k] >= 0 && page[1][k] >= 0) {
+                const int64_t at = (page[0][k] * p.page_stride + slot[0][k] % ps * p.slot_stride) * unit;
+                *reinterpret_cast<uint4 *>(keys + at) = key[k];
+                *reinterpret_cast<uint4 *>(values + at) = value[k];
+            }
     }
 }
 
@@ -115,9 +249,31 @@ __global__ void __launch_bounds__(256) move_kernel(const __grid_constant__ Paged
 
 cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const PagedPool &p = a.p;
-    choose_slots_kernel<<<dim3(p.kv_heads, p.sequences), kChooseThreads, 0, s>>>(a);
+    cudaError_t e;
+    if (p.capacity <= 2 * kChooseChunk) {
+        choose_slots_kernel<1><<<dim3(p.kv_heads, p.sequences), kChooseThreads, 0, s>>>(a);
+        e = cudaGetLastError();
+    } else {
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(8 * p.kv_heads, p.sequences);
+        config.blockDim = dim3(kChooseThreads);
+        config.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 8;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        config.attrs = attr;
+        config.numAttrs = 1;
+        e = cudaLaunchKernelEx(&config, choose_slots_kernel<8>, a);
+    }
+    if (e != cudaSuccess)
+        return e;
     const int row16 = p.head_dim * (p.type == 0 ? 4 : 2) / 16;
-    move_kernel<<<dim3(8, p.kv_heads, p.sequences), 256, 0, s>>>(a, row16);
+    /* blocks of an item: enough for all SMs together, no more than its pairs can feed */
+    const int items = p.kv_heads * p.sequences, groups = kMoveThreads / row16;
+    const int most = (p.capacity / 2 + groups * kFlight - 1) / (groups * kFlight);
+    const int blocks = std::max(1, std::min(most, std::max(8, 2048 / items)));
+    move_kernel<<<dim3(blocks, p.kv_heads, p.sequences), kMoveThreads, 0, s>>>(a, row16);
     count_launches(2);
     return cudaGetLastError();
 }

@@ -95,6 +95,8 @@ void check_view(const nut_paged_view &v) {
     if (!aligned16(v.keys) || !aligned16(v.values) || v.page_stride % unit != 0 ||
         v.head_stride % unit != 0 || v.slot_stride % unit != 0)
         raise(NUT_INVALID_ARGUMENT, "keys, values and strides must be multiples of 16 bytes");
+    if (!aligned16(v.bounds))
+        raise(NUT_INVALID_ARGUMENT, "bounds must be a multiple of 16 bytes");
     if (v.page_stride < 0 || v.head_stride < 0 || v.slot_stride < 0)
         raise(NUT_INVALID_ARGUMENT, "negative stride");
     if ((v.page_stride || v.head_stride || v.slot_stride) &&

@@ -2,103 +2,235 @@
  *
  * score(page) = max_g u_g U sum_d max(x_gd M_d, x_gd L_d), with x the query
  * head in 8 bits, M and L the page's greatest and least key in 8 bits, u and
- * U powers of two.  The sum is at most 256 * 127 * 128 < 2^24 in size, so
- * it is exact in an int and in fp32, whatever its order.
+ * U powers of two.  As max(x M, x L) = max(x, 0) M + min(x, 0) L, the sum is
+ * one product of [M | L] with [max(x, 0) | min(x, 0)]: mma.sync m16n8k32 in
+ * 8 bits, 16 pages by the 8 query heads of a group.  The sum is at most
+ * 256 * 127 * 128 < 2^24 in size, so it is exact in an int and in fp32,
+ * whatever its order.
+ *
+ * Bytes bound it: 2 head_dim + 4 of each page and kv head, a 32nd of what
+ * the page's 16 keys and values take in 16 bits.
  */
 #include <cstdint>
 #include <cuda_runtime.h>
 
 #include "kernels.h"
 #include "paged.cuh"
+#include "paged_choose.cuh"
+#include "stream.cuh"
 
 namespace nut {
 namespace {
 
-/* Warp per page: its score for one row and kv head. */
+constexpr int kWarps = 8;
+constexpr int kPages = 16;  /* of a warp's product */
+constexpr int kHeads = 8;   /* of a warp's product */
+constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
+
+/* Queries of one row and up to 8 heads in 8 bits, a warp for each head:
+ * [max(x, 0) | min(x, 0)] in `width` bytes, zeros behind; their units. */
 template <typename R>
-__global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ PagedSelect a) {
-    const PagedPool &p = a.p;
-    const int head = blockIdx.y, r = blockIdx.z, lane = threadIdx.x & 31;
-    const int j = int(blockIdx.x) * 8 + int(threadIdx.x >> 5);
-    int length;
-    const int s = row_span(p, a.row_sequence, a.row_length, r, length);
-    const int pages = (length + p.page_size - 1) / p.page_size, D = p.head_dim;
-    if (j >= pages)
-        return;
-    float best = -INFINITY;
-    if (j < a.sink_pages || j >= pages - a.recent_pages) {
-        best = INFINITY;
-    } else {
-        const int page = checked_page(p, s, j);
-        if (page >= 0) {
-            const int64_t at = int64_t(page) * p.kv_heads + head;
-            const int8_t *b = p.bounds + at * 2 * D;
-            for (int g = 0; g < p.group; g++) {
-                const R *q = static_cast<const R *>(a.q) + r * a.q_stride +
-                             int64_t(head * p.group + g) * D;
-                float top = 0.0f;
-                for (int d = lane; d < D; d += 32)
-                    top = fmaxf(top, fabsf(finite_key(to_float(q[d]))));
-                const float u = unit_of(warp_max(top)), inv = u > 0.0f ? 1.0f / u : 0.0f;
-                int sum = 0;
-                for (int d = lane; d < D; d += 32) {
-                    const int x = int(rintf(finite_key(to_float(q[d])) * inv));
-                    sum += max(x * b[d], x * b[D + d]);
-                }
-                sum = __reduce_add_sync(0xffffffffu, sum);
-                best = fmaxf(best, float(sum) * u);
-            }
-            best *= p.bound_scales[at];
+__device__ void quantise_queries(const PagedSelect &a, int row, int first_head, int heads, int width,
+                                 int pitch, int8_t *to, float *units) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.p.head_dim;
+    static_assert(kWarps == kHeads, "a warp for each head");
+    const R *q = static_cast<const R *>(a.q) + row * a.q_stride + int64_t(first_head + warp) * D;
+    int8_t *out = to + warp * pitch;
+    float v[8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int d = lane + 32 * i;
+        v[i] = warp < heads && d < D ? finite_key(to_float(q[d])) : 0.0f;
+        top = fmaxf(top, fabsf(v[i]));
+    }
+    const float u = unit_of(warp_max(top)), inv = u > 0.0f ? 1.0f / u : 0.0f; /* exact */
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int d = lane + 32 * i;
+        if (d < D) {
+            const int x = int(rintf(v[i] * inv));
+            out[d] = int8_t(max(x, 0));
+            out[D + d] = int8_t(min(x, 0));
         }
     }
+    for (int d = 2 * D + lane; d < width; d += 32)
+        out[d] = 0;
     if (lane == 0)
-        a.scores[(int64_t(r) * p.kv_heads + head) * p.max_pages + j] = best;
+        units[warp] = u;
 }
+
+/* Scores of 16 pages at a time for the rows of a block, KC 64-byte pieces
+ * of bounds a page.  A lane loads 16 neighbouring bytes of two pages for two
+ * products: which 32 of the 64 bytes meet in one product does not matter as
+ * long as both operands take the same ones. */
+template <typename R, int KC>
+__global__ void __launch_bounds__(kWarps * 32)
+    score_kernel(const __grid_constant__ PagedSelect a, int rows_each, int pages_each) {
+    constexpr int kWidth = KC * 64, kPitch = kWidth + 64; /* pitch: rows in different banks */
+    extern __shared__ __align__(16) int8_t queries[]; /* [rows_each][8][kPitch] */
+    __shared__ float units[kMostRows][kHeads];
+    const PagedPool &p = a.p;
+    const int head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3, D = p.head_dim;
+    const int row0 = int(blockIdx.z) * rows_each, rows = min(rows_each, a.rows - row0);
+    const int j_from = int(blockIdx.x) * pages_each, j_to = j_from + pages_each;
+
+    for (int gq = 0; gq < p.group; gq += kHeads) {
+        const int heads = min(kHeads, p.group - gq);
+        if (gq > 0)
+            __syncthreads();
+        for (int i = 0; i < rows; i++)
+            quantise_queries<R>(a, row0 + i, head * p.group + gq, heads, kWidth, kPitch,
+                                queries + i * kHeads * kPitch, units[i]);
+        __syncthreads();
+        for (int j0 = j_from + warp * kPages; j0 < j_to; j0 += kWarps * kPages) {
+            uint4 bound[2][KC];
+            float scale[2] = {0.0f, 0.0f};
+            bool there[2] = {false, false};
+            int held = -1; /* whose bounds these are */
+            for (int i = 0; i < rows; i++) {
+                int length;
+                const int s = row_span(p, a.row_sequence, a.row_length, row0 + i, length);
+                const int pages = (length + p.page_size - 1) / p.page_size;
+                if (j0 >= pages)
+                    continue;
+                if (s != held) {
+                    held = s;
+                    const int known = (checked_length(p, p.lengths[s]) + p.page_size - 1) / p.page_size;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int j = j0 + g + 8 * h;
+                        /* all of the sequence: the next rows may see more of it */
+                        const int page = j < max(known, pages) && j < p.max_pages ? checked_page(p, s, j) : -1;
+                        there[h] = page >= 0;
+                        const int64_t at = int64_t(page) * p.kv_heads + head;
+                        const uint4 *b = reinterpret_cast<const uint4 *>(p.bounds + at * 2 * D);
+                        scale[h] = there[h] ? p.bound_scales[at] : 0.0f;
+#pragma unroll
+                        for (int c = 0; c < KC; c++)
+                            bound[h][c] = there[h] && c * 4 + t < D / 8 ? __ldg(b + c * 4 + t) : make_uint4(0, 0, 0, 0);
+                    }
+                }
+                int acc[4] = {0, 0, 0, 0};
+                const int8_t *x = queries + (i * kHeads + g) * kPitch + t * 16;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const uint4 b = *reinterpret_cast<const uint4 *>(x + c * 64);
+                    const uint32_t lo[4] = {bound[0][c].x, bound[1][c].x, bound[0][c].y, bound[1][c].y};
+                    const uint32_t hi[4] = {bound[0][c].z, bound[1][c].z, bound[0][c].w, bound[1][c].w};
+                    mma_s8(acc, lo, b.x, b.y);
+                    mma_s8(acc, hi, b.z, b.w);
+                }
+                /* this lane: pages g and g + 8, heads 2 t and 2 t + 1 */
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float best = 2 * t < heads ? float(acc[2 * h]) * units[i][2 * t] : -INFINITY;
+                    if (2 * t + 1 < heads)
+                        best = fmaxf(best, float(acc[2 * h + 1]) * units[i][2 * t + 1]);
+                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+                    best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+                    const int j = j0 + g + 8 * h;
+                    if (t == 0 && j < pages) {
+                        float *to = a.scores + (int64_t(row0 + i) * p.kv_heads + head) * p.max_pages + j;
+                        float v = there[h] ? best * scale[h] : -INFINITY;
+                        if (gq > 0)
+                            v = fmaxf(v, *to);
+                        if (j < a.sink_pages || j >= pages - a.recent_pages)
+                            v = INFINITY;
+                        *to = v;
+                    }
+                }
+            }
+        }
+    }
+}
+
+struct PageKeys {
+    const float *score;
+    __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[kOwn]) const {
+        float v[kOwn];
+        load_own(score + i, there, v);
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            k[e] = e < there ? ordered_bits(v[e]) : 0u;
+    }
+};
 
 __global__ void __launch_bounds__(kChooseThreads)
     choose_pages_kernel(const __grid_constant__ PagedSelect a) {
     __shared__ ChooseScratch scratch;
     const PagedPool &p = a.p;
-    const int head = blockIdx.x, r = blockIdx.y;
+    const int head = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     int length;
     row_span(p, a.row_sequence, a.row_length, r, length);
     const int pages = (length + p.page_size - 1) / p.page_size;
     const int64_t at = int64_t(r) * p.kv_heads + head;
-    const float *score = a.scores + at * p.max_pages;
+    const PageKeys key{a.scores + at * p.max_pages};
     int32_t *out = a.selected + at * a.n_selected;
-    uint32_t threshold;
+    uint32_t first[kOwn], threshold;
     int quota;
-    choose_largest([=](int i) { return ordered_bits(score[i]); }, pages, a.n_selected, scratch,
-                   threshold, quota);
+    own_keys(key, 0, pages, first);
+    choose_largest<1>(key, pages, pages, a.n_selected, first, scratch, threshold, quota);
     int ties = 0, n = 0;
-    for (int i0 = 0; i0 < pages; i0 += blockDim.x) {
-        const int i = i0 + threadIdx.x;
-        const uint32_t k = i < pages ? ordered_bits(score[i]) : 0u;
-        const bool tie = i < pages && k == threshold;
-        int total;
-        const int rank = ties + block_rank(tie, scratch.warp[0], total);
+    for (int base = 0; base < pages; base += kChooseChunk) {
+        uint32_t k[kOwn];
+        if (base == 0) {
+#pragma unroll
+            for (int e = 0; e < kOwn; e++)
+                k[e] = first[e];
+        } else {
+            own_keys(key, base, pages, k);
+        }
+        const int i0 = base + tid * kOwn;
+        int mine = 0, total;
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            mine += i0 + e < pages && k[e] == threshold;
+        int rank = ties + block_before(mine, scratch, 0, total);
         ties += total;
-        const bool chosen = i < pages && (k > threshold || (tie && rank < quota));
-        const int to = n + block_rank(chosen, scratch.warp[1], total);
+        uint32_t chosen = 0;
+#pragma unroll
+        for (int e = 0; e < kOwn; e++)
+            if (i0 + e < pages && (k[e] > threshold || (k[e] == threshold && rank++ < quota)))
+                chosen |= 1u << e;
+        int to = n + block_before(__popc(chosen), scratch, 1, total);
         n += total;
-        if (chosen)
-            out[to] = i;
+        for (; chosen; chosen &= chosen - 1)
+            out[to++] = i0 + __ffs(chosen) - 1;
     }
-    for (int i = n + threadIdx.x; i < a.n_selected; i += blockDim.x)
+    for (int i = n + tid; i < a.n_selected; i += kChooseThreads)
         out[i] = -1;
+}
+
+template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cudaStream_t s) {
+    const PagedPool &p = a.p;
+    /* rows that may share a sequence share its bounds in registers */
+    const int rows_each = a.row_sequence ? kMostRows : 1, pages_each = kWarps * kPages;
+    const int bytes = rows_each * kHeads * (KC * 64 + 64);
+    const dim3 grid((p.max_pages + pages_each - 1) / pages_each, p.kv_heads,
+                    (a.rows + rows_each - 1) / rows_each);
+    score_kernel<R, KC><<<grid, kWarps * 32, bytes, s>>>(a, rows_each, pages_each);
+    return cudaGetLastError();
+}
+
+template <typename R> cudaError_t scores(const PagedSelect &a, cudaStream_t s) {
+    const int D = a.p.head_dim;
+    return D <= 32    ? launch_scores<R, 1>(a, s)
+           : D <= 64  ? launch_scores<R, 2>(a, s)
+           : D <= 96  ? launch_scores<R, 3>(a, s)
+           : D <= 128 ? launch_scores<R, 4>(a, s)
+                      : launch_scores<R, 8>(a, s);
 }
 
 } // namespace
 
 cudaError_t paged_select(const PagedSelect &a, cudaStream_t s) {
     const PagedPool &p = a.p;
-    const dim3 grid((p.max_pages + 7) / 8, p.kv_heads, a.rows);
-    if (a.type == 0)
-        score_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (a.type == 1)
-        score_kernel<__half><<<grid, 256, 0, s>>>(a);
-    else
-        score_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    const cudaError_t e = a.type == 0   ? scores<float>(a, s)
+                          : a.type == 1 ? scores<__half>(a, s)
+                                        : scores<__nv_bfloat16>(a, s);
+    if (e != cudaSuccess)
+        return e;
     choose_pages_kernel<<<dim3(p.kv_heads, a.rows), kChooseThreads, 0, s>>>(a);
     count_launches(2);
     return cudaGetLastError();

@@ -742,6 +742,54 @@ def test_eviction_leaves_the_attention_to_the_kept_tokens(gpu):
     check_attention(torch, pool, q, out, lse, [(0, 100), (1, 100)], 1 / 8, "f32")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,page,n", [([10001], 2, 700), ([9000, 300, 8193 * 2], 2, 5000)], ids=str)
+def test_select_among_thousands_of_pages(gpu, lens, page, n):
+    import torch
+    pool = Pool(torch, lens, 4, 1, 8, page, "f16", bounds=True, fill=False)
+    for s in range(len(lens)):
+        t = torch.arange(lens[s])
+        pages = pool.table_cpu[s].long()[t // page].cuda()
+        pool.keys[pages, :, (t % page).cuda()] = pool.k[s].permute(1, 0, 2).cuda()
+    pool.cache.summarise()
+    q = torch.randn(len(lens), 4, 8, generator=pool.g).cuda()
+    want = select_reference(pool, q, list(enumerate(lens)), n, 1, 2)
+    assert np.array_equal(run_select(torch, pool, q, "f32", len(lens), n, 1, 2), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [False, True], ids=["distinct", "ties"])
+@pytest.mark.parametrize("lens,budget", [([40001, 9000, 0, 5], 3000), ([33000], 32999), ([8200, 8193], 8192)], ids=str)
+def test_evict_from_long_caches(gpu, lens, budget, tied):
+    """Capacities beyond what one block holds."""
+    import torch
+    KV, D, ps = 2, 8, 64
+    pool = Pool(torch, lens, KV, KV, D, ps, "f16", fill=False)
+    for s, n in enumerate(lens):
+        t = torch.arange(n)
+        pages = pool.table_cpu[s].long()[t // ps].cuda()
+        pool.keys[pages, :, (t % ps).cuda()] = pool.k[s].permute(1, 0, 2).cuda()
+        pool.values[pages, :, (t % ps).cuda()] = pool.v[s].permute(1, 0, 2).cuda()
+    S, cap, g = len(lens), pool.capacity, pool.g
+    w = torch.randint(0, 3, (S, KV, cap), generator=g).float() if tied else torch.randn(S, KV, cap, generator=g).exp()
+    pos = torch.rand(S, KV, cap, generator=g).argsort(-1).int()
+    seen = torch.full((S,), cap, dtype=torch.int32)
+    dw, dp, dseen = w.cuda(), pos.cuda(), seen.cuda()
+    pool.cache.evict(dw.data_ptr(), dp.data_ptr(), dseen.data_ptr(), budget, sinks=4, recent=100,
+                     new_lengths=pool.lengths.data_ptr(), weights_out=dw.data_ptr(), positions_out=dp.data_ptr())
+    pool.cache.check()
+    source, left = evict_reference(pool, w, pos, seen, budget, 4, 100)
+    assert pool.lengths.cpu().tolist() == left
+    for s, n in enumerate(lens):
+        m = left[s]
+        for h in range(KV):
+            src = source[s, h]
+            assert torch.equal(pool.read(pool.keys, s, m)[h], pool.k[s][h][src])
+            assert torch.equal(pool.read(pool.values, s, m)[h], pool.v[s][h][src])
+            assert torch.equal(dw.cpu()[s, h, :m], w[s, h][src]) and not bool(dw.cpu()[s, h, m:n].any())
+            assert torch.equal(dp.cpu()[s, h, :m], pos[s, h][src]) and bool((dp.cpu()[s, h, m:n] == -1).all())
+
+
 # ---------------------------------------------------------------------------
 # refusals
 
