@@ -102,7 +102,7 @@ __device__ void choose_largest(const Key &key, int n, int all, int want, const u
         quota = want <= 0 ? 0 : all;
         return;
     }
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x;
     uint32_t prefix = 0;
     int left = want;
     for (int pass = 0; pass < 3; pass++) {
@@ -119,19 +119,11 @@ __device__ void choose_largest(const Key &key, int n, int all, int want, const u
             } else {
                 own_keys(key, base, n, k);
             }
-            if (base + (tid & ~31) * kOwn >= n)
-                continue; /* nothing in this warp */
 #pragma unroll
-            for (int e = 0; e < kOwn; e++) {
-                /* one addition for each bin among the warp's keys: scores
-                 * crowd into few bins */
-                const bool in = base + tid * kOwn + e < n &&
-                                (pass == 0 || (k[e] >> (shift + bits)) == (prefix >> (shift + bits)));
-                const uint32_t bin = in ? (k[e] >> shift) & ((1u << bits) - 1u) : 0xffffffffu;
-                const uint32_t same = __match_any_sync(0xffffffffu, bin);
-                if (in && lane == __ffs(same) - 1)
-                    atomicAdd(&s.hist[bin], __popc(same));
-            }
+            for (int e = 0; e < kOwn; e++)
+                if (base + tid * kOwn + e < n &&
+                    (pass == 0 || (k[e] >> (shift + bits)) == (prefix >> (shift + bits))))
+                    atomicAdd(&s.hist[(k[e] >> shift) & ((1u << bits) - 1u)], 1);
         }
         __syncthreads();
         const int *hist = s.hist;

@@ -195,9 +195,10 @@ __global__ void __launch_bounds__(kChooseThreads)
 }
 
 /* Keys and values of the pairs: a group of row16 threads moves a row of
- * row16 16-byte pieces, kFlight pairs at a time so that the look-ups and the
- * rows of several are on their way together. */
-constexpr int kMoveThreads = 256, kFlight = 4;
+ * row16 16-byte pieces.  One pair at a time: 51 us for 242 MB in 256-byte
+ * rows; with 2, 4 and 8 in flight in a thread the rows in flight on the chip
+ * lie further apart and it took 53, 59 and 85. */
+constexpr int kMoveThreads = 256;
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ PagedEvict a, int row16) {
     const PagedPool &p = a.p;
@@ -210,38 +211,21 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const int groups = kMoveThreads / row16, group = threadIdx.x / row16, piece = threadIdx.x % row16;
     if (group >= groups)
         return;
-    const int ps = p.page_size, all = gridDim.x * groups;
+    const int ps = p.page_size;
     const int64_t unit = p.type == 0 ? 4 : 2;
     char *keys = static_cast<char *>(p.keys) + int64_t(head) * p.head_stride * unit + piece * 16;
     char *values = static_cast<char *>(p.values) + int64_t(head) * p.head_stride * unit + piece * 16;
-    for (int i0 = blockIdx.x * groups + group; i0 < n; i0 += all * kFlight) {
-        int slot[2][kFlight], page[2][kFlight];
-#pragma unroll
-        for (int k = 0; k < kFlight; k++) {
-            const int i = i0 + k * all;
-            slot[0][k] = i < n ? holes[i] : -1;
-            slot[1][k] = i < n ? sources[i] : -1;
-        }
-#pragma unroll
-        for (int k = 0; k < kFlight; k++)
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-                page[x][k] = slot[x][k] >= 0 ? checked_page(p, s, slot[x][k] / ps) : -1;
-        uint4 key[kFlight], value[kFlight];
-#pragma unroll
-        for (int k = 0; k < kFlight; k++)
-            if (page[0][k] >= 0 && page[1][k] >= 0) {
-                const int64_t at = (page[1][k] * p.page_stride + slot[1][k] % ps * p.slot_stride) * unit;
-                key[k] = *reinterpret_cast<const uint4 *>(keys + at);
-                value[k] = *reinterpret_cast<const uint4 *>(values + at);
-            }
-#pragma unroll
-        for (int k = 0; k < kFlight; k++)
-            if (page[0][k] >= 0 && page[1][k] >= 0) {
-                const int64_t at = (page[0][k] * p.page_stride + slot[0][k] % ps * p.slot_stride) * unit;
-                *reinterpret_cast<uint4 *>(keys + at) = key[k];
-                *reinterpret_cast<uint4 *>(values + at) = value[k];
-            }
+    for (int i = blockIdx.x * groups + group; i < n; i += gridDim.x * groups) {
+        const int to = holes[i], from = sources[i];
+        const int page_to = checked_page(p, s, to / ps), page_from = checked_page(p, s, from / ps);
+        if (page_to < 0 || page_from < 0)
+            continue;
+        const int64_t src = (page_from * p.page_stride + from % ps * p.slot_stride) * unit;
+        const int64_t dst = (page_to * p.page_stride + to % ps * p.slot_stride) * unit;
+        const uint4 k = *reinterpret_cast<const uint4 *>(keys + src);
+        const uint4 v = *reinterpret_cast<const uint4 *>(values + src);
+        *reinterpret_cast<uint4 *>(keys + dst) = k;
+        *reinterpret_cast<uint4 *>(values + dst) = v;
     }
 }
 
@@ -271,7 +255,7 @@ cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const int row16 = p.head_dim * (p.type == 0 ? 4 : 2) / 16;
     /* blocks of an item: enough for all SMs together, no more than its pairs can feed */
     const int items = p.kv_heads * p.sequences, groups = kMoveThreads / row16;
-    const int most = (p.capacity / 2 + groups * kFlight - 1) / (groups * kFlight);
+    const int most = (p.capacity / 2 + groups - 1) / groups;
     const int blocks = std::max(1, std::min(most, std::max(8, 2048 / items)));
     move_kernel<<<dim3(blocks, p.kv_heads, p.sequences), kMoveThreads, 0, s>>>(a, row16);
     count_launches(2);
