@@ -2,11 +2,12 @@
 /* Choosing the largest of many 32-bit keys, ties to the lowest index: page
  * selection and slot eviction of the paged KV cache.
  *
- * A radix select by 11, 11 and 10 bits from the top.  One block, or the
- * blocks of a cluster that each hold a run of the keys and add their
- * histograms over distributed shared memory.  A thread owns kOwn
- * neighbouring keys of every chunk of kOwn * threads, and while the block's
- * run is a single chunk keeps them in registers over all passes. */
+ * search_largest: few keys, in the registers of four warps; the threshold is
+ * found two bits at a time by counting the keys at or above three candidates,
+ * 16 rounds without atomics or scans.
+ * choose_largest: any number of keys, by histograms of 11, 11 and 10 bits
+ * from the top; one block, or the blocks of a cluster that each hold a run
+ * of the keys and add their histograms over distributed shared memory. */
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -15,7 +16,7 @@ namespace nut {
 
 constexpr int kChooseThreads = 512;
 constexpr int kChooseWarps = kChooseThreads / 32;
-constexpr int kOwn = 8;
+constexpr int kOwn = 8; /* neighbouring keys a thread holds of a chunk */
 constexpr int kChooseChunk = kOwn * kChooseThreads;
 constexpr int kBins = 2048;
 
@@ -46,25 +47,96 @@ __device__ __forceinline__ int block_before(int count, ChooseScratch &s, int tur
     return before + upto - count;
 }
 
-/* 8 neighbouring words from x; aligned: 16-byte loads. */
-template <typename T> __device__ __forceinline__ void load_own(const T *x, int there, T (&v)[kOwn]) {
-    static_assert(sizeof(T) == 4 && kOwn == 8, "two 16-byte loads");
-    if (there >= kOwn && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(x);
-        *reinterpret_cast<uint4 *>(v + 4) = *reinterpret_cast<const uint4 *>(x + 4);
+/* N neighbouring words from x, zeros behind the first `there`; aligned:
+ * 16-byte loads. */
+template <int N, typename T> __device__ __forceinline__ void load_own(const T *x, int there, T (&v)[N]) {
+    static_assert(sizeof(T) == 4 && N % 4 == 0, "16-byte loads");
+    if (there >= N && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4)
+            *reinterpret_cast<uint4 *>(v + e) = *reinterpret_cast<const uint4 *>(x + e);
     } else {
 #pragma unroll
-        for (int e = 0; e < kOwn; e++)
+        for (int e = 0; e < N; e++)
             v[e] = e < there ? x[e] : T(0);
     }
 }
 
+constexpr int kFewWarps = 4;
+
+/* Sums of two counts (below 2^16 each) over kFewWarps warps, for every thread. */
+struct FewSums {
+    int2 (*scratch)[kFewWarps]; /* [2] */
+    int turn = 0;
+    __device__ __forceinline__ void operator()(int &a, int &b) {
+        a = __reduce_add_sync(0xffffffffu, a);
+        b = __reduce_add_sync(0xffffffffu, b);
+        if ((threadIdx.x & 31) == 0)
+            scratch[turn][threadIdx.x >> 5] = make_int2(a, b);
+        __syncthreads();
+        a = b = 0;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; w++) {
+            a += scratch[turn][w].x;
+            b += scratch[turn][w].y;
+        }
+        turn ^= 1;
+    }
+};
+
+/* The `want` (1 .. number of keys - 1) largest of the block's keys, N a
+ * thread, 0 where a thread has fewer: a key is chosen when it is above
+ * `threshold`, or equal to it and one of the first `quota` such.  Invariant:
+ * at least `want` keys are >= prefix, `above` are beyond the digits so far. */
+template <int N>
+__device__ __forceinline__ void search_largest(const uint32_t (&k)[N], int want, FewSums &sum, uint32_t &threshold,
+                                               int &quota) {
+    uint32_t prefix = 0;
+    int above = 0;
+    for (int shift = 30; shift >= 0; shift -= 2) {
+        const uint32_t c1 = prefix + (1u << shift), c2 = prefix + (2u << shift), c3 = prefix + (3u << shift);
+        int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            n1 += k[e] >= c1;
+            n2 += k[e] >= c2;
+            n3 += k[e] >= c3;
+        }
+        n1 |= n2 << 16;
+        sum(n1, n3);
+        n2 = int(uint32_t(n1) >> 16);
+        n1 &= 0xffff;
+        int here = -1; /* keys at or above the new prefix, where it moved */
+        if (n3 >= want) {
+            prefix = c3;
+            here = n3;
+        } else if (n2 >= want) {
+            prefix = c2;
+            here = n2;
+            above = n3;
+        } else if (n1 >= want) {
+            prefix = c1;
+            here = n1;
+            above = n2;
+        } else {
+            above = n1;
+        }
+        if (here == want) { /* no key is left to tell apart */
+            threshold = prefix - 1u;
+            quota = 0;
+            return;
+        }
+    }
+    threshold = prefix;
+    quota = want - above;
+}
+
 /* The keys of this thread in the chunk that starts at `base`; 0 beyond n.
- * key.own(i, there, k) makes the first `there` of keys i .. i + 7. */
-template <typename Key>
-__device__ __forceinline__ void own_keys(const Key &key, int base, int n, uint32_t (&k)[kOwn]) {
-    const int i0 = base + int(threadIdx.x) * kOwn;
-    key.own(i0, max(0, min(kOwn, n - i0)), k);
+ * key.own(i, there, k) makes the first `there` of keys i .. i + N - 1. */
+template <int N, typename Key>
+__device__ __forceinline__ void own_keys(const Key &key, int base, int n, uint32_t (&k)[N]) {
+    const int i0 = base + int(threadIdx.x) * N;
+    key.own(i0, max(0, min(N, n - i0)), k);
 }
 
 /* Adds `value` of every block of the cluster, for blocks of lower rank only
@@ -92,10 +164,10 @@ __device__ __forceinline__ void cluster_before(int value, ChooseScratch &s, int 
 
 /* The `want` largest of all keys of the cluster (key(0) .. key(n - 1) in
  * this block, `all` in the cluster): a key is chosen when it is above
- * `threshold`, or equal to it and one of the first `quota` such.  k holds
- * the block's first chunk. */
-template <int kBlocks, typename Key>
-__device__ void choose_largest(const Key &key, int n, int all, int want, const uint32_t (&first)[kOwn],
+ * `threshold`, or equal to it and one of the first `quota` such.  `first`
+ * holds the block's first chunk, N keys a thread. */
+template <int kBlocks, int N, typename Key>
+__device__ void choose_largest(const Key &key, int n, int all, int want, const uint32_t (&first)[N],
                                ChooseScratch &s, uint32_t &threshold, int &quota) {
     if (want <= 0 || want >= all) {
         threshold = want <= 0 ? 0xffffffffu : 0u;
@@ -110,18 +182,18 @@ __device__ void choose_largest(const Key &key, int n, int all, int want, const u
         for (int i = tid; i < kBins; i += kChooseThreads)
             s.hist[i] = 0;
         __syncthreads();
-        for (int base = 0; base < n; base += kChooseChunk) {
-            uint32_t k[kOwn];
+        for (int base = 0; base < n; base += N * kChooseThreads) {
+            uint32_t k[N];
             if (base == 0) {
 #pragma unroll
-                for (int e = 0; e < kOwn; e++)
+                for (int e = 0; e < N; e++)
                     k[e] = first[e];
             } else {
                 own_keys(key, base, n, k);
             }
 #pragma unroll
-            for (int e = 0; e < kOwn; e++)
-                if (base + tid * kOwn + e < n &&
+            for (int e = 0; e < N; e++)
+                if (base + tid * N + e < n &&
                     (pass == 0 || (k[e] >> (shift + bits)) == (prefix >> (shift + bits))))
                     atomicAdd(&s.hist[(k[e] >> shift) & ((1u << bits) - 1u)], 1);
         }

@@ -26,14 +26,14 @@ struct SlotKeys {
     const int32_t *positions;
     int sinks;
     int64_t recent_from;
-    __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[kOwn]) const {
-        float w[kOwn];
-        int32_t at[kOwn];
+    template <int N> __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[N]) const {
+        float w[N];
+        int32_t at[N];
         load_own(weights + i, there, w);
         if (positions)
             load_own(positions + i, there, at);
 #pragma unroll
-        for (int e = 0; e < kOwn; e++) {
+        for (int e = 0; e < N; e++) {
             k[e] = w[e] != w[e] ? 0u : ordered_bits(w[e]);
             if (positions && (at[e] < sinks || at[e] >= recent_from))
                 k[e] = ordered_bits(INFINITY);
@@ -43,155 +43,182 @@ struct SlotKeys {
     }
 };
 
-/* kBlocks blocks (a cluster) for each sequence and kv head, each with a run
- * of the slots. */
-template <int kBlocks>
+/* What both forms of the choice know of an item. */
+struct SlotItem {
+    int length, m;      /* slots now, slots to keep */
+    int64_t item, at;   /* its number, its first slot in the arrays */
+    int32_t *holes, *sources;
+    SlotKeys key;
+    __device__ SlotItem(const PagedEvict &a, int s, int head) {
+        const PagedPool &p = a.p;
+        length = checked_length(p, p.lengths[s]);
+        m = min(length, a.budget);
+        item = int64_t(s) * p.kv_heads + head;
+        at = item * p.capacity;
+        holes = a.pairs + at;
+        sources = holes + p.capacity / 2;
+        key = SlotKeys{a.weights + at, a.positions ? a.positions + at : nullptr, a.sinks,
+                       a.recent ? int64_t(a.seen[s]) - a.recent : INT64_MAX};
+    }
+};
+
+/* The slots i0 .. i0 + there - 1 as holes (to be filled) and sources. */
+__device__ __forceinline__ void holes_and_sources(uint32_t kept, int i0, int there, int m, uint32_t &hole,
+                                                  uint32_t &source) {
+    const uint32_t low = (1u << max(0, min(there, m - i0))) - 1u; /* those below m */
+    hole = low & ~kept;
+    source = kept & ~low;
+}
+
+__device__ __forceinline__ void list_slots(uint32_t mask, int i0, int32_t *to) {
+    for (; mask; mask &= mask - 1)
+        *to++ = i0 + __ffs(mask) - 1;
+}
+
+/* Weights and positions of slots i, or an empty slot's. */
+__device__ __forceinline__ void keep_slot(const PagedEvict &a, int64_t to, int64_t from) {
+    a.weights_out[to] = a.weights[from];
+    if (a.positions)
+        a.positions_out[to] = a.positions[from];
+}
+__device__ __forceinline__ void clear_slot(const PagedEvict &a, int64_t at) {
+    a.weights_out[at] = 0.0f;
+    if (a.positions)
+        a.positions_out[at] = -1;
+}
+
+/* Up to N * kChooseThreads slots: a block for each sequence and kv head,
+ * all keys in registers. */
+template <int N>
+__global__ void __launch_bounds__(kChooseThreads)
+    choose_few_slots_kernel(const __grid_constant__ PagedEvict a) {
+    __shared__ ChooseScratch scratch;
+    const SlotItem x(a, blockIdx.y, blockIdx.x);
+    const int tid = threadIdx.x, i0 = tid * N, there = max(0, min(N, x.length - i0));
+    uint32_t k[N], threshold;
+    x.key.own(i0, there, k);
+    int quota, total;
+    choose_largest<1>(x.key, x.length, x.length, x.m, k, scratch, threshold, quota);
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        ties += e < there && k[e] == threshold;
+    int rank = block_before(ties, scratch, 0, total);
+    uint32_t kept = 0, hole, source;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (e < there && (k[e] > threshold || (k[e] == threshold && rank++ < quota)))
+            kept |= 1u << e;
+    holes_and_sources(kept, i0, there, x.m, hole, source);
+    /* holes and sources in one scan: below 2^15 of each */
+    const int before = block_before(__popc(hole) | (__popc(source) << 16), scratch, 1, total);
+    list_slots(hole, i0, x.holes + (before & 0xffff));
+    list_slots(source, i0, x.sources + (before >> 16));
+    const int pairs = total & 0xffff;
+    if (tid == 0) {
+        a.counts[x.item * 2] = pairs;
+        a.counts[x.item * 2 + 1] = x.m;
+    }
+    /* kept slots first: a hole's own entry is overwritten after */
+    if (a.weights_out != a.weights || a.positions_out != a.positions)
+        for (int i = tid; i < x.m; i += kChooseThreads)
+            keep_slot(a, x.at + i, x.at + i);
+    __syncthreads();
+    for (int i = tid; i < pairs; i += kChooseThreads)
+        keep_slot(a, x.at + x.holes[i], x.at + x.sources[i]);
+    __syncthreads();
+    for (int i = x.m + tid; i < x.length; i += kChooseThreads)
+        clear_slot(a, x.at + i);
+}
+
+/* Any number of slots: a cluster of kBlocks blocks for each sequence and kv
+ * head, each with a run of the slots. */
+constexpr int kBlocks = 8;
+
 __global__ void __launch_bounds__(kChooseThreads)
     choose_slots_kernel(const __grid_constant__ PagedEvict a) {
     __shared__ ChooseScratch scratch;
-    const PagedPool &p = a.p;
-    const int rank = int(blockIdx.x) % kBlocks, head = int(blockIdx.x) / kBlocks, s = blockIdx.y;
-    const int tid = threadIdx.x;
-    const int length = checked_length(p, p.lengths[s]), m = min(length, a.budget);
-    /* runs of whole groups of kOwn slots */
-    const int run = (length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn;
-    const int from = min(rank * run, length), n = min(run, length - from);
-    const int64_t item = int64_t(s) * p.kv_heads + head, at = item * p.capacity;
-    const float *w = a.weights + at + from;
-    const int32_t *pos = a.positions ? a.positions + at + from : nullptr;
-    const int64_t recent_from = a.recent ? int64_t(a.seen[s]) - a.recent : INT64_MAX;
-    const SlotKeys key{w, pos, a.sinks, recent_from};
+    const int rank = int(blockIdx.x) % kBlocks, tid = threadIdx.x;
+    const SlotItem x(a, blockIdx.y, int(blockIdx.x) / kBlocks);
+    const int run = (x.length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn; /* whole groups of kOwn */
+    const int from = min(rank * run, x.length), n = min(run, x.length - from);
+    SlotKeys key = x.key;
+    key.weights += from;
+    key.positions += key.positions ? from : 0;
     uint32_t first[kOwn], threshold;
-    int quota;
+    int quota, total, all;
     own_keys(key, 0, n, first);
-    choose_largest<kBlocks>(key, n, length, m, first, scratch, threshold, quota);
+    choose_largest<kBlocks>(key, n, x.length, x.m, first, scratch, threshold, quota);
 
-    /* ties, holes and sources of the blocks before this one */
-    int ties = 0, holes_n = 0, sources_n = 0;
-    int32_t *holes = a.pairs + at, *sources = holes + p.capacity / 2;
-    if constexpr (kBlocks > 1) {
-        int mine = 0, total, all;
-        for (int base = 0; base < n; base += kChooseChunk) {
-            uint32_t k[kOwn];
-            own_keys(key, base, n, k);
-#pragma unroll
-            for (int e = 0; e < kOwn; e++)
-                mine += base + tid * kOwn + e < n && k[e] == threshold;
-        }
-        block_before(mine, scratch, 0, total);
-        cluster_before<kBlocks>(total, scratch, 0, ties, all);
-        /* kept slots below m and from m on, up to this block's run, follow
-         * from the counts of kept ones */
-    }
-    auto flags = [&](int base, int rank0, const uint32_t (&k)[kOwn], uint32_t &kept) {
-        const int i0 = base + tid * kOwn;
-        kept = 0;
+    auto ties_in = [&](int base, const uint32_t(&k)[kOwn]) {
+        int ties = 0;
 #pragma unroll
         for (int e = 0; e < kOwn; e++)
-            if (i0 + e < n && (k[e] > threshold || (k[e] == threshold && rank0++ < quota)))
-                kept |= 1u << e;
+            ties += base + tid * kOwn + e < n && k[e] == threshold;
+        return ties;
     };
-    auto own_mask = [&](int base) { /* this thread's slots of the chunk, and those of them below m */
-        const int i0 = base + tid * kOwn;
-        const int there = max(0, min(kOwn, n - i0)), low = max(0, min(there, m - from - i0));
-        return make_uint2((1u << there) - 1u, (1u << low) - 1u);
-    };
-    if constexpr (kBlocks > 1) {
-        int h = 0, q = 0, t0 = ties, total, all;
+    /* walks this block's slots: each(holes, sources, first slot) */
+    int ties_before = 0;
+    auto walk = [&](auto each) {
+        int ties = ties_before;
         for (int base = 0; base < n; base += kChooseChunk) {
-            uint32_t k[kOwn], kept;
+            uint32_t k[kOwn], kept = 0, hole, source;
             own_keys(key, base, n, k);
-            int mine = 0;
+            int tie_rank = ties + block_before(ties_in(base, k), scratch, 0, total);
+            ties += total;
+            const int i0 = base + tid * kOwn, there = max(0, min(kOwn, n - i0));
 #pragma unroll
             for (int e = 0; e < kOwn; e++)
-                mine += base + tid * kOwn + e < n && k[e] == threshold;
-            const int rank0 = t0 + block_before(mine, scratch, 0, total);
-            t0 += total;
-            flags(base, rank0, k, kept);
-            const uint2 own = own_mask(base);
-            h += __popc(own.y & ~kept);
-            q += __popc(kept & ~own.y);
-            __syncthreads(); /* before the scan's scratch is used again */
+                if (e < there && (k[e] > threshold || (k[e] == threshold && tie_rank++ < quota)))
+                    kept |= 1u << e;
+            holes_and_sources(kept, from + i0, there, x.m, hole, source);
+            each(hole, source, from + i0);
+            __syncthreads(); /* the scan's scratch is free again */
         }
-        block_before(h, scratch, 1, total);
-        cluster_before<kBlocks>(total, scratch, 1, holes_n, all);
-        __syncthreads();
-        block_before(q, scratch, 1, total);
-        cluster_before<kBlocks>(total, scratch, 2, sources_n, all);
-        __syncthreads();
-    }
-    int ties_seen = ties;
+    };
+    /* ties, holes and sources in the blocks before this one */
+    int mine = 0, holes_n, sources_n, pairs;
     for (int base = 0; base < n; base += kChooseChunk) {
-        uint32_t k[kOwn], kept;
-        if (base == 0) {
-#pragma unroll
-            for (int e = 0; e < kOwn; e++)
-                k[e] = first[e];
-        } else {
-            own_keys(key, base, n, k);
-        }
-        int mine = 0, total;
-#pragma unroll
-        for (int e = 0; e < kOwn; e++)
-            mine += base + tid * kOwn + e < n && k[e] == threshold;
-        const int rank0 = ties_seen + block_before(mine, scratch, 0, total);
-        ties_seen += total;
-        flags(base, rank0, k, kept);
-        const uint2 own = own_mask(base);
-        uint32_t hole = own.y & ~kept, source = kept & ~own.y;
-        /* both counts in one scan */
-        const int both = __popc(hole) | (__popc(source) << 16);
-        const int before = block_before(both, scratch, 1, total);
-        int to = holes_n + (before & 0xffff), of = sources_n + (before >> 16);
+        uint32_t k[kOwn];
+        own_keys(key, base, n, k);
+        mine += ties_in(base, k);
+    }
+    block_before(mine, scratch, 0, total);
+    cluster_before<kBlocks>(total, scratch, 0, ties_before, all);
+    int holes_here = 0, sources_here = 0;
+    walk([&](uint32_t hole, uint32_t source, int) {
+        holes_here += __popc(hole);
+        sources_here += __popc(source);
+    });
+    block_before(holes_here, scratch, 1, total);
+    cluster_before<kBlocks>(total, scratch, 1, holes_n, pairs);
+    __syncthreads();
+    block_before(sources_here, scratch, 1, total);
+    cluster_before<kBlocks>(total, scratch, 2, sources_n, all);
+    __syncthreads();
+    walk([&](uint32_t hole, uint32_t source, int i0) {
+        const int before = block_before(__popc(hole) | (__popc(source) << 16), scratch, 1, total);
+        list_slots(hole, i0, x.holes + holes_n + (before & 0xffff));
+        list_slots(source, i0, x.sources + sources_n + (before >> 16));
         holes_n += total & 0xffff;
         sources_n += total >> 16;
-        const int i0 = from + base + tid * kOwn;
-        for (; hole; hole &= hole - 1)
-            holes[to++] = i0 + __ffs(hole) - 1;
-        for (; source; source &= source - 1)
-            sources[of++] = i0 + __ffs(source) - 1;
+    });
+    if (rank == 0 && tid == 0) {
+        a.counts[x.item * 2] = pairs;
+        a.counts[x.item * 2 + 1] = x.m;
     }
-    /* the last block of the run has seen them all */
-    if (rank == kBlocks - 1 && tid == 0) {
-        a.counts[item * 2] = holes_n;
-        a.counts[item * 2 + 1] = m;
-        scratch.shared[3] = holes_n;
-    }
-    const float *w0 = a.weights + at;
-    const int32_t *pos0 = a.positions ? a.positions + at : nullptr;
     /* kept slots first: a hole's own entry is overwritten after */
-    const int low = max(0, min(n, m - from));
-    if (a.weights_out != a.weights)
-        for (int i = tid; i < low; i += kChooseThreads)
-            a.weights_out[at + from + i] = w[i];
-    if (pos && a.positions_out != a.positions)
-        for (int i = tid; i < low; i += kChooseThreads)
-            a.positions_out[at + from + i] = pos[i];
-    int pairs;
-    if constexpr (kBlocks > 1) {
-        auto cluster = cooperative_groups::this_cluster();
-        __threadfence();
-        cluster.sync();
-        pairs = *cluster.map_shared_rank(&scratch.shared[3], kBlocks - 1);
-    } else {
-        __syncthreads();
-        pairs = holes_n;
-    }
-    for (int i = rank * kChooseThreads + tid; i < pairs; i += kBlocks * kChooseThreads) {
-        const int to = holes[i], of = sources[i];
-        a.weights_out[at + to] = w0[of];
-        if (pos)
-            a.positions_out[at + to] = pos0[of];
-    }
-    if constexpr (kBlocks > 1)
-        cooperative_groups::this_cluster().sync(); /* sources read, and shared memory done with */
-    else
-        __syncthreads();
-    for (int i = low + tid; i < n; i += kChooseThreads) {
-        a.weights_out[at + from + i] = 0.0f;
-        if (pos)
-            a.positions_out[at + from + i] = -1;
-    }
+    const int whole = kBlocks * kChooseThreads, me = rank * kChooseThreads + tid;
+    if (a.weights_out != a.weights || a.positions_out != a.positions)
+        for (int i = me; i < x.m; i += whole)
+            keep_slot(a, x.at + i, x.at + i);
+    __threadfence();
+    cooperative_groups::this_cluster().sync();
+    for (int i = me; i < pairs; i += whole)
+        keep_slot(a, x.at + x.holes[i], x.at + x.sources[i]);
+    cooperative_groups::this_cluster().sync(); /* sources read, and shared memory done with */
+    for (int i = x.m + me; i < x.length; i += whole)
+        clear_slot(a, x.at + i);
 }
 
 /* Keys and values of the pairs: a group of row16 threads moves a row of
@@ -234,21 +261,25 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
 cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     cudaError_t e;
-    if (p.capacity <= 2 * kChooseChunk) {
-        choose_slots_kernel<1><<<dim3(p.kv_heads, p.sequences), kChooseThreads, 0, s>>>(a);
+    if (p.capacity <= 16 * kChooseThreads) {
+        const dim3 grid(p.kv_heads, p.sequences);
+        if (p.capacity <= 4 * kChooseThreads)
+            choose_few_slots_kernel<4><<<grid, kChooseThreads, 0, s>>>(a);
+        else
+            choose_few_slots_kernel<16><<<grid, kChooseThreads, 0, s>>>(a);
         e = cudaGetLastError();
     } else {
         cudaLaunchConfig_t config{};
-        config.gridDim = dim3(8 * p.kv_heads, p.sequences);
+        config.gridDim = dim3(kBlocks * p.kv_heads, p.sequences);
         config.blockDim = dim3(kChooseThreads);
         config.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 8;
+        attr[0].val.clusterDim.x = kBlocks;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         config.attrs = attr;
         config.numAttrs = 1;
-        e = cudaLaunchKernelEx(&config, choose_slots_kernel<8>, a);
+        e = cudaLaunchKernelEx(&config, choose_slots_kernel, a);
     }
     if (e != cudaSuccess)
         return e;

@@ -147,11 +147,11 @@ __global__ void __launch_bounds__(kWarps * 32)
 
 struct PageKeys {
     const float *score;
-    __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[kOwn]) const {
-        float v[kOwn];
+    template <int N> __device__ __forceinline__ void own(int i, int there, uint32_t (&k)[N]) const {
+        float v[N];
         load_own(score + i, there, v);
 #pragma unroll
-        for (int e = 0; e < kOwn; e++)
+        for (int e = 0; e < N; e++)
             k[e] = e < there ? ordered_bits(v[e]) : 0u;
     }
 };
@@ -202,6 +202,63 @@ __global__ void __launch_bounds__(kChooseThreads)
         out[i] = -1;
 }
 
+/* The same for at most 128 N pages, N neighbouring ones a thread.  For 512
+ * pages, two thousand times over, the other form takes 34 us and this one 12. */
+constexpr int kFewThreads = kFewWarps * 32;
+
+template <int N>
+__global__ void __launch_bounds__(kFewThreads)
+    choose_few_pages_kernel(const __grid_constant__ PagedSelect a) {
+    __shared__ int2 counts[2][kFewWarps];
+    __shared__ int scans[2][kFewWarps];
+    const PagedPool &p = a.p;
+    const int head = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int length;
+    row_span(p, a.row_sequence, a.row_length, r, length);
+    const int pages = (length + p.page_size - 1) / p.page_size, want = min(a.n_selected, pages);
+    const int64_t at = int64_t(r) * p.kv_heads + head;
+    int32_t *out = a.selected + at * a.n_selected;
+    const PageKeys key{a.scores + at * p.max_pages};
+    uint32_t k[N], threshold = 0;
+    const int i0 = tid * N, there = max(0, min(N, pages - i0));
+    key.own(i0, there, k);
+    int quota = want;
+    if (want < pages) {
+        FewSums sum{counts};
+        search_largest(k, want, sum, threshold, quota);
+    }
+    auto before = [&](int count, int turn) {
+        int upto = count;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            upto += lane >= x ? v : 0;
+        }
+        if (lane == 31)
+            scans[turn][warp] = upto;
+        __syncthreads();
+        int less = upto - count;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; w++)
+            less += w < warp ? scans[turn][w] : 0;
+        return less;
+    };
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        ties += e < there && k[e] == threshold;
+    int rank = before(ties, 0);
+    uint32_t chosen = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (e < there && (k[e] > threshold || (k[e] == threshold && rank++ < quota)))
+            chosen |= 1u << e;
+    for (int to = before(__popc(chosen), 1); chosen; chosen &= chosen - 1)
+        out[to++] = i0 + __ffs(chosen) - 1;
+    for (int i = want + tid; i < a.n_selected; i += kFewThreads)
+        out[i] = -1;
+}
+
 template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     /* rows that may share a sequence share its bounds in registers */
@@ -231,7 +288,13 @@ cudaError_t paged_select(const PagedSelect &a, cudaStream_t s) {
                                         : scores<__nv_bfloat16>(a, s);
     if (e != cudaSuccess)
         return e;
-    choose_pages_kernel<<<dim3(p.kv_heads, a.rows), kChooseThreads, 0, s>>>(a);
+    const dim3 items(p.kv_heads, a.rows);
+    if (p.max_pages <= 4 * kFewThreads)
+        choose_few_pages_kernel<4><<<items, kFewThreads, 0, s>>>(a);
+    else if (p.max_pages <= 8 * kFewThreads)
+        choose_few_pages_kernel<8><<<items, kFewThreads, 0, s>>>(a);
+    else
+        choose_pages_kernel<<<items, kChooseThreads, 0, s>>>(a);
     count_launches(2);
     return cudaGetLastError();
 }
