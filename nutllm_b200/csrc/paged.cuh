@@ -6,9 +6,38 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "kernels.h"
 #include "paged.h"
 
 namespace nut {
+
+/* The paged kernels are launched while the kernel before them in the stream
+ * still runs: what it wrote may be read, and its buffers written, after
+ * begin_kernel(), which also lets the next one be launched. */
+__device__ __forceinline__ void begin_kernel() {
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t bytes, cudaStream_t stream,
+                          int cluster, Args... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = bytes;
+    config.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    count_launches(1);
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -34,6 +63,12 @@ __device__ __forceinline__ int checked_length(const PagedPool &p, int length) {
         return 0;
     }
     return length;
+}
+
+/* Page number of logical page j of sequence s, or -1. */
+__device__ __forceinline__ int lookup(const PagedPool &p, int s, int j) {
+    const int page = p.table[int64_t(s) * p.max_pages + j];
+    return unsigned(page) < unsigned(p.n_pages) ? page : -1;
 }
 
 /* Page number of logical page j of sequence s, or -1 (recorded). */

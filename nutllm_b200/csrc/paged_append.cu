@@ -12,7 +12,6 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
-#include "kernels.h"
 #include "paged.cuh"
 
 namespace nut {
@@ -139,10 +138,11 @@ __device__ void page_bounds(const PagedPool &p, int page, int head, int used) {
  * the value. */
 template <typename R, typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ PagedAppend a) {
+    begin_kernel();
     const PagedPool &p = a.p;
     const int head = blockIdx.y, s = blockIdx.z;
-    const int row0 = a.starts[s], row1 = a.starts[s + 1], stored = p.lengths[s];
-    const int n = row1 - row0, length = checked_length(p, stored);
+    const int row0 = a.starts[s], row1 = a.starts[s + 1];
+    const int n = row1 - row0, length = checked_length(p, p.lengths[s]);
     if (n == 0)
         return;
     if (row0 < 0 || n < 0 || row1 > a.rows || n > a.max_new || n > length) {
@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) summarise_kernel(const __grid_constant__ PagedPool p) {
+    begin_kernel();
     const int j = blockIdx.x, head = blockIdx.y, s = blockIdx.z;
     const int used = min(checked_length(p, p.lengths[s]) - j * p.page_size, p.page_size);
     if (used <= 0)
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) summarise_kernel(const __grid_consta
         page_bounds<T>(p, page, head, used);
 }
 
-template <typename R, typename T> void launch_append(const PagedAppend &a, cudaStream_t s) {
+template <typename R, typename T> cudaError_t launch_append(const PagedAppend &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     /* pages that max_new consecutive slots can touch */
     const dim3 grid((a.max_new + p.page_size - 2) / p.page_size + 1, p.kv_heads, p.sequences);
@@ -243,10 +244,8 @@ template <typename R, typename T> void launch_append(const PagedAppend &a, cudaS
         bits |= reinterpret_cast<uintptr_t>(x);
     for (int64_t stride : {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride})
         bits |= uintptr_t(stride) * sizeof(R);
-    if ((bits & 15) == 0)
-        append_kernel<R, T, true><<<grid, kThreads, 0, s>>>(a);
-    else
-        append_kernel<R, T, false><<<grid, kThreads, 0, s>>>(a);
+    return launch_kernel((bits & 15) == 0 ? append_kernel<R, T, true> : append_kernel<R, T, false>, grid,
+                         kThreads, 0, s, 1, a);
 }
 
 } // namespace
@@ -254,29 +253,18 @@ template <typename R, typename T> void launch_append(const PagedAppend &a, cudaS
 cudaError_t paged_append(const PagedAppend &a, cudaStream_t s) {
     const bool wide = a.type == 0;
     if (a.p.type == 0)
-        launch_append<float, float>(a, s);
-    else if (a.p.type == 1 && wide)
-        launch_append<float, __half>(a, s);
-    else if (a.p.type == 1)
-        launch_append<__half, __half>(a, s);
-    else if (wide)
-        launch_append<float, __nv_bfloat16>(a, s);
-    else
-        launch_append<__nv_bfloat16, __nv_bfloat16>(a, s);
-    count_launches(1);
-    return cudaGetLastError();
+        return launch_append<float, float>(a, s);
+    if (a.p.type == 1)
+        return wide ? launch_append<float, __half>(a, s) : launch_append<__half, __half>(a, s);
+    return wide ? launch_append<float, __nv_bfloat16>(a, s) : launch_append<__nv_bfloat16, __nv_bfloat16>(a, s);
 }
 
 cudaError_t paged_summarise(const PagedPool &p, cudaStream_t s) {
     const dim3 grid(p.max_pages, p.kv_heads, p.sequences);
-    if (p.type == 0)
-        summarise_kernel<float><<<grid, kThreads, 0, s>>>(p);
-    else if (p.type == 1)
-        summarise_kernel<__half><<<grid, kThreads, 0, s>>>(p);
-    else
-        summarise_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(p);
-    count_launches(1);
-    return cudaGetLastError();
+    const auto kernel = p.type == 0   ? summarise_kernel<float>
+                        : p.type == 1 ? summarise_kernel<__half>
+                                      : summarise_kernel<__nv_bfloat16>;
+    return launch_kernel(kernel, grid, kThreads, 0, s, 1, p);
 }
 
 } // namespace nut

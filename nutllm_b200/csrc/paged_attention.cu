@@ -16,7 +16,6 @@
 #include <type_traits>
 #include <cuda_runtime.h>
 
-#include "kernels.h"
 #include "paged.cuh"
 #include "stream.cuh"
 
@@ -701,6 +700,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
             mbar_init(&full[0][0] + i, 1);
         fence_barrier_init();
     }
+    begin_kernel();
 
     /* this CTA's share of the line of tiles: thread i sums a run of rows */
     const int run = (a.rows + kThreads - 1) / kThreads;
@@ -967,6 +967,7 @@ __global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ Pa
     const PagedPool &p = a.p;
     const int head = blockIdx.y, r = blockIdx.z;
     int length;
+    begin_kernel();
     row_span(p, a.row_sequence, a.row_length, r, length);
     const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity;
     const int64_t h0 = int64_t(r) * p.heads + head * p.group;
@@ -1003,15 +1004,11 @@ cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
     const int64_t slots = a.selected ? int64_t(a.n_selected) * p.page_size : p.capacity;
     const int64_t tiles = items * ((slots + tile - 1) / tile);
     const int64_t ctas = int64_t(a.sms) * per_sm;
-    attention_kernel<Op, R><<<unsigned(tiles < ctas ? tiles : ctas), threads, bytes, s>>>(a);
-    count_launches(1);
-    e = cudaGetLastError();
+    e = launch_kernel(attention_kernel<Op, R>, dim3(unsigned(tiles < ctas ? tiles : ctas)), threads, bytes, s, 1, a);
     if (e != cudaSuccess || !a.weights)
         return e;
     const unsigned blocks = unsigned((p.capacity + 1023) / 1024);
-    weights_kernel<<<dim3(blocks, p.kv_heads, a.rows), 256, 0, s>>>(a);
-    count_launches(1);
-    return cudaGetLastError();
+    return launch_kernel(weights_kernel, dim3(blocks, p.kv_heads, a.rows), 256, 0, s, 1, a);
 }
 
 template <typename T, typename R> cudaError_t launch_halves(const PagedAttention &a, cudaStream_t s) {

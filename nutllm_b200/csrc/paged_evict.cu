@@ -14,7 +14,6 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
-#include "kernels.h"
 #include "paged.cuh"
 #include "paged_choose.cuh"
 
@@ -93,6 +92,7 @@ template <int N>
 __global__ void __launch_bounds__(kChooseThreads)
     choose_few_slots_kernel(const __grid_constant__ PagedEvict a) {
     __shared__ ChooseScratch scratch;
+    begin_kernel();
     const SlotItem x(a, blockIdx.y, blockIdx.x);
     const int tid = threadIdx.x, i0 = tid * N, there = max(0, min(N, x.length - i0));
     uint32_t k[N], threshold;
@@ -138,6 +138,7 @@ constexpr int kBlocks = 8;
 __global__ void __launch_bounds__(kChooseThreads)
     choose_slots_kernel(const __grid_constant__ PagedEvict a) {
     __shared__ ChooseScratch scratch;
+    begin_kernel();
     const int rank = int(blockIdx.x) % kBlocks, tid = threadIdx.x;
     const SlotItem x(a, blockIdx.y, int(blockIdx.x) / kBlocks);
     const int run = (x.length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn; /* whole groups of kOwn */
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const PagedPool &p = a.p;
     const int head = blockIdx.y, s = blockIdx.z;
     const int64_t item = int64_t(s) * p.kv_heads + head;
+    begin_kernel();
     const int n = a.counts[item * 2];
     if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0)
         a.new_lengths[s] = a.counts[item * 2 + 1];
@@ -260,27 +262,13 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
 
 cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const PagedPool &p = a.p;
-    cudaError_t e;
-    if (p.capacity <= 16 * kChooseThreads) {
-        const dim3 grid(p.kv_heads, p.sequences);
-        if (p.capacity <= 4 * kChooseThreads)
-            choose_few_slots_kernel<4><<<grid, kChooseThreads, 0, s>>>(a);
-        else
-            choose_few_slots_kernel<16><<<grid, kChooseThreads, 0, s>>>(a);
-        e = cudaGetLastError();
-    } else {
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(kBlocks * p.kv_heads, p.sequences);
-        config.blockDim = dim3(kChooseThreads);
-        config.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = kBlocks;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        config.attrs = attr;
-        config.numAttrs = 1;
-        e = cudaLaunchKernelEx(&config, choose_slots_kernel, a);
-    }
+    const dim3 all(p.kv_heads, p.sequences);
+    const cudaError_t e =
+        p.capacity <= 4 * kChooseThreads ? launch_kernel(choose_few_slots_kernel<4>, all, kChooseThreads, 0, s, 1, a)
+        : p.capacity <= 16 * kChooseThreads
+            ? launch_kernel(choose_few_slots_kernel<16>, all, kChooseThreads, 0, s, 1, a)
+            : launch_kernel(choose_slots_kernel, dim3(kBlocks * p.kv_heads, p.sequences), kChooseThreads, 0, s,
+                            kBlocks, a);
     if (e != cudaSuccess)
         return e;
     const int row16 = p.head_dim * (p.type == 0 ? 4 : 2) / 16;
@@ -288,9 +276,7 @@ cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const int items = p.kv_heads * p.sequences, groups = kMoveThreads / row16;
     const int most = (p.capacity / 2 + groups - 1) / groups;
     const int blocks = std::max(1, std::min(most, std::max(8, 2048 / items)));
-    move_kernel<<<dim3(blocks, p.kv_heads, p.sequences), kMoveThreads, 0, s>>>(a, row16);
-    count_launches(2);
-    return cudaGetLastError();
+    return launch_kernel(move_kernel, dim3(blocks, p.kv_heads, p.sequences), kMoveThreads, 0, s, 1, a, row16);
 }
 
 } // namespace nut

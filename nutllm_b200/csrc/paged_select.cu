@@ -14,7 +14,6 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
-#include "kernels.h"
 #include "paged.cuh"
 #include "paged_choose.cuh"
 #include "stream.cuh"
@@ -27,90 +26,119 @@ constexpr int kPages = 16;  /* of a warp's product */
 constexpr int kHeads = 8;   /* of a warp's product */
 constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
 
-/* Queries of one row and up to 8 heads in 8 bits, a warp for each head:
- * [max(x, 0) | min(x, 0)] in `width` bytes, zeros behind; their units. */
-template <typename R>
-__device__ void quantise_queries(const PagedSelect &a, int row, int first_head, int heads, int width,
-                                 int pitch, int8_t *to, float *units) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.p.head_dim;
-    static_assert(kWarps == kHeads, "a warp for each head");
-    const R *q = static_cast<const R *>(a.q) + row * a.q_stride + int64_t(first_head + warp) * D;
-    int8_t *out = to + warp * pitch;
-    float v[8], top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        v[i] = warp < heads && d < D ? finite_key(to_float(q[d])) : 0.0f;
-        top = fmaxf(top, fabsf(v[i]));
-    }
-    const float u = unit_of(warp_max(top)), inv = u > 0.0f ? 1.0f / u : 0.0f; /* exact */
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        if (d < D) {
-            const int x = int(rintf(v[i] * inv));
-            out[d] = int8_t(max(x, 0));
-            out[D + d] = int8_t(min(x, 0));
-        }
-    }
-    for (int d = 2 * D + lane; d < width; d += 32)
-        out[d] = 0;
-    if (lane == 0)
-        units[warp] = u;
-}
-
 /* Scores of 16 pages at a time for the rows of a block, KC 64-byte pieces
  * of bounds a page.  A lane loads 16 neighbouring bytes of two pages for two
  * products: which 32 of the 64 bytes meet in one product does not matter as
- * long as both operands take the same ones. */
+ * long as both operands take the same ones.  The first pages' bounds are on
+ * their way (three look-ups one after another) while the queries are put
+ * into 8 bits. */
 template <typename R, int KC>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
     score_kernel(const __grid_constant__ PagedSelect a, int rows_each, int pages_each) {
     constexpr int kWidth = KC * 64, kPitch = kWidth + 64; /* pitch: rows in different banks */
-    extern __shared__ __align__(16) int8_t queries[]; /* [rows_each][8][kPitch] */
+    constexpr int kBatch = 4;                             /* heads of a warp that load together */
+    extern __shared__ __align__(16) int8_t queries[];     /* [rows_each][8][kPitch] */
     __shared__ float units[kMostRows][kHeads];
+    __shared__ int sequence_of[kMostRows], pages_of[kMostRows], limit_of[kMostRows];
     const PagedPool &p = a.p;
     const int head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3, D = p.head_dim;
     const int row0 = int(blockIdx.z) * rows_each, rows = min(rows_each, a.rows - row0);
     const int j_from = int(blockIdx.x) * pages_each, j_to = j_from + pages_each;
+    begin_kernel();
+    if (int(threadIdx.x) < rows) {
+        int length;
+        sequence_of[threadIdx.x] = row_span(p, a.row_sequence, a.row_length, row0 + int(threadIdx.x), length);
+        pages_of[threadIdx.x] = (length + p.page_size - 1) / p.page_size;
+    }
+    __syncthreads();
+    int most = 0, limit = 0; /* pages of any row; of any row of this thread's row's sequence */
+    for (int i = 0; i < rows; i++) {
+        most = max(most, pages_of[i]);
+        if (int(threadIdx.x) < rows && sequence_of[i] == sequence_of[threadIdx.x])
+            limit = max(limit, pages_of[i]);
+    }
+    if (int(threadIdx.x) < rows)
+        limit_of[threadIdx.x] = limit;
+    __syncthreads();
+    if (j_from >= most)
+        return;
+
+    uint4 bound[2][KC];
+    float scale[2];
+    bool there[2];
+    int held = -1, held_j = -1; /* whose bounds these are */
+    auto hold = [&](int i, int j0) {
+        const int s = sequence_of[i], to = limit_of[i];
+        held = s;
+        held_j = j0;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int j = j0 + g + 8 * h;
+            const int page = j < to ? lookup(p, s, j) : -1;
+            there[h] = page >= 0;
+            const int64_t at = int64_t(page) * p.kv_heads + head;
+            const uint4 *b = reinterpret_cast<const uint4 *>(p.bounds + at * 2 * D);
+            scale[h] = there[h] ? p.bound_scales[at] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+                bound[h][c] = there[h] && c * 4 + t < D / 8 ? b[c * 4 + t] : make_uint4(0, 0, 0, 0);
+        }
+    };
+    hold(0, j_from + warp * kPages);
 
     for (int gq = 0; gq < p.group; gq += kHeads) {
         const int heads = min(kHeads, p.group - gq);
         if (gq > 0)
             __syncthreads();
-        for (int i = 0; i < rows; i++)
-            quantise_queries<R>(a, row0 + i, head * p.group + gq, heads, kWidth, kPitch,
-                                queries + i * kHeads * kPitch, units[i]);
-        __syncthreads();
-        for (int j0 = j_from + warp * kPages; j0 < j_to; j0 += kWarps * kPages) {
-            uint4 bound[2][KC];
-            float scale[2] = {0.0f, 0.0f};
-            bool there[2] = {false, false};
-            int held = -1; /* whose bounds these are */
-            for (int i = 0; i < rows; i++) {
-                int length;
-                const int s = row_span(p, a.row_sequence, a.row_length, row0 + i, length);
-                const int pages = (length + p.page_size - 1) / p.page_size;
-                if (j0 >= pages)
-                    continue;
-                if (s != held) {
-                    held = s;
-                    const int known = (checked_length(p, p.lengths[s]) + p.page_size - 1) / p.page_size;
+        /* queries in 8 bits, a warp for each (row, head): [max(x, 0) |
+         * min(x, 0)], and their units; what lies behind meets zeros */
+        const int pairs = rows * heads;
+        for (int b = warp; b < pairs; b += kWarps * kBatch) {
+            float v[kBatch][KC]; /* KC * 64 bytes are KC * 32 dims */
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int j = j0 + g + 8 * h;
-                        /* all of the sequence: the next rows may see more of it */
-                        const int page = j < max(known, pages) && j < p.max_pages ? checked_page(p, s, j) : -1;
-                        there[h] = page >= 0;
-                        const int64_t at = int64_t(page) * p.kv_heads + head;
-                        const uint4 *b = reinterpret_cast<const uint4 *>(p.bounds + at * 2 * D);
-                        scale[h] = there[h] ? p.bound_scales[at] : 0.0f;
+            for (int i = 0; i < kBatch; i++) {
+                const int pair = b + i * kWarps, row = pair / heads, h = pair - row * heads;
+                const R *q = static_cast<const R *>(a.q) + int64_t(row0 + row) * a.q_stride +
+                             int64_t(head * p.group + gq + h) * D;
 #pragma unroll
-                        for (int c = 0; c < KC; c++)
-                            bound[h][c] = there[h] && c * 4 + t < D / 8 ? __ldg(b + c * 4 + t) : make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < KC; c++) {
+                    const int d = lane + 32 * c;
+                    v[i][c] = pair < pairs && d < D ? finite_key(to_float(q[d])) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                const int pair = b + i * kWarps, row = pair / heads, h = pair - row * heads;
+                if (pair >= pairs)
+                    break;
+                float top = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+                    top = fmaxf(top, fabsf(v[i][c]));
+                const float u = unit_of(warp_max(top)), inv = u > 0.0f ? 1.0f / u : 0.0f; /* exact */
+                int8_t *out = queries + (row * kHeads + h) * kPitch;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    const int d = lane + 32 * c;
+                    if (d < D) {
+                        const int x = int(rintf(v[i][c] * inv));
+                        out[d] = int8_t(max(x, 0));
+                        out[D + d] = int8_t(min(x, 0));
                     }
                 }
+                if (lane == 0)
+                    units[row][h] = u;
+            }
+        }
+        __syncthreads();
+        for (int j0 = j_from + warp * kPages; j0 < min(j_to, most); j0 += kWarps * kPages) {
+            for (int i = 0; i < rows; i++) {
+                const int s = sequence_of[i], pages = pages_of[i];
+                if (j0 >= pages)
+                    continue;
+                if (s != held || j0 != held_j)
+                    hold(i, j0);
                 int acc[4] = {0, 0, 0, 0};
                 const int8_t *x = queries + (i * kHeads + g) * kPitch + t * 16;
 #pragma unroll
@@ -137,6 +165,8 @@ __global__ void __launch_bounds__(kWarps * 32)
                             v = fmaxf(v, *to);
                         if (j < a.sink_pages || j >= pages - a.recent_pages)
                             v = INFINITY;
+                        else if (!there[h])
+                            paged_fail(p, kPagedBadPage);
                         *to = v;
                     }
                 }
@@ -162,6 +192,7 @@ __global__ void __launch_bounds__(kChooseThreads)
     const PagedPool &p = a.p;
     const int head = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     int length;
+    begin_kernel();
     row_span(p, a.row_sequence, a.row_length, r, length);
     const int pages = (length + p.page_size - 1) / p.page_size;
     const int64_t at = int64_t(r) * p.kv_heads + head;
@@ -214,6 +245,7 @@ __global__ void __launch_bounds__(kFewThreads)
     const PagedPool &p = a.p;
     const int head = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int length;
+    begin_kernel();
     row_span(p, a.row_sequence, a.row_length, r, length);
     const int pages = (length + p.page_size - 1) / p.page_size, want = min(a.n_selected, pages);
     const int64_t at = int64_t(r) * p.kv_heads + head;
@@ -262,12 +294,17 @@ __global__ void __launch_bounds__(kFewThreads)
 template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     /* rows that may share a sequence share its bounds in registers */
-    const int rows_each = a.row_sequence ? kMostRows : 1, pages_each = kWarps * kPages;
+    const int rows_each = a.row_sequence ? kMostRows : 1;
     const int bytes = rows_each * kHeads * (KC * 64 + 64);
-    const dim3 grid((p.max_pages + pages_each - 1) / pages_each, p.kv_heads,
-                    (a.rows + rows_each - 1) / rows_each);
-    score_kernel<R, KC><<<grid, kWarps * 32, bytes, s>>>(a, rows_each, pages_each);
-    return cudaGetLastError();
+    /* a block's queries are made once for all of its pages: as many of them
+     * as still leave two blocks for each SM (36 against 51 us with 128) */
+    int pages_each = kWarps * kPages * 4;
+    const int row_blocks = (a.rows + rows_each - 1) / rows_each;
+    const auto chunks = [&] { return (p.max_pages + pages_each - 1) / pages_each; };
+    while (pages_each > kWarps * kPages && int64_t(chunks()) * p.kv_heads * row_blocks < 2 * kMaxSms)
+        pages_each /= 2;
+    return launch_kernel(score_kernel<R, KC>, dim3(chunks(), p.kv_heads, row_blocks), kWarps * 32, bytes, s, 1, a,
+                         rows_each, pages_each);
 }
 
 template <typename R> cudaError_t scores(const PagedSelect &a, cudaStream_t s) {
@@ -290,13 +327,10 @@ cudaError_t paged_select(const PagedSelect &a, cudaStream_t s) {
         return e;
     const dim3 items(p.kv_heads, a.rows);
     if (p.max_pages <= 4 * kFewThreads)
-        choose_few_pages_kernel<4><<<items, kFewThreads, 0, s>>>(a);
-    else if (p.max_pages <= 8 * kFewThreads)
-        choose_few_pages_kernel<8><<<items, kFewThreads, 0, s>>>(a);
-    else
-        choose_pages_kernel<<<items, kChooseThreads, 0, s>>>(a);
-    count_launches(2);
-    return cudaGetLastError();
+        return launch_kernel(choose_few_pages_kernel<4>, items, kFewThreads, 0, s, 1, a);
+    if (p.max_pages <= 8 * kFewThreads)
+        return launch_kernel(choose_few_pages_kernel<8>, items, kFewThreads, 0, s, 1, a);
+    return launch_kernel(choose_pages_kernel, items, kChooseThreads, 0, s, 1, a);
 }
 
 } // namespace nut

@@ -528,6 +528,66 @@ def test_calls_follow_their_stream_and_replay_in_graphs(gpu):
         check_attention(torch, pool, q, out, lse, list(enumerate(lens)), 1 / 8, "f32", chosen.cpu().numpy())
 
 
+@pytest.mark.gpu
+def test_replays_read_what_has_changed_since(gpu):
+    """A whole step as a graph, replayed while every input it reads is rewritten in place, and the same without a graph: each
+    kernel starts while the one before it runs, and must not meet stale values."""
+    import torch
+    H, KV, D, ps, S, n = 8, 2, 64, 16, 3, 4
+    pool = Pool(torch, [150, 60, 33], H, KV, D, ps, "f16", bounds=True, track=True, max_pages=20, spare=40)
+    pool.cache.summarise()
+    side = torch.cuda.Stream()
+    dev = dict(device="cuda")
+    k, v, q = torch.zeros(S, KV, D, **dev), torch.zeros(S, KV, D, **dev), torch.zeros(S, H, D, **dev)
+    starts = torch.arange(S + 1, dtype=torch.int32, **dev)
+    cos, sin = torch.zeros(400, D // 2, **dev), torch.zeros(400, D // 2, **dev)
+    turned, out, sparse = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    chosen = torch.zeros(S, KV, n, dtype=torch.int32, **dev)
+    w, w_out = torch.zeros(S, KV, pool.capacity, **dev), torch.zeros(S, KV, pool.capacity, **dev)
+    c = pool.cache
+
+    def step(stream, wait):
+        def then(f, *a, **kw):
+            f(*a, **kw)
+            if wait:
+                torch.cuda.synchronize()
+        then(c.append, q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), S, 1, cos=cos.data_ptr(), sin=sin.data_ptr(),
+             rope_rows=400, q_out=turned.data_ptr(), stream=stream)
+        then(c.attention, turned.data_ptr(), out.data_ptr(), S, weights=w.data_ptr(), weights_out=w_out.data_ptr(), stream=stream)
+        then(c.select, turned.data_ptr(), chosen.data_ptr(), S, n, stream=stream)
+        then(c.attention, turned.data_ptr(), sparse.data_ptr(), S, selected=chosen.data_ptr(), n_selected=n, stream=stream)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(side.cuda_stream, False)
+    results = (turned, out, sparse, chosen, w_out, pool.bounds, pool.scales)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for i in range(12):
+        # new values in the same places; the table is shuffled and the lengths move on
+        for x in (k, v, q, cos, sin, w):
+            x.copy_(torch.randn(x.shape, generator=g, **dev))
+        pool.keys.copy_(torch.randn(pool.keys.shape, generator=g, **dev))
+        pool.values.copy_(torch.randn(pool.values.shape, generator=g, **dev))
+        pool.table[:, :10] = torch.randperm(pool.n_pages, generator=g, **dev)[:30].int().reshape(3, 10)
+        pool.lengths.copy_(torch.tensor([150 + i % 5, 61 - 7 * (i % 3), 33 + i], dtype=torch.int32))
+        torch.cuda.synchronize()
+        before = [x.clone() for x in (pool.keys, pool.values)]
+        got = []
+        for way in ("apart", "together", "graph"):
+            pool.keys.copy_(before[0])
+            pool.values.copy_(before[1])
+            if way == "graph":
+                graph.replay()
+            else:
+                step(torch.cuda.current_stream().cuda_stream, way == "apart")
+            torch.cuda.synchronize()
+            got.append([x.clone() for x in results])
+        pool.cache.check()
+        for way in (1, 2):
+            assert all(torch.equal(a, b) for a, b in zip(got[0], got[way])), (i, way)
+
+
 # ---------------------------------------------------------------------------
 # selection
 
