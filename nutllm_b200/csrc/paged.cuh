@@ -11,13 +11,12 @@
 
 namespace nut {
 
-/* The paged kernels are launched while the kernel before them in the stream
- * still runs: what it wrote may be read, and its buffers written, after
- * begin_kernel(), which also lets the next one be launched. */
-__device__ __forceinline__ void begin_kernel() {
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-}
+/* The paged kernels are set up while the kernel before them in the stream
+ * drains: what that one wrote may be read, and its buffers written, after
+ * begin_kernel().  (None lets the next one in earlier than its own last
+ * block: waiting blocks of the attention would crowd the kernel they wait for,
+ * 97 against 82 us for a sparse step of 32 sequences.) */
+__device__ __forceinline__ void begin_kernel() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 template <typename... Params, typename... Args>
 cudaError_t launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t bytes, cudaStream_t stream,

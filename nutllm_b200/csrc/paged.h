@@ -43,9 +43,16 @@ struct PagedAppend {
 };
 
 struct PagedAttention {
-    CUtensorMap key_map, value_map; /* (dim, slot, kv head, page), boxes of 128 bytes x `box` slots */
+    /* (dim, slot, 128-byte column, kv head, page), in boxes of 16 slots by all
+     * columns; where page_size is no multiple of 16 or head_dim none of a
+     * column there is but one column, head_dim wide, and boxes are 128 bytes
+     * of `box` slots */
+    CUtensorMap key_map, value_map;
     PagedPool p;
     int box; /* the greatest power of two up to 16 that divides page_size */
+    int whole_columns;
+    uint64_t page_magic; /* v / page_size = v * magic >> shift for v < 2^31 */
+    int page_shift;
     const void *q;
     void *out;
     int64_t q_stride, out_stride;
@@ -91,6 +98,11 @@ struct PagedEvict {
     int32_t *pairs;  /* [sequences][kv_heads][capacity]: holes, then sources from the far end */
     int32_t *counts; /* [sequences][kv_heads][2]: pairs, old length */
 };
+
+/* 128-byte columns of a row as the attention lays it out in shared memory. */
+inline int paged_columns(int type, int D) {
+    return type == 0 ? (D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8) : (D <= 64 ? 1 : D <= 128 ? 2 : D <= 192 ? 3 : 4);
+}
 
 cudaError_t paged_append(const PagedAppend &a, cudaStream_t s);
 cudaError_t paged_summarise(const PagedPool &p, cudaStream_t s);

@@ -32,13 +32,13 @@ constexpr float kSlack = 8.0f; /* log2 by which a logit may pass the maximum in 
 constexpr uint64_t kPagedWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-/* One box of the pool to shared memory: columns x .. x + 128 bytes, the map's
- * rows from slot y, of kv head h and page w; arrives on `bar`. */
-__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, int x, int y, int h, int w,
+/* One box of the pool to shared memory: from column x of 128-byte column b,
+ * the map's slots from y, kv head h, page w; arrives on `bar`. */
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, int x, int y, int b, int h, int w,
                                          uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-                 "[%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(to),
-                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(h), "r"(w)
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::"r"(to),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(b), "r"(h), "r"(w)
                  : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
@@ -761,47 +761,37 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     Item in, x;
     bool more = feed.next(a, items_per_row, kTile, in);
 
-    /* lane i < boxes: where box i of this warp's chunk of in.tile lies, and how
-     * many of its slots count */
-    int next_page = 0, next_slot = 0, next_count = 0;
-    auto locate = [&] {
-        const int v = in.tile * kTile + warp * kChunk + lane * box;
-        next_count = 0;
-        if (!more || lane >= boxes || v >= in.span)
-            return;
-        int j = v / p.page_size;
-        next_slot = v - j * p.page_size;
-        if (a.selected) {
-            j = a.selected[(int64_t(in.row) * p.kv_heads + in.index / groups) * a.n_selected + j];
-            if (j < 0 || j >= p.max_pages || j * p.page_size + next_slot >= in.length)
-                return;
-        }
-        next_page = checked_page(p, in.sequence, j);
-        if (next_page >= 0)
-            next_count = min(box, in.length - j * p.page_size - next_slot);
+    /* Where this warp's chunks of the next 32 / boxes tiles of an item lie, a
+     * box a lane (box i of chunk k in lane k boxes + i), and how many of a
+     * box's slots count.  One look-up, two round trips long, serves that many
+     * chunks, and is made that many ahead. */
+    struct Batch {
+        int page, slot, count, tiles, head;
     };
-    auto issue = [&](int stage) {
-        const uint32_t to = ring_at + stage * Op::kStageBytes + lane * box * 128;
-        const bool mine = next_count > 0 && !dead;
-        const uint32_t valid =
-            __reduce_or_sync(0xffffffffu, mine ? ((1u << next_count) - 1u) << (lane * box) : 0u);
-        const int n = __popc(__ballot_sync(0xffffffffu, mine));
-        uint64_t *bar = &full[warp][stage];
-        if (lane == 0) {
-            masks[warp][stage] = valid;
-            if (n > 0)
-                mbar_expect_tx(bar, n * box * 128 * 2 * Op::kBlocks);
-        }
-        __syncwarp();
-        const int head = in.index / groups;
-        if (mine)
-#pragma unroll
-            for (int b = 0; b < Op::kBlocks; b++) {
-                copy_box(to + b * kBlock, &a.key_map, b * kBoxWidth, next_slot, head, next_page, smem_u32(bar));
-                copy_box(to + (Op::kBlocks + b) * kBlock, &a.value_map, b * kBoxWidth, next_slot, head, next_page,
-                         smem_u32(bar));
+    const int my_chunk = lane / boxes, my_box = lane - my_chunk * boxes;
+    auto plan = [&](Batch &b) {
+        b.count = b.tiles = 0;
+        if (!more)
+            return;
+        const int v = (in.tile + my_chunk) * kTile + warp * kChunk + my_box * box;
+        b.tiles = min(32 / boxes, in.tile1 - in.tile);
+        b.head = in.index / groups;
+        if (my_chunk < b.tiles && v < in.span) {
+            int j = int((uint64_t(unsigned(v)) * a.page_magic) >> a.page_shift);
+            b.slot = v - j * p.page_size;
+            bool there = true;
+            if (a.selected) {
+                j = a.selected[(int64_t(in.row) * p.kv_heads + b.head) * a.n_selected + j];
+                there = j >= 0 && j < p.max_pages && j * p.page_size + b.slot < in.length;
             }
-        if (more && ++in.tile == in.tile1) {
+            if (there) {
+                b.page = checked_page(p, in.sequence, j);
+                if (b.page >= 0)
+                    b.count = min(box, in.length - j * p.page_size - b.slot);
+            }
+        }
+        in.tile += b.tiles;
+        if (in.tile == in.tile1) {
             more = feed.next(a, items_per_row, kTile, in);
             if (more && warp == 0) { /* its queries, on their way to L2 */
                 const char *q = reinterpret_cast<const char *>(
@@ -811,10 +801,52 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
                     asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + lane * 128));
             }
         }
-        locate();
+    };
+    Batch now{}, then{};
+    int used = 0; /* chunks of `now` that have been issued */
+    auto issue = [&](int stage) {
+        if (used == now.tiles) {
+            now = then;
+            used = 0;
+            plan(then);
+        }
+        const uint32_t to = ring_at + stage * Op::kStageBytes + my_box * box * 128;
+        const bool mine = now.count > 0 && my_chunk == used && !dead;
+        const uint32_t valid = __reduce_or_sync(0xffffffffu, mine ? ((1u << now.count) - 1u) << (my_box * box) : 0u);
+        const uint32_t bar = smem_u32(&full[warp][stage]);
+        if (boxes > 1) {
+            const int n = __popc(__ballot_sync(0xffffffffu, mine));
+            if (lane == 0) {
+                masks[warp][stage] = valid;
+                if (n > 0)
+                    mbar_expect_tx(&full[warp][stage], n * box * 128 * 2 * Op::kBlocks);
+            }
+            __syncwarp();
+        } else {
+            if (lane == 0)
+                masks[warp][stage] = valid;
+            if (mine)
+                mbar_expect_tx(&full[warp][stage], Op::kStageBytes);
+        }
+        if (mine) {
+            if (a.whole_columns) {
+                copy_box(to, &a.key_map, 0, now.slot, 0, now.head, now.page, bar);
+                copy_box(to + Op::kBlocks * kBlock, &a.value_map, 0, now.slot, 0, now.head, now.page, bar);
+            } else {
+#pragma unroll
+                for (int b = 0; b < Op::kBlocks; b++) {
+                    copy_box(to + b * kBlock, &a.key_map, b * kBoxWidth, now.slot, 0, now.head, now.page, bar);
+                    copy_box(to + (Op::kBlocks + b) * kBlock, &a.value_map, b * kBoxWidth, now.slot, 0, now.head,
+                             now.page, bar);
+                }
+            }
+        }
+        if (used < now.tiles)
+            used++;
     };
 
-    locate();
+    plan(now);
+    plan(then);
     for (int i = 0; i < kStages - 1; i++)
         issue(i);
     /* rows that see nothing */

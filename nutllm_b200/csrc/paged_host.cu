@@ -111,9 +111,9 @@ using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                  CUtensorMapFloatOOBfill);
 
-/* The pool as (dim, slot, kv head, page), read in boxes of 128 bytes by
- * `box` slots; dims behind head_dim read as zeros. */
-CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box) {
+/* The pool as the attention's tensor map (PagedAttention::key_map); dims
+ * behind head_dim read as zeros. */
+CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box, bool whole) {
     static const EncodeTiled encode = [] {
         void *f = nullptr;
         cudaDriverEntryPointQueryResult q{};
@@ -128,13 +128,17 @@ CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box) {
     const CUtensorMapDataType type = p.type == NUT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : p.type == NUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.page_size), cuuint64_t(p.kv_heads),
+    const int width = int(128 / size);
+    const cuuint64_t dims[5] = {cuuint64_t(whole ? width : p.head_dim), cuuint64_t(p.page_size),
+                                cuuint64_t(whole ? p.head_dim / width : 1), cuuint64_t(p.kv_heads),
                                 cuuint64_t(p.n_pages)};
-    const cuuint64_t strides[3] = {cuuint64_t(p.slot_stride) * size, cuuint64_t(p.head_stride) * size,
+    const cuuint64_t strides[4] = {cuuint64_t(p.slot_stride) * size, 128, cuuint64_t(p.head_stride) * size,
                                    cuuint64_t(p.page_stride) * size};
-    const cuuint32_t boxes[4] = {cuuint32_t(128 / size), cuuint32_t(box), 1, 1}, steps[4] = {1, 1, 1, 1};
+    const cuuint32_t columns = cuuint32_t(nut::paged_columns(p.type, p.head_dim));
+    const cuuint32_t boxes[5] = {cuuint32_t(width), cuuint32_t(box), whole ? columns : 1, 1, 1};
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     CUtensorMap map;
-    if (encode(&map, type, 4, base, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    if (encode(&map, type, 5, base, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         raise(NUT_INVALID_ARGUMENT, "the pool's strides cannot be mapped");
@@ -157,6 +161,9 @@ struct nut_paged {
     nut::PagedPool pool{};
     CUtensorMap key_map{}, value_map{};
     int box = 16;
+    bool whole_columns = false;
+    uint64_t page_magic = 0;
+    int page_shift = 32;
     int max_rows = 0;
     bool track = false;
     int sms = 0;
@@ -228,8 +235,13 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         h->sms = std::min(h->sms, nut::kMaxSms);
         while (p.page_size % h->box != 0)
             h->box /= 2;
-        h->key_map = pool_map(p, p.keys, h->box);
-        h->value_map = pool_map(p, p.values, h->box);
+        /* ceil(2^(32 + s) / page_size) with 2^s < page_size <= 2^(s + 1): exact below 2^31 */
+        while ((int64_t(1) << (h->page_shift - 31)) < p.page_size)
+            h->page_shift++;
+        h->page_magic = ((uint64_t(1) << h->page_shift) + p.page_size - 1) / p.page_size;
+        h->whole_columns = h->box == 16 && p.head_dim % (p.type == NUT_F32 ? 32 : 64) == 0;
+        h->key_map = pool_map(p, p.keys, h->box, h->whole_columns);
+        h->value_map = pool_map(p, p.values, h->box, h->whole_columns);
         const size_t items = size_t(p.sequences) * p.kv_heads;
         size_t bytes = 0;
         const auto part = [&](size_t count, size_t size) {
@@ -411,6 +423,9 @@ nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *arg
         a.key_map = h->key_map;
         a.value_map = h->value_map;
         a.box = h->box;
+        a.whole_columns = h->whole_columns;
+        a.page_shift = h->page_shift;
+        a.page_magic = h->page_magic;
         DeviceScope scope(h->device);
         cuda_check(nut::paged_attention(a, static_cast<cudaStream_t>(stream)), "paged attention");
     });
