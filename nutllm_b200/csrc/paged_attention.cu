@@ -42,6 +42,7 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, in
                  : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;\n" ::: "memory"); }
 
 /* Waits for a stage without sleeping; false after kPagedWaitNs. */
 __device__ __forceinline__ bool stage_wait(uint64_t *bar, uint32_t parity) {
@@ -527,7 +528,8 @@ template <typename Op> struct Plan {
     static constexpr int kBytes = kWarps * (kRing + kScratchBytes) + 2 * kOutputBytes + 1024; /* to align */
     static constexpr int kFit = 228 * 1024 / (kBytes + 2048);
     static constexpr int kPerSm = kFit < Op::kMaxPerSm ? (kFit > 1 ? kFit : 1) : Op::kMaxPerSm;
-    static_assert(kWarps * kRing >= kMaxSms * kPerSm * kRows * 4, "an item's parts have their factors there");
+    static_assert(kWarps * kRing >= kMaxSms * kPerSm * kRows * 4 + 128 + kOutputBytes,
+                  "the factors of an item's parts and one part fit there");
 };
 
 /* Slots of a row that the kernel walks: its length, or the listed pages. */
@@ -543,64 +545,49 @@ template <typename R> __device__ __forceinline__ void store4(R *to, float4 v) {
 }
 
 /* Joins the `parts` parts of an item left by CTAs c0, c0 + 1, ...; run by
- * the whole CTA that arrived last.  Warps first turn the parts' maxima and
- * sums into one factor exp(m_c - m) / l per part and head, in shared memory;
- * then a thread adds 4 dims of the parts' outputs with many loads in flight
- * (one after another, 37 parts cost 200 us; this way 6). */
-template <typename R, int kWarps>
-__device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, int c0, int parts, int r, int first_head,
-                           int heads, float *factor) {
+ * the whole CTA that arrived last.  Bulk copies bring the parts to shared
+ * memory while the warps turn their maxima and sums into one factor
+ * exp(m_c - m) / l per part and head.  (Read by one load after another, 37
+ * parts cost 200 us; with sixteen in flight a thread, 7.)  */
+template <typename R, int DP, int kWarps>
+__device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, int c0, int parts, int r,
+                                        int first_head, int heads, char *space, int bytes, uint64_t *bar,
+                                        uint32_t &phase) {
     const PagedPool &p = a.p;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     /* an item that starts inside its first CTA's share lies in that one's second slot */
     const float *first = a.partial + (int64_t(c0) * 2 + (inside ? 1 : 0)) * kPartialFloats;
     const float *rest = a.partial + (int64_t(c0) * 2 + 2) * kPartialFloats;
     auto part = [&](int c) { return c == 0 ? first : rest + int64_t(c - 1) * 2 * kPartialFloats; };
-    /* outputs of the first parts are on their way while the factors are made */
-    constexpr int kFlight = 16;
-    const int quads = p.head_dim / 4;
-    float4 x[kFlight];
-    auto fetch = [&](int i, int c0) {
-        const int at = 2 * kRows + i / quads * kMaxDim + i % quads * 4;
-#pragma unroll
-        for (int k = 0; k < kFlight; k++)
-            x[k] = c0 + k < parts ? __ldcg(reinterpret_cast<const float4 *>(part(c0 + k) + at))
-                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float *factor = reinterpret_cast<float *>(space);
+    const int head_room = (parts * kRows * 4 + 127) / 128 * 128;
+    const int size = heads * DP * 4; /* of a part's outputs */
+    const int most = (bytes - head_room) / size;
+    float *copies = reinterpret_cast<float *>(space + head_room);
+    auto fetch = [&](int c, int n) { /* by warp 0 */
+        fence_proxy_async(); /* others' stores, seen by this thread, before its copies */
+        if (lane == 0)
+            mbar_expect_tx(bar, n * size);
+        __syncwarp();
+        for (int k = lane; k < n; k += 32)
+            bulk_g2s(copies + k * (size / 4), part(c + k) + 2 * kRows, size, bar);
     };
-    if (threadIdx.x < heads * quads)
-        fetch(threadIdx.x, 0);
+    if (warp == 0)
+        fetch(0, min(parts, most));
     for (int g = warp; g < heads; g += kWarps) {
-        /* the first 64 parts' statistics in registers, both loads together */
-        float m0[2], l0[2], top = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int c = lane + 32 * k;
-            m0[k] = c < parts ? __ldcg(part(c) + g) : -INFINITY;
-            l0[k] = c < parts ? __ldcg(part(c) + kRows + g) : 0.0f;
-            top = fmaxf(top, m0[k]);
-        }
-        for (int c = lane + 64; c < parts; c += 32)
+        float top = -INFINITY, sum = 0.0f;
+        for (int c = lane; c < parts; c += 32)
             top = fmaxf(top, __ldcg(part(c) + g));
         top = warp_max(top);
         const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            m0[k] = exp2f(m0[k] - base);
-            sum = l0[k] != 0.0f ? fmaf(l0[k], m0[k], sum) : sum;
-        }
-        for (int c = lane + 64; c < parts; c += 32) {
+        for (int c = lane; c < parts; c += 32) {
             const float f = exp2f(__ldcg(part(c) + g) - base), l = __ldcg(part(c) + kRows + g);
             factor[c * kRows + g] = f;
             sum = l != 0.0f ? fmaf(l, f, sum) : sum;
         }
         sum = warp_sum(sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (lane + 32 * k < parts)
-                factor[(lane + 32 * k) * kRows + g] = m0[k] * inv;
-        for (int c = lane + 64; c < parts; c += 32)
+        for (int c = lane; c < parts; c += 32)
             factor[c * kRows + g] *= inv;
         if (lane == 0) {
             const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
@@ -611,23 +598,38 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * quads; i += kWarps * 32) {
-        const int g = i / quads;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 0; c < parts; c += kFlight) {
-            if (c > 0 || i >= kWarps * 32)
-                fetch(i, c);
+    constexpr int kQuads = (kRows * DP / 4 + kWarps * 32 - 1) / (kWarps * 32); /* 4-dim pieces a thread may have */
+    float4 o[kQuads];
 #pragma unroll
-            for (int k = 0; k < kFlight; k++) {
-                const float f = c + k < parts ? factor[(c + k) * kRows + g] : 0.0f;
-                o.x = fmaf(x[k].x, f, o.x);
-                o.y = fmaf(x[k].y, f, o.y);
-                o.z = fmaf(x[k].z, f, o.z);
-                o.w = fmaf(x[k].w, f, o.w);
-            }
+    for (int q = 0; q < kQuads; q++)
+        o[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = 0; c < parts; c += most) {
+        const int n = min(parts - c, most);
+        if (!stage_wait(bar, phase))
+            paged_fail(p, kPagedTimeout);
+        phase ^= 1;
+#pragma unroll
+        for (int q = 0; q < kQuads; q++) {
+            const int i = (q * kWarps * 32 + tid) * 4, g = i / DP;
+            if (g < heads)
+                for (int k = 0; k < n; k++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(copies + k * (size / 4) + i);
+                    const float f = factor[(c + k) * kRows + g];
+                    o[q].x = fmaf(x.x, f, o[q].x);
+                    o[q].y = fmaf(x.y, f, o[q].y);
+                    o[q].z = fmaf(x.z, f, o[q].z);
+                    o[q].w = fmaf(x.w, f, o[q].w);
+                }
         }
-        store4<R>(static_cast<R *>(a.out) + r * a.out_stride + int64_t(first_head + g) * p.head_dim +
-                      i % quads * 4, o);
+        __syncthreads();
+        if (warp == 0 && c + n < parts)
+            fetch(c + n, min(parts - c - n, most));
+    }
+#pragma unroll
+    for (int q = 0; q < kQuads; q++) {
+        const int i = (q * kWarps * 32 + tid) * 4, g = i / DP, d = i % DP;
+        if (g < heads && d < p.head_dim)
+            store4<R>(static_cast<R *>(a.out) + r * a.out_stride + int64_t(first_head + g) * p.head_dim + d, o[q]);
     }
 }
 
@@ -639,12 +641,12 @@ __device__ __forceinline__ int line_of(int tiles) { return tiles == 0 ? 0 : tile
 struct Item {
     int row, sequence, length, span, tiles, index; /* index within the row */
     int tile, tile0, tile1;
-    int64_t first; /* where its first tile lies on the line */
+    int first; /* where its first tile lies on the line */
 };
 
 /* Walks the items of a share. */
 struct Cursor {
-    int64_t pos, last, in_row; /* place on the line, end, place within the row's items */
+    int pos, last, in_row; /* place on the line, end, place within the row's items */
     int r;
 
     __device__ __forceinline__ bool next(const PagedAttention &a, int items_per_row, int tile_slots, Item &x) {
@@ -657,16 +659,16 @@ struct Cursor {
                 continue;
             }
             const int len = line_of(x.tiles);
-            x.index = int(in_row / len);
-            const int place = int(in_row - int64_t(x.index) * len);
-            const int taken = int(min(int64_t(len - place), last - pos));
+            x.index = in_row / len;
+            const int place = in_row - x.index * len;
+            const int taken = min(len - place, last - pos);
             x.row = r;
             x.tile = x.tile0 = max(place - kItemCost, 0);
             x.tile1 = place + taken - kItemCost;
             x.first = pos - place + kItemCost;
             pos += taken;
             in_row += taken;
-            if (in_row >= int64_t(len) * items_per_row) {
+            if (in_row >= len * items_per_row) {
                 in_row = 0;
                 r++;
             }
@@ -677,6 +679,13 @@ struct Cursor {
     }
 };
 
+/* Places of one of row r's items. */
+__device__ __noinline__ int places_of(const PagedAttention &a, int r, int tile_slots) {
+    int length;
+    row_span(a.p, a.row_sequence, a.row_length, r, length);
+    return line_of((walked(a, length) + tile_slots - 1) / tile_slots);
+}
+
 template <typename Op, typename R>
 __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     attention_kernel(const __grid_constant__ PagedAttention a) {
@@ -686,10 +695,9 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     extern __shared__ char smem_raw[];
     char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint32_t masks[kWarps][kStages];
-    __shared__ uint64_t full[kWarps][kStages];
+    __shared__ uint64_t full[kWarps][kStages], joined;
     __shared__ float maxima[2][kWarps][kRows], sums[2][kWarps][kRows], factors[kWarps][kRows];
-    __shared__ int64_t warp_sum64[kWarps], found_place;
-    __shared__ int found_row, arrived_last[2];
+    __shared__ int warp_sums[kWarps], found_row, found_place, arrived_last[2];
     __shared__ Item shared[2]; /* items that other CTAs have parts of: the first and the last at most */
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -698,6 +706,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     if (tid == 0) {
         for (int i = 0; i < kWarps * kStages; i++)
             mbar_init(&full[0][0] + i, 1);
+        mbar_init(&joined, 1);
         fence_barrier_init();
     }
     begin_kernel();
@@ -705,36 +714,32 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     /* this CTA's share of the line of tiles: thread i sums a run of rows */
     const int run = (a.rows + kThreads - 1) / kThreads;
     const int r0 = min(tid * run, a.rows), r1 = min(r0 + run, a.rows);
-    int64_t mine = 0;
-    for (int r = r0; r < r1; r++) {
-        int length;
-        row_span(p, a.row_sequence, a.row_length, r, length);
-        mine += line_of((walked(a, length) + kTile - 1) / kTile);
-    }
-    int64_t upto = mine;
+    int mine = 0;
+#pragma unroll 1
+    for (int r = r0; r < r1; r++)
+        mine += places_of(a, r, kTile);
+    int upto = mine;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, x);
+        const int v = __shfl_up_sync(0xffffffffu, upto, x);
         upto += lane >= x ? v : 0;
     }
     if (lane == 31)
-        warp_sum64[warp] = upto;
+        warp_sums[warp] = upto;
     __syncthreads();
-    int64_t total = 0;
+    int total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
-        upto += w < warp ? warp_sum64[w] : 0;
-        total += warp_sum64[w];
+        upto += w < warp ? warp_sums[w] : 0;
+        total += warp_sums[w];
     }
     total *= items_per_row;
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x, start = int64_t(blockIdx.x) * share;
-    const int64_t before = upto - mine;
-    if (start < total && start >= before * items_per_row && start < upto * items_per_row) {
-        int64_t at = before * items_per_row;
+    const int share = (total + int(gridDim.x) - 1) / int(gridDim.x), start = int(blockIdx.x) * share;
+    int at = (upto - mine) * items_per_row;
+    if (start < total && start >= at && start < upto * items_per_row)
+#pragma unroll 1
         for (int r = r0; r < r1; r++) {
-            int length;
-            row_span(p, a.row_sequence, a.row_length, r, length);
-            const int64_t n = int64_t(line_of((walked(a, length) + kTile - 1) / kTile)) * items_per_row;
+            const int n = run == 1 ? mine * items_per_row : places_of(a, r, kTile) * items_per_row;
             if (start < at + n) {
                 found_row = r;
                 found_place = start - at;
@@ -742,7 +747,6 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
             }
             at += n;
         }
-    }
     __syncthreads();
 
     char *ring = smem + warp * Plan<Op>::kRing;
@@ -953,7 +957,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
             const float4 v = *reinterpret_cast<const float4 *>(outputs + (kRows + g) * DP + d);
             const float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
             if (!whole)
-                *reinterpret_cast<float4 *>(part + 2 * kRows + g * kMaxDim + d) = o;
+                *reinterpret_cast<float4 *>(part + 2 * kRows + g * DP + d) = o;
             else if (d < D)
                 store4<R>(static_cast<R *>(a.out) + x.row * a.out_stride + int64_t(first_head + g) * D + d, o);
         }
@@ -972,7 +976,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     if (tid < parts) {
         const Item &y = shared[tid];
         int *counter = a.counters + int64_t(y.row) * items_per_row + y.index, before_me;
-        const int others = int((y.first + y.tiles - 1) / share - y.first / share);
+        const int others = (y.first + y.tiles - 1) / share - y.first / share;
         /* releases the block's parts (ordered before by the barrier) and
          * acquires the others' */
         asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;\n" : "=r"(before_me) : "l"(counter) : "memory");
@@ -981,34 +985,64 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
             *counter = 0;
     }
     __syncthreads();
+    uint32_t join_phase = 0;
     for (int i = 0; i < parts; i++)
         if (arrived_last[i]) {
             const Item &y = shared[i];
-            const int64_t c0 = y.first / share, c1 = (y.first + y.tiles - 1) / share;
-            join_parts<R, kWarps>(a, y.first > c0 * share, int(c0), int(c1 - c0) + 1, y.row,
+            const int c0 = y.first / share, c1 = (y.first + y.tiles - 1) / share;
+            join_parts<R, DP, kWarps>(a, y.first > c0 * share, c0, c1 - c0 + 1, y.row,
                                       y.index / groups * p.group + y.index % groups * kRows,
-                                      min(kRows, p.group - y.index % groups * kRows),
-                                      reinterpret_cast<float *>(smem));
+                                      min(kRows, p.group - y.index % groups * kRows), smem, kWarps * Plan<Op>::kRing,
+                                      &joined, join_phase);
             __syncthreads();
         }
 }
 
 /* weights_out[t] = weights[t] + sum over the group of exp(z_t - lse): every
- * slot has one writer, so the order of the sum is fixed. */
-__global__ void __launch_bounds__(256) weights_kernel(const __grid_constant__ PagedAttention a) {
+ * slot has one writer, so the order of the sum is fixed.  Four slots a
+ * thread; kVec: their addresses are multiples of 16 bytes. */
+constexpr int kWeightThreads = 256;
+
+template <bool kVec>
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_constant__ PagedAttention a) {
+    begin_kernel();
     const PagedPool &p = a.p;
     const int head = blockIdx.y, r = blockIdx.z;
     int length;
-    begin_kernel();
     row_span(p, a.row_sequence, a.row_length, r, length);
-    const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity;
+    const int t = (int(blockIdx.x) * kWeightThreads + int(threadIdx.x)) * 4;
+    if (t >= length)
+        return;
+    const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity + t;
     const int64_t h0 = int64_t(r) * p.heads + head * p.group;
-    for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < length; t += gridDim.x * blockDim.x) {
-        float w = 0.0f;
-        for (int g = 0; g < p.group; g++)
-            w += exp2f(a.logits[(h0 + g) * p.capacity + t] - a.lse2[h0 + g]);
-        a.weights_out[to + t] = a.weights[to + t] + w;
+    const float *z = a.logits + h0 * p.capacity + t;
+    const int n = min(4, length - t);
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int g = 0; g < p.group; g++) {
+        const float lse2 = a.lse2[h0 + g];
+        float x[4];
+        if constexpr (kVec) {
+            *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(z + int64_t(g) * p.capacity);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[i] = i < n ? z[int64_t(g) * p.capacity + i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] += exp2f(x[i] - lse2);
     }
+    if (kVec && n == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(a.weights + to);
+        *reinterpret_cast<float4 *>(a.weights_out + to) =
+            make_float4(x.x + w[0], x.y + w[1], x.z + w[2], x.w + w[3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n)
+            a.weights_out[to + i] = a.weights[to + i] + w[i];
 }
 
 template <typename Op, typename R>
@@ -1039,8 +1073,11 @@ cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
     e = launch_kernel(attention_kernel<Op, R>, dim3(unsigned(tiles < ctas ? tiles : ctas)), threads, bytes, s, 1, a);
     if (e != cudaSuccess || !a.weights)
         return e;
-    const unsigned blocks = unsigned((p.capacity + 1023) / 1024);
-    return launch_kernel(weights_kernel, dim3(blocks, p.kv_heads, a.rows), 256, 0, s, 1, a);
+    const unsigned blocks = unsigned((p.capacity + 4 * kWeightThreads - 1) / (4 * kWeightThreads));
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.weights_out) |
+                           uintptr_t(p.capacity) * 4;
+    return launch_kernel((bits & 15) == 0 ? weights_kernel<true> : weights_kernel<false>,
+                         dim3(blocks, p.kv_heads, a.rows), kWeightThreads, 0, s, 1, a);
 }
 
 template <typename T, typename R> cudaError_t launch_halves(const PagedAttention &a, cudaStream_t s) {
