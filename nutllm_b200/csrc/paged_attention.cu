@@ -528,7 +528,7 @@ template <typename Op> struct Plan {
     static constexpr int kBytes = kWarps * (kRing + kScratchBytes) + 2 * kOutputBytes + 1024; /* to align */
     static constexpr int kFit = 228 * 1024 / (kBytes + 2048);
     static constexpr int kPerSm = kFit < Op::kMaxPerSm ? (kFit > 1 ? kFit : 1) : Op::kMaxPerSm;
-    static_assert(kWarps * kRing >= kMaxSms * kPerSm * kRows * 4 + 128 + kOutputBytes,
+    static_assert(kWarps * kRing >= kMaxSms * kPerSm * kRows * 4 + 128 + kOutputBytes + 2 * kRows * 4,
                   "the factors of an item's parts and one part fit there");
 };
 
@@ -546,7 +546,7 @@ template <typename R> __device__ __forceinline__ void store4(R *to, float4 v) {
 
 /* Joins the `parts` parts of an item left by CTAs c0, c0 + 1, ...; run by
  * the whole CTA that arrived last.  Bulk copies bring the parts to shared
- * memory while the warps turn their maxima and sums into one factor
+ * memory, and the warps turn their maxima and sums into one factor
  * exp(m_c - m) / l per part and head.  (Read by one load after another, 37
  * parts cost 200 us; with sixteen in flight a thread, 7.)  */
 template <typename R, int DP, int kWarps>
@@ -561,7 +561,7 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
     auto part = [&](int c) { return c == 0 ? first : rest + int64_t(c - 1) * 2 * kPartialFloats; };
     float *factor = reinterpret_cast<float *>(space);
     const int head_room = (parts * kRows * 4 + 127) / 128 * 128;
-    const int size = heads * DP * 4; /* of a part's outputs */
+    const int size = (2 * kRows + heads * DP) * 4, pitch = size / 4; /* of a part */
     const int most = (bytes - head_room) / size;
     float *copies = reinterpret_cast<float *>(space + head_room);
     auto fetch = [&](int c, int n) { /* by warp 0 */
@@ -570,18 +570,23 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
             mbar_expect_tx(bar, n * size);
         __syncwarp();
         for (int k = lane; k < n; k += 32)
-            bulk_g2s(copies + k * (size / 4), part(c + k) + 2 * kRows, size, bar);
+            bulk_g2s(copies + k * pitch, part(c + k), size, bar);
     };
     if (warp == 0)
         fetch(0, min(parts, most));
+    const bool fit = parts <= most; /* then the statistics are read from the copies too */
+    if (!stage_wait(bar, phase))
+        paged_fail(p, kPagedTimeout);
+    phase ^= 1;
+    auto statistic = [&](int c, int i) { return fit ? copies[c * pitch + i] : __ldcg(part(c) + i); };
     for (int g = warp; g < heads; g += kWarps) {
         float top = -INFINITY, sum = 0.0f;
         for (int c = lane; c < parts; c += 32)
-            top = fmaxf(top, __ldcg(part(c) + g));
+            top = fmaxf(top, statistic(c, g));
         top = warp_max(top);
         const float base = top == -INFINITY ? 0.0f : top;
         for (int c = lane; c < parts; c += 32) {
-            const float f = exp2f(__ldcg(part(c) + g) - base), l = __ldcg(part(c) + kRows + g);
+            const float f = exp2f(statistic(c, g) - base), l = statistic(c, kRows + g);
             factor[c * kRows + g] = f;
             sum = l != 0.0f ? fmaf(l, f, sum) : sum;
         }
@@ -605,15 +610,17 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
         o[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c = 0; c < parts; c += most) {
         const int n = min(parts - c, most);
-        if (!stage_wait(bar, phase))
-            paged_fail(p, kPagedTimeout);
-        phase ^= 1;
+        if (c > 0) {
+            if (!stage_wait(bar, phase))
+                paged_fail(p, kPagedTimeout);
+            phase ^= 1;
+        }
 #pragma unroll
         for (int q = 0; q < kQuads; q++) {
             const int i = (q * kWarps * 32 + tid) * 4, g = i / DP;
             if (g < heads)
                 for (int k = 0; k < n; k++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(copies + k * (size / 4) + i);
+                    const float4 x = *reinterpret_cast<const float4 *>(copies + k * pitch + 2 * kRows + i);
                     const float f = factor[(c + k) * kRows + g];
                     o[q].x = fmaf(x.x, f, o[q].x);
                     o[q].y = fmaf(x.y, f, o[q].y);
@@ -908,7 +915,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         }
 
         /* the warps' states meet: a common maximum, then outputs in a fixed
-         * order, warps 0 and 1 first, 2 and 3 on top */
+         * order, two warps at a time */
         float(&top)[kWarps][kRows] = maxima[turn], (&sum)[kWarps][kRows] = sums[turn];
         turn ^= 1;
         op.statistics(top[warp], sum[warp]);
@@ -946,9 +953,10 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         if (warp < 2)
             op.template output<false>(outputs + warp * kRows * DP, factor);
         __syncthreads();
-        if (kWarps > 2) {
-            if (warp >= 2)
-                op.template output<true>(outputs + (warp - 2) * kRows * DP, factor);
+#pragma unroll
+        for (int w = 2; w < kWarps; w += 2) {
+            if (warp / 2 == w / 2)
+                op.template output<true>(outputs + warp % 2 * kRows * DP, factor);
             __syncthreads();
         }
         for (int i = tid; i < heads * (DP / 4); i += kThreads) {
