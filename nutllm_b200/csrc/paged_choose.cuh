@@ -2,8 +2,8 @@
 /* Choosing the largest of many 32-bit keys, ties to the lowest index: page
  * selection and slot eviction of the paged KV cache.
  *
- * search_largest: few keys, in the registers of four warps; the threshold is
- * found two bits at a time by counting the keys at or above three candidates,
+ * search_largest: few keys, in the registers of a warp or of four; the
+ * threshold is found two bits at a time by counting the keys at or above three candidates,
  * 16 rounds without atomics or scans.
  * choose_largest: any number of keys, by histograms of 11, 11 and 10 bits
  * from the top; one block, or the blocks of a cluster that each hold a run
@@ -84,12 +84,20 @@ struct FewSums {
     }
 };
 
-/* The `want` (1 .. number of keys - 1) largest of the block's keys, N a
+/* The same over a warp. */
+struct WarpSums {
+    __device__ __forceinline__ void operator()(int &a, int &b) {
+        a = __reduce_add_sync(0xffffffffu, a);
+        b = __reduce_add_sync(0xffffffffu, b);
+    }
+};
+
+/* The `want` (1 .. number of keys - 1) largest of the group's keys, N a
  * thread, 0 where a thread has fewer: a key is chosen when it is above
  * `threshold`, or equal to it and one of the first `quota` such.  Invariant:
  * at least `want` keys are >= prefix, `above` are beyond the digits so far. */
-template <int N>
-__device__ __forceinline__ void search_largest(const uint32_t (&k)[N], int want, FewSums &sum, uint32_t &threshold,
+template <int N, typename Sum>
+__device__ __forceinline__ void search_largest(const uint32_t (&k)[N], int want, Sum &sum, uint32_t &threshold,
                                                int &quota) {
     uint32_t prefix = 0;
     int above = 0;

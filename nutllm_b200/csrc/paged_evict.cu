@@ -262,13 +262,17 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
 
 cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s) {
     const PagedPool &p = a.p;
+    /* keys a thread holds: no more than the table needs (12 instead of 16 for
+     * 5000 slots leaves room for another block on the SM: 23 against 26 us) */
     const dim3 all(p.kv_heads, p.sequences);
+    const int each = (p.capacity + kChooseThreads - 1) / kChooseThreads;
     const cudaError_t e =
-        p.capacity <= 4 * kChooseThreads ? launch_kernel(choose_few_slots_kernel<4>, all, kChooseThreads, 0, s, 1, a)
-        : p.capacity <= 16 * kChooseThreads
-            ? launch_kernel(choose_few_slots_kernel<16>, all, kChooseThreads, 0, s, 1, a)
-            : launch_kernel(choose_slots_kernel, dim3(kBlocks * p.kv_heads, p.sequences), kChooseThreads, 0, s,
-                            kBlocks, a);
+        each <= 4    ? launch_kernel(choose_few_slots_kernel<4>, all, kChooseThreads, 0, s, 1, a)
+        : each <= 8  ? launch_kernel(choose_few_slots_kernel<8>, all, kChooseThreads, 0, s, 1, a)
+        : each <= 12 ? launch_kernel(choose_few_slots_kernel<12>, all, kChooseThreads, 0, s, 1, a)
+        : each <= 16 ? launch_kernel(choose_few_slots_kernel<16>, all, kChooseThreads, 0, s, 1, a)
+                     : launch_kernel(choose_slots_kernel, dim3(kBlocks * p.kv_heads, p.sequences), kChooseThreads,
+                                     0, s, kBlocks, a);
     if (e != cudaSuccess)
         return e;
     const int row16 = p.head_dim * (p.type == 0 ? 4 : 2) / 16;

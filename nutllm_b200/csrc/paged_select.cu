@@ -25,19 +25,60 @@ constexpr int kWarps = 8;
 constexpr int kPages = 16;  /* of a warp's product */
 constexpr int kHeads = 8;   /* of a warp's product */
 constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
+constexpr int kFusedPages = 512; /* most pages of a row that its block chooses from at once */
+
+/* A warp writes the `n` first-ranked of a row's `pages` scores (at most 32 N,
+ * in shared memory) to out, ascending, -1 behind. */
+template <int N>
+__device__ __forceinline__ void choose_in_warp(const float *score, int pages, int n, int32_t *out) {
+    const int lane = threadIdx.x & 31, i0 = lane * N, want = min(n, pages);
+    uint32_t k[N], threshold = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        k[e] = i0 + e < pages ? ordered_bits(score[i0 + e]) : 0u;
+    int quota = want;
+    if (want < pages) {
+        WarpSums sum;
+        search_largest(k, want, sum, threshold, quota);
+    }
+    auto before = [&](int count) {
+        int upto = count;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, x);
+            upto += lane >= x ? v : 0;
+        }
+        return upto - count;
+    };
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        ties += i0 + e < pages && k[e] == threshold;
+    int rank = before(ties);
+    uint32_t chosen = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (i0 + e < pages && (k[e] > threshold || (k[e] == threshold && rank++ < quota)))
+            chosen |= 1u << e;
+    for (int to = before(__popc(chosen)); chosen; chosen &= chosen - 1)
+        out[to++] = i0 + __ffs(chosen) - 1;
+    for (int i = want + lane; i < n; i += 32)
+        out[i] = -1;
+}
 
 /* Scores of 16 pages at a time for the rows of a block, KC 64-byte pieces
  * of bounds a page.  A lane loads 16 neighbouring bytes of two pages for two
  * products: which 32 of the 64 bytes meet in one product does not matter as
  * long as both operands take the same ones.  The first pages' bounds are on
  * their way (three look-ups one after another) while the queries are put
- * into 8 bits. */
-template <typename R, int KC>
+ * into 8 bits.  kFused: the block has all of its rows' pages, keeps the
+ * scores in shared memory and chooses, a warp for each row. */
+template <typename R, int KC, bool kFused>
 __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
     score_kernel(const __grid_constant__ PagedSelect a, int rows_each, int pages_each) {
     constexpr int kWidth = KC * 64, kPitch = kWidth + 64; /* pitch: rows in different banks */
     constexpr int kBatch = 4;                             /* heads of a warp that load together */
-    extern __shared__ __align__(16) int8_t queries[];     /* [rows_each][8][kPitch] */
+    extern __shared__ __align__(16) int8_t queries[];     /* [rows_each][8][kPitch], kFused: then the scores */
     __shared__ float units[kMostRows][kHeads];
     __shared__ int sequence_of[kMostRows], pages_of[kMostRows], limit_of[kMostRows];
     const PagedPool &p = a.p;
@@ -45,6 +86,7 @@ __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
     const int g = lane >> 2, t = lane & 3, D = p.head_dim;
     const int row0 = int(blockIdx.z) * rows_each, rows = min(rows_each, a.rows - row0);
     const int j_from = int(blockIdx.x) * pages_each, j_to = j_from + pages_each;
+    float *kept = reinterpret_cast<float *>(queries + rows_each * kHeads * kPitch); /* [rows_each][kFusedPages] */
     begin_kernel();
     if (int(threadIdx.x) < rows) {
         int length;
@@ -61,7 +103,7 @@ __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
     if (int(threadIdx.x) < rows)
         limit_of[threadIdx.x] = limit;
     __syncthreads();
-    if (j_from >= most)
+    if (!kFused && j_from >= most)
         return;
 
     uint4 bound[2][KC];
@@ -159,7 +201,8 @@ __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
                     best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
                     const int j = j0 + g + 8 * h;
                     if (t == 0 && j < pages) {
-                        float *to = a.scores + (int64_t(row0 + i) * p.kv_heads + head) * p.max_pages + j;
+                        float *to = kFused ? kept + i * kFusedPages + j
+                                           : a.scores + (int64_t(row0 + i) * p.kv_heads + head) * p.max_pages + j;
                         float v = there[h] ? best * scale[h] : -INFINITY;
                         if (gq > 0)
                             v = fmaxf(v, *to);
@@ -171,6 +214,18 @@ __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
                     }
                 }
             }
+        }
+    }
+    if constexpr (kFused) {
+        static_assert(kWarps >= kMostRows, "a warp for each row");
+        __syncthreads();
+        if (warp < rows) {
+            int32_t *out = a.selected + (int64_t(row0 + warp) * p.kv_heads + head) * a.n_selected;
+            const float *score = kept + warp * kFusedPages;
+            if (pages_of[warp] <= kFusedPages / 4)
+                choose_in_warp<kFusedPages / 128>(score, pages_of[warp], a.n_selected, out);
+            else
+                choose_in_warp<kFusedPages / 32>(score, pages_of[warp], a.n_selected, out);
         }
     }
 }
@@ -233,8 +288,8 @@ __global__ void __launch_bounds__(kChooseThreads)
         out[i] = -1;
 }
 
-/* The same for at most 128 N pages, N neighbouring ones a thread.  For 512
- * pages, two thousand times over, the other form takes 34 us and this one 12. */
+/* The same for at most 128 N pages, N neighbouring ones a thread: for 1024
+ * pages, 256 times over, the other form takes 7.8 us and this one 6.2. */
 constexpr int kFewThreads = kFewWarps * 32;
 
 template <int N>
@@ -296,6 +351,9 @@ template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cu
     /* rows that may share a sequence share its bounds in registers */
     const int rows_each = a.row_sequence ? kMostRows : 1;
     const int bytes = rows_each * kHeads * (KC * 64 + 64);
+    if (p.max_pages <= kFusedPages)
+        return launch_kernel(score_kernel<R, KC, true>, dim3(1, p.kv_heads, (a.rows + rows_each - 1) / rows_each),
+                             kWarps * 32, bytes + rows_each * kFusedPages * 4, s, 1, a, rows_each, kFusedPages);
     /* a block's queries are made once for all of its pages: as many of them
      * as still leave two blocks for each SM (36 against 51 us with 128) */
     int pages_each = kWarps * kPages * 4;
@@ -303,7 +361,7 @@ template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cu
     const auto chunks = [&] { return (p.max_pages + pages_each - 1) / pages_each; };
     while (pages_each > kWarps * kPages && int64_t(chunks()) * p.kv_heads * row_blocks < 2 * kMaxSms)
         pages_each /= 2;
-    return launch_kernel(score_kernel<R, KC>, dim3(chunks(), p.kv_heads, row_blocks), kWarps * 32, bytes, s, 1, a,
+    return launch_kernel(score_kernel<R, KC, false>, dim3(chunks(), p.kv_heads, row_blocks), kWarps * 32, bytes, s, 1, a,
                          rows_each, pages_each);
 }
 
@@ -325,9 +383,9 @@ cudaError_t paged_select(const PagedSelect &a, cudaStream_t s) {
                                         : scores<__nv_bfloat16>(a, s);
     if (e != cudaSuccess)
         return e;
+    if (p.max_pages <= kFusedPages)
+        return cudaSuccess;
     const dim3 items(p.kv_heads, a.rows);
-    if (p.max_pages <= 4 * kFewThreads)
-        return launch_kernel(choose_few_pages_kernel<4>, items, kFewThreads, 0, s, 1, a);
     if (p.max_pages <= 8 * kFewThreads)
         return launch_kernel(choose_few_pages_kernel<8>, items, kFewThreads, 0, s, 1, a);
     return launch_kernel(choose_pages_kernel, items, kChooseThreads, 0, s, 1, a);
