@@ -468,6 +468,38 @@ def test_attention_passes_infinities_on(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("types", [("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")], ids=lambda t: "-".join(t))
+def test_infinite_keys_in_16_bits_keep_their_sign(gpu, types):
+    """The lower terms of a split query do not turn an infinite logit into NaN: -inf takes no weight."""
+    import torch
+    pool = Pool(torch, [40], 4, 1, 64, 16, types[0])
+    pool.keys[int(pool.table_cpu[0, 1]), 0, 3, 5] = float("inf")  # slot 19
+    dt = dtypes(torch)[types[1]]
+    q = torch.randn(1, 4, 64, generator=pool.g)
+    q[:, :, 5] = -torch.rand(1, 4, generator=pool.g) - 0.1
+    q = q.to(dt).cuda()
+    out, lse = torch.zeros_like(q), torch.zeros(1, 4, device="cuda")
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), 1, dtype=KINDS[types[1]], lse=lse.data_ptr())
+    pool.cache.check()
+    keep = [t for t in range(40) if t != 19]
+    want, want_lse, _, dz, mass = head_reference(torch, q.cpu()[0], pool.k[0][0][keep], pool.v[0][0][keep], 1 / 8)
+    close_out(torch, out.cpu()[0], want, dz, mass, 39, types[1])
+    assert bool(((lse.cpu()[0].double() - want_lse).abs() <= dz[:, 0] + 48 * EPS + 4 * EPS * want_lse.abs()).all())
+
+
+@pytest.mark.gpu
+def test_one_sequence_among_many_rows_and_places(gpu):
+    """More rows than threads of a block, most of them idle, on a table far wider than the lengths."""
+    import torch
+    lens = [0] * 300
+    for s, n in ((0, 1), (7, 33), (128, 70), (255, 16), (299, 129)):
+        lens[s] = n
+    pool = Pool(torch, lens, 4, 2, 64, 16, "bf16", max_pages=1000)
+    q, out, lse = run_attention(torch, pool, "f32", 300)
+    check_attention(torch, pool, q, out, lse, list(enumerate(lens)), 1 / 8, "f32")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f16", "f32"])
 def test_offsets_pass_32_bits(gpu, kind):
     """A pool of more than 2^32 elements, the sequence in its first and last pages."""
