@@ -65,14 +65,13 @@ struct PagedAttention {
     float scale;
     float *logits; /* [sequences][heads][capacity] with weights, in log2 */
     float *lse2;   /* [sequences][heads] with weights, in log2 */
-    float *partial; /* [CTAs][2][kPartialFloats]: items shared between CTAs */
+    float *partial; /* [CTAs][2][paged_part_floats]: items shared between CTAs */
     int *counters;  /* [max_rows][items of a row], 0 between calls */
     int sms;
 };
 
-/* A CTA's part of an attention item: maxima [8], sums [8], outputs [8][256]. */
-constexpr int kMaxDim = 256;
-constexpr int kPartialFloats = 8 * 2 + 8 * kMaxDim;
+/* A CTA's part of an attention item: maxima [8], sums [8], outputs [8][padded dim]. */
+constexpr int paged_part_floats(int padded) { return 8 * 2 + 8 * padded; }
 constexpr int kMaxCtasPerSm = 3;
 constexpr int kMaxSms = 160;
 constexpr int kMaxDevices = 64;
@@ -99,9 +98,14 @@ struct PagedEvict {
     int32_t *counts; /* [sequences][kv_heads][2]: pairs, old length */
 };
 
-/* 128-byte columns of a row as the attention lays it out in shared memory. */
+/* head_dim as the attention's kernels are made for. */
+inline int paged_padded_dim(int type, int D) {
+    return type == 0 ? (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256)
+                     : (D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256);
+}
+/* 128-byte columns of such a row in shared memory. */
 inline int paged_columns(int type, int D) {
-    return type == 0 ? (D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 4 : 8) : (D <= 64 ? 1 : D <= 128 ? 2 : D <= 192 ? 3 : 4);
+    return (paged_padded_dim(type, D) * (type == 0 ? 4 : 2) + 127) / 128;
 }
 
 cudaError_t paged_append(const PagedAppend &a, cudaStream_t s);

@@ -553,6 +553,7 @@ template <typename R, int DP, int kWarps>
 __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, int c0, int parts, int r,
                                         int first_head, int heads, char *space, int bytes, uint64_t *bar,
                                         uint32_t &phase) {
+    constexpr int kPartialFloats = paged_part_floats(DP);
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     /* an item that starts inside its first CTA's share lies in that one's second slot */
@@ -922,7 +923,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         __syncthreads();
         float(&factor)[kRows] = factors[warp];
         const bool whole = x.tile0 == 0 && x.tile1 == x.tiles;
-        float *part = a.partial + (int64_t(blockIdx.x) * 2 + (x.first <= start ? 0 : 1)) * kPartialFloats;
+        float *part = a.partial + (int64_t(blockIdx.x) * 2 + (x.first <= start ? 0 : 1)) * paged_part_floats(DP);
         if (lane < kRows) {
             float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -1089,27 +1090,31 @@ cudaError_t launch(const PagedAttention &a, cudaStream_t s) {
 }
 
 template <typename T, typename R> cudaError_t launch_halves(const PagedAttention &a, cudaStream_t s) {
-    const int D = a.p.head_dim;
-    if (D <= 64)
+    switch (paged_padded_dim(a.p.type, a.p.head_dim)) {
+    case 64:
         return launch<Halves<T, R, 64>, R>(a, s);
-    if (D <= 96)
+    case 96:
         return launch<Halves<T, R, 96>, R>(a, s);
-    if (D <= 128)
+    case 128:
         return launch<Halves<T, R, 128>, R>(a, s);
-    if (D <= 192)
+    case 192:
         return launch<Halves<T, R, 192>, R>(a, s);
-    return launch<Halves<T, R, 256>, R>(a, s);
+    default:
+        return launch<Halves<T, R, 256>, R>(a, s);
+    }
 }
 
 template <int NQ> cudaError_t launch_wide(const PagedAttention &a, cudaStream_t s) {
-    const int D = a.p.head_dim;
-    if (D <= 32)
+    switch (paged_padded_dim(a.p.type, a.p.head_dim)) {
+    case 32:
         return launch<Wide<NQ, 32>, float>(a, s);
-    if (D <= 64)
+    case 64:
         return launch<Wide<NQ, 64>, float>(a, s);
-    if (D <= 128)
+    case 128:
         return launch<Wide<NQ, 128>, float>(a, s);
-    return launch<Wide<NQ, 256>, float>(a, s);
+    default:
+        return launch<Wide<NQ, 256>, float>(a, s);
+    }
 }
 
 } // namespace

@@ -4,6 +4,7 @@
 #include <climits>
 #include <cmath>
 #include <memory>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
@@ -58,10 +59,26 @@ struct DeviceScope {
     }
 };
 
-template <typename T> T *dev_alloc(size_t count, const char *what) {
-    void *p = nullptr;
-    cuda_check(cudaMalloc(&p, (count == 0 ? 1 : count) * sizeof(T)), what);
-    return static_cast<T *>(p);
+/* Workspaces come from a memory pool of this library's own on each device,
+ * which keeps up to 64 MB that handles gave back: a handle is made in some 20
+ * us, where cudaMalloc and cudaFree take 300 to 400 each. */
+cudaMemPool_t workspace_pool(int device) {
+    static std::mutex lock;
+    static cudaMemPool_t pools[nut::kMaxDevices] = {};
+    if (device < 0 || device >= nut::kMaxDevices)
+        raise(NUT_INVALID_ARGUMENT, "device out of range");
+    const std::lock_guard<std::mutex> hold(lock);
+    if (!pools[device]) {
+        cudaMemPoolProps props{};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = device;
+        cuda_check(cudaMemPoolCreate(&pools[device], &props), "create workspace pool");
+        uint64_t keep = uint64_t(64) << 20;
+        cuda_check(cudaMemPoolSetAttribute(pools[device], cudaMemPoolAttrReleaseThreshold, &keep),
+                   "size workspace pool");
+    }
+    return pools[device];
 }
 
 constexpr int64_t kMaxGrid = 65535; /* sequences and rows are grid dimensions */
@@ -172,8 +189,10 @@ struct nut_paged {
     float *partial = nullptr, *logits = nullptr, *lse2 = nullptr, *scores = nullptr;
     int32_t *pairs = nullptr, *counts = nullptr;
     ~nut_paged() {
-        if (block)
-            cudaFree(block);
+        if (block) {
+            cudaDeviceSynchronize(); /* calls in flight, on any stream, still use it */
+            cudaFreeAsync(block, nullptr);
+        }
     }
 };
 
@@ -253,12 +272,16 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         const size_t error = part(1, 4);
         const size_t counters = part(size_t(h->max_rows) * p.kv_heads * ((p.group + 7) / 8), 4);
         const size_t zeroed = bytes;
-        const size_t partial = part(size_t(h->sms) * nut::kMaxCtasPerSm * 2 * nut::kPartialFloats, 4);
+        const size_t partial = part(size_t(h->sms) * nut::kMaxCtasPerSm * 2 *
+                                        nut::paged_part_floats(nut::paged_padded_dim(p.type, p.head_dim)),
+                                    4);
         const size_t pairs = part(items * p.capacity, 4), counts = part(items * 2, 4);
         const size_t logits = part(h->track ? size_t(p.sequences) * p.heads * p.capacity : 0, 4);
         const size_t lse2 = part(h->track ? size_t(p.sequences) * p.heads : 0, 4);
         const size_t scores = part(p.bounds ? size_t(h->max_rows) * p.kv_heads * p.max_pages : 0, 4);
-        h->block = dev_alloc<char>(bytes, "alloc workspace");
+        void *block = nullptr;
+        cuda_check(cudaMallocFromPoolAsync(&block, bytes, workspace_pool(device), nullptr), "alloc workspace");
+        h->block = static_cast<char *>(block);
         const auto floats = [&](size_t at) { return reinterpret_cast<float *>(h->block + at); };
         const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(h->block + at); };
         p.error = h->error = ints(error);
@@ -269,7 +292,7 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         h->logits = floats(logits);
         h->lse2 = floats(lse2);
         h->scores = floats(scores);
-        cuda_check(cudaMemset(h->block, 0, zeroed), "clear workspace");
+        cuda_check(cudaMemsetAsync(h->block, 0, zeroed, nullptr), "clear workspace");
         cuda_check(cudaStreamSynchronize(nullptr), "finish workspace");
         *out = h.release();
     });
