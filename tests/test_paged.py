@@ -1011,3 +1011,48 @@ def test_the_device_reports_what_it_cannot_serve(gpu):
     reported("rotation table")
     attend()
     pool.cache.check()
+
+
+# groups of every width share products between rows, or do not
+PACKED = [(1, 1), (2, 1), (6, 2), (8, 2), (10, 2), (7, 1), (16, 2), (18, 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 1], ids=["block chooses", "scores in memory"])
+@pytest.mark.parametrize("heads,kv", PACKED)
+def test_select_for_rows_of_mixed_sequences(gpu, heads, kv, page):
+    """Neighbouring rows of one sequence and of others, of unequal lengths, in blocks of whole and of ragged size."""
+    import torch
+    lens = [600, 130, 0]
+    pool = Pool(torch, lens, heads, kv, 32, page, "f16", bounds=True, max_rows=21)
+    pool.cache.summarise()
+    rows = [(0, 600), (0, 1), (0, 17), (1, 130), (1, 0), (0, 599), (0, 600), (1, 64),
+            (2, 0), (1, 130), (0, 300), (0, 301), (0, 302), (0, 303), (1, 5), (1, 6),
+            (1, 129), (0, 33), (0, 600), (0, 16), (1, 100)]
+    q = torch.randn(len(rows), heads, 32, generator=pool.g).cuda()
+    seq = torch.tensor([s for s, _ in rows], dtype=torch.int32, device="cuda")
+    length = torch.tensor([n for _, n in rows], dtype=torch.int32, device="cuda")
+    got = run_select(torch, pool, q, "f32", len(rows), 9, 1, 2, row_sequence=seq.data_ptr(), row_length=length.data_ptr())
+    assert np.array_equal(got, select_reference(pool, q, rows, 9, 1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf], ids=str)
+@pytest.mark.parametrize("length", [300, 700, 9000])
+def test_select_writes_distinct_pages_whatever_the_scores(gpu, length, scale):
+    """Scales that no summary writes: the choice is arbitrary, but of n pages of the row, in order, and no more."""
+    import torch
+    pool = Pool(torch, [length], 4, 2, 8, 1, "f16", bounds=True)
+    pool.cache.summarise()
+    pool.scales[::3] = scale
+    if math.isnan(scale):
+        pool.scales.view(torch.int32)[::6] = 0x7fffffff
+    q = torch.randn(1, 4, 8, generator=pool.g).cuda()
+    for n in (1, 40, length - 1):
+        got = torch.full((1, 2, n + 8), 99999, dtype=torch.int32, device="cuda")
+        pool.cache.select(q.data_ptr(), got.data_ptr(), 1, n, dtype=KINDS["f32"], sink_pages=1, recent_pages=1)
+        pool.cache.check()
+        flat = got.cpu().numpy().reshape(-1)
+        assert (flat[2 * n:] == 99999).all()
+        for chosen in flat[:2 * n].reshape(2, n):
+            assert (np.diff(chosen) > 0).all() and chosen[0] >= 0 and chosen[-1] < length
