@@ -3,8 +3,9 @@
  * selection and slot eviction of the paged KV cache.
  *
  * search_largest: few keys, in the registers of a warp or of four; the
- * threshold is found two bits at a time by counting the keys at or above three candidates,
- * 16 rounds without atomics or scans.
+ * threshold is found between the least and the greatest of them, a quarter
+ * of what is left at a time, by counting the keys at or above three
+ * candidates: no atomics, no scans.
  * choose_largest: any number of keys, by histograms of 11, 11 and 10 bits
  * from the top; one block, or the blocks of a cluster that each hold a run
  * of the keys and add their histograms over distributed shared memory. */
@@ -64,23 +65,35 @@ template <int N, typename T> __device__ __forceinline__ void load_own(const T *x
 
 constexpr int kFewWarps = 4;
 
-/* Sums of two counts (below 2^16 each) over kFewWarps warps, for every thread. */
+/* Sums of two counts (below 2^16 each) over kFewWarps warps, and the least
+ * and greatest of two keys, for every thread. */
 struct FewSums {
     int2 (*scratch)[kFewWarps]; /* [2] */
     int turn = 0;
-    __device__ __forceinline__ void operator()(int &a, int &b) {
-        a = __reduce_add_sync(0xffffffffu, a);
-        b = __reduce_add_sync(0xffffffffu, b);
+    __device__ __forceinline__ const int2 *all(int a, int b) {
         if ((threadIdx.x & 31) == 0)
             scratch[turn][threadIdx.x >> 5] = make_int2(a, b);
         __syncthreads();
+        const int2 *of = scratch[turn];
+        turn ^= 1;
+        return of;
+    }
+    __device__ __forceinline__ void operator()(int &a, int &b) {
+        const int2 *of = all(__reduce_add_sync(0xffffffffu, a), __reduce_add_sync(0xffffffffu, b));
         a = b = 0;
 #pragma unroll
         for (int w = 0; w < kFewWarps; w++) {
-            a += scratch[turn][w].x;
-            b += scratch[turn][w].y;
+            a += of[w].x;
+            b += of[w].y;
         }
-        turn ^= 1;
+    }
+    __device__ __forceinline__ void range(uint32_t &lo, uint32_t &hi) {
+        const int2 *of = all(int(__reduce_min_sync(0xffffffffu, lo)), int(__reduce_max_sync(0xffffffffu, hi)));
+#pragma unroll
+        for (int w = 0; w < kFewWarps; w++) {
+            lo = min(lo, uint32_t(of[w].x));
+            hi = max(hi, uint32_t(of[w].y));
+        }
     }
 };
 
@@ -90,19 +103,65 @@ struct WarpSums {
         a = __reduce_add_sync(0xffffffffu, a);
         b = __reduce_add_sync(0xffffffffu, b);
     }
+    __device__ __forceinline__ void range(uint32_t &lo, uint32_t &hi) {
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+    }
 };
 
 /* The `want` (1 .. number of keys - 1) largest of the group's keys, N a
  * thread, 0 where a thread has fewer: a key is chosen when it is above
- * `threshold`, or equal to it and one of the first `quota` such.  Invariant:
- * at least `want` keys are >= prefix, `above` are beyond the digits so far. */
+ * `threshold`, or equal to it and one of the first `quota` such.  Keys of
+ * +inf stand outside the range that is searched: a few of them (pages that
+ * are always read) would stretch it.  (From the top bit down, two bits a
+ * round, 256 choices among 1024 pages took 6.4 us; so, 5.8.)  Invariant: at least `want` keys are
+ * >= lo; `above` of them, fewer than `want`, are >= hi. */
 template <int N, typename Sum>
 __device__ __forceinline__ void search_largest(const uint32_t (&k)[N], int want, Sum &sum, uint32_t &threshold,
                                                int &quota) {
-    uint32_t prefix = 0;
-    int above = 0;
-    for (int shift = 30; shift >= 0; shift -= 2) {
-        const uint32_t c1 = prefix + (1u << shift), c2 = prefix + (2u << shift), c3 = prefix + (3u << shift);
+    constexpr uint32_t kTop = 0xff800000u; /* ordered_bits(+inf) */
+    uint32_t lo = ~0u, hi = 0;
+    int above = 0, here = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        above += k[e] >= kTop;
+        here += k[e] != 0;
+        lo = min(lo, k[e] != 0 ? k[e] : ~0u);
+        hi = max(hi, k[e] < kTop ? k[e] : 0u);
+    }
+    sum.range(lo, hi);
+    sum(above, here);
+    if (here < want) { /* keys of 0, too, are chosen */
+        threshold = 0;
+        quota = want - here;
+        return;
+    }
+    if (above >= want) {
+        int last = 0, none = 0; /* some NaN have all bits set */
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            last += k[e] == ~0u;
+        sum(last, none);
+        if (last >= want) {
+            threshold = ~0u;
+            quota = want;
+            return;
+        }
+        lo = kTop;
+        hi = ~0u;
+        here = above;
+        above = last;
+    } else {
+        hi++;
+    }
+    while (here != want) { /* otherwise no key is left to tell apart */
+        if (hi - lo == 1) {
+            threshold = lo;
+            quota = want - above;
+            return;
+        }
+        const uint32_t left = hi - lo, step = max(left / 4, 1u); /* lo < c1 <= c2 <= c3 < hi */
+        const uint32_t c1 = lo + step, c2 = lo + left / 2, c3 = hi - step;
         int n1 = 0, n2 = 0, n3 = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -114,29 +173,26 @@ __device__ __forceinline__ void search_largest(const uint32_t (&k)[N], int want,
         sum(n1, n3);
         n2 = int(uint32_t(n1) >> 16);
         n1 &= 0xffff;
-        int here = -1; /* keys at or above the new prefix, where it moved */
         if (n3 >= want) {
-            prefix = c3;
+            lo = c3;
             here = n3;
         } else if (n2 >= want) {
-            prefix = c2;
+            lo = c2;
             here = n2;
+            hi = c3;
             above = n3;
         } else if (n1 >= want) {
-            prefix = c1;
+            lo = c1;
             here = n1;
+            hi = c2;
             above = n2;
         } else {
+            hi = c1;
             above = n1;
         }
-        if (here == want) { /* no key is left to tell apart */
-            threshold = prefix - 1u;
-            quota = 0;
-            return;
-        }
     }
-    threshold = prefix;
-    quota = want - above;
+    threshold = lo - 1u;
+    quota = 0;
 }
 
 /* The keys of this thread in the chunk that starts at `base`; 0 beyond n.
