@@ -4,7 +4,7 @@
  * head in 8 bits, M and L the page's greatest and least key in 8 bits, u and
  * U powers of two.  As max(x M, x L) = max(x, 0) M + min(x, 0) L, the sum is
  * one product of [M | L] with [max(x, 0) | min(x, 0)]: mma.sync m16n8k32 in
- * 8 bits, 16 pages by the 8 query heads of a group.  The sum is at most
+ * 8 bits, 16 pages by 8 query heads (of one row, or of two or four).  The sum is at most
  * 256 * 127 * 128 < 2^24 in size, so it is exact in an int and in fp32,
  * whatever its order.
  *
@@ -12,7 +12,8 @@
  * page's 16 keys and values take in 16 bits.  35 MB of them (32 sequences of
  * up to 1,024 pages, 8 heads of 128) take 15 us, bound by the look-ups that
  * precede them (length, table, bounds) and the blocks' barriers, and choosing
- * 64 of each 6 us more.
+ * 64 of each 6 us more.  256 rows of one prompt choosing 64 of 512 pages
+ * take 32 us: 11 of them the choice, a warp for each row's.
  */
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -26,7 +27,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kPages = 16;  /* of a warp's product */
-constexpr int kHeads = 8;   /* of a warp's product */
+constexpr int kHeads = 8;   /* columns of a warp's product */
 constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
 constexpr int kFusedPages = 512; /* most pages of a row that its block chooses from at once */
 
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kChooseThreads)
 }
 
 /* The same for at most 128 N pages, N neighbouring ones a thread: for 1024
- * pages, 256 times over, the other form takes 7.8 us and this one 6.2. */
+ * pages, 256 times over, the other form takes 7.8 us and this one 5.8. */
 constexpr int kFewThreads = kFewWarps * 32;
 
 template <int N>
