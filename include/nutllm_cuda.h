@@ -432,9 +432,11 @@ nut_status nut_paged_summarise(nut_paged *paged, void *stream);
 /* out[r][h] = sum_t w_t v_t with w = softmax_t(scale q[r][h] . k_t) over the
  * first row_length[r] slots of sequence row_sequence[r], kv head
  * h / (heads / kv_heads).  A row that sees nothing gives zeros and
- * lse = -infinity.  Sums, the softmax and its statistics are fp32 and the
- * operands enter unrounded (16-bit caches: queries and weights are split
- * into two or three 16-bit terms).
+ * lse = -infinity.  Sums, the softmax and its statistics are fp32.  What
+ * multiplies a 16-bit cache is split into 16-bit terms: fp32 queries and
+ * their weights keep 22 bits (fp16) or 24 (bf16), the weights of bf16 rows
+ * 16; weights below 2^-21 of a row's greatest on an fp16 cache are exact to
+ * 2^-43 of it.
  * `selected` restricts row r, kv head g to the pages whose numbers within the
  * sequence are listed, in any order, -1 for none; a page listed twice counts
  * twice.  With weights / weights_out (one row per sequence, no `selected`)

@@ -134,13 +134,21 @@ __device__ __forceinline__ float plus_terms(float hi, float rest) {
  * plus c of row g + 8, which lie in the same thread, is the fp32 logit at no
  * further cost.  The weights of the second product are split the same way.
  * fp16's two terms hold 22 bits (fp32 queries are first scaled by a power
- * of two into its range), bf16's two hold 16; with fp32 rows a third bf16
- * term goes through a second mma. */
+ * of two into its range), bf16's two hold 16, less than a bf16 output's
+ * rounding loses; with fp32 rows a third bf16 term goes through a second mma.
+ * fp16 ends at 2^-24, below which what many small weights add up to would be
+ * lost beside one great one (a quarter of an output made of 2,047 weights
+ * 18 nats below the greatest).  So its weights are 2^kLift times as great, at
+ * most 2^15 with kSlack, and their second terms, at most 2^4, kLow times that,
+ * which the accumulators of rows 8-15, theirs alone, undo at the end: a weight
+ * is within 2^-22 of itself or 2^-43 of the greatest. */
 template <typename T, typename R, int DP_> struct Halves {
     static constexpr int DP = DP_, kWarps = 4;
     static constexpr bool kThird = std::is_same<T, __nv_bfloat16>::value && std::is_same<R, float>::value;
     static constexpr bool kScaled = std::is_same<T, __half>::value && std::is_same<R, float>::value;
     static constexpr bool kSplitQ = std::is_same<R, float>::value;
+    static constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f; /* log2 */
+    static constexpr float kLow = std::is_same<T, __half>::value ? 2048.0f : 1.0f;
     static constexpr int kMaxPerSm = DP >= 128 && kThird ? 2 : 3; /* by registers */
     static constexpr int kBlocks = (DP * 2 + 127) / 128; /* 128-byte columns of a row */
     static constexpr int kStageBytes = 2 * kBlocks * kBlock;
@@ -256,8 +264,8 @@ template <typename T, typename R, int DP_> struct Halves {
                         z[int64_t(g) * stride + 8 * i + 2 * t + j] = s2[i][j];
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        /* the maximum in use may lag behind by kSlack: weights then reach 2^8,
-         * which costs no precision, and outputs are rarely rescaled */
+        /* the maximum in use may lag behind by kSlack: weights then reach 2^8
+         * (times 2^kLift), and outputs are rarely rescaled */
         const float next = top > m + kSlack || m == -INFINITY ? fmaxf(m, top) : m;
         if (__any_sync(0xffffffffu, next != m)) {
             const float keep = m == next ? 1.0f : exp2f(m - next);
@@ -271,7 +279,7 @@ template <typename T, typename R, int DP_> struct Halves {
             }
             m = next;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = m == -INFINITY ? 0.0f : m - kLift;
         uint32_t hi[2], lo[2], p3[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -279,7 +287,7 @@ template <typename T, typename R, int DP_> struct Halves {
             l += w0 + w1;
             hi[i] = Pair<T>::pack(w0, w1);
             const float2 r = left_of<T>(w0, w1, hi[i]);
-            lo[i] = Pair<T>::pack(r.x, r.y);
+            lo[i] = Pair<T>::pack(r.x * kLow, r.y * kLow);
             if constexpr (kThird) {
                 const float2 r3 = left_of<T>(r.x, r.y, lo[i]);
                 p3[i] = Pair<T>::pack(r3.x, r3.y);
@@ -300,13 +308,13 @@ template <typename T, typename R, int DP_> struct Halves {
         }
     }
 
-    /* This warp's maxima and sums of the 8 heads. */
+    /* This warp's maxima, kLift below the real ones, and sums of the 8 heads. */
     __device__ __forceinline__ void statistics(float *maxima, float *sums) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (t == 0) {
-            maxima[g] = m;
+            maxima[g] = m - kLift;
             sums[g] = l;
         }
     }
@@ -319,7 +327,8 @@ template <typename T, typename R, int DP_> struct Halves {
             float2 *to = reinterpret_cast<float2 *>(out + g * DP + n * 8 + 2 * t);
             float2 v = make_float2(0.0f, 0.0f);
             if (f != 0.0f)
-                v = make_float2(plus_terms(o[n][0], o[n][2]) * f, plus_terms(o[n][1], o[n][3]) * f);
+                v = make_float2(plus_terms(o[n][0], o[n][2] * (1.0f / kLow)) * f,
+                                plus_terms(o[n][1], o[n][3] * (1.0f / kLow)) * f);
             if (kAdd)
                 v = make_float2(v.x + to->x, v.y + to->y);
             *to = v;

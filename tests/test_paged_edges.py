@@ -1,0 +1,50 @@
+"""The paged KV cache operators where a call is easily answered wrongly: rows
+with one token far above the others, special values in used slots, wrong
+numbers in device memory, and sizes at the ends of their ranges.  Tolerances
+are those of test_paged.py, or derived beside the test."""
+import math
+
+import pytest
+
+from tests.test_paged import EPS, KINDS, TYPES, Pool, dtypes, head_reference
+
+# ---------------------------------------------------------------------------
+# attention
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("gap", [10.0, 14.0, 16.0, 18.0])
+def test_tokens_far_below_the_greatest_keep_their_share(gpu, types, gap):
+    """One token `gap` nats above all others has a value of 0, so that the output is what the others add up to.  512 rows of one
+    sequence: an item then lies in one or two blocks, and its warps walk hundreds of slots.
+
+    A weight is off by the logits' error (one product, its unit and the subtraction: 4 eps of the gap), by 2^-22 (16-bit caches:
+    two terms; bf16: 2^-17 where the rows are bf16, whose weights have two terms of 8 bits) and, in fp16, by 2^-43 of the greatest
+    weight.  The sums are chains of n / 64 products of 16 slots a warp, and the denominator's of n / 16."""
+    import torch
+    n, D, rows = 2048, 64, 512
+    pool = Pool(torch, [n], 4, 1, D, 16, types[0], max_rows=rows, fill=False)
+    dt = dtypes(torch)
+    k = torch.zeros(1, n, D)
+    k[0, 5, 0] = gap
+    v = 500 + 1000 * torch.rand(1, n, D, generator=pool.g)
+    v[0, 5] = 0.0
+    k, v = k.to(dt[types[0]]), v.to(dt[types[0]])
+    pool.put(0, k, v, 0)
+    q = torch.zeros(rows, 4, D, dtype=dt[types[1]])
+    q[:, :, 0] = 1.0
+    q, seq = q.cuda(), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(rows, 4, device="cuda")
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), rows, dtype=KINDS[types[1]], scale=1.0, lse=lse.data_ptr(),
+                         row_sequence=seq.data_ptr())
+    pool.cache.check()
+    want, want_lse, _, _, mass = head_reference(torch, q[0, :1].cpu(), k[0], v[0], 1.0)
+    tol = 8 * EPS * gap + (n / 16 + 64) * EPS + 2.0 ** -22
+    tol += {"f32": 0.0, "f16": 2.0 ** -43 * math.exp(gap), "bf16": 2.0 ** -17 if types[1] == "bf16" else 0.0}[types[0]]
+    tol = tol * mass
+    if types[1] != "f32":
+        tol = tol + (want.abs() + tol) * torch.finfo(dt[types[1]]).eps / 2 + (2.0 ** -25 if types[1] == "f16" else 0.0)
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"error {float((err / want).max()):.2e} of the output, {float((err / tol).max()):.1f} of the bound"
+    assert float((lse.cpu().double() - want_lse).abs().max()) <= 8 * EPS * gap + (n / 16 + 8) * EPS
