@@ -301,9 +301,12 @@ template <typename T, typename R, int DP_> struct Halves {
             Pair<T>::mma(o[2 * n], hi[0], lo[0], hi[1], lo[1], b[0], b[1]);
             Pair<T>::mma(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b[2], b[3]);
             if constexpr (kThird) {
-                /* into the rows of the second terms */
-                Pair<T>::mma(o[2 * n], 0u, p3[0], 0u, p3[1], b[0], b[1]);
-                Pair<T>::mma(o[2 * n + 1], 0u, p3[0], 0u, p3[1], b[2], b[3]);
+                /* into the rows of the second terms; the first ones get a
+                 * weight of 2^-126, beside which an infinite value stays
+                 * infinite where 0 would make it NaN */
+                constexpr uint32_t kTiny = 0x00800080u;
+                Pair<T>::mma(o[2 * n], kTiny, p3[0], kTiny, p3[1], b[0], b[1]);
+                Pair<T>::mma(o[2 * n + 1], kTiny, p3[0], kTiny, p3[1], b[2], b[3]);
             }
         }
     }

@@ -48,3 +48,19 @@ def test_tokens_far_below_the_greatest_keep_their_share(gpu, types, gap):
     err = (out.cpu().double() - want).abs()
     assert bool((err <= tol).all()), f"error {float((err / want).max()):.2e} of the output, {float((err / tol).max()):.1f} of the bound"
     assert float((lse.cpu().double() - want_lse).abs().max()) <= 8 * EPS * gap + (n / 16 + 8) * EPS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [t for t in TYPES if t[1] != "f16"], ids=lambda t: "-".join(t))
+def test_infinite_values_reach_the_output(gpu, types):
+    """An infinite value with a weight of its own makes its dimension infinite."""
+    import torch
+    pool = Pool(torch, [30], 2, 1, 64, 16, types[0])
+    page = int(pool.table_cpu[0, 1])
+    pool.values[page, 0, 3, 6], pool.values[page, 0, 4, 9] = float("inf"), -float("inf")
+    q = torch.randn(1, 2, 64, generator=pool.g).to(dtypes(torch)[types[1]]).cuda()
+    out = torch.zeros_like(q)
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), 1, dtype=KINDS[types[1]])
+    pool.cache.check()
+    assert bool((out[0, :, 6] == math.inf).all()) and bool((out[0, :, 9] == -math.inf).all())
+    assert bool(torch.isfinite(out[0, :, [d for d in range(64) if d not in (6, 9)]]).all())
