@@ -556,11 +556,16 @@ __device__ __forceinline__ int walked(const PagedAttention &a, int length) {
     return length == 0 ? 0 : a.selected ? a.n_selected * a.p.page_size : length;
 }
 
+/* An output in its type; infinities stay (from_float would saturate them, and
+ * a mean of fp16 values has no other way beyond 65504). */
+template <typename R> __device__ __forceinline__ R output_of(float v) { return from_float<R>(v); }
+template <> __device__ __forceinline__ __half output_of<__half>(float v) { return __float2half_rn(v); }
+
 template <typename R> __device__ __forceinline__ void store4(R *to, float4 v) {
-    to[0] = from_float<R>(v.x);
-    to[1] = from_float<R>(v.y);
-    to[2] = from_float<R>(v.z);
-    to[3] = from_float<R>(v.w);
+    to[0] = output_of<R>(v.x);
+    to[1] = output_of<R>(v.y);
+    to[2] = output_of<R>(v.z);
+    to[3] = output_of<R>(v.w);
 }
 
 /* Joins the `parts` parts of an item left by CTAs c0, c0 + 1, ...; run by

@@ -64,3 +64,21 @@ def test_infinite_values_reach_the_output(gpu, types):
     pool.cache.check()
     assert bool((out[0, :, 6] == math.inf).all()) and bool((out[0, :, 9] == -math.inf).all())
     assert bool(torch.isfinite(out[0, :, [d for d in range(64) if d not in (6, 9)]]).all())
+
+
+@pytest.mark.gpu
+def test_infinite_values_reach_fp16_rows(gpu):
+    """Outputs are rounded to fp16, not saturated: infinities stay, and a mean of the largest finite values stays finite."""
+    import torch
+    pool = Pool(torch, [30], 2, 1, 64, 16, "f16")
+    page = int(pool.table_cpu[0, 1])
+    pool.values[page, 0, 3, 6], pool.values[page, 0, 4, 9] = float("inf"), -float("inf")
+    for j in range(2):
+        pool.values[int(pool.table_cpu[0, j]), 0, :, 11] = 65504.0
+    q = torch.randn(1, 2, 64, generator=pool.g).half().cuda()
+    out = torch.zeros_like(q)
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), 1, dtype=KINDS["f16"])
+    pool.cache.check()
+    assert bool((out[0, :, 6] == math.inf).all()) and bool((out[0, :, 9] == -math.inf).all())
+    assert bool((out[0, :, 11] == 65504.0).all())
+    assert bool(torch.isfinite(out[0, :, [d for d in range(64) if d not in (6, 9)]]).all())
