@@ -371,9 +371,23 @@ template <typename R, int KC> cudaError_t launch_scores(const PagedSelect &a, cu
     /* rows that may share a sequence share its bounds in registers */
     const int rows_each = a.row_sequence ? kMostRows : 1;
     const int bytes = max(rows_each << columns_of(p.group), kHeads) * (KC * 64 + 64);
-    if (p.max_pages <= kFusedPages)
-        return launch_kernel(score_kernel<R, KC, true>, dim3(1, p.kv_heads, (a.rows + rows_each - 1) / rows_each),
-                             kWarps * 32, bytes + rows_each * kFusedPages * 4, s, 1, a, rows_each, kFusedPages);
+    if (p.max_pages <= kFusedPages) {
+        const auto kernel = score_kernel<R, KC, true>;
+        /* 8 rows of more than 4 heads of more than 128 dims take 52 KB */
+        constexpr int kMostBytes = kMostRows * (kHeads * (KC * 64 + 64) + kFusedPages * 4);
+        if constexpr (kMostBytes > 40 * 1024) {
+            static bool raised[kMaxDevices] = {};
+            int device = 0;
+            cudaError_t e = cudaGetDevice(&device);
+            if (e == cudaSuccess && !raised[device % kMaxDevices])
+                e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
+            if (e != cudaSuccess)
+                return e;
+            raised[device % kMaxDevices] = true;
+        }
+        return launch_kernel(kernel, dim3(1, p.kv_heads, (a.rows + rows_each - 1) / rows_each), kWarps * 32,
+                             bytes + rows_each * kFusedPages * 4, s, 1, a, rows_each, kFusedPages);
+    }
     /* a block's queries are made once for all of its pages: as many of them
      * as still leave two blocks for each SM (36 against 51 us with 128) */
     int pages_each = kWarps * kPages * 4;

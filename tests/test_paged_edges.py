@@ -4,9 +4,10 @@ numbers in device memory, and sizes at the ends of their ranges.  Tolerances
 are those of test_paged.py, or derived beside the test."""
 import math
 
+import numpy as np
 import pytest
 
-from tests.test_paged import EPS, KINDS, TYPES, Pool, dtypes, head_reference
+from tests.test_paged import EPS, KINDS, TYPES, Pool, dtypes, head_reference, run_select, select_reference
 
 # ---------------------------------------------------------------------------
 # attention
@@ -82,3 +83,25 @@ def test_infinite_values_reach_fp16_rows(gpu):
     assert bool((out[0, :, 6] == math.inf).all()) and bool((out[0, :, 9] == -math.inf).all())
     assert bool((out[0, :, 11] == 65504.0).all())
     assert bool(torch.isfinite(out[0, :, [d for d in range(64) if d not in (6, 9)]]).all())
+
+
+# ---------------------------------------------------------------------------
+# selection
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(5, 1, 136), (8, 1, 256), (16, 2, 160), (16, 1, 256), (32, 2, 200)], ids=str)
+@pytest.mark.parametrize("page", [16, 1], ids=["block chooses", "scores in memory"])
+def test_select_for_rows_of_wide_heads(gpu, shape, page):
+    """Rows of given sequences, more than 4 query heads of more than 128 dims a kv head."""
+    import torch
+    H, KV, D = shape
+    lens = [600, 130]
+    pool = Pool(torch, lens, H, KV, D, page, "f16", bounds=True, max_rows=11)
+    pool.cache.summarise()
+    rows = [(0, 600), (0, 1), (0, 17), (1, 130), (1, 0), (0, 599), (0, 600), (1, 64), (0, 300), (0, 301), (1, 5)]
+    q = torch.randn(len(rows), H, D, generator=pool.g).cuda()
+    seq = torch.tensor([s for s, _ in rows], dtype=torch.int32, device="cuda")
+    length = torch.tensor([n for _, n in rows], dtype=torch.int32, device="cuda")
+    got = run_select(torch, pool, q, "f32", len(rows), 9, 1, 2, row_sequence=seq.data_ptr(), row_length=length.data_ptr())
+    assert np.array_equal(got, select_reference(pool, q, rows, 9, 1, 2))
