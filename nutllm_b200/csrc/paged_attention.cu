@@ -1058,7 +1058,9 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
     float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int g = 0; g < p.group; g++) {
-        const float lse2 = a.lse2[h0 + g];
+        float lse2 = a.lse2[h0 + g];
+        if (lse2 == -INFINITY) /* every logit was: the head sees nothing */
+            lse2 = INFINITY;
         float x[4];
         if constexpr (kVec) {
             *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(z + int64_t(g) * p.capacity);

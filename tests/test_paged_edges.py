@@ -85,6 +85,29 @@ def test_infinite_values_reach_fp16_rows(gpu):
     assert bool(torch.isfinite(out[0, :, [d for d in range(64) if d not in (6, 9)]]).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+def test_logits_that_are_all_minus_infinity_add_no_weight(gpu, types):
+    """A row that gives every slot a weight of 0 is a row that sees nothing."""
+    import torch
+    lens = [40, 20]
+    pool = Pool(torch, lens, 4, 2, 64, 16, types[0], track=True)
+    for j in range(3):
+        pool.keys[int(pool.table_cpu[0, j]), :, :, 2] = float("inf")
+    q = torch.randn(2, 4, 64, generator=pool.g)
+    q[0, :, 2] = -1.0
+    q = q.to(dtypes(torch)[types[1]]).cuda()
+    out, lse = torch.full_like(q, 7.0), torch.zeros(2, 4, device="cuda")
+    w = torch.rand(2, 2, pool.capacity, generator=pool.g).cuda()
+    before = w.clone()
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), 2, dtype=KINDS[types[1]], lse=lse.data_ptr(), weights=w.data_ptr(),
+                         weights_out=w.data_ptr())
+    pool.cache.check()
+    assert not bool(out[0].any()) and bool((lse[0] == -math.inf).all())
+    assert torch.equal(w[0], before[0]) and torch.equal(w[1, :, 20:], before[1, :, 20:])
+    assert bool(torch.isfinite(w[1]).all()) and abs(float((w[1] - before[1]).sum()) - 4) < 1e-4
+
+
 # ---------------------------------------------------------------------------
 # selection
 
