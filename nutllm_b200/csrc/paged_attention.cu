@@ -912,6 +912,9 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         for (; x.tile < x.tile1; x.tile++) {
             issue(stage == 0 ? kStages - 1 : stage - 1);
             const uint32_t valid = masks[warp][stage];
+            float *z = !kLean && a.weights ? a.logits + (int64_t(x.row) * p.heads + first_head) * p.capacity +
+                                                 x.tile * kTile + warp * kChunk
+                                           : nullptr;
             bool arrived = valid != 0;
             if (arrived) {
                 arrived = stage_wait(&full[warp][stage], (phases >> stage) & 1);
@@ -933,12 +936,16 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
                                          : "memory");
                     __syncwarp();
                 }
-                float *z = !kLean && a.weights ? a.logits + (int64_t(x.row) * p.heads + first_head) * p.capacity +
-                                           x.tile * kTile + warp * kChunk
-                                     : nullptr;
                 op.step(at, valid, scratch, z, p.capacity, heads);
                 if (valid != 0xffffu)
                     fence_async(); /* the zeros, before the stage is filled again */
+            }
+            if (z != nullptr && (!arrived || valid != 0xffffu)) {
+                /* slots in use that could not be read have no weight */
+                const int used = min(kChunk, x.length - (x.tile * kTile + warp * kChunk));
+                for (int i = lane; i < heads * kChunk; i += 32)
+                    if (i % kChunk < used && !(arrived && ((valid >> (i % kChunk)) & 1)))
+                        z[int64_t(i / kChunk) * p.capacity + i % kChunk] = -INFINITY;
             }
             __syncwarp();
             stage = stage + 1 == kStages ? 0 : stage + 1;

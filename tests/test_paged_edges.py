@@ -108,6 +108,44 @@ def test_logits_that_are_all_minus_infinity_add_no_weight(gpu, types):
     assert bool(torch.isfinite(w[1]).all()) and abs(float((w[1] - before[1]).sum()) - 4) < 1e-4
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("bad", ["one page", "every page"])
+def test_slots_of_a_bad_page_receive_no_weight(gpu, types, bad):
+    """Whatever an earlier call left in the workspace: what is not read adds nothing, and the other slots get the weights of an
+    attention without it."""
+    import torch
+    n = 75
+    pool = Pool(torch, [n], 4, 2, 64, 16, types[0], track=True)
+    q = torch.randn(1, 4, 64, generator=pool.g).to(dtypes(torch)[types[1]]).cuda()
+    out = torch.zeros_like(q)
+    w = torch.zeros(1, 2, pool.capacity, device="cuda")
+
+    def attend():
+        pool.cache.attention(q.data_ptr(), out.data_ptr(), 1, dtype=KINDS[types[1]], weights=w.data_ptr(), weights_out=w.data_ptr())
+
+    attend()  # leaves logits
+    pool.cache.check()
+    start = torch.rand(1, 2, pool.capacity, generator=pool.g)
+    w.copy_(start)
+    if bad == "one page":
+        pool.table[0, 1] = pool.n_pages
+        read = [t for t in range(n) if not 16 <= t < 32]
+    else:
+        pool.table[0, :5] = -1
+        read = []
+    attend()
+    with pytest.raises(IndexError, match="page number"):
+        pool.cache.check()
+    got, want = w.cpu().double(), start.double()
+    for h in range(2):
+        _, _, x, dz, _ = head_reference(torch, q.cpu()[0, 2 * h:2 * h + 2], pool.k[0][h][read], pool.v[0][h][read], 1 / 8)
+        want[0, h, read] += x.sum(0)
+        tol = torch.zeros(pool.capacity, dtype=torch.float64)
+        tol[read] = ((2 * dz + (n + 64) * EPS) * x).sum(0) + 6 * EPS * want[0, h, read]
+        assert bool(((got[0, h] - want[0, h]).abs() <= tol).all())
+
+
 # ---------------------------------------------------------------------------
 # selection
 
