@@ -184,22 +184,27 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
     const int64_t base = int64_t(page) * p.page_stride + int64_t(head) * p.head_stride + o;
     T *keys = static_cast<T *>(p.keys) + base, *values = static_cast<T *>(p.values) + base;
     const int heads = a.q ? p.group : 0, units = heads + 2;
+    /* whether slot t's position has a rotation, where there are any: rows without one are skipped */
+    const auto turns = [&](int t) {
+        const int64_t pos = int64_t(t) + ahead;
+        return !a.cos || (pos >= 0 && pos < a.rope_rows);
+    };
     if (group < groups)
         for (int e = group; e < (t1 - t0) * units; e += groups) {
             const int t = t0 + e / units, unit = e % units;
             const int64_t row = row0 + (t - first), column = int64_t(head * p.group + unit) * D + o;
             float v[8], c[4], z[4];
+            if (!turns(t)) {
+                paged_fail(p, kPagedBadPosition);
+                continue;
+            }
             const R *x = unit < heads    ? static_cast<const R *>(a.q) + row * a.q_stride + column
                          : unit == heads ? static_cast<const R *>(a.k) + row * a.k_stride + head * D + o
                                          : static_cast<const R *>(a.v) + row * a.v_stride + head * D + o;
             load4<kVec>(x, v);
             load4<kVec>(x + half, v + 4);
-            const int64_t pos = int64_t(t) + ahead;
             if (a.cos && unit <= heads) {
-                const bool there = pos >= 0 && pos < a.rope_rows;
-                if (!there)
-                    paged_fail(p, kPagedBadPosition);
-                const int64_t turn = (there ? pos * half : 0) + o / 2;
+                const int64_t turn = (int64_t(t) + ahead) * half + o / 2;
                 load2<kVec>(a.cos + turn, c);
                 load2<kVec>(a.cos + turn + half / 2, c + 2);
                 load2<kVec>(a.sin + turn, z);
@@ -224,6 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
     if (a.positions || a.weights) {
         const int64_t at = (int64_t(s) * p.kv_heads + head) * p.capacity;
         for (int t = t0 + threadIdx.x; t < t1; t += kThreads) {
+            if (!turns(t))
+                continue;
             if (a.positions)
                 a.positions[at + t] = t + ahead;
             if (a.weights)

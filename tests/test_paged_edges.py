@@ -166,3 +166,34 @@ def test_select_for_rows_of_wide_heads(gpu, shape, page):
     length = torch.tensor([n for _, n in rows], dtype=torch.int32, device="cuda")
     got = run_select(torch, pool, q, "f32", len(rows), 9, 1, 2, row_sequence=seq.data_ptr(), row_length=length.data_ptr())
     assert np.array_equal(got, select_reference(pool, q, rows, 9, 1, 2))
+
+
+# ---------------------------------------------------------------------------
+# append
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_append_skips_rows_without_a_rotation(gpu, kind):
+    """A position outside the table is reported, and its row stored nowhere; the other rows are."""
+    import torch
+    lens, H, KV, D = [6, 20, 9], 4, 2, 64
+    pool = Pool(torch, lens, H, KV, D, 16, kind)
+    q, k, v = (torch.randn(6, n, D, generator=pool.g).cuda() for n in (H, KV, KV))
+    starts = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda")
+    seen = torch.tensor([1, 21, 9], dtype=torch.int32, device="cuda")  # positions -1, 0; 19, 20; 7, 8
+    turn = torch.ones(20, D // 2, device="cuda"), torch.zeros(20, D // 2, device="cuda")
+    q_out = torch.full_like(q, 7.0)
+    w, at = torch.full((3, KV, pool.capacity), 5.0, device="cuda"), torch.full((3, KV, pool.capacity), -3, dtype=torch.int32, device="cuda")
+    want = [x.clone() for x in (pool.keys, pool.values, q_out, w, at)]
+    for row, (s, slot) in {1: (0, 5), 2: (1, 18), 4: (2, 7), 5: (2, 8)}.items():
+        page = int(pool.table_cpu[s, slot // 16])
+        want[0][page, :, slot % 16], want[1][page, :, slot % 16] = k[row].to(want[0].dtype), v[row].to(want[1].dtype)
+        want[2][row], want[3][s, :, slot], want[4][s, :, slot] = q[row], 0.0, (0, 0, 19, 0, 7, 8)[row]
+    want[4][0, :, 5] = 0
+    pool.cache.append(q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), 6, 2, q_out=q_out.data_ptr(), cos=turn[0].data_ptr(),
+                      sin=turn[1].data_ptr(), rope_rows=20, seen=seen.data_ptr(), positions=at.data_ptr(), weights=w.data_ptr())
+    with pytest.raises(IndexError, match="rotation table"):
+        pool.cache.check()
+    for got, x in zip((pool.keys, pool.values, q_out, w, at), want):
+        assert torch.equal(got.nan_to_num(77.0) if got.is_floating_point() else got, x.nan_to_num(77.0) if x.is_floating_point() else x)
