@@ -488,7 +488,9 @@ nut_status nut_paged_select(nut_paged *paged, const nut_paged_select_args *args,
  * order of slots does not matter to the attention.  weights_out and
  * positions_out (which may be weights / positions) receive the moved
  * entries, 0 and -1 in the slots given up, and new_lengths (which may be
- * the view's lengths) min(length, budget).  Key bounds are not recomputed
+ * the view's lengths) min(length, budget).  A sequence with a bad length or,
+ * where it has to be trimmed, a bad page number stays as it is in all of
+ * these.  Key bounds are not recomputed
  * (nut_paged_summarise). */
 typedef struct nut_paged_evict_args {
     const float *weights;     /* [sequences][kv_heads][max_pages * page_size] */

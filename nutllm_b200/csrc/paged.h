@@ -95,7 +95,7 @@ struct PagedEvict {
     float *weights_out;
     int32_t *positions_out;
     int32_t *pairs;  /* [sequences][kv_heads][capacity]: holes, then sources from the far end */
-    int32_t *counts; /* [sequences][kv_heads][2]: pairs, old length */
+    int32_t *counts; /* [sequences][kv_heads][2]: pairs, new length (-1: as it was) */
 };
 
 /* head_dim as the attention's kernels are made for. */

@@ -47,12 +47,14 @@ struct SlotKeys {
 /* What both forms of the choice know of an item. */
 struct SlotItem {
     int length, m;      /* slots now, slots to keep */
+    bool bad;           /* the length is not one the table can hold */
     int64_t item, at;   /* its number, its first slot in the arrays */
     int32_t *holes, *sources;
     SlotKeys key;
     __device__ SlotItem(const PagedEvict &a, int s, int head) {
         const PagedPool &p = a.p;
         length = checked_length(p, p.lengths[s]);
+        bad = length != p.lengths[s];
         m = min(length, a.budget);
         item = int64_t(s) * p.kv_heads + head;
         at = item * p.capacity;
@@ -62,6 +64,31 @@ struct SlotItem {
                        a.recent ? int64_t(a.seen[s]) - a.recent : INT64_MAX};
     }
 };
+
+/* What forbids to trim a sequence: a bad length, or, where tokens will move, a
+ * page outside the pool.  Such a sequence is left as it is (counts of 0 and
+ * -1).  `me` of `threads` threads has its first page on the way from the
+ * start (0.5 us of a choice among few). */
+struct Pages {
+    int s, me, threads, end, first;
+    __device__ __forceinline__ Pages(const PagedPool &p, const SlotItem &x, int s_, int me_, int threads_)
+        : s(s_), me(me_), threads(threads_), end(x.m < x.length ? (x.length - 1) / p.page_size + 1 : 0), first(0) {
+        if (me < end)
+            first = p.table[int64_t(s) * p.max_pages + me];
+    }
+    __device__ __forceinline__ bool forbid(const PagedPool &p, const SlotItem &x) const {
+        bool bad = unsigned(first) >= unsigned(p.n_pages);
+        for (int j = me + threads; j < end; j += threads)
+            bad |= lookup(p, s, j) < 0;
+        if (bad)
+            paged_fail(p, kPagedBadPage);
+        return bad || x.bad;
+    }
+};
+__device__ __forceinline__ void leave(const PagedEvict &a, const SlotItem &x) {
+    a.counts[x.item * 2] = 0;
+    a.counts[x.item * 2 + 1] = -1;
+}
 
 /* The slots i0 .. i0 + there - 1 as holes (to be filled) and sources. */
 __device__ __forceinline__ void holes_and_sources(uint32_t kept, int i0, int there, int m, uint32_t &hole,
@@ -98,14 +125,21 @@ __global__ void __launch_bounds__(kChooseThreads)
     const SlotItem x(a, blockIdx.y, blockIdx.x);
     const int tid = threadIdx.x, i0 = tid * N, there = max(0, min(N, x.length - i0));
     uint32_t k[N], threshold;
+    const Pages pages(a.p, x, blockIdx.y, tid, kChooseThreads);
     x.key.own(i0, there, k);
     int quota, total;
     choose_largest<1>(x.key, x.length, x.length, x.m, k, scratch, threshold, quota);
-    int ties = 0;
+    /* counted with the ties, below 2^14 of them */
+    int ties = int(pages.forbid(a.p, x)) << 16;
 #pragma unroll
     for (int e = 0; e < N; e++)
         ties += e < there && k[e] == threshold;
-    int rank = block_before(ties, scratch, 0, total);
+    int rank = block_before(ties, scratch, 0, total) & 0xffff;
+    if (total >> 16) {
+        if (tid == 0)
+            leave(a, x);
+        return;
+    }
     uint32_t kept = 0, hole, source;
 #pragma unroll
     for (int e = 0; e < N; e++)
@@ -143,6 +177,15 @@ __global__ void __launch_bounds__(kChooseThreads)
     begin_kernel();
     const int rank = int(blockIdx.x) % kBlocks, tid = threadIdx.x;
     const SlotItem x(a, blockIdx.y, int(blockIdx.x) / kBlocks);
+    int none, forbidden;
+    const Pages pages(a.p, x, blockIdx.y, rank * kChooseThreads + tid, kBlocks * kChooseThreads);
+    cluster_before<kBlocks>(__syncthreads_or(pages.forbid(a.p, x)), scratch, 3, none, forbidden);
+    if (forbidden) {
+        if (rank == 0 && tid == 0)
+            leave(a, x);
+        cooperative_groups::this_cluster().sync(); /* shared memory done with */
+        return;
+    }
     const int run = (x.length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn; /* whole groups of kOwn */
     const int from = min(rank * run, x.length), n = min(run, x.length - from);
     SlotKeys key = x.key;
@@ -236,8 +279,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constan
     const int64_t item = int64_t(s) * p.kv_heads + head;
     begin_kernel();
     const int n = a.counts[item * 2];
-    if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0)
-        a.new_lengths[s] = a.counts[item * 2 + 1];
+    const int left = a.counts[item * 2 + 1];
+    if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0 && left >= 0)
+        a.new_lengths[s] = left;
     const int32_t *holes = a.pairs + item * p.capacity, *sources = holes + p.capacity / 2;
     const int groups = kMoveThreads / row16, group = threadIdx.x / row16, piece = threadIdx.x % row16;
     if (group >= groups)

@@ -197,3 +197,50 @@ def test_append_skips_rows_without_a_rotation(gpu, kind):
         pool.cache.check()
     for got, x in zip((pool.keys, pool.values, q_out, w, at), want):
         assert torch.equal(got.nan_to_num(77.0) if got.is_floating_point() else got, x.nan_to_num(77.0) if x.is_floating_point() else x)
+
+
+# ---------------------------------------------------------------------------
+# eviction
+
+
+def eviction(torch, lens, max_pages=None, kv=2):
+    pool = Pool(torch, lens, kv, kv, 64, 16, "f16", max_pages=max_pages)
+    S, cap = len(lens), pool.capacity
+    w = torch.rand(S, kv, cap, generator=pool.g)
+    at = torch.arange(cap, dtype=torch.int32).expand(S, kv, cap).contiguous()
+    return pool, w.cuda(), at.cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_pages", [8, 600], ids=["a block", "a cluster"])
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in place"])
+@pytest.mark.parametrize("bad", ["length", "page"])
+def test_evict_leaves_a_sequence_alone_that_it_cannot_serve(gpu, max_pages, in_place, bad):
+    """A bad length or page number is reported, and nothing of its sequence changes; the other one is trimmed."""
+    import torch
+    pool, w, at = eviction(torch, [100, 90], max_pages)
+    if bad == "length":
+        pool.lengths[0] = pool.capacity + 1
+    else:
+        pool.table[0, 2] = -1
+    seen = torch.tensor([100, 90], dtype=torch.int32, device="cuda")
+    wo, po, left = (w, at, pool.lengths) if in_place else (torch.full_like(w, 9.0), torch.full_like(at, 9), torch.full_like(pool.lengths, 9))
+    of = [x[0].clone() for x in (wo, po, left)]
+    mine = pool.table_cpu[0, :7].long().cuda()
+    before = pool.keys[mine].clone(), pool.values[mine].clone()
+    want_w = w[1].cpu()
+    pool.cache.evict(w.data_ptr(), at.data_ptr(), seen.data_ptr(), 50, sinks=2, recent=3, new_lengths=left.data_ptr(),
+                     weights_out=wo.data_ptr(), positions_out=po.data_ptr())
+    with pytest.raises(IndexError, match="length" if bad == "length" else "page number"):
+        pool.cache.check()
+    for got, x in zip((wo, po, left), of):
+        assert torch.equal(got[0], x)
+    assert torch.equal(pool.keys[mine].nan_to_num(7.0), before[0].nan_to_num(7.0))
+    assert torch.equal(pool.values[mine].nan_to_num(7.0), before[1].nan_to_num(7.0))
+    assert int(left[1]) == 50
+    for h in range(2):
+        key = want_w[h, :90].clone()
+        key[:2], key[87:90] = 2.0, 2.0
+        kept = key.sort(descending=True, stable=True).indices[:50]
+        assert sorted(po.cpu()[1, h, :50].tolist()) == sorted(kept.tolist())
+        assert bool((po.cpu()[1, h, 50:90] == -1).all())
