@@ -465,8 +465,9 @@ nut_status nut_paged_attention(nut_paged *paged, const nut_paged_attention_args 
  * under which |x| <= 127,
  *   score(page) = max over the group's heads of
  *                 u * bound_scale * sum_d max(x_d greatest_d, x_d least_d).
- * Every term is an integer times a power of two, so the score is exact and
- * the choice does not depend on the order of any sum.  The first sink_pages
+ * Every term is an integer times a power of two, so the score is exact (up
+ * to fp32's greatest numbers, which stand for what lies beyond them) and the
+ * choice does not depend on the order of any sum.  The first sink_pages
  * and the last recent_pages pages of the row's length come before all
  * others; then the highest scores, ties to the lowest page.  selected[r][g]
  * receives the min(n_selected, pages) chosen ones ascending, then -1. */

@@ -6,7 +6,8 @@
  * one product of [M | L] with [max(x, 0) | min(x, 0)]: mma.sync m16n8k32 in
  * 8 bits, 16 pages by 8 query heads (of one row, or of two or four).  The sum is at most
  * 256 * 127 * 128 < 2^24 in size, so it is exact in an int and in fp32,
- * whatever its order.
+ * whatever its order; what the units carry beyond fp32's range counts as its
+ * greatest number.
  *
  * It reads 2 head_dim + 4 bytes of each page and kv head, a 32nd of what the
  * page's 16 keys and values take in 16 bits.  35 MB of them (32 sequences of
@@ -29,6 +30,7 @@ constexpr int kWarps = 8;
 constexpr int kPages = 16;  /* of a warp's product */
 constexpr int kHeads = 8;   /* columns of a warp's product */
 constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
+constexpr float kMostFloat = 3.402823466e38f;
 constexpr int kFusedPages = 512; /* most pages of a row that its block chooses from at once */
 
 /* A warp writes the `n` first-ranked of a row's `pages` scores (at most 32 N,
@@ -223,7 +225,8 @@ __global__ void __launch_bounds__(kWarps * 32, KC <= 4 ? 3 : 2)
                     if (j < pages) {
                         float *to = kFused ? kept + row * kFusedPages + j
                                            : a.scores + (int64_t(row0 + row) * p.kv_heads + head) * p.max_pages + j;
-                        float v = there[h] ? best * scale[h] : -INFINITY;
+                        /* beyond fp32's range (pages with infinite keys): below the pages that are always read */
+                        float v = there[h] ? fminf(fmaxf(best * scale[h], -kMostFloat), kMostFloat) : -INFINITY;
                         if (gq > 0)
                             v = fmaxf(v, *to);
                         if (j < a.sink_pages || j >= pages - a.recent_pages)

@@ -168,6 +168,29 @@ def test_select_for_rows_of_wide_heads(gpu, shape, page):
     assert np.array_equal(got, select_reference(pool, q, rows, 9, 1, 2))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 1], ids=["block chooses", "scores in memory"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_scores_beyond_fp32_stay_behind_the_pages_that_are_always_read(gpu, page, kind):
+    """Infinite keys count as the largest finite float, whose products with a query pass fp32's range: such scores are equal to
+    one another, below the sinks and the recent pages and above all others."""
+    import torch
+    pages = 40 if page == 16 else 700
+    pool = Pool(torch, [pages * page], 4, 2, 64, page, kind, bounds=True)
+    for j in (7, 9):
+        pool.keys[int(pool.table_cpu[0, j]), :, 0, 3] = float("inf")
+    pool.keys[int(pool.table_cpu[0, 11]), :, :, 5] = float("inf")  # every key of the page: no score above -inf
+    pool.cache.summarise()
+    q = torch.randn(1, 4, 64, generator=pool.g)
+    q[:, :, 3], q[:, :, 5] = 3.0, -3.0
+    q = q.cuda()
+    for n, want in ((2, [0, pages - 1]), (3, [0, 7, pages - 1]), (4, [0, 7, 9, pages - 1])):
+        got = run_select(torch, pool, q, "f32", 1, n, 1, 1)
+        assert got.tolist() == [[want, want]]
+    most = run_select(torch, pool, q, "f32", 1, pages - 1, 1, 1)
+    assert most.tolist() == [[[j for j in range(pages) if j != 11]] * 2]
+
+
 # ---------------------------------------------------------------------------
 # append
 
