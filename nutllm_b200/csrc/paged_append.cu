@@ -143,8 +143,11 @@ __device__ void page_bounds(const PagedPool &p, int page, int head, int used) {
     for (int k = 0; k < kEach; k++) {
         const int d = threadIdx.x + k * kThreads;
         if (d < D) {
-            p.bounds[at * 2 * D + d] = int8_t(ceilf(hi[k] * inv));
-            p.bounds[at * 2 * D + D + d] = int8_t(floorf(lo[k] * inv));
+            /* a key below 2^-149 of the unit is not a whole 0 of it */
+            const float most_units = hi[k] > 0.0f ? fmaxf(ceilf(hi[k] * inv), 1.0f) : ceilf(hi[k] * inv);
+            const float least_units = lo[k] < 0.0f ? fminf(floorf(lo[k] * inv), -1.0f) : floorf(lo[k] * inv);
+            p.bounds[at * 2 * D + d] = int8_t(most_units);
+            p.bounds[at * 2 * D + D + d] = int8_t(least_units);
         }
     }
     if (threadIdx.x == 0)

@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.test_paged import EPS, KINDS, TYPES, Pool, dtypes, head_reference, run_select, select_reference
+from tests.test_paged import EPS, KINDS, TYPES, Pool, check_bounds, dtypes, head_reference, run_select, select_reference
 
 # ---------------------------------------------------------------------------
 # attention
@@ -189,6 +189,25 @@ def test_scores_beyond_fp32_stay_behind_the_pages_that_are_always_read(gpu, page
         assert got.tolist() == [[want, want]]
     most = run_select(torch, pool, q, "f32", 1, pages - 1, 1, 1)
     assert most.tolist() == [[[j for j in range(pages) if j != 11]] * 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_bounds_hold_keys_far_below_the_unit(gpu, kind):
+    """A key so small beside the page's greatest that it is no whole number of units: its bound is one unit, not none."""
+    import torch
+    pool = Pool(torch, [2], 1, 1, 16, 4, kind, bounds=True, fill=False)
+    k = torch.zeros(2, 16)
+    k[0, 3], k[1, 4] = 3e38, float("-inf")
+    k[:, 5], k[:, 6] = 1e-30, -1e-30
+    k[0, 7], k[1, 7], k[:, 8] = 1e-38, -1e-38, 1e-3
+    k = k.to(dtypes(torch)[kind])
+    pool.put(0, k[None], k[None], 0)
+    pool.cache.summarise()
+    pool.cache.check()
+    check_bounds(pool, 0, 2)
+    b = pool.bounds.cpu()[int(pool.table_cpu[0, 0]), 0]
+    assert b[:, 5].tolist() == [1, 0] and b[:, 6].tolist() == [0, -1] and b[:, 7].tolist() == [1, -1]
 
 
 # ---------------------------------------------------------------------------
