@@ -67,6 +67,13 @@ __device__ __forceinline__ bool stage_wait(uint64_t *bar, uint32_t parity) {
     }
 }
 
+/* A wait of this thread that gave up: recorded, and the copy, which may still
+ * be on its way, gets that time once more before its place is used again. */
+__device__ __noinline__ void gave_up(const PagedPool &p, uint64_t *bar, uint32_t parity) {
+    paged_fail(p, kPagedTimeout);
+    stage_wait(bar, parity);
+}
+
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -601,7 +608,7 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
         fetch(0, min(parts, most));
     const bool fit = parts <= most; /* then the statistics are read from the copies too */
     if (!stage_wait(bar, phase))
-        paged_fail(p, kPagedTimeout);
+        gave_up(p, bar, phase);
     phase ^= 1;
     auto statistic = [&](int c, int i) { return fit ? copies[c * pitch + i] : __ldcg(part(c) + i); };
     for (int g = warp; g < heads; g += kWarps) {
@@ -637,7 +644,7 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
         const int n = min(parts - c, most);
         if (c > 0) {
             if (!stage_wait(bar, phase))
-                paged_fail(p, kPagedTimeout);
+                gave_up(p, bar, phase);
             phase ^= 1;
         }
 #pragma unroll
@@ -917,12 +924,13 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
                                            : nullptr;
             bool arrived = valid != 0;
             if (arrived) {
-                arrived = stage_wait(&full[warp][stage], (phases >> stage) & 1);
-                phases ^= 1u << stage;
+                /* the lanes give up together: what follows needs the whole warp */
+                arrived = __all_sync(0xffffffffu, stage_wait(&full[warp][stage], (phases >> stage) & 1));
                 if (!arrived) {
-                    paged_fail(p, kPagedTimeout);
+                    gave_up(p, &full[warp][stage], (phases >> stage) & 1);
                     dead = true;
                 }
+                phases ^= 1u << stage;
             }
             if (arrived) {
                 const uint32_t at = ring_at + stage * Op::kStageBytes;
