@@ -412,9 +412,11 @@ nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *arg
             raise(NUT_INVALID_ARGUMENT, "n_selected must be positive");
         if (g.selected && g.n_selected * p.page_size > (int64_t(1) << 30))
             raise(NUT_LENGTH_ERROR, "too many selected pages");
-        /* the kernel counts tiles of at least 32 slots, and 3 for each item, in 32 bits */
+        /* the kernel counts tiles of at least 32 slots, and 3 for each item, in 32 bits; its
+         * blocks' shares are rounded up, and pass the end by less than a place a block */
         const int64_t slots = g.selected ? g.n_selected * p.page_size : p.capacity;
-        if (g.rows * p.kv_heads * ((p.group + 7) / 8) * (slots / 32 + 4) > INT_MAX)
+        if (g.rows * p.kv_heads * ((p.group + 7) / 8) * (slots / 32 + 4) >
+            INT_MAX - nut::kMaxSms * nut::kMaxCtasPerSm)
             raise(NUT_LENGTH_ERROR, "too many rows for so long a table: split the call");
         if ((g.weights == nullptr) != (g.weights_out == nullptr))
             raise(NUT_INVALID_ARGUMENT, "weights and weights_out go together");

@@ -7,6 +7,7 @@ import math
 import numpy as np
 import pytest
 
+import nutllm_b200 as nb
 from tests.test_paged import EPS, KINDS, TYPES, Pool, check_bounds, dtypes, head_reference, run_select, select_reference
 
 # ---------------------------------------------------------------------------
@@ -144,6 +145,19 @@ def test_slots_of_a_bad_page_receive_no_weight(gpu, types, bad):
         tol = torch.zeros(pool.capacity, dtype=torch.float64)
         tol[read] = ((2 * dz + (n + 64) * EPS) * x).sum(0) + 6 * EPS * want[0, h, read]
         assert bool(((got[0, h] - want[0, h]).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_attention_leaves_room_behind_its_line_of_tiles(gpu):
+    """42,966 rows over a table of 49,977 pages of 32 slots come to 2^31 - 2 places: the blocks' shares, rounded up, would pass
+    32 bits."""
+    import torch
+    x = torch.zeros(4096, device="cuda")
+    p = x.data_ptr()
+    cache = nb.PagedCache(p, p, p, p, sequences=1, max_pages=49977, n_pages=1, page_size=32, heads=1, kv_heads=1, head_dim=8,
+                          max_rows=42966)
+    with pytest.raises(nb.LengthError, match="split the call"):
+        cache.attention(p, p, 42966, row_sequence=p)
 
 
 # ---------------------------------------------------------------------------
