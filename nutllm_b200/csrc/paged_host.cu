@@ -410,7 +410,7 @@ nut_status nut_paged_attention(nut_paged *h, const nut_paged_attention_args *arg
         check_rows(*h, g.rows, g.row_sequence);
         if (g.selected && g.n_selected <= 0)
             raise(NUT_INVALID_ARGUMENT, "n_selected must be positive");
-        if (g.selected && g.n_selected * p.page_size > (int64_t(1) << 30))
+        if (g.selected && g.n_selected > (int64_t(1) << 30) / p.page_size)
             raise(NUT_LENGTH_ERROR, "too many selected pages");
         /* the kernel counts tiles of at least 32 slots, and 3 for each item, in 32 bits; its
          * blocks' shares are rounded up, and pass the end by less than a place a block */

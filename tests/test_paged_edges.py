@@ -160,6 +160,17 @@ def test_attention_leaves_room_behind_its_line_of_tiles(gpu):
         cache.attention(p, p, 42966, row_sequence=p)
 
 
+@pytest.mark.gpu
+def test_attention_refuses_lists_beyond_any_table(gpu):
+    import torch
+    pool = Pool(torch, [10, 20], 4, 2, 64, 16, "f16", bounds=True)
+    x = torch.zeros(4096, device="cuda")
+    p = x.data_ptr()
+    for n in (1 << 27, 1 << 60, (1 << 60) + 1, (1 << 63) - 1):
+        with pytest.raises(nb.LengthError, match="paged: "):
+            pool.cache.attention(p, p, 2, selected=p, n_selected=n)
+
+
 # ---------------------------------------------------------------------------
 # selection
 
