@@ -365,6 +365,9 @@ nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, voi
             raise(NUT_LENGTH_ERROR, "too many rows");
         if (g.max_new > p.capacity)
             raise(NUT_LENGTH_ERROR, "more new tokens than a sequence can hold");
+        /* a block counts a page's rows and steps beyond them by its threads */
+        if (std::min<int64_t>(g.max_new, p.page_size) * ((g.q ? p.group : 0) + 2) > INT_MAX - 1024)
+            raise(NUT_LENGTH_ERROR, "too many rows for one page: append fewer at a time");
         if (g.rows == 0 || g.max_new == 0)
             return;
         a.q = g.q;

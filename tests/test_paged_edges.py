@@ -266,6 +266,17 @@ def test_append_skips_rows_without_a_rotation(gpu, kind):
         assert torch.equal(got.nan_to_num(77.0) if got.is_floating_point() else got, x.nan_to_num(77.0) if x.is_floating_point() else x)
 
 
+@pytest.mark.gpu
+def test_append_refuses_pages_whose_rows_it_cannot_count(gpu):
+    """A page of 2^24 slots with 127 query heads a kv head has more rows than 32 bits count."""
+    import torch
+    x = torch.zeros(4096, device="cuda")
+    p = x.data_ptr()
+    cache = nb.PagedCache(p, p, p, p, sequences=1, max_pages=1, n_pages=1, page_size=1 << 24, heads=127, kv_heads=1, head_dim=8)
+    with pytest.raises(nb.LengthError, match="paged: "):
+        cache.append(p, p, p, p, 1 << 24, 1 << 24, q_out=p)
+
+
 # ---------------------------------------------------------------------------
 # eviction
 
