@@ -24,9 +24,11 @@ struct Failure {
 [[noreturn]] void raise(nut_status s, const std::string &m) { throw Failure{s, "paged: " + m}; }
 
 void cuda_check(cudaError_t e, const char *what) {
-    if (e != cudaSuccess)
+    if (e != cudaSuccess) {
+        cudaGetLastError(); /* reported here: the next call's own check is not to find it */
         throw Failure{NUT_RUNTIME_ERROR,
                       std::string("cuda: ") + what + ": " + cudaGetErrorString(e)};
+    }
 }
 
 template <typename F> nut_status guarded(F &&body) {

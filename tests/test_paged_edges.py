@@ -322,3 +322,21 @@ def test_evict_leaves_a_sequence_alone_that_it_cannot_serve(gpu, max_pages, in_p
         kept = key.sort(descending=True, stable=True).indices[:50]
         assert sorted(po.cpu()[1, h, :50].tolist()) == sorted(kept.tolist())
         assert bool((po.cpu()[1, h, 50:90] == -1).all())
+
+
+# ---------------------------------------------------------------------------
+# errors
+
+
+@pytest.mark.gpu
+def test_a_failed_call_leaves_no_error_for_the_next_one(gpu):
+    """A workspace beyond the device's memory is refused, and the library's next call, which checks its launch, does not find
+    that error."""
+    import torch
+    a, c = torch.ones(4096, device="cuda"), torch.zeros(16, 16, device="cuda")
+    p = a.data_ptr()
+    with pytest.raises(RuntimeError, match="workspace"):
+        nb.PagedCache(p, p, p, p, sequences=65535, max_pages=1 << 20, n_pages=1, page_size=1 << 10, heads=64, kv_heads=1, head_dim=64,
+                      track_weights=True)
+    nb.matmul_f32_async(p, p, c.data_ptr(), 16, 64, 16, torch.cuda.current_stream().cuda_stream)
+    assert bool((c == 64).all())
