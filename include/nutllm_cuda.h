@@ -441,7 +441,9 @@ nut_status nut_paged_summarise(nut_paged *paged, void *stream);
  * sequence are listed, in any order, -1 for none; a page listed twice counts
  * twice.  With weights / weights_out (one row per sequence, no `selected`)
  *   weights_out[s][g][t] = weights[s][g][t] + sum of w_t over the group's heads
- * for the slots in use; the two may be the same buffer. */
+ * for the slots in use; the two may be the same buffer.  (A prompt's tokens
+ * are ranked by attending its newest rows a second time, one row of every
+ * sequence a call, with row_length.) */
 typedef struct nut_paged_attention_args {
     const void *q; /* [rows][heads][head_dim] */
     void *out;

@@ -11,6 +11,8 @@ checkpoint to load); what it shows is how the operators go together:
   attention  over each sequence's own pages; with a budget it also collects
              the attention weight each cached token received
   select + attention  the same over the pages whose keys can match best
+             (a prompt's tokens receive that of its newest rows, attended to
+             a second time, one row of every sequence a call)
   evict      once a sequence outgrows its budget by a page or more, then its
              pages behind the budget go back to the pool
 
@@ -27,6 +29,7 @@ import torch
 import nutllm_b200 as nb
 
 PROMPT_ROWS = 512  # prompt rows of one attention call
+PROMPT_WINDOW = 32  # newest prompt rows whose attention ranks a prompt's tokens for eviction
 TYPES = {torch.float32: nb.F32, torch.float16: nb.F16, torch.bfloat16: nb.BF16}
 
 
@@ -127,6 +130,18 @@ class PagedSession:
                 row_length=length[i:].data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
         return out
 
+    def weigh_prompt(self, layer: int, q: torch.Tensor, starts: torch.Tensor, news: list) -> None:
+        """Collects the attention weight that the newest rows of each sequence's prompt (q, as append() gave it) give to
+        its tokens: weights are collected from one row per sequence, so a call for each place from the end."""
+        t, new = self.layers[layer], starts[1:] - starts[:-1]
+        weights = t["weights"].data_ptr()
+        for back in range(min(PROMPT_WINDOW, max(news))):
+            rows = q[(starts[1:].long() - 1 - back).clamp(min=0)]
+            length = torch.where(new > back, self.lengths - back, 0).int()  # 0: sees nothing, adds nothing
+            out = torch.empty_like(rows)
+            t["cache"].attention(rows.data_ptr(), out.data_ptr(), rows.shape[0], dtype=TYPES[q.dtype], row_length=length.data_ptr(),
+                                 weights=weights, weights_out=weights, stream=torch.cuda.current_stream().cuda_stream)
+
     def trim(self) -> bool:
         """Evicts down to the budget where a sequence is a page or more beyond it; whether it did."""
         if not self.budget or max(self.length) < self.budget + self.page_size:
@@ -171,6 +186,8 @@ def decode(session: PagedSession, weights: list, prompts: list, steps: int) -> t
     upto = torch.cat([torch.arange(1, n + 1) for n in news]).int().cuda()
     for i, (qkv, out) in enumerate(weights):
         q = session.append(i, norm(x) @ qkv, starts, max(news))
+        if session.budget:
+            session.weigh_prompt(i, q, starts, news)
         x = x + session.attend_prompt(i, q, seq, upto) @ out
     h, got = norm(x[starts[1:].long() - 1]), []
     for _ in range(steps):

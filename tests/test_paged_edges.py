@@ -340,3 +340,40 @@ def test_a_failed_call_leaves_no_error_for_the_next_one(gpu):
                       track_weights=True)
     nb.matmul_f32_async(p, p, c.data_ptr(), 16, 64, 16, torch.cuda.current_stream().cuda_stream)
     assert bool((c == 64).all())
+
+
+# ---------------------------------------------------------------------------
+# the serving loop
+
+
+@pytest.mark.gpu
+def test_prompts_beyond_the_budget_keep_the_tokens_their_last_rows_attend_to(gpu):
+    """The first trim, before any step: of each prompt's tokens those stay that its newest 32 rows give most weight (first
+    layer, in 64 bits; a weight is a sum of 128 softmax weights in fp32, off by less than 1e-5 of the greatest)."""
+    import torch
+    from tests.test_paged_demo import D, HEADS, KV, LAYERS, setup as make
+    lens, budget, sinks, recent = [100, 20, 70], 48, 2, 8
+    demo, weights, prompts = make(torch, lens)
+    session = demo.PagedSession(3, LAYERS, HEADS, KV, D, pages=20, max_pages=8, dtype=torch.float32, budget=budget, sinks=sinks,
+                                recent=recent)
+    demo.decode(session, weights, prompts, 1)
+    session.check()
+    assert session.length == [49, 21, 49]
+    for s in (0, 2):
+        n = lens[s]
+        x = demo.norm(prompts[s].double()) @ weights[0][0].double()
+        turn = torch.polar(torch.ones(n, 1, D // 2).double(), torch.arange(n)[:, None, None] * 10000.0 ** (
+            -torch.arange(0, D, 2).double() / D)).cuda()
+        qk = torch.view_as_real(torch.view_as_complex(x[:, :(HEADS + KV) * D].reshape(n, -1, D // 2, 2).contiguous()) * turn)
+        qk = qk.reshape(n, HEADS + KV, D).transpose(0, 1)
+        z = qk[:HEADS, n - 32:] @ qk[HEADS:].repeat_interleave(HEADS // KV, 0).transpose(1, 2) / D ** 0.5
+        late = torch.arange(n, device="cuda") > torch.arange(n - 32, n, device="cuda")[:, None]
+        w = torch.softmax(z.masked_fill(late, -math.inf), -1).sum(1).reshape(KV, -1, n).sum(1).cpu()
+        for h in range(KV):
+            kept = session.layers[0]["positions"][s, h, :budget].long().cpu()
+            stays = torch.zeros(n, dtype=torch.bool)
+            stays[kept] = True
+            assert int(stays.sum()) == budget and bool(stays[:sinks].all()) and bool(stays[n - recent:].all())
+            free = torch.ones(n, dtype=torch.bool)
+            free[:sinks], free[n - recent:] = False, False
+            assert float(w[h][stays & free].min()) >= float(w[h][~stays].max()) - 1e-5 * float(w[h].max())
