@@ -74,12 +74,13 @@ class PagedSession:
 
     def extend(self, news: list) -> torch.Tensor:
         """Makes room for news[s] more tokens of each sequence; the rows' `starts`."""
+        pages = [-(-(self.length[s] + n) // self.page_size) for s, n in enumerate(news)]
+        if max(pages) > self.table.shape[1] or sum(pages) - sum(map(len, self.owned)) > len(self.free):
+            raise RuntimeError("paged session: out of pages")
         for s, n in enumerate(news):
             self.length[s] += n
             self.seen[s] += n
-            while len(self.owned[s]) * self.page_size < self.length[s]:
-                if not self.free or len(self.owned[s]) == self.table.shape[1]:
-                    raise RuntimeError("paged session: out of pages")
+            while len(self.owned[s]) < pages[s]:
                 page = self.free.pop()
                 self.table[s, len(self.owned[s])] = page
                 self.owned[s].append(page)

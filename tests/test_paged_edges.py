@@ -377,3 +377,22 @@ def test_prompts_beyond_the_budget_keep_the_tokens_their_last_rows_attend_to(gpu
             free = torch.ones(n, dtype=torch.bool)
             free[:sinks], free[n - recent:] = False, False
             assert float(w[h][stays & free].min()) >= float(w[h][~stays].max()) - 1e-5 * float(w[h].max())
+
+
+@pytest.mark.gpu
+def test_a_refused_extension_leaves_the_session_as_it_was(gpu):
+    import torch
+    from nutllm_b200 import paged_demo as demo
+    session = demo.PagedSession(2, 1, 4, 2, 32, pages=6, max_pages=4)
+    session.extend([20, 30])
+
+    def state():
+        return (list(session.length), list(session.seen), list(session.free), [list(p) for p in session.owned],
+                session.table.tolist(), session.lengths.tolist())
+
+    before = state()
+    for news in ([20, 30], [0, 40], [65, 0]):  # more pages than are free, more than the table holds (two ways)
+        with pytest.raises(RuntimeError, match="out of pages"):
+            session.extend(news)
+        assert state() == before
+    assert session.extend([12, 1]).tolist() == [0, 12, 13] and session.lengths.tolist() == [32, 31]
