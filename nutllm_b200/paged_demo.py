@@ -181,6 +181,8 @@ def decode(session: PagedSession, weights: list, prompts: list, steps: int) -> t
     """Prompts (hidden rows [n][dim] of each sequence), then `steps` tokens of every sequence, each fed the hidden
     row before it; the last hidden rows of all steps [steps][sequences][dim]."""
     news = [len(p) for p in prompts]
+    if not all(news):
+        raise ValueError("paged session: empty prompt")
     starts = session.extend(news)
     x = torch.cat(prompts)
     seq = torch.repeat_interleave(torch.arange(len(news)), torch.tensor(news)).int().cuda()

@@ -396,3 +396,12 @@ def test_a_refused_extension_leaves_the_session_as_it_was(gpu):
             session.extend(news)
         assert state() == before
     assert session.extend([12, 1]).tolist() == [0, 12, 13] and session.lengths.tolist() == [32, 31]
+
+
+
+def test_the_loop_refuses_empty_prompts():
+    """Their first step would be fed another sequence's row."""
+    import torch
+    from nutllm_b200 import paged_demo as demo
+    with pytest.raises(ValueError, match="empty prompt"):
+        demo.decode(None, [], [torch.zeros(3, 8), torch.zeros(0, 8)], 1)
