@@ -35,7 +35,9 @@ constexpr int kBlock = kChunk * 128; /* a chunk's 128-byte columns, in the 128-b
 /* What an item costs besides its tiles, in tiles: with 0, 1, 2 and 3 a batch
  * whose shares hold 1 to 20 items took 147, 108, 101 and 100 us. */
 constexpr int kItemCost = 3;
-constexpr float kSlack = 8.0f; /* log2 by which a logit may pass the maximum in use */
+/* log2 by which a logit may pass the maximum in use: with kLift, which may
+ * round to 8 beside a maximum of 2^24 or more, 2^15 at most */
+constexpr float kSlack = 7.0f;
 constexpr uint64_t kPagedWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -271,9 +273,9 @@ template <typename T, typename R, int DP_> struct Halves {
                         z[int64_t(g) * stride + 8 * i + 2 * t + j] = s2[i][j];
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        /* the maximum in use may lag behind by kSlack: weights then reach 2^8
-         * (times 2^kLift), and outputs are rarely rescaled */
-        const float next = top > m + kSlack || m == -INFINITY ? fmaxf(m, top) : m;
+        /* the maximum in use may lag behind by kSlack (the difference is exact
+         * where it matters): outputs are rarely rescaled */
+        const float next = top - m > kSlack || m == -INFINITY ? fmaxf(m, top) : m;
         if (__any_sync(0xffffffffu, next != m)) {
             const float keep = m == next ? 1.0f : exp2f(m - next);
             l *= keep;

@@ -171,6 +171,32 @@ def test_attention_refuses_lists_beyond_any_table(gpu):
             pool.cache.attention(p, p, 2, selected=p, n_selected=n)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+@pytest.mark.parametrize("step", [2, 4, 8], ids=lambda s: f"+{s}")
+@pytest.mark.parametrize("power", [23, 24, 25, 26, 27])
+def test_logits_beyond_whole_numbers_stay_finite(gpu, types, power, step):
+    """Logits of 2^23 and more, where fp32 counts in steps of 1 to 16: whatever the maximum in use rounds to, weights stay in
+    their type's range.  The later half of the slots lies `step` (times log 2) higher, or the same where that is less than a
+    step: outputs lie between the values of the two."""
+    import torch
+    n, rows, D = 256, 512, 64
+    pool = Pool(torch, [n], 4, 1, D, 16, types[0], max_rows=rows, fill=False)
+    k = torch.zeros(1, n, D)
+    k[:, :, 0], k[:, n // 2:, 1] = 2.0 ** 14, step * 2.0 ** (14 - power)
+    v = torch.ones(1, n, D)
+    v[:, n // 2:] = 2.0
+    pool.put(0, k.to(pool.keys.dtype), v.to(pool.keys.dtype), 0)
+    q = torch.zeros(rows, 4, D)
+    q[:, :, :2] = 1.0
+    q, seq = q.to(dtypes(torch)[types[1]]).cuda(), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    out = torch.zeros_like(q)
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), rows, dtype=KINDS[types[1]], scale=2.0 ** (power - 14) * math.log(2.0),
+                         row_sequence=seq.data_ptr())
+    pool.cache.check()
+    assert bool(((out >= 1.0) & (out <= 2.0)).all())
+
+
 # ---------------------------------------------------------------------------
 # selection
 
