@@ -177,15 +177,9 @@ __global__ void __launch_bounds__(kChooseThreads)
     begin_kernel();
     const int rank = int(blockIdx.x) % kBlocks, tid = threadIdx.x;
     const SlotItem x(a, blockIdx.y, int(blockIdx.x) / kBlocks);
-    int none, forbidden;
     const Pages pages(a.p, x, blockIdx.y, rank * kChooseThreads + tid, kBlocks * kChooseThreads);
-    cluster_before<kBlocks>(__syncthreads_or(pages.forbid(a.p, x)), scratch, 3, none, forbidden);
-    if (forbidden) {
-        if (rank == 0 && tid == 0)
-            leave(a, x);
-        cooperative_groups::this_cluster().sync(); /* shared memory done with */
-        return;
-    }
+    if (tid == 0)
+        scratch.shared[3] = 0;
     const int run = (x.length + kBlocks * kOwn - 1) / (kBlocks * kOwn) * kOwn; /* whole groups of kOwn */
     const int from = min(rank * run, x.length), n = min(run, x.length - from);
     SlotKeys key = x.key;
@@ -230,7 +224,20 @@ __global__ void __launch_bounds__(kChooseThreads)
         mine += ties_in(base, k);
     }
     block_before(mine, scratch, 0, total);
+    if (pages.forbid(a.p, x))
+        scratch.shared[3] = 1;
     cluster_before<kBlocks>(total, scratch, 0, ties_before, all);
+    /* read behind the same barrier of the cluster */
+    int forbidden = 0;
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+        forbidden |= *cooperative_groups::this_cluster().map_shared_rank(&scratch.shared[3], b);
+    if (forbidden) {
+        if (rank == 0 && tid == 0)
+            leave(a, x);
+        cooperative_groups::this_cluster().sync(); /* shared memory done with */
+        return;
+    }
     int holes_here = 0, sources_here = 0;
     walk([&](uint32_t hole, uint32_t source, int) {
         holes_here += __popc(hole);
