@@ -69,13 +69,6 @@ __device__ __forceinline__ bool stage_wait(uint64_t *bar, uint32_t parity) {
     }
 }
 
-/* A wait of this thread that gave up: recorded, and the copy, which may still
- * be on its way, gets that time once more before its place is used again. */
-__device__ __noinline__ void gave_up(const PagedPool &p, uint64_t *bar, uint32_t parity) {
-    paged_fail(p, kPagedTimeout);
-    stage_wait(bar, parity);
-}
-
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -609,8 +602,10 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
     if (warp == 0)
         fetch(0, min(parts, most));
     const bool fit = parts <= most; /* then the statistics are read from the copies too */
-    if (!stage_wait(bar, phase))
-        gave_up(p, bar, phase);
+    if (!stage_wait(bar, phase)) {
+        paged_fail(p, kPagedTimeout);
+        stage_wait(bar, phase); /* once more before its place is used again */
+    }
     phase ^= 1;
     auto statistic = [&](int c, int i) { return fit ? copies[c * pitch + i] : __ldcg(part(c) + i); };
     for (int g = warp; g < heads; g += kWarps) {
@@ -645,8 +640,10 @@ __device__ __noinline__ void join_parts(const PagedAttention &a, bool inside, in
     for (int c = 0; c < parts; c += most) {
         const int n = min(parts - c, most);
         if (c > 0) {
-            if (!stage_wait(bar, phase))
-                gave_up(p, bar, phase);
+            if (!stage_wait(bar, phase)) {
+                paged_fail(p, kPagedTimeout);
+                stage_wait(bar, phase);
+            }
             phase ^= 1;
         }
 #pragma unroll
@@ -719,6 +716,19 @@ struct Cursor {
         return false;
     }
 };
+
+/* Logits of a box of slots whose page is a bad one: they give no weight.  By
+ * the lane that found it; where the logits are made it would cost the kernel
+ * registers (42 against 39 us for 16 sequences of up to 4,096 slots, bf16,
+ * fp32 rows). */
+__device__ __noinline__ void no_weight(const PagedAttention &a, int row, int index, int slot) {
+    const PagedPool &p = a.p;
+    const int groups = (p.group + kRows - 1) / kRows, in_group = index % groups * kRows;
+    float *z = a.logits + (int64_t(row) * p.heads + index / groups * p.group + in_group) * p.capacity + slot;
+    for (int g = 0; g < min(kRows, p.group - in_group); g++)
+        for (int i = 0; i < a.box; i++)
+            z[int64_t(g) * p.capacity + i] = -INFINITY;
+}
 
 /* Places of one of row r's items. */
 __device__ __noinline__ int places_of(const PagedAttention &a, int r, int tile_slots) {
@@ -800,7 +810,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
     const int D = p.head_dim, box = kLean ? kChunk : a.box, boxes = kLean ? 1 : kChunk / box;
     constexpr int kBoxWidth = 128 / sizeof(T);
     uint32_t phases = 0;
-    bool dead = false; /* a wait gave up: nothing more is read */
+    uint32_t late = 0; /* stages whose copy did not arrive: then nothing more is read */
 
     /* The copies run ahead of the arithmetic by kStages - 1 chunks, through
      * the ends of items: under load a round trip to memory takes 3 us, and an
@@ -836,6 +846,8 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
                 b.page = checked_page(p, in.sequence, j);
                 if (b.page >= 0)
                     b.count = min(box, in.length - j * p.page_size - b.slot);
+                else if (!kLean && a.weights)
+                    no_weight(a, in.row, in.index, v);
             }
         }
         in.tile += b.tiles;
@@ -859,7 +871,7 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
             plan(then);
         }
         const uint32_t to = ring_at + stage * Op::kStageBytes + my_box * box * 128;
-        const bool mine = now.count > 0 && my_chunk == used && !dead;
+        const bool mine = now.count > 0 && my_chunk == used && late == 0;
         const uint32_t valid = __reduce_or_sync(0xffffffffu, mine ? ((1u << now.count) - 1u) << (my_box * box) : 0u);
         const uint32_t bar = smem_u32(&full[warp][stage]);
         if (boxes > 1) {
@@ -921,18 +933,16 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         for (; x.tile < x.tile1; x.tile++) {
             issue(stage == 0 ? kStages - 1 : stage - 1);
             const uint32_t valid = masks[warp][stage];
-            float *z = !kLean && a.weights ? a.logits + (int64_t(x.row) * p.heads + first_head) * p.capacity +
-                                                 x.tile * kTile + warp * kChunk
-                                           : nullptr;
             bool arrived = valid != 0;
             if (arrived) {
                 /* the lanes give up together: what follows needs the whole warp */
                 arrived = __all_sync(0xffffffffu, stage_wait(&full[warp][stage], (phases >> stage) & 1));
-                if (!arrived) {
-                    gave_up(p, &full[warp][stage], (phases >> stage) & 1);
-                    dead = true;
+                if (arrived) {
+                    phases ^= 1u << stage;
+                } else {
+                    paged_fail(p, kPagedTimeout);
+                    late |= 1u << stage;
                 }
-                phases ^= 1u << stage;
             }
             if (arrived) {
                 const uint32_t at = ring_at + stage * Op::kStageBytes;
@@ -946,16 +956,12 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
                                          : "memory");
                     __syncwarp();
                 }
+                float *z = !kLean && a.weights ? a.logits + (int64_t(x.row) * p.heads + first_head) * p.capacity +
+                                           x.tile * kTile + warp * kChunk
+                                     : nullptr;
                 op.step(at, valid, scratch, z, p.capacity, heads);
                 if (valid != 0xffffu)
                     fence_async(); /* the zeros, before the stage is filled again */
-            }
-            if (z != nullptr && (!arrived || valid != 0xffffu)) {
-                /* slots in use that could not be read have no weight */
-                const int used = min(kChunk, x.length - (x.tile * kTile + warp * kChunk));
-                for (int i = lane; i < heads * kChunk; i += 32)
-                    if (i % kChunk < used && !(arrived && ((valid >> (i % kChunk)) & 1)))
-                        z[int64_t(i / kChunk) * p.capacity + i % kChunk] = -INFINITY;
             }
             __syncwarp();
             stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -1023,6 +1029,8 @@ __global__ void __launch_bounds__(Plan<Op>::kThreads, Plan<Op>::kPerSm)
         }
         __syncthreads(); /* outputs and factors are free again */
     }
+    for (; late != 0; late &= late - 1) /* once more, before the stages are used again */
+        stage_wait(&full[warp][__ffs(late) - 1], (phases >> (__ffs(late) - 1)) & 1);
     if (parts == 0)
         return;
 
@@ -1068,6 +1076,7 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
     const int t = (int(blockIdx.x) * kWeightThreads + int(threadIdx.x)) * 4;
     if (t >= length)
         return;
+    const int error = *p.error;
     const int64_t to = (int64_t(r) * p.kv_heads + head) * p.capacity + t;
     const int64_t h0 = int64_t(r) * p.heads + head * p.group;
     const float *z = a.logits + h0 * p.capacity + t;
@@ -1090,6 +1099,8 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
         for (int i = 0; i < 4; i++)
             w[i] += exp2f(x[i] - lse2);
     }
+    if (error & kPagedTimeout) /* logits may be missing */
+        return;
     if (kVec && n == 4) {
         const float4 x = *reinterpret_cast<const float4 *>(a.weights + to);
         *reinterpret_cast<float4 *>(a.weights_out + to) =
