@@ -396,7 +396,13 @@ nut_status nut_paged_destroy(nut_paged *paged);
  * calls' device-resident arguments (NUT_OUT_OF_RANGE: a page number outside
  * the pool, a length outside the table, a row's sequence, a position beyond
  * the rotation table, inconsistent `starts`), clearing it.  The work that
- * met it was skipped: nothing outside the caller's buffers is touched. */
+ * met it was skipped: an append stores no row without a slot or a position;
+ * an attention leaves out the slots of a bad page, which get no weight, and
+ * a row of a bad length or sequence sees nothing; a selection ranks a bad
+ * page last; an eviction leaves its sequence as it is.  Nothing outside the
+ * caller's buffers is touched.  NUT_DEVICE_TIMEOUT: a copy from the pool did
+ * not arrive within seconds; the outputs since are not to be used, and
+ * weights_out was not written. */
 nut_status nut_paged_error(nut_paged *paged, void *stream);
 
 /* Appends new tokens.  The rows of sequence s are starts[s] ..
@@ -462,8 +468,8 @@ typedef struct nut_paged_attention_args {
 nut_status nut_paged_attention(nut_paged *paged, const nut_paged_attention_args *args,
                                void *stream);
 
-/* Chooses pages for each row and kv head by a score that bounds the logits:
- * with each query head in 8 bits, x = rint(q / u), u the least power of two
+/* Chooses pages for each row and kv head by a score that bounds the logits up
+ * to the queries' rounding: with each query head in 8 bits, x = rint(q / u), u the least power of two
  * under which |x| <= 127,
  *   score(page) = max over the group's heads of
  *                 u * bound_scale * sum_d max(x_d greatest_d, x_d least_d).
@@ -485,7 +491,8 @@ nut_status nut_paged_select(nut_paged *paged, const nut_paged_select_args *args,
 
 /* Trims each sequence to `budget` slots, for each kv head on its own: kept
  * are the tokens with position < sinks or >= seen - recent, then those with
- * most weight (ties: the lowest slot; a NaN weight is the least).  The kept
+ * most weight (ties: the lowest slot; a NaN weight is the least, an infinite
+ * one ranks with the protected tokens).  The kept
  * tokens in slots from the new length on move into the freed slots below
  * it, both taken in ascending order; keys were rotated when stored, so the
  * order of slots does not matter to the attention.  weights_out and

@@ -94,7 +94,7 @@ struct PagedEvict {
     int32_t *new_lengths;
     float *weights_out;
     int32_t *positions_out;
-    int32_t *pairs;  /* [sequences][kv_heads][capacity]: holes, then sources from the far end */
+    int32_t *pairs;  /* [sequences][kv_heads][capacity]: holes from the start on, sources from the middle on */
     int32_t *counts; /* [sequences][kv_heads][2]: pairs, new length (-1: as it was) */
 };
 

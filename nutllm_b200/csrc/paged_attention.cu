@@ -16,7 +16,8 @@
  * are 545 MB and take 100 us (5.45 TB/s, 83 % of a measured copy; 4 us pass
  * before the first keys arrive and 5 at the end to join).  Where the pages
  * come out of L2 (256 queries of one prompt, 2.1 GB) it is the latency of a
- * warp's own products and softmax, 130 us.  Calls of a few tiles are a chain
+ * warp's own products and softmax, 128 us; dense rows of a prompt re-read the
+ * cache for every row (512 rows behind 8,192 slots: 1.3 ms).  Calls of a few tiles are a chain
  * of round trips: 37 slots take 6.7 us.
  */
 #include <cstdint>
@@ -533,8 +534,9 @@ template <int NQ, int DP> struct Scratch<Wide<NQ, DP>> {
 };
 
 /* Stages of a warp's ring.  With 8 KB stages, three and two CTAs an SM stream
- * from HBM faster than two and three CTAs (100 against 110 us for 545 MB); out
- * of L2 it is the other way round (203 against 183 us for 2.1 GB). */
+ * from HBM faster than two and three CTAs (100 against 103 us for 545 MB, 57
+ * against 59.5 for 250 MB of listed pages); out of L2 it is the other way round
+ * (129 against 115.5 us for 2.1 GB). */
 constexpr int stages_of(int stage_bytes) { return stage_bytes <= 4096 ? 4 : stage_bytes <= 12288 ? 3 : 2; }
 
 /* Shared memory: each warp's ring of stages and scratch, and two outputs of

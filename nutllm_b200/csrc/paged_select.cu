@@ -31,7 +31,12 @@ constexpr int kPages = 16;  /* of a warp's product */
 constexpr int kHeads = 8;   /* columns of a warp's product */
 constexpr int kMostRows = 8; /* of a block, where rows can share a sequence */
 constexpr float kMostFloat = 3.402823466e38f;
-constexpr int kFusedPages = 512; /* most pages of a row that its block chooses from at once */
+/* Most pages of a row that its block chooses from at once, in shared memory
+ * and 16 registers a lane.  A table of 512 and of 513 pages, which the forms
+ * below take in a second launch: 32 sequences 15.9 against 13.4 + 5.9 us, 256
+ * prompt rows 26.7 against 26.2 + 13.4 (bounds out of L2).  1,024 against 1,025
+ * pages, from registers and from histograms: 14.4 + 5.7 against 15.1 + 8.1. */
+constexpr int kFusedPages = 512;
 
 /* A warp writes the `n` first-ranked of a row's `pages` scores (at most 32 N,
  * in shared memory) to out, ascending, -1 behind.  Lanes own every 32nd
