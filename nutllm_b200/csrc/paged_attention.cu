@@ -283,7 +283,7 @@ template <typename T, typename R, int DP_> struct Halves {
             m = next;
         }
         const float base = m == -INFINITY ? 0.0f : m - kLift;
-        uint32_t hi[2], lo[2], p3[2];
+        uint32_t hi[2], lo[2], p3[2], tiny[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const float w0 = exp2f(s2[i][0] - base), w1 = exp2f(s2[i][1] - base);
@@ -294,6 +294,9 @@ template <typename T, typename R, int DP_> struct Halves {
             if constexpr (kThird) {
                 const float2 r3 = left_of<T>(r.x, r.y, lo[i]);
                 p3[i] = Pair<T>::pack(r3.x, r3.y);
+                const __nv_bfloat162 t = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&hi[i]),
+                                                 __float2bfloat162_rn(0x1p-40f));
+                tiny[i] = *reinterpret_cast<const uint32_t *>(&t);
             }
         }
         const uint32_t vrow = at + kBlocks * kBlock + (lane & 15) * 128, vx = ((lane >> 4) ^ (lane & 7)) * 16;
@@ -304,12 +307,11 @@ template <typename T, typename R, int DP_> struct Halves {
             Pair<T>::mma(o[2 * n], hi[0], lo[0], hi[1], lo[1], b[0], b[1]);
             Pair<T>::mma(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b[2], b[3]);
             if constexpr (kThird) {
-                /* into the rows of the second terms; the first ones get a
-                 * weight of 2^-126, beside which an infinite value stays
-                 * infinite where 0 would make it NaN */
-                constexpr uint32_t kTiny = 0x00800080u;
-                Pair<T>::mma(o[2 * n], kTiny, p3[0], kTiny, p3[1], b[0], b[1]);
-                Pair<T>::mma(o[2 * n + 1], kTiny, p3[0], kTiny, p3[1], b[2], b[3]);
+                /* into the rows of the second terms; the first ones get 2^-40
+                 * of their weight, which changes nothing, but where 0 would
+                 * make an infinite value NaN */
+                Pair<T>::mma(o[2 * n], tiny[0], p3[0], tiny[1], p3[1], b[0], b[1]);
+                Pair<T>::mma(o[2 * n + 1], tiny[0], p3[0], tiny[1], p3[1], b[2], b[3]);
             }
         }
     }

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import nutllm_b200 as nb
-from tests.test_paged import EPS, KINDS, TYPES, Pool, check_bounds, dtypes, head_reference, run_select, select_reference
+from tests.test_paged import EPS, KINDS, TYPES, Pool, check_bounds, close_out, dtypes, head_reference, run_select, select_reference
 
 # ---------------------------------------------------------------------------
 # attention
@@ -195,6 +195,31 @@ def test_logits_beyond_whole_numbers_stay_finite(gpu, types, power, step):
                          row_sequence=seq.data_ptr())
     pool.cache.check()
     assert bool(((out >= 1.0) & (out <= 2.0)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(t))
+def test_greatest_values_without_weight_add_nothing(gpu, types):
+    """Tokens whose weight underflows (keys 200 nats below) may hold the greatest finite values."""
+    import torch
+    n = 60
+    pool = Pool(torch, [n], 4, 1, 64, 16, types[0])
+    most = torch.finfo(pool.values.dtype).max
+    dead = [3, 17, 18, 40]
+    for t in dead:
+        page = int(pool.table_cpu[0, t // 16])
+        pool.keys[page, 0, t % 16] = 0.0
+        pool.keys[page, 0, t % 16, 5] = -1600.0
+        pool.values[page, 0, t % 16] = most
+    q = torch.randn(1, 4, 64, generator=pool.g)
+    q[:, :, 5] = 1.0
+    q = q.to(dtypes(torch)[types[1]]).cuda()
+    out = torch.zeros_like(q)
+    pool.cache.attention(q.data_ptr(), out.data_ptr(), 1, dtype=KINDS[types[1]])
+    pool.cache.check()
+    keep = [t for t in range(n) if t not in dead]
+    want, _, _, dz, mass = head_reference(torch, q.cpu()[0], pool.k[0][0][keep], pool.v[0][0][keep], 1 / 8)
+    close_out(torch, out.cpu()[0], want, dz, mass, n, types[1])
 
 
 # ---------------------------------------------------------------------------
