@@ -968,6 +968,11 @@ for _packed, _args in ((_APPEND, PagedAppendArgs), (_ATTENTION, PagedAttentionAr
                        (_SELECT, PagedSelectArgs), (_EVICT, PagedEvictArgs)):
     if _packed.size != C.sizeof(_args):
         raise ImportError(f"nutllm_b200: {_args.__name__} is not laid out as it is packed")
+_MISFIT = (struct.error, OverflowError)
+
+
+def _misfit(e: Exception) -> ValueError:
+    return ValueError(f"paged: an argument does not fit its field ({e})")
 
 
 class PagedCache:
@@ -1016,8 +1021,11 @@ class PagedCache:
         stores keys and values in each sequence's newest slots
         (nut_paged_append).  Rows of sequence s: starts[s] .. starts[s+1]-1;
         `lengths` already counts them."""
-        args = _APPEND.pack(q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, starts,
-                            rows, max_new, cos, sin, rope_rows, seen, positions, weights, dtype)
+        try:
+            args = _APPEND.pack(q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, starts,
+                                rows, max_new, cos, sin, rope_rows, seen, positions, weights, dtype)
+        except _MISFIT as e:
+            raise _misfit(e) from None
         status = self._append(self.handle, args, stream)
         if status:
             _check(status)
@@ -1029,8 +1037,11 @@ class PagedCache:
         """Attention of each row over its sequence's slots, or over the pages
         listed in `selected` (nut_paged_attention); with weights, adds the
         attention weight each slot received into weights_out."""
-        args = _ATTENTION.pack(q, out, q_stride, out_stride, lse, row_sequence, row_length,
-                               selected, n_selected, weights, weights_out, rows, scale, dtype)
+        try:
+            args = _ATTENTION.pack(q, out, q_stride, out_stride, lse, row_sequence, row_length,
+                                   selected, n_selected, weights, weights_out, rows, scale, dtype)
+        except _MISFIT as e:
+            raise _misfit(e) from None
         status = self._attention(self.handle, args, stream)
         if status:
             _check(status)
@@ -1040,8 +1051,11 @@ class PagedCache:
                row_sequence: int = 0, row_length: int = 0, stream: int = 0) -> None:
         """Writes the numbers of the n_selected pages whose keys can match
         each row's queries best, ascending, -1 behind (nut_paged_select)."""
-        args = _SELECT.pack(q, q_stride, row_sequence, row_length, selected, n_selected,
-                            sink_pages, recent_pages, rows, dtype)
+        try:
+            args = _SELECT.pack(q, q_stride, row_sequence, row_length, selected, n_selected,
+                                sink_pages, recent_pages, rows, dtype)
+        except _MISFIT as e:
+            raise _misfit(e) from None
         status = self._select(self.handle, args, stream)
         if status:
             _check(status)
@@ -1051,8 +1065,11 @@ class PagedCache:
               stream: int = 0) -> None:
         """Trims every sequence and kv head to the `budget` slots with most
         accumulated weight (nut_paged_evict)."""
-        args = _EVICT.pack(weights, positions, seen, budget, sinks, recent, new_lengths,
-                           weights_out, positions_out)
+        try:
+            args = _EVICT.pack(weights, positions, seen, budget, sinks, recent, new_lengths,
+                               weights_out, positions_out)
+        except _MISFIT as e:
+            raise _misfit(e) from None
         status = self._evict(self.handle, args, stream)
         if status:
             _check(status)

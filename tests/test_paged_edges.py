@@ -456,3 +456,17 @@ def test_the_loop_refuses_empty_prompts():
     from nutllm_b200 import paged_demo as demo
     with pytest.raises(ValueError, match="empty prompt"):
         demo.decode(None, [], [torch.zeros(3, 8), torch.zeros(0, 8)], 1)
+
+
+@pytest.mark.gpu
+def test_numbers_that_do_not_fit_are_refused_like_others(gpu):
+    """Arguments beyond the structures' fields raise ValueError from the call, as other wrong ones do."""
+    import torch
+    pool = Pool(torch, [10, 20], 4, 2, 64, 16, "f16", bounds=True)
+    c, p = pool.cache, torch.zeros(4096, device="cuda").data_ptr()
+    for call, args, more in ((c.attention, (p, p, 1 << 63), {}), (c.attention, (p, p, 2), dict(dtype=1 << 31)),
+                             (c.attention, (p, p, 2), dict(scale=1e300)),
+                             (c.select, (p, p, 2, 1 << 63), {}), (c.append, (0, p, p, p, 1 << 63, 1), {}),
+                             (c.evict, (p, 0, 0, -1 << 64), dict(new_lengths=p, weights_out=p))):
+        with pytest.raises(ValueError, match="paged: "):
+            call(*args, **more)
