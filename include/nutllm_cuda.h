@@ -385,7 +385,10 @@ typedef struct nut_paged_view {
 
 /* A handle on a pool: the view and this library's workspace for it.  The
  * operators enqueue on `stream` (a cudaStream_t, NULL = the legacy default
- * stream) and return without synchronising; none allocates.  Calls of one
+ * stream) and return without synchronising; none allocates.  The workspace
+ * takes 4 bytes for every sequence, kv head and slot of the table (what an
+ * eviction moves), with bounds 4 for every row, kv head and page, with
+ * track_weights 4 for every sequence, head and slot.  Calls of one
  * handle share its workspace: issue them on one stream or order the streams
  * with events. */
 typedef struct nut_paged nut_paged;
