@@ -516,6 +516,188 @@ typedef struct nut_paged_evict_args {
 } nut_paged_evict_args;
 nut_status nut_paged_evict(nut_paged *paged, const nut_paged_evict_args *args, void *stream);
 
+/* ---- Decoding that branches --------------------------------------------- */
+
+/* The reference follows one continuation of one sequence
+ * (generate_tokens_cached, src/generate.cpp:174-216).  Here several
+ * continuations share a paged cache: trees of drafted tokens that one pass
+ * verifies (nut_paged_append_at, nut_paged_tree_attention,
+ * nut_paged_compact), and beams (nut_beam_select) whose pages fork
+ * (nut_pages_update, nut_paged_copy).  All of it stays on the device and can
+ * be captured in a graph. */
+
+/* nut_paged_append with a position of its own for each row (drafted tokens
+ * of one depth share one): row_position [rows]; args->seen is not read.  A
+ * row whose position is negative or has no rotation is skipped. */
+nut_status nut_paged_append_at(nut_paged *paged, const nut_paged_append_args *args,
+                               const int32_t *row_position, void *stream);
+
+/* Workspace for nut_paged_tree_attention calls of up to max_new (1 to
+ * NUT_TREE_MAX) drafted tokens a sequence.  Allocates, so not within a
+ * capture.  Called again with more it allocates anew; what earlier captures
+ * use stays until the handle goes. */
+#define NUT_TREE_MAX 1024
+nut_status nut_paged_reserve_tree(nut_paged *paged, int64_t max_new);
+
+/* Attention of the drafted tokens of every sequence in one pass over its
+ * cache.  The rows of sequence s are starts[s] .. starts[s + 1] - 1; with n
+ * of them they are the tokens in its slots P .. P + n - 1, P = lengths[s] - n.
+ * Row r sees the slots below P and slot P + j where bit j % 32 of
+ * mask[r][j / 32] is set (itself only with its own bit; bits from n on are
+ * not read):
+ *   out[r][h] = sum_t w_t v_t,  w = softmax_t(scale q[r][h] . k_t)
+ * over the slots it sees, kv head h / (heads / kv_heads).  A row that sees
+ * nothing gives zeros and lse = -infinity.  Masks need not be those of a
+ * tree.  Whatever is stored in slots that a row does not see, infinities and
+ * NaN included, has no part in its outputs; an infinity or NaN among the
+ * values it sees makes that dimension of its output infinite or NaN.  Sums,
+ * the softmax and its statistics are fp32.  Products are formed from 16-bit
+ * terms where the cache has 16 bits: fp32 queries and their weights in two
+ * (fp16) or three (bf16) of them, rows of the cache's type in one (weights
+ * within 2^-8 of themselves on bf16, 2^-11 on fp16, and summed as rounded).
+ * Rows behind starts[sequences] are left as they were.  A sequence whose
+ * `starts` do not ascend within `rows` is skipped (its rows stay); where its
+ * length is bad or n exceeds it or max_new, its rows see nothing; slots of a
+ * bad page are not seen.  All of these are reported (nut_paged_error). */
+typedef struct nut_paged_tree_args {
+    const void *q; /* [rows][heads][head_dim] */
+    void *out;
+    int64_t q_stride, out_stride; /* elements between rows; 0: contiguous */
+    float *lse;            /* [rows][heads] natural log of the softmax sum, or NULL */
+    const int32_t *starts; /* [sequences + 1], ascending from 0 */
+    const uint32_t *mask;  /* [rows][mask_words] */
+    int64_t mask_words;    /* at least max_new / 32, rounded up */
+    int64_t rows;          /* rows there are: starts[sequences] or more */
+    int64_t max_new;       /* most rows of one sequence, as reserved or fewer */
+    float scale;           /* 0: 1 / sqrt(head_dim) */
+    int32_t type;          /* of q and out: NUT_F32 or the cache's */
+} nut_paged_tree_args;
+nut_status nut_paged_tree_attention(nut_paged *paged, const nut_paged_tree_args *args,
+                                    void *stream);
+
+/* Keeps the accepted ones of each sequence's drafted tokens next to one
+ * another: with n = starts[s + 1] - starts[s] and P = lengths[s] - n, the
+ * keys and values of slot P + accepted[s][i] move to slot P + i, and
+ * new_lengths[s] = P + the number accepted.  accepted[s] holds ascending
+ * numbers below n, then -1.  positions and weights (each or NULL) move with
+ * them.  A sequence with a bad length, starts, list or page is left as it is
+ * (new_lengths[s] = lengths[s]) and reported.  new_lengths may be the view's
+ * lengths.  Key bounds are not recomputed (nut_paged_summarise). */
+typedef struct nut_paged_compact_args {
+    const int32_t *starts;   /* [sequences + 1] */
+    const int32_t *accepted; /* [sequences][n_accepted] */
+    int64_t n_accepted;      /* up to NUT_TREE_MAX */
+    int32_t *new_lengths;    /* [sequences] */
+    int32_t *positions;      /* [sequences][kv_heads][max_pages * page_size], or NULL */
+    float *weights;          /* same shape, or NULL */
+} nut_paged_compact_args;
+nut_status nut_paged_compact(nut_paged *paged, const nut_paged_compact_args *args, void *stream);
+
+/* Copies pages: keys and values of the first slots[i] slots (NULL: of all)
+ * of page source[i] to page target[i], and its key bounds where the pool has
+ * them.  Entries with both -1 are passed over, other pages outside the pool
+ * are reported and passed over.  No target may be listed twice or be a
+ * source. */
+typedef struct nut_paged_copy_args {
+    const int32_t *source, *target; /* [count] */
+    const int32_t *slots;           /* [count], or NULL */
+    int64_t count;
+} nut_paged_copy_args;
+nut_status nut_paged_copy(nut_paged *paged, const nut_paged_copy_args *args, void *stream);
+
+/* The pages of many sequences, in the CALLER's device memory: the table and
+ * lengths of one or more nut_paged (a model's layers share them), how many
+ * holders each page has, and which pages have none.
+ *   refs        entries of the table that hold a page (used pages of every
+ *               sequence), plus what the caller holds itself (a prompt kept
+ *               for later, say)
+ *   free_pages  its first free_count[0] entries are the pages without a
+ *               holder; pages are taken from the end of them and given back
+ *               there */
+typedef struct nut_pages_view {
+    int32_t *table;      /* [sequences][max_pages] */
+    int32_t *lengths;    /* [sequences] */
+    int32_t *refs;       /* [n_pages] */
+    int32_t *free_pages; /* [n_pages] */
+    int32_t *free_count; /* [1] */
+    int64_t sequences, max_pages, n_pages, page_size;
+} nut_pages_view;
+
+/* A handle on them with this library's workspace (8 to 12 bytes a page, 4 for
+ * every entry of the table); as for nut_paged, calls of one handle are
+ * ordered by the caller, and none of them allocates. */
+typedef struct nut_pages nut_pages;
+
+nut_status nut_pages_create(const nut_pages_view *view, int device, nut_pages **out);
+nut_status nut_pages_destroy(nut_pages *pages);
+/* Synchronises `stream` and reports what earlier updates met, clearing it:
+ * NUT_LENGTH_ERROR (not enough free pages) or NUT_OUT_OF_RANGE (an argument,
+ * a table entry or the book out of range). */
+nut_status nut_pages_error(nut_pages *pages, void *stream);
+
+/* Every sequence s continues sequence parent[s] (-1: nothing): it keeps the
+ * first k = min(keep[s], length of parent[s]) slots and gets room for add[s]
+ * more; lengths[s] = k + add[s].  All sequences change at once.
+ *   - Pages of kept slots are shared with every other sequence that keeps
+ *     them.
+ *   - Where add[s] > 0 and the page of slot k - 1 is only partly kept, s
+ *     writes to it.  If others hold that page too, s gets a page of its own
+ *     instead, and copy_from[s], copy_to[s], copy_slots[s] say what
+ *     nut_paged_copy has to copy in each layer (-1, -1, 0: nothing); when all
+ *     of its holders are sequences that write to it in this call, the first
+ *     of them keeps it.
+ *   - New pages are taken from the end of free_pages in order of s, and
+ *     within s a copy's page first, then ascending.
+ *   - Pages that lost their last holder are then given back, ascending;
+ *     they cannot be taken by the same call.
+ * Table entries behind a sequence's last page stay as they were.  If a
+ * parent, keep, add, length or page is out of range, a sequence outgrows its
+ * table, or the free pages do not suffice, nothing changes: the copy lists
+ * are all -1 (and 0), and the error is kept for nut_pages_error. */
+typedef struct nut_pages_update_args {
+    const int32_t *parent; /* [sequences]; NULL: itself */
+    const int32_t *keep;   /* [sequences], not negative; NULL: all */
+    const int32_t *add;    /* [sequences], not negative; NULL: none */
+    int32_t *copy_from, *copy_to, *copy_slots; /* [sequences] each; NULL, all three, only without `add` */
+} nut_pages_update_args;
+nut_status nut_pages_update(nut_pages *pages, const nut_pages_update_args *args, void *stream);
+
+/* Beam search's choice for up to `sequences` requests of `beams` beams each
+ * over a vocabulary, the n_out best of each request.  n_out up to
+ * NUT_BEAM_MAX_OUT.  The handle holds the workspace; calls of one handle
+ * are ordered by the caller, and none of them allocates. */
+#define NUT_BEAM_MAX_OUT 64
+typedef struct nut_beam nut_beam;
+nut_status nut_beam_create(int64_t sequences, int64_t beams, int64_t vocab, int64_t n_out,
+                           int device, nut_beam **out);
+nut_status nut_beam_destroy(nut_beam *beam);
+
+/* Of the candidates (beam b, token t) of request s with
+ *   score(b, t) = scores[s][b] + logits[s beams + b][t] - log sum_u exp(logits[..][u])
+ * (the sum in fp32 with the parts joined in fp64, scores compared in fp64) the
+ * n_out greatest in descending order, ties to the lowest beam, then the lowest
+ * token.  A finished beam has one candidate, (b, eos) with score scores[s][b],
+ * and its logits are not read.  NaN counts as -infinity in logits and scores,
+ * a logit of +infinity as the greatest finite float; candidates of
+ * score -infinity rank last.  Where there are fewer candidates than n_out,
+ * rows and tokens are -1 and scores -infinity behind them.  The choice does
+ * not depend on timing.  out_scores and out_finished may be scores and finished
+ * where n_out is beams. */
+typedef struct nut_beam_select_args {
+    const void *logits;      /* [sequences * beams][vocab] */
+    int64_t logits_stride;   /* elements between rows; 0: vocab */
+    const float *scores;     /* [sequences][beams] */
+    const uint8_t *finished; /* [sequences][beams], or NULL: none */
+    float *out_scores;       /* [sequences][n_out], rounded to fp32 */
+    int32_t *out_rows;       /* s * beams + b: a row of logits, and a `parent` of nut_pages_update */
+    int32_t *out_tokens;
+    uint8_t *out_finished;   /* the beam's, or 1 where the token is eos; or NULL */
+    int64_t sequences;       /* as created or fewer */
+    int32_t eos;             /* -1: none */
+    int32_t type;            /* of logits */
+} nut_beam_select_args;
+nut_status nut_beam_select(nut_beam *beam, const nut_beam_select_args *args, void *stream);
+
 /* ---- Greedy head without allocation ------------------------------------ */
 
 /* Largest batch of nut_greedy_head_static. */

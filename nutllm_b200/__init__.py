@@ -171,6 +171,40 @@ class PagedEvictArgs(C.Structure):
         (n, C.c_void_p) for n in ("new_lengths", "weights_out", "positions_out")]
 
 
+class PagedTreeArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("lse", C.c_void_p), ("starts", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_words", C.c_int64), ("rows", C.c_int64),
+                ("max_new", C.c_int64), ("scale", C.c_float), ("type", C.c_int32)]
+
+
+class PagedCompactArgs(C.Structure):
+    _fields_ = [("starts", C.c_void_p), ("accepted", C.c_void_p), ("n_accepted", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("new_lengths", "positions", "weights")]
+
+
+class PagedCopyArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("source", "target", "slots")] + [("count", C.c_int64)]
+
+
+class PagesView(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in (
+        "table", "lengths", "refs", "free_pages", "free_count")] + [
+        (n, C.c_int64) for n in ("sequences", "max_pages", "n_pages", "page_size")]
+
+
+class PagesUpdateArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in (
+        "parent", "keep", "add", "copy_from", "copy_to", "copy_slots")]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("scores", "finished", "out_scores", "out_rows", "out_tokens",
+                                  "out_finished")] + [
+        ("sequences", C.c_int64), ("eos", C.c_int32), ("type", C.c_int32)]
+
+
 # --------------------------------------------------------------------------
 # library loading
 
@@ -254,8 +288,19 @@ def cuda_lib() -> C.CDLL:
         _declare(lib, "nut_paged_error", [_P, _P])
         _declare(lib, "nut_paged_summarise", [_P, _P])
         for op, kind in (("append", PagedAppendArgs), ("attention", PagedAttentionArgs),
-                         ("select", PagedSelectArgs), ("evict", PagedEvictArgs)):
+                         ("select", PagedSelectArgs), ("evict", PagedEvictArgs),
+                         ("tree_attention", PagedTreeArgs), ("compact", PagedCompactArgs),
+                         ("copy", PagedCopyArgs)):
             _declare(lib, f"nut_paged_{op}", [_P, C.POINTER(kind), _P])
+        _declare(lib, "nut_paged_append_at", [_P, C.POINTER(PagedAppendArgs), _P, _P])
+        _declare(lib, "nut_paged_reserve_tree", [_P, _I64])
+        _declare(lib, "nut_pages_create", [C.POINTER(PagesView), C.c_int, C.POINTER(_P)])
+        _declare(lib, "nut_pages_destroy", [_P])
+        _declare(lib, "nut_pages_error", [_P, _P])
+        _declare(lib, "nut_pages_update", [_P, C.POINTER(PagesUpdateArgs), _P])
+        _declare(lib, "nut_beam_create", [_I64, _I64, _I64, _I64, C.c_int, C.POINTER(_P)])
+        _declare(lib, "nut_beam_destroy", [_P])
+        _declare(lib, "nut_beam_select", [_P, C.POINTER(BeamSelectArgs), _P])
         _cuda = lib
     return _cuda
 
@@ -964,15 +1009,28 @@ _APPEND = struct.Struct("@4P4qPqqPPqPPPi4x")
 _ATTENTION = struct.Struct("@PPqqPPPPqPPqfi")
 _SELECT = struct.Struct("@PqPPP4qi4x")
 _EVICT = struct.Struct("@PPPqqqPPP")
+_TREE = struct.Struct("@PPqqPPPqqqfi")
+_COMPACT = struct.Struct("@PPqPPP")
+_COPY = struct.Struct("@PPPq")
+_UPDATE = struct.Struct("@6P")
+_BEAM = struct.Struct("@Pq6Pqii")
 for _packed, _args in ((_APPEND, PagedAppendArgs), (_ATTENTION, PagedAttentionArgs),
-                       (_SELECT, PagedSelectArgs), (_EVICT, PagedEvictArgs)):
+                       (_SELECT, PagedSelectArgs), (_EVICT, PagedEvictArgs),
+                       (_TREE, PagedTreeArgs), (_COMPACT, PagedCompactArgs),
+                       (_COPY, PagedCopyArgs), (_UPDATE, PagesUpdateArgs),
+                       (_BEAM, BeamSelectArgs)):
     if _packed.size != C.sizeof(_args):
         raise ImportError(f"nutllm_b200: {_args.__name__} is not laid out as it is packed")
 _MISFIT = (struct.error, OverflowError)
 
 
-def _misfit(e: Exception) -> ValueError:
-    return ValueError(f"paged: an argument does not fit its field ({e})")
+def _misfit(e: Exception, part: str = "paged") -> ValueError:
+    return ValueError(f"{part}: an argument does not fit its field ({e})")
+
+
+def _packed(lib: C.CDLL, name: str):
+    """An entry point that takes (handle, arguments as bytes, stream)."""
+    return C.CFUNCTYPE(C.c_int, _P, _P, _P)(C.cast(getattr(lib, name), _P).value)
 
 
 class PagedCache:
@@ -1007,26 +1065,30 @@ class PagedCache:
         lib = cuda_lib()
         _check(lib.nut_paged_create(C.byref(view), device, C.byref(h)))
         self.handle = h
-        packed = C.CFUNCTYPE(C.c_int, _P, _P, _P)  # arguments as bytes
-        self._append, self._attention, self._select, self._evict = (
-            packed(C.cast(getattr(lib, f"nut_paged_{op}"), _P).value)
-            for op in ("append", "attention", "select", "evict"))
+        self._append, self._attention, self._select, self._evict, self._tree, self._compact, self._copy = (
+            _packed(lib, f"nut_paged_{op}") for op in (
+                "append", "attention", "select", "evict", "tree_attention", "compact", "copy"))
+        self._append_at = C.CFUNCTYPE(C.c_int, _P, _P, _P, _P)(C.cast(lib.nut_paged_append_at, _P).value)
 
     def append(self, q: int, k: int, v: int, starts: int, rows: int, max_new: int, *,
                dtype: int = F32, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0,
                q_out: int = 0, q_out_stride: int = 0, cos: int = 0, sin: int = 0,
                rope_rows: int = 0, seen: int = 0, positions: int = 0, weights: int = 0,
-               stream: int = 0) -> None:
+               row_position: int = 0, stream: int = 0) -> None:
         """Rotates the new rows' queries (into q_out; q may be 0) and keys and
         stores keys and values in each sequence's newest slots
         (nut_paged_append).  Rows of sequence s: starts[s] .. starts[s+1]-1;
-        `lengths` already counts them."""
+        `lengths` already counts them.  With row_position (int32 [rows]) each
+        row has a position of its own (nut_paged_append_at)."""
         try:
             args = _APPEND.pack(q, k, v, q_out, q_stride, k_stride, v_stride, q_out_stride, starts,
                                 rows, max_new, cos, sin, rope_rows, seen, positions, weights, dtype)
         except _MISFIT as e:
             raise _misfit(e) from None
-        status = self._append(self.handle, args, stream)
+        if row_position:
+            status = self._append_at(self.handle, args, row_position, stream)
+        else:
+            status = self._append(self.handle, args, stream)
         if status:
             _check(status)
 
@@ -1074,6 +1136,53 @@ class PagedCache:
         if status:
             _check(status)
 
+    def reserve_tree(self, max_new: int) -> None:
+        """Workspace for tree_attention() of up to max_new drafted tokens a
+        sequence (nut_paged_reserve_tree); not within a capture."""
+        if not -1 << 63 <= max_new < 1 << 63:
+            raise _misfit(OverflowError("max_new"))
+        _check(cuda_lib().nut_paged_reserve_tree(self.handle, max_new))
+
+    def tree_attention(self, q: int, out: int, starts: int, mask: int, rows: int, max_new: int,
+                       mask_words: int, *, dtype: int = F32, scale: float = 0.0, q_stride: int = 0,
+                       out_stride: int = 0, lse: int = 0, stream: int = 0) -> None:
+        """Attention of the drafted tokens in each sequence's newest slots over
+        its earlier slots and those of the drafted tokens that `mask` (32 bits
+        to a word, [rows][mask_words]) names (nut_paged_tree_attention)."""
+        try:
+            args = _TREE.pack(q, out, q_stride, out_stride, lse, starts, mask, mask_words, rows,
+                              max_new, scale, dtype)
+        except _MISFIT as e:
+            raise _misfit(e) from None
+        status = self._tree(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def compact(self, starts: int, accepted: int, n_accepted: int, *, new_lengths: int,
+                positions: int = 0, weights: int = 0, stream: int = 0) -> None:
+        """Moves the accepted ones of each sequence's drafted tokens (ascending
+        numbers in int32 [sequences][n_accepted], -1 behind) to where the
+        drafted tokens begin (nut_paged_compact)."""
+        try:
+            args = _COMPACT.pack(starts, accepted, n_accepted, new_lengths, positions, weights)
+        except _MISFIT as e:
+            raise _misfit(e) from None
+        status = self._compact(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def copy_pages(self, source: int, target: int, count: int, *, slots: int = 0,
+                   stream: int = 0) -> None:
+        """Copies the first slots[i] slots (0: all slots) of page source[i] to
+        page target[i]; -1 and -1: nothing (nut_paged_copy)."""
+        try:
+            args = _COPY.pack(source, target, slots, count)
+        except _MISFIT as e:
+            raise _misfit(e) from None
+        status = self._copy(self.handle, args, stream)
+        if status:
+            _check(status)
+
     def summarise(self, stream: int = 0) -> None:
         """Recomputes the key bounds of every used page (nut_paged_summarise)."""
         _check(cuda_lib().nut_paged_summarise(self.handle, stream))
@@ -1086,6 +1195,102 @@ class PagedCache:
     def close(self) -> None:
         if getattr(self, "handle", None):
             cuda_lib().nut_paged_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PageBook:
+    """The pages of many sequences that may share them (nut_pages), in device
+    memory of the caller; pointers as for PagedCache, whose table and lengths
+    these are.
+
+    refs        int32 [n_pages], table entries (and callers) that hold a page
+    free_pages  int32 [n_pages], of which the first free_count[0] are free
+
+    update() enqueues on `stream` and does not synchronise; calls of one object
+    must be ordered as on one stream."""
+
+    def __init__(self, table: int, lengths: int, refs: int, free_pages: int, free_count: int, *,
+                 sequences: int, max_pages: int, n_pages: int, page_size: int, device: int = 0):
+        self.handle = None
+        view = PagesView(table, lengths, refs, free_pages, free_count, sequences, max_pages,
+                         n_pages, page_size)
+        h = C.c_void_p()
+        lib = cuda_lib()
+        _check(lib.nut_pages_create(C.byref(view), device, C.byref(h)))
+        self.handle = h
+        self._update = _packed(lib, "nut_pages_update")
+
+    def update(self, *, parent: int = 0, keep: int = 0, add: int = 0, copy_from: int = 0,
+               copy_to: int = 0, copy_slots: int = 0, stream: int = 0) -> None:
+        """Every sequence s continues parent[s] (0: itself; an entry of -1:
+        nothing), keeps its first keep[s] slots (0: all) and gets room for
+        add[s] more (0: none); all int32 [sequences].  Pages are shared, split
+        and given back as needed (nut_pages_update); what copy_from, copy_to
+        and copy_slots receive is for copy_pages() of every layer."""
+        try:
+            args = _UPDATE.pack(parent, keep, add, copy_from, copy_to, copy_slots)
+        except _MISFIT as e:
+            raise _misfit(e, "pages") from None
+        status = self._update(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def check(self, stream: int = 0) -> None:
+        """Synchronises `stream`; raises OverflowError if an update lacked free
+        pages, IndexError if it met something out of range (nut_pages_error)."""
+        _check(cuda_lib().nut_pages_error(self.handle, stream))
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            cuda_lib().nut_pages_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class BeamSearch:
+    """Beam search's choice for up to `sequences` requests of `beams` beams over
+    `vocab` tokens, n_out of them each (nut_beam)."""
+
+    def __init__(self, sequences: int, beams: int, vocab: int, n_out: int, *, device: int = 0):
+        self.handle = None
+        if not all(-1 << 63 <= n < 1 << 63 for n in (sequences, beams, vocab, n_out)):
+            raise _misfit(OverflowError("dimension"), "beam")
+        h = C.c_void_p()
+        lib = cuda_lib()
+        _check(lib.nut_beam_create(sequences, beams, vocab, n_out, device, C.byref(h)))
+        self.handle = h
+        self.sequences = sequences
+        self._select = _packed(lib, "nut_beam_select")
+
+    def select(self, logits: int, scores: int, out_scores: int, out_rows: int, out_tokens: int, *,
+               dtype: int = F32, logits_stride: int = 0, finished: int = 0, eos: int = -1,
+               out_finished: int = 0, sequences: Optional[int] = None, stream: int = 0) -> None:
+        """The n_out best continuations of each request's beams by
+        scores + log softmax(logits) (nut_beam_select), all device addresses:
+        their scores, rows of the logits (sequence * beams + beam) and tokens."""
+        try:
+            args = _BEAM.pack(logits, logits_stride, scores, finished, out_scores, out_rows, out_tokens,
+                              out_finished, self.sequences if sequences is None else sequences, eos, dtype)
+        except _MISFIT as e:
+            raise _misfit(e, "beam") from None
+        status = self._select(self.handle, args, stream)
+        if status:
+            _check(status)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            cuda_lib().nut_beam_destroy(self.handle)
             self.handle = None
 
     def __del__(self):

@@ -52,6 +52,11 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
     return __float2bfloat16_rn(v);
 }
 
+/* An output in its type; infinities stay (from_float would saturate them, and
+ * a mean of fp16 values has no other way beyond 65504). */
+template <typename R> __device__ __forceinline__ R output_of(float v) { return from_float<R>(v); }
+template <> __device__ __forceinline__ __half output_of<__half>(float v) { return __float2half_rn(v); }
+
 __device__ __forceinline__ void paged_fail(const PagedPool &p, int bit) { atomicOr(p.error, bit); }
 
 /* Slots in use of sequence s; 0, with the error recorded, when the length

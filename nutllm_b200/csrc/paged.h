@@ -40,6 +40,7 @@ struct PagedAppend {
     int rows, max_new, rope_rows, type;
     int32_t *positions;
     float *weights;
+    const int32_t *row_position; /* [rows], or NULL: by the slots */
 };
 
 struct PagedAttention {
@@ -98,11 +99,57 @@ struct PagedEvict {
     int32_t *counts; /* [sequences][kv_heads][2]: pairs, new length (-1: as it was) */
 };
 
+struct PagedCompact {
+    PagedPool p;
+    const int32_t *starts, *accepted;
+    int n_accepted;
+    int32_t *new_lengths, *positions;
+    float *weights;
+    int32_t *order; /* [sequences]: blocks that are through, 0 between calls */
+};
+
+struct PagedCopy {
+    PagedPool p;
+    const int32_t *source, *target, *slots;
+    int count;
+};
+
+constexpr int kTreeMost = 1024;   /* drafted tokens of a sequence */
+constexpr int kTreeMostBox = 128; /* slots of a box of the tree attention's maps */
+constexpr int kTreeCtasPerSm = 2;
+
+struct PagedTree {
+    /* (dim, slot, 128-byte column, kv head, page) in boxes of one column by
+     * `box` slots; the column is the whole row where head_dim is no multiple of it */
+    CUtensorMap key_map, value_map;
+    PagedPool p;
+    int box, box_shift, whole_columns;
+    uint64_t page_magic;
+    int page_shift;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    float *lse;
+    const int32_t *starts;
+    const uint32_t *mask;
+    int mask_words, rows, max_new, type;
+    float scale;
+    float *partial; /* [CTAs][2][part_floats] */
+    int4 *joins;    /* [CTAs]: the item that begins in a CTA and ends in another */
+    int64_t part_floats;
+    int sms;
+};
+
 /* head_dim as the attention's kernels are made for. */
 inline int paged_padded_dim(int type, int D) {
     return type == 0 ? (D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256)
                      : (D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256);
 }
+/* What the tree attention's kernels want of a pool (paged_tree.cu): floats of
+ * a CTA's part of an item, and the most places on the line of tiles. */
+int64_t tree_part_floats(const PagedPool &p, int max_new);
+int64_t tree_most_places(const PagedPool &p, int max_new, int64_t rows);
+
 /* 128-byte columns of such a row in shared memory. */
 inline int paged_columns(int type, int D) {
     return (paged_padded_dim(type, D) * (type == 0 ? 4 : 2) + 127) / 128;
@@ -113,5 +160,8 @@ cudaError_t paged_summarise(const PagedPool &p, cudaStream_t s);
 cudaError_t paged_attention(const PagedAttention &a, cudaStream_t s);
 cudaError_t paged_select(const PagedSelect &a, cudaStream_t s);
 cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s);
+cudaError_t paged_compact(const PagedCompact &a, cudaStream_t s);
+cudaError_t paged_copy(const PagedCopy &a, cudaStream_t s);
+cudaError_t paged_tree(const PagedTree &a, cudaStream_t s);
 
 } // namespace nut

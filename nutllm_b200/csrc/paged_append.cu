@@ -159,8 +159,9 @@ __device__ void page_bounds(const PagedPool &p, int page, int head, int used) {
  * and write neighbouring 16 bytes) and walks the page's new
  * (token, unit) rows, a unit being one of the group's query heads, the key or
  * the value.  1536 threads on an SM: registers for 1280 and 2048 took 61 and
- * 65 us where this takes 56 (12 prompts, 297 MB). */
-template <int kThreads, typename R, typename T, bool kVec>
+ * 65 us where this takes 56 (12 prompts, 297 MB).  kAt: rows have positions
+ * of their own (nut_paged_append_at). */
+template <int kThreads, typename R, typename T, bool kVec, bool kAt>
 __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
     append_kernel(const __grid_constant__ PagedAppend a) {
     begin_kernel();
@@ -182,7 +183,10 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
     const int page = checked_page(p, s, j);
     if (page < 0)
         return;
-    const int ahead = a.seen ? a.seen[s] - length : 0; /* position less slot */
+    const int ahead = !kAt && a.seen ? a.seen[s] - length : 0; /* position less slot */
+    const auto position = [&](int t) {
+        return kAt ? int64_t(a.row_position[row0 + (t - first)]) : int64_t(t) + ahead;
+    };
     const int D = p.head_dim, half = D / 2, octets = D / 8, groups = kThreads / octets;
     const int o = threadIdx.x % octets * 4, group = threadIdx.x / octets;
     const int64_t base = int64_t(page) * p.page_stride + int64_t(head) * p.head_stride + o;
@@ -190,8 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
     const int heads = a.q ? p.group : 0, units = heads + 2;
     /* whether slot t's position has a rotation, where there are any: rows without one are skipped */
     const auto turns = [&](int t) {
-        const int64_t pos = int64_t(t) + ahead;
-        return !a.cos || (pos >= 0 && pos < a.rope_rows);
+        const int64_t pos = position(t);
+        return (!kAt && !a.cos) || (pos >= 0 && (!a.cos || pos < a.rope_rows));
     };
     if (group < groups)
         for (int e = group; e < (t1 - t0) * units; e += groups) {
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
             load4<kVec>(x, v);
             load4<kVec>(x + half, v + 4);
             if (a.cos && unit <= heads) {
-                const int64_t turn = (int64_t(t) + ahead) * half + o / 2;
+                const int64_t turn = position(t) * half + o / 2;
                 load2<kVec>(a.cos + turn, c);
                 load2<kVec>(a.cos + turn + half / 2, c + 2);
                 load2<kVec>(a.sin + turn, z);
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
             if (!turns(t))
                 continue;
             if (a.positions)
-                a.positions[at + t] = t + ahead;
+                a.positions[at + t] = int(position(t));
             if (a.weights)
                 a.weights[at + t] = 0.0f;
         }
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kSummaryThreads) summarise_kernel(const __grid
         page_bounds<kSummaryThreads, T>(p, page, head, used);
 }
 
-template <typename R, typename T> cudaError_t launch_append(const PagedAppend &a, cudaStream_t s) {
+template <typename R, typename T, bool kAt> cudaError_t launch_append_by(const PagedAppend &a, cudaStream_t s) {
     const PagedPool &p = a.p;
     /* pages that max_new consecutive slots can touch */
     const dim3 grid((a.max_new + p.page_size - 2) / p.page_size + 1, p.kv_heads, p.sequences);
@@ -276,8 +280,14 @@ template <typename R, typename T> cudaError_t launch_append(const PagedAppend &a
      * token of 3 rows: 4.2 against 5.7 us for 2048 pages), two warps */
     const int64_t octets = int64_t(std::min(a.max_new, p.page_size)) * ((a.q ? p.group : 0) + 2) * (p.head_dim / 8);
     if (octets <= 64)
-        return launch_kernel(vec ? append_kernel<64, R, T, true> : append_kernel<64, R, T, false>, grid, 64, 0, s, 1, a);
-    return launch_kernel(vec ? append_kernel<128, R, T, true> : append_kernel<128, R, T, false>, grid, 128, 0, s, 1, a);
+        return launch_kernel(vec ? append_kernel<64, R, T, true, kAt> : append_kernel<64, R, T, false, kAt>, grid, 64, 0,
+                             s, 1, a);
+    return launch_kernel(vec ? append_kernel<128, R, T, true, kAt> : append_kernel<128, R, T, false, kAt>, grid, 128, 0,
+                         s, 1, a);
+}
+
+template <typename R, typename T> cudaError_t launch_append(const PagedAppend &a, cudaStream_t s) {
+    return a.row_position ? launch_append_by<R, T, true>(a, s) : launch_append_by<R, T, false>(a, s);
 }
 
 } // namespace

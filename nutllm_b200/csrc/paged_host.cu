@@ -4,88 +4,20 @@
 #include <climits>
 #include <cmath>
 #include <memory>
-#include <mutex>
-#include <stdexcept>
 #include <string>
+#include <vector>
 
 #include <cuda_runtime.h>
 
-#include "../../include/nutllm_cuda.h"
-#include "kernels.h"
-#include "paged.h"
+#include "abi.h"
 
 namespace {
 
-struct Failure {
-    nut_status status;
-    std::string message;
-};
+using namespace nut::abi;
 
 [[noreturn]] void raise(nut_status s, const std::string &m) { throw Failure{s, "paged: " + m}; }
 
-void cuda_check(cudaError_t e, const char *what) {
-    if (e != cudaSuccess) {
-        cudaGetLastError(); /* reported here: the next call's own check is not to find it */
-        throw Failure{NUT_RUNTIME_ERROR,
-                      std::string("cuda: ") + what + ": " + cudaGetErrorString(e)};
-    }
-}
-
-template <typename F> nut_status guarded(F &&body) {
-    try {
-        body();
-        return NUT_OK;
-    } catch (const Failure &f) {
-        nut::set_last_error(f.message);
-        return f.status;
-    } catch (const std::bad_alloc &) {
-        nut::set_last_error("nutllm: host allocation failed");
-        return NUT_RUNTIME_ERROR;
-    } catch (const std::exception &e) {
-        nut::set_last_error(e.what());
-        return NUT_RUNTIME_ERROR;
-    }
-}
-
-/* Makes the handle's device current where it is not, and restores it. */
-struct DeviceScope {
-    int previous = 0, device;
-    explicit DeviceScope(int d) : device(d) {
-        cuda_check(cudaGetDevice(&previous), "get device");
-        if (previous != device)
-            cuda_check(cudaSetDevice(device), "set device");
-    }
-    ~DeviceScope() {
-        if (previous != device)
-            cudaSetDevice(previous);
-    }
-};
-
-/* Workspaces come from a memory pool of this library's own on each device,
- * which keeps up to 64 MB that handles gave back: a handle is made in some 20
- * us, where cudaMalloc and cudaFree take 300 to 400 each. */
-cudaMemPool_t workspace_pool(int device) {
-    static std::mutex lock;
-    static cudaMemPool_t pools[nut::kMaxDevices] = {};
-    if (device < 0 || device >= nut::kMaxDevices)
-        raise(NUT_INVALID_ARGUMENT, "device out of range");
-    const std::lock_guard<std::mutex> hold(lock);
-    if (!pools[device]) {
-        cudaMemPoolProps props{};
-        props.allocType = cudaMemAllocationTypePinned;
-        props.location.type = cudaMemLocationTypeDevice;
-        props.location.id = device;
-        cuda_check(cudaMemPoolCreate(&pools[device], &props), "create workspace pool");
-        uint64_t keep = uint64_t(64) << 20;
-        cuda_check(cudaMemPoolSetAttribute(pools[device], cudaMemPoolAttrReleaseThreshold, &keep),
-                   "size workspace pool");
-    }
-    return pools[device];
-}
-
 constexpr int64_t kMaxGrid = 65535; /* sequences and rows are grid dimensions */
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 void check_view(const nut_paged_view &v) {
     if (!v.keys || !v.values || !v.table || !v.lengths)
@@ -130,9 +62,10 @@ using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                  CUtensorMapFloatOOBfill);
 
-/* The pool as the attention's tensor map (PagedAttention::key_map); dims
- * behind head_dim read as zeros. */
-CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box, bool whole) {
+/* The pool as the attention's tensor map (PagedAttention::key_map), or the
+ * tree attention's with boxes of one column; dims behind head_dim read as
+ * zeros. */
+CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box, bool whole, bool one_column = false) {
     static const EncodeTiled encode = [] {
         void *f = nullptr;
         cudaDriverEntryPointQueryResult q{};
@@ -154,7 +87,7 @@ CUtensorMap pool_map(const nut::PagedPool &p, void *base, int box, bool whole) {
     const cuuint64_t strides[4] = {cuuint64_t(p.slot_stride) * size, 128, cuuint64_t(p.head_stride) * size,
                                    cuuint64_t(p.page_stride) * size};
     const cuuint32_t columns = cuuint32_t(nut::paged_columns(p.type, p.head_dim));
-    const cuuint32_t boxes[5] = {cuuint32_t(width), cuuint32_t(box), whole ? columns : 1, 1, 1};
+    const cuuint32_t boxes[5] = {cuuint32_t(width), cuuint32_t(box), whole && !one_column ? columns : 1, 1, 1};
     const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
     CUtensorMap map;
     if (encode(&map, type, 5, base, dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -189,11 +122,21 @@ struct nut_paged {
     char *block = nullptr; /* one allocation, cut into the parts below */
     int *error = nullptr, *counters = nullptr;
     float *partial = nullptr, *logits = nullptr, *lse2 = nullptr, *scores = nullptr;
-    int32_t *pairs = nullptr, *counts = nullptr;
+    int32_t *pairs = nullptr, *counts = nullptr, *order = nullptr;
+    /* nut_paged_reserve_tree */
+    CUtensorMap tree_key_map{}, tree_value_map{};
+    int tree_box = 0, tree_box_shift = 0, tree_max = 0;
+    bool tree_whole_columns = false;
+    std::vector<char *> tree_blocks; /* the last is in use; captured calls may use the others */
+    float *tree_partial = nullptr;
+    int4 *tree_joins = nullptr;
+    int64_t tree_part_floats = 0;
     ~nut_paged() {
         if (block) {
             cudaDeviceSynchronize(); /* calls in flight, on any stream, still use it */
             cudaFreeAsync(block, nullptr);
+            for (char *b : tree_blocks)
+                cudaFreeAsync(b, nullptr);
         }
     }
 };
@@ -270,9 +213,10 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
             bytes += (count * size + 255) / 256 * 256;
             return at;
         };
-        /* zeroed at first: the error word and the counters */
+        /* zeroed at first: the error word, the counters and the compaction's order */
         const size_t error = part(1, 4);
         const size_t counters = part(size_t(h->max_rows) * p.kv_heads * ((p.group + 7) / 8), 4);
+        const size_t order = part(size_t(p.sequences), 4);
         const size_t zeroed = bytes;
         const size_t partial = part(size_t(h->sms) * nut::kMaxCtasPerSm * 2 *
                                         nut::paged_part_floats(nut::paged_padded_dim(p.type, p.head_dim)),
@@ -288,6 +232,7 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(h->block + at); };
         p.error = h->error = ints(error);
         h->counters = ints(counters);
+        h->order = ints(order);
         h->partial = floats(partial);
         h->pairs = ints(pairs);
         h->counts = ints(counts);
@@ -339,7 +284,7 @@ nut_status nut_paged_error(nut_paged *h, void *stream) {
     });
 }
 
-nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, void *stream) {
+static nut_status append(nut_paged *h, const nut_paged_append_args *args, const int32_t *row_position, void *stream) {
     return guarded([&] {
         if (!h || !args)
             raise(NUT_INVALID_ARGUMENT, "null argument");
@@ -378,6 +323,7 @@ nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, voi
         a.q_out = g.q_out;
         a.starts = g.starts;
         a.seen = g.seen;
+        a.row_position = row_position;
         a.cos = g.rope_cos;
         a.sin = g.rope_sin;
         a.rows = int(g.rows);
@@ -389,6 +335,20 @@ nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, voi
         DeviceScope scope(h->device);
         cuda_check(nut::paged_append(a, static_cast<cudaStream_t>(stream)), "paged append");
     });
+}
+
+nut_status nut_paged_append(nut_paged *h, const nut_paged_append_args *args, void *stream) {
+    return append(h, args, nullptr, stream);
+}
+
+nut_status nut_paged_append_at(nut_paged *h, const nut_paged_append_args *args, const int32_t *row_position,
+                               void *stream) {
+    return guarded([&] {
+               if (!row_position)
+                   raise(NUT_INVALID_ARGUMENT, "null row_position");
+           }) == NUT_OK
+               ? append(h, args, row_position, stream)
+               : NUT_INVALID_ARGUMENT;
 }
 
 nut_status nut_paged_summarise(nut_paged *h, void *stream) {
@@ -531,6 +491,151 @@ nut_status nut_paged_evict(nut_paged *h, const nut_paged_evict_args *args, void 
         a.counts = h->counts;
         DeviceScope scope(h->device);
         cuda_check(nut::paged_evict(a, static_cast<cudaStream_t>(stream)), "paged evict");
+    });
+}
+
+nut_status nut_paged_reserve_tree(nut_paged *h, int64_t max_new) {
+    return guarded([&] {
+        if (!h)
+            raise(NUT_INVALID_ARGUMENT, "null handle");
+        if (max_new <= 0)
+            raise(NUT_INVALID_ARGUMENT, "max_new must be positive");
+        if (max_new > NUT_TREE_MAX)
+            raise(NUT_LENGTH_ERROR, "more drafted tokens than NUT_TREE_MAX");
+        if (max_new <= h->tree_max)
+            return;
+        const nut::PagedPool &p = h->pool;
+        if (max_new * p.group > (1 << 24))
+            raise(NUT_LENGTH_ERROR, "too many rows for one kv head");
+        DeviceScope scope(h->device);
+        if (h->tree_box == 0) {
+            int box = nut::kTreeMostBox, shift = 0;
+            while (p.page_size % box != 0)
+                box /= 2;
+            while ((1 << shift) < box)
+                shift++;
+            const bool whole = p.head_dim % (p.type == NUT_F32 ? 32 : 64) == 0;
+            h->tree_key_map = pool_map(p, p.keys, box, whole, true);
+            h->tree_value_map = pool_map(p, p.values, box, whole, true);
+            h->tree_whole_columns = whole;
+            h->tree_box_shift = shift;
+            h->tree_box = box;
+        }
+        const int64_t floats = nut::tree_part_floats(p, int(max_new));
+        const size_t joins = (size_t(h->sms) * nut::kTreeCtasPerSm * sizeof(int4) + 255) / 256 * 256;
+        const size_t bytes = joins + size_t(h->sms) * nut::kTreeCtasPerSm * 2 * floats * sizeof(float);
+        h->tree_blocks.reserve(h->tree_blocks.size() + 1);
+        void *block = nullptr;
+        cuda_check(cudaMallocFromPoolAsync(&block, bytes, workspace_pool(h->device), nullptr), "alloc tree workspace");
+        h->tree_blocks.push_back(static_cast<char *>(block));
+        cuda_check(cudaStreamSynchronize(nullptr), "finish tree workspace");
+        h->tree_joins = reinterpret_cast<int4 *>(h->tree_blocks.back());
+        h->tree_partial = reinterpret_cast<float *>(h->tree_blocks.back() + joins);
+        h->tree_part_floats = floats;
+        h->tree_max = int(max_new);
+    });
+}
+
+nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_tree_args &g = *args;
+        const nut::PagedPool &p = h->pool;
+        if (!g.q || !g.out || !g.starts || !g.mask)
+            raise(NUT_INVALID_ARGUMENT, "null q, out, starts or mask");
+        check_row_type(*h, g.type);
+        if (g.rows < 0 || g.max_new < 0)
+            raise(NUT_INVALID_ARGUMENT, "negative row count");
+        if (g.max_new > h->tree_max)
+            raise(NUT_LENGTH_ERROR, "more drafted tokens than reserved (nut_paged_reserve_tree)");
+        if (g.rows > INT_MAX || g.mask_words > INT_MAX)
+            raise(NUT_LENGTH_ERROR, "too many rows or mask words");
+        if (g.mask_words < (g.max_new + 31) / 32)
+            raise(NUT_INVALID_ARGUMENT, "mask_words must cover max_new");
+        if (!std::isfinite(g.scale))
+            raise(NUT_INVALID_ARGUMENT, "scale must be finite");
+        nut::PagedTree a{};
+        a.q_stride = stride_of(g.q_stride, int64_t(p.heads) * p.head_dim, "q_stride");
+        a.out_stride = stride_of(g.out_stride, int64_t(p.heads) * p.head_dim, "out_stride");
+        /* the line of tiles is counted in 32 bits */
+        if (nut::tree_most_places(p, int(g.max_new), g.rows) > INT_MAX - 2 * nut::kMaxSms * nut::kTreeCtasPerSm)
+            raise(NUT_LENGTH_ERROR, "too many rows for so long a table: split the call");
+        if (g.rows == 0 || g.max_new == 0)
+            return;
+        a.p = p;
+        a.key_map = h->tree_key_map;
+        a.value_map = h->tree_value_map;
+        a.box = h->tree_box;
+        a.box_shift = h->tree_box_shift;
+        a.whole_columns = h->tree_whole_columns;
+        a.page_shift = h->page_shift;
+        a.page_magic = h->page_magic;
+        a.q = g.q;
+        a.out = g.out;
+        a.lse = g.lse;
+        a.starts = g.starts;
+        a.mask = g.mask;
+        a.mask_words = int(g.mask_words);
+        a.rows = int(g.rows);
+        a.max_new = int(g.max_new);
+        a.type = g.type;
+        a.scale = g.scale != 0.0f ? g.scale : float(1.0 / std::sqrt(double(p.head_dim)));
+        a.partial = h->tree_partial;
+        a.joins = h->tree_joins;
+        a.part_floats = h->tree_part_floats;
+        a.sms = h->sms;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_tree(a, static_cast<cudaStream_t>(stream)), "paged tree attention");
+    });
+}
+
+nut_status nut_paged_compact(nut_paged *h, const nut_paged_compact_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_compact_args &g = *args;
+        if (!g.starts || !g.new_lengths || (!g.accepted && g.n_accepted != 0))
+            raise(NUT_INVALID_ARGUMENT, "null starts, accepted or new_lengths");
+        if (g.n_accepted < 0)
+            raise(NUT_INVALID_ARGUMENT, "negative n_accepted");
+        if (g.n_accepted > NUT_TREE_MAX)
+            raise(NUT_LENGTH_ERROR, "more accepted tokens than NUT_TREE_MAX");
+        nut::PagedCompact a{};
+        a.p = h->pool;
+        a.starts = g.starts;
+        a.accepted = g.accepted;
+        a.n_accepted = int(g.n_accepted);
+        a.new_lengths = g.new_lengths;
+        a.positions = g.positions;
+        a.weights = g.weights;
+        a.order = h->order;
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_compact(a, static_cast<cudaStream_t>(stream)), "paged compact");
+    });
+}
+
+nut_status nut_paged_copy(nut_paged *h, const nut_paged_copy_args *args, void *stream) {
+    return guarded([&] {
+        if (!h || !args)
+            raise(NUT_INVALID_ARGUMENT, "null argument");
+        const nut_paged_copy_args &g = *args;
+        if (g.count < 0)
+            raise(NUT_INVALID_ARGUMENT, "negative count");
+        if (g.count == 0)
+            return;
+        if (!g.source || !g.target)
+            raise(NUT_INVALID_ARGUMENT, "null source or target");
+        if (g.count > INT_MAX)
+            raise(NUT_LENGTH_ERROR, "too many pages");
+        nut::PagedCopy a{};
+        a.p = h->pool;
+        a.source = g.source;
+        a.target = g.target;
+        a.slots = g.slots;
+        a.count = int(g.count);
+        DeviceScope scope(h->device);
+        cuda_check(nut::paged_copy(a, static_cast<cudaStream_t>(stream)), "paged copy");
     });
 }
 

@@ -1,0 +1,409 @@
+/* Attention of drafted tokens over the paged KV cache
+ * (nut_paged_tree_attention): fp32 arithmetic on any types, and the joining of
+ * split items.
+ *
+ *   z_t = scale q . k_t,  m = max z,  l = sum exp(z_t - m),
+ *   out = sum exp(z_t - m) v_t / l,   lse = m + log l
+ * over the slots a row sees, in one pass with a running maximum and sum.
+ *
+ * A tile is 64 slots, read once for all of an item's rows, in fp32 in shared
+ * memory; 256 threads form the products as 4 rows by slots, then 4 rows by
+ * dims.  FFMA and its operands' shared-memory reads bound it (16 products to
+ * five 16-byte reads); 16-bit caches take it only where the tensor cores'
+ * kernel has no form.
+ */
+#include <algorithm>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "paged_tree.cuh"
+
+namespace nut {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 64;
+
+/* kRows: 16 or 64 rows of an item. */
+template <int kRows, int DP> struct WidePlan {
+    static constexpr int kPitch = DP + 4; /* floats: rows begin 4 banks apart */
+    static constexpr int kWeights = kTile + 4;
+    static constexpr int kFloats = kRows * kPitch + kTile * kPitch + kRows * kWeights;
+    static constexpr int kBytes = kFloats * 4;
+    static constexpr int kAcross = kThreads / (kRows / 4); /* threads that share 4 rows */
+    static constexpr int kSlots = kTile / kAcross;         /* slots of a thread */
+    static constexpr int kPieces = (DP / 4 + kAcross - 1) / kAcross; /* 4-dim pieces of a thread */
+    static constexpr int kOfRow = kThreads / kRows;        /* threads of a row's softmax */
+    static constexpr int kPerSm = kBytes <= 110 * 1024 ? 2 : 1;
+};
+
+template <typename T> __device__ __forceinline__ void load_four(const T *x, float *v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(x);
+    } else {
+        const uint2 a = *reinterpret_cast<const uint2 *>(x);
+        const T *e = reinterpret_cast<const T *>(&a);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            v[i] = to_float(e[i]);
+    }
+}
+
+template <int kRows, int DP, typename T, typename R>
+__global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_kernel(const __grid_constant__ PagedTree a) {
+    using W = WidePlan<kRows, DP>;
+    extern __shared__ float4 smem_raw[];
+    float *queries = reinterpret_cast<float *>(smem_raw), *cached = queries + kRows * W::kPitch,
+          *weights = cached + kTile * W::kPitch;
+    __shared__ int64_t places[kTile]; /* elements from the pool's start, -1: no such slot */
+    __shared__ float maxima[kRows], sums[kRows], factors[kRows];
+    const PagedPool &p = a.p;
+    const int tid = threadIdx.x, D = p.head_dim;
+    begin_kernel();
+    int share;
+    TreeCursor cursor = tree_share<kThreads>(a, kTile, kRows, share);
+    tree_blind_rows<R>(a);
+    const int start = cursor.pos;
+    const int r0 = tid / W::kAcross * 4, c0 = tid % W::kAcross; /* of the products */
+    const int soft_row = tid / W::kOfRow, soft_at = tid % W::kOfRow;
+    const float unit = a.scale * kTreeLog2e;
+    int4 join = make_int4(0, 0, 0, 0);
+
+    TreeItem x;
+    while (cursor.next(a, kTile, kRows, x)) {
+        __syncthreads();
+        for (int i = tid; i < kRows * (DP / 4); i += kThreads) {
+            const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (r < x.rows && d < D) {
+                int64_t row;
+                int h;
+                tree_row(a, x.span.row0, x.head, x.first_row + r, row, h);
+                const R *q = static_cast<const R *>(a.q) + row * a.q_stride + int64_t(h) * D + d;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v[j] = to_float(q[j]);
+            }
+            *reinterpret_cast<float4 *>(queries + r * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        if (tid < kRows) {
+            maxima[tid] = -INFINITY;
+            sums[tid] = 0.0f;
+        }
+        float o[4][W::kPieces][4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int k = 0; k < W::kPieces; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[r][k][j] = 0.0f;
+
+        for (int tile = x.tile0; tile < x.tile1; tile++) {
+            const int t0 = tile * kTile;
+            if (tid < kTile) {
+                const int t = t0 + tid;
+                int64_t at = -1;
+                if (t < x.span.length) {
+                    const int j = t / p.page_size, page = checked_page(p, x.sequence, j);
+                    if (page >= 0)
+                        at = int64_t(page) * p.page_stride + int64_t(x.head) * p.head_stride +
+                             int64_t(t - j * p.page_size) * p.slot_stride;
+                }
+                places[tid] = at;
+            }
+            __syncthreads();
+            const auto fetch = [&](const void *pool) {
+                for (int i = tid; i < kTile * (DP / 4); i += kThreads) {
+                    const int t = i / (DP / 4), d = i % (DP / 4) * 4;
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (places[t] >= 0 && d < D)
+                        load_four(static_cast<const T *>(pool) + places[t] + d, v);
+                    *reinterpret_cast<float4 *>(cached + t * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            };
+            fetch(p.keys);
+            __syncthreads();
+            float z[4][W::kSlots];
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int k = 0; k < W::kSlots; k++)
+                    z[r][k] = 0.0f;
+#pragma unroll 4
+            for (int d = 0; d < DP; d += 4) {
+                float4 q[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    q[r] = *reinterpret_cast<const float4 *>(queries + (r0 + r) * W::kPitch + d);
+#pragma unroll
+                for (int k = 0; k < W::kSlots; k++) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cached + (c0 + k * W::kAcross) * W::kPitch + d);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        z[r][k] = fmaf(q[r].x, c.x, z[r][k]);
+                        z[r][k] = fmaf(q[r].y, c.y, z[r][k]);
+                        z[r][k] = fmaf(q[r].z, c.z, z[r][k]);
+                        z[r][k] = fmaf(q[r].w, c.w, z[r][k]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int k = 0; k < W::kSlots; k++)
+                    weights[(r0 + r) * W::kWeights + c0 + k * W::kAcross] = z[r][k] * unit;
+            __syncthreads();
+            fetch(p.values); /* in flight during the softmax */
+
+            /* softmax: kOfRow threads a row, 64 / kOfRow neighbouring slots each */
+            constexpr int kEach = kTile / W::kOfRow;
+            const int s0 = soft_at * kEach;
+            float *own = weights + soft_row * W::kWeights + s0;
+            float v[kEach], top = -INFINITY;
+            {
+                uint32_t sees = 0;
+                const int base = t0 + s0 - x.span.prefix;
+                if (soft_row < x.rows) {
+                    if (base <= -kEach) {
+                        sees = ~0u;
+                    } else {
+                        const int node = (x.first_row + soft_row) / p.group;
+                        sees = tree_sees(a.mask + (int64_t(x.span.row0) + node) * a.mask_words, base, x.span.n);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kEach; j++) {
+                    v[j] = ((sees >> j) & 1) && places[s0 + j] >= 0 ? own[j] : -INFINITY;
+                    top = fmaxf(top, v[j]);
+                }
+            }
+#pragma unroll
+            for (int e = W::kOfRow / 2; e > 0; e >>= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+            const float before = maxima[soft_row], next = fmaxf(before, top);
+            const float from = next == -INFINITY ? 0.0f : next;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kEach; j++) {
+                const float w = exp2f(v[j] - from);
+                own[j] = w;
+                sum += w;
+            }
+#pragma unroll
+            for (int e = W::kOfRow / 2; e > 0; e >>= 1)
+                sum += __shfl_xor_sync(0xffffffffu, sum, e);
+            if (soft_at == 0) {
+                const float keep = before == next ? 1.0f : exp2f(before - next);
+                factors[soft_row] = keep;
+                maxima[soft_row] = next;
+                sums[soft_row] = sums[soft_row] * keep + sum;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float keep = factors[r0 + r];
+#pragma unroll
+                for (int k = 0; k < W::kPieces; k++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[r][k][j] *= keep;
+            }
+            /* values that a row does not see may be infinite or NaN: a weight of 0 takes no part */
+            const bool drafted = t0 + kTile > x.span.prefix;
+#pragma unroll 4
+            for (int t = 0; t < kTile; t++) {
+                float w[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    w[r] = weights[(r0 + r) * W::kWeights + t];
+#pragma unroll
+                for (int k = 0; k < W::kPieces; k++) {
+                    const int d = (c0 + k * W::kAcross) * 4;
+                    if (d >= DP)
+                        break;
+                    const float4 c = *reinterpret_cast<const float4 *>(cached + t * W::kPitch + d);
+                    const float e[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            o[r][k][j] = fmaf(w[r], drafted && w[r] == 0.0f ? 0.0f : e[j], o[r][k][j]);
+                }
+            }
+            __syncthreads();
+        }
+
+        const bool whole = x.whole();
+        const TreePart part = tree_part(a, blockIdx.x, x.first <= start ? 0 : 1, x.rows);
+        if (tid < x.rows) {
+            const float m = maxima[tid], l = sums[tid];
+            if (whole) {
+                int64_t row;
+                int h;
+                tree_row(a, x.span.row0, x.head, x.first_row + tid, row, h);
+                if (a.lse)
+                    a.lse[row * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kTreeLn2;
+            } else {
+                part.maxima[tid] = m;
+                part.sums[tid] = l;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int f = r0 + r;
+            if (f >= x.rows)
+                break;
+            int64_t row;
+            int h;
+            tree_row(a, x.span.row0, x.head, x.first_row + f, row, h);
+            const float inv = !whole ? 1.0f : sums[f] == 0.0f ? 0.0f : 1.0f / sums[f];
+#pragma unroll
+            for (int k = 0; k < W::kPieces; k++) {
+                const int d = (c0 + k * W::kAcross) * 4;
+                if (d >= D)
+                    break;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (whole)
+                        static_cast<R *>(a.out)[row * a.out_stride + int64_t(h) * D + d + j] = output_of<R>(o[r][k][j] * inv);
+                    else
+                        part.out[int64_t(f) * D + d + j] = o[r][k][j];
+                }
+            }
+        }
+        if (!whole && x.tile0 == 0)
+            join = tree_join(x, share);
+    }
+    if (tid == 0)
+        a.joins[blockIdx.x] = join;
+}
+
+/* ---- joining the parts of an item --------------------------------------- */
+
+constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 32;
+
+/* A warp joins a row: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m).  Lanes
+ * turn the parts' maxima and sums into factors, 32 parts at a time, then take
+ * 4 dims each. */
+template <typename R> __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ PagedTree a, int block_rows) {
+    begin_kernel();
+    const int4 join = a.joins[blockIdx.x];
+    const int parts = join.x, lane = threadIdx.x & 31;
+    if (parts == 0)
+        return;
+    const PagedPool &p = a.p;
+    const int D = p.head_dim, first_row = join.w >> 1, inside = join.w & 1;
+    const int row0 = a.starts[join.y], n = a.starts[join.y + 1] - row0;
+    const int rows = min(block_rows, n * p.group - first_row);
+    const int f = int(blockIdx.y) * kJoinRows + int(threadIdx.x >> 5);
+    if (f >= rows)
+        return;
+    const auto part = [&](int c) { return tree_part(a, blockIdx.x + c, c == 0 ? inside : 0, rows); };
+    float top = -INFINITY;
+    for (int c = lane; c < parts; c += 32)
+        top = fmaxf(top, part(c).maxima[f]);
+    top = warp_max(top);
+    const float from = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    for (int c0 = 0; c0 < parts; c0 += 32) {
+        const int c = c0 + lane, many = min(32, parts - c0);
+        const float factor = c < parts ? exp2f(part(c).maxima[f] - from) : 0.0f;
+        if (c < parts)
+            sum = fmaf(part(c).sums[f], factor, sum);
+#pragma unroll 8
+        for (int i = 0; i < many; i++) {
+            const float w = __shfl_sync(0xffffffffu, factor, i);
+            const float *out = part(c0 + i).out + int64_t(f) * D;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int d = k * 128 + lane * 4;
+                if (d < D && w != 0.0f) {
+                    const float4 v = *reinterpret_cast<const float4 *>(out + d);
+                    o[k].x = fmaf(v.x, w, o[k].x);
+                    o[k].y = fmaf(v.y, w, o[k].y);
+                    o[k].z = fmaf(v.z, w, o[k].z);
+                    o[k].w = fmaf(v.w, w, o[k].w);
+                }
+            }
+        }
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    int64_t row;
+    int h;
+    tree_row(a, row0, join.z, first_row + f, row, h);
+    if (a.lse && lane == 0)
+        a.lse[row * p.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kTreeLn2;
+    R *to = static_cast<R *>(a.out) + row * a.out_stride + int64_t(h) * D;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = k * 128 + lane * 4;
+        if (d < D) {
+            to[d] = output_of<R>(o[k].x * inv);
+            to[d + 1] = output_of<R>(o[k].y * inv);
+            to[d + 2] = output_of<R>(o[k].z * inv);
+            to[d + 3] = output_of<R>(o[k].w * inv);
+        }
+    }
+}
+
+template <int kRows, int DP, typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cudaStream_t s) {
+    using W = WidePlan<kRows, DP>;
+    const auto kernel = wide_kernel<kRows, DP, T, R>;
+    static bool set[kMaxDevices] = {};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    if (!set[device % kMaxDevices]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::kBytes);
+        if (e != cudaSuccess)
+            return e;
+        set[device % kMaxDevices] = true;
+    }
+    static_assert(W::kPerSm <= kTreeCtasPerSm, "the workspace has room for as many");
+    const int ctas = a.sms * W::kPerSm;
+    e = launch_kernel(kernel, dim3(ctas), kThreads, W::kBytes, s, 1, a);
+    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, s);
+}
+
+template <typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cudaStream_t s) {
+    const int D = a.p.head_dim;
+    const bool few = int64_t(a.max_new) * a.p.group <= 16;
+    if (D <= 64)
+        return few ? launch_wide<16, 64, T, R>(a, s) : launch_wide<64, 64, T, R>(a, s);
+    if (D <= 128)
+        return few ? launch_wide<16, 128, T, R>(a, s) : launch_wide<64, 128, T, R>(a, s);
+    return few ? launch_wide<16, 256, T, R>(a, s) : launch_wide<64, 256, T, R>(a, s);
+}
+
+} // namespace
+
+cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaStream_t s) {
+    const int rows = int(std::min<int64_t>(block_rows, int64_t(a.max_new) * a.p.group));
+    const dim3 grid(ctas, (rows + kJoinRows - 1) / kJoinRows);
+    const auto kernel = a.type == 0 ? join_kernel<float> : a.type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>;
+    return launch_kernel(kernel, grid, kJoinThreads, 0, s, 1, a, block_rows);
+}
+
+int64_t tree_part_floats(const PagedPool &p, int max_new) {
+    const int64_t rows = std::min<int64_t>(256, int64_t(max_new) * p.group);
+    return (rows * 2 + 3) / 4 * 4 + rows * p.head_dim;
+}
+
+int64_t tree_most_places(const PagedPool &p, int max_new, int64_t rows) {
+    const int64_t most = std::min<int64_t>(rows, int64_t(p.sequences) * max_new);
+    return (most * p.heads / 16 + int64_t(p.sequences) * p.kv_heads + 1) * (p.capacity / 64 + 1 + kTreeItemCost);
+}
+
+cudaError_t paged_tree(const PagedTree &a, cudaStream_t s) {
+    if (a.p.type == 0)
+        return launch_wide<float, float>(a, s);
+    if (a.p.type == 1)
+        return a.type == 0 ? launch_wide<__half, float>(a, s) : launch_wide<__half, __half>(a, s);
+    return a.type == 0 ? launch_wide<__nv_bfloat16, float>(a, s) : launch_wide<__nv_bfloat16, __nv_bfloat16>(a, s);
+}
+
+} // namespace nut
