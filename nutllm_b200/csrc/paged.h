@@ -115,7 +115,7 @@ struct PagedCopy {
 };
 
 constexpr int kTreeMost = 1024;   /* drafted tokens of a sequence */
-constexpr int kTreeMostBox = 128; /* slots of a box of the tree attention's maps */
+constexpr int kTreeMostBox = 64; /* slots of a box of the tree attention's maps */
 constexpr int kTreeCtasPerSm = 2;
 
 struct PagedTree {
@@ -123,7 +123,7 @@ struct PagedTree {
      * `box` slots; the column is the whole row where head_dim is no multiple of it */
     CUtensorMap key_map, value_map;
     PagedPool p;
-    int box, box_shift, whole_columns;
+    int box, whole_columns, aligned; /* aligned: rows of q and out begin at multiples of 16 bytes */
     uint64_t page_magic;
     int page_shift;
     const void *q;
@@ -163,5 +163,6 @@ cudaError_t paged_evict(const PagedEvict &a, cudaStream_t s);
 cudaError_t paged_compact(const PagedCompact &a, cudaStream_t s);
 cudaError_t paged_copy(const PagedCopy &a, cudaStream_t s);
 cudaError_t paged_tree(const PagedTree &a, cudaStream_t s);
+cudaError_t paged_tree_tc(const PagedTree &a, cudaStream_t s);
 
 } // namespace nut

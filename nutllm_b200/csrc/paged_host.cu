@@ -125,7 +125,7 @@ struct nut_paged {
     int32_t *pairs = nullptr, *counts = nullptr, *order = nullptr;
     /* nut_paged_reserve_tree */
     CUtensorMap tree_key_map{}, tree_value_map{};
-    int tree_box = 0, tree_box_shift = 0, tree_max = 0;
+    int tree_box = 0, tree_max = 0;
     bool tree_whole_columns = false;
     std::vector<char *> tree_blocks; /* the last is in use; captured calls may use the others */
     float *tree_partial = nullptr;
@@ -509,16 +509,13 @@ nut_status nut_paged_reserve_tree(nut_paged *h, int64_t max_new) {
             raise(NUT_LENGTH_ERROR, "too many rows for one kv head");
         DeviceScope scope(h->device);
         if (h->tree_box == 0) {
-            int box = nut::kTreeMostBox, shift = 0;
+            int box = nut::kTreeMostBox;
             while (p.page_size % box != 0)
                 box /= 2;
-            while ((1 << shift) < box)
-                shift++;
             const bool whole = p.head_dim % (p.type == NUT_F32 ? 32 : 64) == 0;
             h->tree_key_map = pool_map(p, p.keys, box, whole, true);
             h->tree_value_map = pool_map(p, p.values, box, whole, true);
             h->tree_whole_columns = whole;
-            h->tree_box_shift = shift;
             h->tree_box = box;
         }
         const int64_t floats = nut::tree_part_floats(p, int(max_new));
@@ -567,7 +564,6 @@ nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *arg
         a.key_map = h->tree_key_map;
         a.value_map = h->tree_value_map;
         a.box = h->tree_box;
-        a.box_shift = h->tree_box_shift;
         a.whole_columns = h->tree_whole_columns;
         a.page_shift = h->page_shift;
         a.page_magic = h->page_magic;
@@ -580,6 +576,8 @@ nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *arg
         a.rows = int(g.rows);
         a.max_new = int(g.max_new);
         a.type = g.type;
+        const int64_t element = g.type == NUT_F32 ? 4 : 2;
+        a.aligned = aligned16(g.q) && aligned16(g.out) && a.q_stride * element % 16 == 0 && a.out_stride * element % 16 == 0;
         a.scale = g.scale != 0.0f ? g.scale : float(1.0 / std::sqrt(double(p.head_dim)));
         a.partial = h->tree_partial;
         a.joins = h->tree_joins;

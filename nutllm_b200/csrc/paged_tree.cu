@@ -399,6 +399,8 @@ int64_t tree_most_places(const PagedPool &p, int max_new, int64_t rows) {
 }
 
 cudaError_t paged_tree(const PagedTree &a, cudaStream_t s) {
+    if (a.p.type != 0 && a.p.head_dim <= 128)
+        return paged_tree_tc(a, s);
     if (a.p.type == 0)
         return launch_wide<float, float>(a, s);
     if (a.p.type == 1)
