@@ -120,12 +120,13 @@ constexpr int kTreeCtasPerSm = 2;
 
 struct PagedTree {
     /* (dim, slot, 128-byte column, kv head, page) in boxes of one column by
-     * `box` slots; the column is the whole row where head_dim is no multiple of it */
-    CUtensorMap key_map, value_map;
+     * `box` slots; the column is the whole row where head_dim is no multiple of
+     * it.  wide_value_map: all columns by 16 slots, where there are such */
+    CUtensorMap key_map, value_map, wide_value_map;
     PagedPool p;
     int box, whole_columns, aligned; /* aligned: rows of q and out begin at multiples of 16 bytes */
-    uint64_t page_magic;
-    int page_shift;
+    uint64_t page_magic, group_magic; /* as PagedAttention's */
+    int page_shift, group_shift;
     const void *q;
     void *out;
     int64_t q_stride, out_stride;

@@ -114,8 +114,8 @@ struct nut_paged {
     CUtensorMap key_map{}, value_map{};
     int box = 16;
     bool whole_columns = false;
-    uint64_t page_magic = 0;
-    int page_shift = 32;
+    uint64_t page_magic = 0, group_magic = 0;
+    int page_shift = 32, group_shift = 32;
     int max_rows = 0;
     bool track = false;
     int sms = 0;
@@ -199,10 +199,14 @@ nut_status nut_paged_create(const nut_paged_view *view, int device, nut_paged **
         h->sms = std::min(h->sms, nut::kMaxSms);
         while (p.page_size % h->box != 0)
             h->box /= 2;
-        /* ceil(2^(32 + s) / page_size) with 2^s < page_size <= 2^(s + 1): exact below 2^31 */
-        while ((int64_t(1) << (h->page_shift - 31)) < p.page_size)
-            h->page_shift++;
-        h->page_magic = ((uint64_t(1) << h->page_shift) + p.page_size - 1) / p.page_size;
+        /* ceil(2^(32 + s) / divisor) with 2^s < divisor <= 2^(s + 1): exact below 2^31 */
+        const auto magic = [](int divisor, uint64_t &factor, int &shift) {
+            while ((int64_t(1) << (shift - 31)) < divisor)
+                shift++;
+            factor = ((uint64_t(1) << shift) + divisor - 1) / divisor;
+        };
+        magic(p.page_size, h->page_magic, h->page_shift);
+        magic(p.group, h->group_magic, h->group_shift);
         h->whole_columns = h->box == 16 && p.head_dim % (p.type == NUT_F32 ? 32 : 64) == 0;
         h->key_map = pool_map(p, p.keys, h->box, h->whole_columns);
         h->value_map = pool_map(p, p.values, h->box, h->whole_columns);
@@ -563,10 +567,13 @@ nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *arg
         a.p = p;
         a.key_map = h->tree_key_map;
         a.value_map = h->tree_value_map;
+        a.wide_value_map = h->value_map;
         a.box = h->tree_box;
         a.whole_columns = h->tree_whole_columns;
         a.page_shift = h->page_shift;
         a.page_magic = h->page_magic;
+        a.group_shift = h->group_shift;
+        a.group_magic = h->group_magic;
         a.q = g.q;
         a.out = g.out;
         a.lse = g.lse;

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
     begin_kernel();
     int share;
     TreeCursor cursor = tree_share<kThreads>(a, kTile, kRows, share);
-    tree_blind_rows<R>(a);
+    tree_blind_rows<R>(a, tid, kThreads);
     const int start = cursor.pos;
     const int r0 = tid / W::kAcross * 4, c0 = tid % W::kAcross; /* of the products */
     const int soft_row = tid / W::kOfRow, soft_at = tid % W::kOfRow;
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                     if (base <= -kEach) {
                         sees = ~0u;
                     } else {
-                        const int node = (x.first_row + soft_row) / p.group;
+                        const int node = tree_node(a, x.first_row + soft_row);
                         sees = tree_sees(a.mask + (int64_t(x.span.row0) + node) * a.mask_words, base, x.span.n);
                     }
                 }
@@ -389,7 +389,7 @@ cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaSt
 }
 
 int64_t tree_part_floats(const PagedPool &p, int max_new) {
-    const int64_t rows = std::min<int64_t>(256, int64_t(max_new) * p.group);
+    const int64_t rows = std::min<int64_t>(128, int64_t(max_new) * p.group);
     return (rows * 2 + 3) / 4 * 4 + rows * p.head_dim;
 }
 

@@ -147,26 +147,31 @@ __device__ __forceinline__ TreeCursor tree_share(const PagedTree &a, int tile, i
     return {start, min(start + share, total), found[0], found[1]};
 }
 
-/* Rows that see nothing; run by all threads of all CTAs. */
-template <typename R> __device__ __forceinline__ void tree_blind_rows(const PagedTree &a) {
+/* Rows that see nothing; run by `threads` threads of every CTA. */
+template <typename R> __device__ __noinline__ void tree_blind_rows(const PagedTree &a, int tid, int threads) {
     const int H = a.p.heads, width = H * a.p.head_dim;
     for (int s = blockIdx.x; s < a.p.sequences; s += gridDim.x) {
         const TreeSpan x = tree_span(a, s);
         if (x.n == 0 || !x.blind)
             continue;
         for (int r = x.row0; r < x.row0 + x.n; r++) {
-            for (int i = threadIdx.x; i < width; i += blockDim.x)
+            for (int i = tid; i < width; i += threads)
                 static_cast<R *>(a.out)[r * a.out_stride + i] = from_float<R>(0.0f);
             if (a.lse)
-                for (int h = threadIdx.x; h < H; h += blockDim.x)
+                for (int h = tid; h < H; h += threads)
                     a.lse[int64_t(r) * H + h] = -INFINITY;
         }
     }
 }
 
-/* Row f of an item: its row in q and out, and its query head. */
+/* Drafted token of row f of a sequence and kv head. */
+__device__ __forceinline__ int tree_node(const PagedTree &a, int f) {
+    return int((uint64_t(unsigned(f)) * a.group_magic) >> a.group_shift);
+}
+
+/* Row f of a sequence and kv head: its row in q and out, and its query head. */
 __device__ __forceinline__ void tree_row(const PagedTree &a, int row0, int head, int f, int64_t &row, int &query_head) {
-    const int node = f / a.p.group;
+    const int node = tree_node(a, f);
     row = row0 + node;
     query_head = head * a.p.group + f - node * a.p.group;
 }

@@ -6,13 +6,14 @@
  * S = Q K^T and outputs O += P V of 128 rows by tcgen05.mma, with S, P and O in
  * tensor memory and a thread for each row in the softmax between them.
  *
- *   warp 8      copies key and value tiles (TMA boxes of a page's slots) into
- *               a ring of stages, and notes which slots there are
- *   warp 9      issues the products
- *   warps 0-3, 4-7   the softmax of two streams, each with its own S, P and O:
- *               the halves of more than 128 rows on the same tiles, else
- *               every other tile of the same rows, joined at the item's end.
- *               While one stream does its softmax the other's products run.
+ *   warps 0-3   the softmax, a thread for each row
+ *   warp 4      copies key and value tiles of 64 slots (TMA boxes of a page's
+ *               slots) into a ring of stages, and notes which slots there are
+ *   warp 5      issues the products: those of the next tile's logits run
+ *               during the softmax
+ * Two such blocks share an SM where the queries leave room: one's products
+ * and copies run while the other is in its softmax, loads its queries or
+ * writes its outputs.
  *
  * Queries in fp32 are split into 16-bit terms that multiply the same keys, and
  * so are their weights: two for fp16 (queries first scaled by a power of two
@@ -36,31 +37,34 @@
 namespace nut {
 namespace {
 
-constexpr int kStreams = 2;
-constexpr int kThreads = kStreams * 128 + 64;
-constexpr int kProducer = kStreams * 4, kIssuer = kProducer + 1; /* warps */
+constexpr int kRows = 128;
+constexpr int kTile = 64;
+constexpr int kProducer = 4, kIssuer = 5; /* warps */
+constexpr int kThreads = 192;
 constexpr uint64_t kTreeWaitNs = 2000000000ull;
 
 /* kTerms: 16-bit terms of a query and of a weight. */
 template <int DP_, int kTerms_> struct TcPlan {
     static constexpr int DP = DP_, kTerms = kTerms_;
-    /* three terms of 128 weights do not fit in their logits' place */
-    static constexpr int kTile = kTerms == 3 ? 64 : 128;
     static constexpr int kColumns = DP / 64; /* of 128 bytes */
-    static constexpr int kQueryTiles = kTerms == 1 ? 2 : 1;
-    static constexpr int kBlockRows = 128 * kQueryTiles;
-    static constexpr int kQueryBytes = 128 * DP * 2;
-    static constexpr int kQueries = kQueryBytes * kQueryTiles * kTerms;
+    static constexpr int kQueryBytes = kRows * DP * 2; /* of a term */
+    static constexpr int kQueries = kQueryBytes * kTerms;
     static constexpr int kStage = kTile * DP * 2;
-    static constexpr int kFit = (227 * 1024 - 1024 - 4096 - kQueries) / kStage; /* beside alignment and static shared memory */
-    static constexpr int kStages = kFit < 10 ? kFit : 10;
+    static constexpr int kSpare = 1024 + 2560; /* alignment, static shared memory and the block's own 1 KB */
+    static constexpr int kPerSm = kQueries + 4 * kStage + kSpare <= 114 * 1024 ? 2 : 1;
+    static constexpr int kFit = ((kPerSm == 2 ? 114 : 227) * 1024 - kSpare - kQueries) / kStage;
+    static constexpr int kStages = kFit < 12 ? kFit : 12;
     static constexpr int kBytes = 1024 + kQueries + kStages * kStage;
-    /* tensor memory: S (P in its place) of both streams, then O of both */
-    static constexpr int kLogits = kTile > kTerms * kTile / 2 ? kTile : kTerms * kTile / 2;
-    static constexpr int kOutputs = kStreams * kLogits;
-    static_assert(kOutputs + kStreams * DP <= 512, "columns of tensor memory");
-    static_assert(kQueries >= 128 * DP * 4, "the streams' outputs meet there");
+    /* tensor memory: S, with P in its place, once or twice; then O */
+    static constexpr int kLogits = kTerms * kTile / 2 > kTile ? kTerms * kTile / 2 : kTile;
+    static constexpr int kMemory = kPerSm == 2 ? 256 : 512;
+    static constexpr int kBuffers = 2 * kLogits + DP <= kMemory ? 2 : 1;
+    static constexpr int kOutputs = kBuffers * kLogits;
+    static_assert(kOutputs + DP <= kMemory, "columns of tensor memory");
+    static_assert(kQueries >= kRows * 128, "the outputs leave through there, 32 dims at a time");
     static_assert(kStages >= 4, "keys of two tiles and values of one are in use at a time");
+    static_assert(kStages / 2 + 2 < 8, "tiles under way: Shared::valid");
+    static_assert(kPerSm <= kTreeCtasPerSm, "the workspace has room for as many");
 };
 
 /* ---- PTX --------------------------------------------------------------- */
@@ -133,12 +137,13 @@ __device__ __forceinline__ float power2(float x) {
     return y;
 }
 
-/* A matrix in 128-byte rows with the 128-byte swizzle, 1024 bytes to 8 rows.
- * Rows along the product's M or N (K-major): `lead` has no meaning.  Rows
- * along its K (MN-major): 8 of K are 1024 bytes, 64 of N are `lead`. */
-__device__ __forceinline__ uint64_t matrix_at(uint32_t addr, uint32_t lead) {
-    return uint64_t((addr >> 4) & 0x3fffu) | uint64_t((lead >> 4) & 0x3fffu) << 16 | uint64_t(1024 >> 4) << 32 |
-           uint64_t(1) << 46 | uint64_t(2) << 61;
+/* A matrix in 128-byte rows with the 128-byte swizzle, 8 rows together.  Rows
+ * along the product's M or N (K-major): 8 of them are `step` bytes from the
+ * next 8, `lead` has no meaning.  Rows along its K (MN-major): 8 of K are
+ * `step` bytes, 64 of N `lead`. */
+__device__ __forceinline__ uint64_t matrix_at(uint32_t addr, uint32_t lead, uint32_t step) {
+    return uint64_t((addr >> 4) & 0x3fffu) | uint64_t(lead >> 4) << 16 | uint64_t(step >> 4) << 32 | uint64_t(1) << 46 |
+           uint64_t(2) << 61;
 }
 /* fp32 accumulators; fp16 or bf16 operands of 128 x K and N x K, B's rows along
  * K if `along_k`. */
@@ -155,6 +160,10 @@ template <> struct Pair<__half> {
         return *reinterpret_cast<const uint32_t *>(&h);
     }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+    static __device__ __forceinline__ uint32_t add_zero_times(uint32_t sum, uint32_t v) {
+        asm("fma.rn.f16x2 %0, %1, %2, %0;\n" : "+r"(sum) : "r"(v), "r"(0u));
+        return sum;
+    }
 };
 template <> struct Pair<__nv_bfloat16> {
     static constexpr uint32_t kInfinite = 0x7f80u;
@@ -165,33 +174,129 @@ template <> struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ float2 unpack(uint32_t v) {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     }
+    static __device__ __forceinline__ uint32_t add_zero_times(uint32_t sum, uint32_t v) {
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;\n" : "+r"(sum) : "r"(v), "r"(0u));
+        return sum;
+    }
 };
 
 /* ---- the kernel ---------------------------------------------------------- */
 
+/* 16 bytes of elements whose address is a multiple of an element only.  (Not
+ * through an array that a pointer reaches: that would lie in local memory, and
+ * each of a thread's loads would wait for the one before.) */
+__device__ __forceinline__ uint4 load_elements(const float *q) {
+    return make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3]));
+}
+template <typename R> __device__ __forceinline__ uint4 load_elements(const R *x) {
+    const unsigned short *q = reinterpret_cast<const unsigned short *>(x);
+    return make_uint4(q[0] | uint32_t(q[1]) << 16, q[2] | uint32_t(q[3]) << 16, q[4] | uint32_t(q[5]) << 16,
+                      q[6] | uint32_t(q[7]) << 16);
+}
+
+/* Four outputs whose address is a multiple of an element only. */
+template <typename R> __device__ __noinline__ void store_elements(R *to, float4 v, bool really) {
+    if (really) {
+        to[0] = output_of<R>(v.x);
+        to[1] = output_of<R>(v.y);
+        to[2] = output_of<R>(v.z);
+        to[3] = output_of<R>(v.w);
+    }
+}
+template <typename R> __device__ __forceinline__ uint32_t pack_outputs(float a, float b) {
+    const R e[2] = {output_of<R>(a), output_of<R>(b)};
+    return *reinterpret_cast<const uint32_t *>(e);
+}
+
+/* Takes infinities and NaN out of 16 bytes of values. */
+template <typename T> __device__ __noinline__ void take_out(uint32_t at) {
+    constexpr uint32_t kInf = Pair<T>::kInfinite;
+    uint32_t e[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3]) : "r"(at));
+    for (int j = 0; j < 4; j++)
+        e[j] &= ~__vcmpeq2(e[j] & (kInf | kInf << 16), kInf | kInf << 16);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
+}
+
+/* Half of a slot's row of a value tile, its 128-byte columns `lead` apart:
+ * zeros where there is no such slot, else infinities and NaN taken out (and
+ * noted).  0 times a value is NaN if it is one of those. */
+template <typename T, int DP>
+__device__ __forceinline__ void clean_values(uint32_t row, int slot, int half, uint32_t lead, bool there, int *odd) {
+    constexpr int kPieces = DP / 16;
+    const auto at = [&](int k) {
+        const int c = half * kPieces + k;
+        return row + (c >> 3) * lead + (((c & 7) ^ (slot & 7)) << 4);
+    };
+    if (!there) {
+#pragma unroll
+        for (int k = 0; k < kPieces; k++)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(at(k)), "r"(0) : "memory");
+        return;
+    }
+    uint32_t zeros[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+        uint32_t e[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3]) : "r"(at(k)));
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            zeros[j] = Pair<T>::add_zero_times(zeros[j], e[j]);
+    }
+    const uint32_t all = (zeros[0] | zeros[1] | zeros[2] | zeros[3]) & 0x7fff7fffu;
+    if (all != 0) {
+        *odd = 1;
+#pragma unroll 1
+        for (int k = 0; k < kPieces; k++)
+            take_out<T>(at(k));
+    }
+}
+
+/* Adds the infinities and NaN among the values of drafted tokens in slots
+ * s0 .. s1 - 1 that a row (mask words `seen`) sees to its outputs of dims
+ * d0 .. d0 + 31, in 16-byte pieces that lie swizzled by the row. */
+template <typename T>
+__device__ __noinline__ void add_odd_values(const PagedTree &a, const TreeItem &x, const uint32_t *seen, int s0, int s1, int d0,
+                                            float4 *out, int row) {
+    const PagedPool &p = a.p;
+    for (int s = s0; s < s1; s++) {
+        const int node = s - x.span.prefix, page = lookup(p, x.sequence, s / p.page_size);
+        if (page < 0 || !((seen[node >> 5] >> (node & 31)) & 1))
+            continue;
+        const T *v = static_cast<const T *>(p.values) + int64_t(page) * p.page_stride + int64_t(x.head) * p.head_stride +
+                     int64_t(s % p.page_size) * p.slot_stride;
+        for (int j = 0; j < 32 && d0 + j < p.head_dim; j++) {
+            const float e = to_float(v[d0 + j]);
+            if (!(fabsf(e) <= 3.402823466e38f))
+                reinterpret_cast<float *>(out + ((j / 4) ^ (row & 7)))[j % 4] += e;
+        }
+    }
+}
+
+constexpr int kNoted = 8;
+
 template <int kStages> struct Shared {
     uint64_t full[kStages], empty[kStages];
     uint64_t queries;                      /* an item's are in shared memory */
-    uint64_t logits[kStreams];             /* a tile's are in tensor memory */
-    uint64_t weights[kStreams];            /* and its weights */
-    uint64_t outputs[kStreams], drained;
-    uint32_t valid[kStages][4];            /* slots there are of a value tile */
-    float unit[128];                       /* of a row's logits (fp32 queries) */
-    float maxima[kStreams][128], sums[kStreams][128];
+    uint64_t logits[2];                    /* a tile's are in tensor memory */
+    uint64_t weights[2];                   /* its weights are; the softmax may be a tile ahead of the products */
+    uint64_t outputs;                      /* its product with the values is done */
+    uint64_t drained;                      /* products in flight after a wait ran out */
+    uint32_t valid[kNoted][2];             /* slots there are of the tiles under way */
+    float unit[kRows];                     /* of a row's logits (fp32 queries) */
     uint32_t tmem;
     int dead;                              /* a wait ran out: nothing more is waited for */
     int odd;                               /* an item's value tiles held infinities or NaN */
 };
 
-/* Where a tile's keys and values lie in the order of copies of an item of n
- * tiles: k0 k1 v0 k2 v1 ... */
+/* Copies of an item of n tiles come in this order: k0 k1 v0 k2 v1 ... */
 __device__ __forceinline__ int place_of_keys(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int place_of_values(int i, int n) { return i == n - 1 ? 2 * i + 1 : 2 * i + 2; }
 
 template <typename T, typename R, typename Plan>
-__global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__ PagedTree a) {
-    constexpr int DP = Plan::DP, kTile = Plan::kTile, kStages = Plan::kStages, kTerms = Plan::kTerms,
-                  kColumns = Plan::kColumns;
+__global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid_constant__ PagedTree a) {
+    constexpr int DP = Plan::DP, kStages = Plan::kStages, kTerms = Plan::kTerms, kColumns = Plan::kColumns,
+                  kBuffers = Plan::kBuffers;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr float kSlack = kTerms > 1 ? 0.0f : kHalf ? 7.0f : 8.0f;
     constexpr float kLift = !kHalf ? -38.0f : kTerms > 1 ? 15.0f : 8.0f; /* log2 of the greatest weight */
@@ -201,34 +306,40 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     const uint32_t queries_at = smem_u32(smem), ring_at = queries_at + Plan::kQueries;
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.head_dim;
+    /* a box of values has all columns of 16 slots where it can */
+    const bool wide = a.box >= 16 && a.whole_columns;
+    const uint32_t values_lead = wide ? 16 * 128 : kTile * 128, values_step = wide ? kColumns * 16 * 128 : 16 * 128;
 
     if (tid == 0) {
         for (int i = 0; i < kStages; i++) {
             mbar_init(&sh.full[i], 1);
             mbar_init(&sh.empty[i], 1);
         }
-        mbar_init(&sh.queries, kStreams * 128);
-        for (int w = 0; w < kStreams; w++) {
-            mbar_init(&sh.logits[w], 1);
-            mbar_init(&sh.weights[w], 128);
-            mbar_init(&sh.outputs[w], 1);
-        }
-        mbar_init(&sh.drained, 1); /* products in flight after a wait ran out */
+        mbar_init(&sh.queries, kRows);
+        mbar_init(&sh.logits[0], 1);
+        mbar_init(&sh.logits[1], 1);
+        mbar_init(&sh.weights[0], kRows);
+        mbar_init(&sh.weights[1], kRows);
+        mbar_init(&sh.outputs, 1);
+        mbar_init(&sh.drained, 1);
         sh.dead = sh.odd = 0;
         fence_barrier_init();
     }
     if (warp == kIssuer) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&sh.tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)),
+                     "n"(Plan::kMemory)
+                     : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
+    if (warp == kProducer && lane < 2)
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(lane == 0 ? &a.key_map : wide ? &a.wide_value_map : &a.value_map) : "memory");
     tc_before();
     begin_kernel();
     int share;
-    TreeCursor cursor = tree_share<kThreads>(a, kTile, Plan::kBlockRows, share); /* synchronises the block */
+    TreeCursor cursor = tree_share<kThreads>(a, kTile, kRows, share); /* synchronises the block */
     tc_after();
     const uint32_t tmem = sh.tmem;
     const int start = cursor.pos;
-    tree_blind_rows<R>(a);
 
     /* Waits for a barrier's phase.  After kTreeWaitNs somewhere nobody waits
      * any more: the roles run through their steps without doing them. */
@@ -259,103 +370,93 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     bool alive = true;
     if (warp == kProducer) {
         const int box = a.box, boxes = kTile / box;
-        const int each = boxes > 32 ? boxes / 32 : 1;       /* boxes of a lane */
+        constexpr int kEach = kTile / 32; /* boxes of one slot are so many a lane */
+        const int each = boxes > 32 ? boxes / 32 : 1;
         const int ahead = boxes > 32 ? 1 : 32 / boxes;      /* tiles of a look-up */
         const int my_tile = boxes > 32 ? 0 : lane / boxes, my_box = boxes > 32 ? lane * each : lane - my_tile * boxes;
         uint32_t issued = 0;
-        while (cursor.next(a, kTile, Plan::kBlockRows, x)) {
+        while (cursor.next(a, kTile, kRows, x)) {
             const int n = x.tile1 - x.tile0;
             /* pages of the tiles from `looked` on, and of the ones after them */
-            int now[4], then[4], looked = -1;
-            const auto look = [&](int i, int (&page)[4]) {
+            int now[kEach], then[kEach], looked = -2 * ahead;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    page[k] = -1;
-                    const int slot = (x.tile0 + i + my_tile) * kTile + (my_box + k) * box;
-                    if (k < each && i + my_tile < n && slot < x.span.length) {
-                        const int j = int((uint64_t(unsigned(slot)) * a.page_magic) >> a.page_shift);
-                        page[k] = checked_page(p, x.sequence, j);
+            for (int k = 0; k < kEach; k++)
+                then[k] = -1;
+#pragma unroll 1
+            for (int step = 0; step < 2 * n; step++) {
+                const bool values = step > 0 && (step % 2 == 0 || step == 2 * n - 1);
+                const int i = values ? (step == 2 * n - 1 ? n - 1 : step / 2 - 1) : (step + 1) / 2;
+                while (!values && i >= looked + 2 * ahead) { /* keys of a tile that was not looked up */
+                    looked += ahead;
+#pragma unroll
+                    for (int k = 0; k < kEach; k++) {
+                        now[k] = then[k];
+                        then[k] = -1;
+                        const int tile = looked + ahead + my_tile;
+                        const int slot = (x.tile0 + tile) * kTile + (my_box + k) * box;
+                        if (k < each && tile < n && slot < x.span.length) {
+                            const int j = int((uint64_t(unsigned(slot)) * a.page_magic) >> a.page_shift);
+                            then[k] = checked_page(p, x.sequence, j);
+                        }
                     }
                 }
-            };
-            /* copies tile i's keys or values */
-            const auto copy = [&](int i, bool values, const int (&page)[4], int offset) {
-                const uint32_t place = base + (values ? place_of_values(i, n) : place_of_keys(i));
+                const uint32_t place = base + step;
                 const int stage = stage_of(place);
                 if (alive && place >= kStages)
                     alive = __all_sync(0xffffffffu, await(&sh.empty[stage], parity_of(place) ^ 1));
                 if (!alive)
-                    return;
-                const bool mine = my_tile == offset;
+                    continue;
+                const bool later = i - looked >= ahead;
+                const bool mine = my_tile == i - looked - (later ? ahead : 0);
                 const int t0 = (x.tile0 + i) * kTile;
-                int many = 0;
+                int page[kEach], many = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    many += mine && page[k] >= 0;
+                for (int k = 0; k < kEach; k++) {
+                    page[k] = mine ? later ? then[k] : now[k] : -1;
+                    many += page[k] >= 0;
+                }
                 const int all = __reduce_add_sync(0xffffffffu, many);
-                if (values) {
-                    uint32_t words[kTile / 32];
+                if (!values) {
+                    const bool full = all == boxes && t0 + kTile <= x.span.length;
+#pragma unroll 1
+                    for (int w = 0; w < kTile / 32; w++) {
+                        uint32_t bits = full ? ~0u : 0u;
+                        if (!full) {
 #pragma unroll
-                    for (int w = 0; w < kTile / 32; w++)
-                        words[w] = ~0u;
-                    if (all < boxes || t0 + kTile > x.span.length) {
-#pragma unroll
-                        for (int w = 0; w < kTile / 32; w++) {
-                            uint32_t bits = 0;
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
+                            for (int k = 0; k < kEach; k++) {
                                 /* the box's slots that there are, as they lie in this word */
                                 const int from = (my_box + k) * box - 32 * w;
                                 const int to = min(from + box, x.span.length - t0 - 32 * w);
-                                if (mine && page[k] >= 0 && from < 32 && to > 0 && to > from)
+                                if (page[k] >= 0 && from < 32 && to > 0 && to > from)
                                     bits |= (to >= 32 ? ~0u : (1u << to) - 1u) & (from <= 0 ? ~0u : ~0u << from);
                             }
-                            words[w] = __reduce_or_sync(0xffffffffu, bits);
+                            bits = __reduce_or_sync(0xffffffffu, bits);
                         }
+                        if (lane == 0)
+                            sh.valid[(base / 2 + i) % kNoted][w] = bits;
                     }
-                    if (lane == 0)
-#pragma unroll
-                        for (int w = 0; w < kTile / 32; w++)
-                            sh.valid[stage][w] = words[w];
                 }
                 if (lane == 0)
                     mbar_expect_tx(&sh.full[stage], uint32_t(all) * box * 128 * kColumns);
                 __syncwarp();
                 const uint32_t to = ring_at + stage * Plan::kStage, bar = smem_u32(&sh.full[stage]);
-                const CUtensorMap *map = values ? &a.value_map : &a.key_map;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (mine && page[k] >= 0) {
-                        const int slot = t0 + (my_box + k) * box;
-                        const int j = int((uint64_t(unsigned(slot)) * a.page_magic) >> a.page_shift);
-                        const int y = slot - j * p.page_size;
+                for (int k = 0; k < kEach; k++)
+                    if (page[k] >= 0) {
+                        const int in_tile = (my_box + k) * box, slot = t0 + in_tile;
+                        const int y = slot - int((uint64_t(unsigned(slot)) * a.page_magic) >> a.page_shift) * p.page_size;
+                        if (values && wide) {
+#pragma unroll 1
+                            for (int t = 0; t < box; t += 16)
+                                copy_box(to + (in_tile + t) * kColumns * 128, &a.wide_value_map, 0, y + t, 0, x.head, page[k], bar);
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < kColumns; c++)
-                            copy_box(to + c * kTile * 128 + (my_box + k) * box * 128, map, a.whole_columns ? 0 : c * 64, y,
-                                     a.whole_columns ? c : 0, x.head, page[k], bar);
+                            for (int c = 0; c < kColumns; c++)
+                                copy_box(to + c * kTile * 128 + in_tile * 128, values ? &a.value_map : &a.key_map,
+                                         a.whole_columns ? 0 : c * 64, y, a.whole_columns ? c : 0, x.head, page[k], bar);
+                        }
                     }
-                issued = max(issued, place + 1);
-            };
-            look(0, now);
-            looked = 0;
-            look(ahead, then);
-            copy(0, false, now, 0);
-            for (int i = 0; i < n; i++) {
-                /* keys of tile i + 1, then values of tile i */
-                if (i + 1 < n) {
-                    if (i + 1 - looked < ahead)
-                        copy(i + 1, false, now, i + 1 - looked);
-                    else
-                        copy(i + 1, false, then, i + 1 - looked - ahead);
-                }
-                copy(i, true, now, i - looked);
-                if (i + 1 - looked == ahead) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        now[k] = then[k];
-                    looked += ahead;
-                    look(looked + ahead, then);
-                }
+                issued = place + 1;
             }
             base += 2 * n;
         }
@@ -369,113 +470,59 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     } else if (warp == kIssuer) {
         if (lane == 0) {
             constexpr uint32_t kShapeS = shape_of<T>(kTile, false), kShapeO = shape_of<T>(DP, true);
-            uint32_t items = 0, turns[kStreams] = {0, 0};
-            /* S of a stream = Q K^T */
-            const auto logits = [&](int w, int query_tile, uint32_t place) {
-                const uint32_t k = ring_at + stage_of(place) * Plan::kStage;
-#pragma unroll
-                for (int t = 0; t < kTerms; t++) {
-                    const uint32_t q = queries_at + (t * Plan::kQueryTiles + query_tile) * Plan::kQueryBytes;
-#pragma unroll
-                    for (int s = 0; s < DP / 16; s++)
-                        mma_ss(tmem + w * Plan::kLogits, matrix_at(q + s / 4 * (128 * 128) + s % 4 * 32, 16),
-                               matrix_at(k + s / 4 * (kTile * 128) + s % 4 * 32, 16), kShapeS, t > 0 || s > 0);
-                }
-            };
-            /* O of a stream += P V */
-            const auto outputs = [&](int w, uint32_t place, bool first) {
-                const uint32_t v = ring_at + stage_of(place) * Plan::kStage;
+            uint32_t items = 0, tiles = 0; /* of the items before */
+            /* logits of tile i of the item, from its keys */
+            const auto logits = [&](int i) {
+                const uint32_t place = base + place_of_keys(i), buffer = (tiles + i) % kBuffers;
+                if (alive)
+                    alive = await(&sh.full[stage_of(place)], parity_of(place));
+                if (!alive)
+                    return;
+                tc_after();
+                const uint64_t k = matrix_at(ring_at + stage_of(place) * Plan::kStage, 16, 1024);
+                const uint64_t q = matrix_at(queries_at, 16, 1024);
 #pragma unroll
                 for (int t = 0; t < kTerms; t++)
 #pragma unroll
-                    for (int s = 0; s < kTile / 16; s++)
-                        mma_ts(tmem + Plan::kOutputs + w * DP, tmem + w * Plan::kLogits + t * (kTile / 2) + s * 8,
-                               matrix_at(v + s * 2048, kTile * 128), kShapeO, !first || t > 0 || s > 0);
+                    for (int s = 0; s < DP / 16; s++)
+                        mma_ss(tmem + buffer * Plan::kLogits,
+                               q + ((t * Plan::kQueryBytes + s / 4 * (kRows * 128) + s % 4 * 32) >> 4),
+                               k + ((s / 4 * (kTile * 128) + s % 4 * 32) >> 4), kShapeS, t > 0 || s > 0);
+                tc_commit(&sh.logits[buffer]);
+                tc_commit(&sh.empty[stage_of(place)]);
             };
-            const auto arrived = [&](uint32_t place) {
-                if (alive)
-                    alive = await(&sh.full[stage_of(place)], parity_of(place));
-                if (alive)
-                    tc_after();
-            };
-            while (cursor.next(a, kTile, Plan::kBlockRows, x)) {
+            while (cursor.next(a, kTile, kRows, x)) {
                 const int n = x.tile1 - x.tile0;
-                const bool both = x.rows > 128; /* streams take halves of the rows, else every other tile */
                 if (alive)
                     alive = await(&sh.queries, items & 1);
                 items++;
-                if (both) {
-                    arrived(base);
-                    if (alive)
-                        for (int w = 0; w < 2; w++) {
-                            logits(w, w % Plan::kQueryTiles, base);
-                            tc_commit(&sh.logits[w]);
-                        }
-                    if (alive)
-                        tc_commit(&sh.empty[stage_of(base)]);
-                    for (int i = 0; i < n; i++) {
-                        const uint32_t values = base + place_of_values(i, n), keys = base + place_of_keys(i + 1);
-                        if (i + 1 < n)
-                            arrived(keys);
-                        arrived(values);
-#pragma unroll
-                        for (int w = 0; w < 2; w++) {
-                            if (alive)
-                                alive = await(&sh.weights[w], turns[w] & 1);
-                            turns[w]++;
-                            if (!alive)
-                                continue;
-                            tc_after();
-                            outputs(w, values, i == 0);
-                            if (i + 1 < n) {
-                                logits(w, w % Plan::kQueryTiles, keys);
-                                tc_commit(&sh.logits[w]);
-                            } else {
-                                tc_commit(&sh.outputs[w]);
-                            }
-                        }
-                        if (alive) {
-                            tc_commit(&sh.empty[stage_of(values)]);
-                            if (i + 1 < n)
-                                tc_commit(&sh.empty[stage_of(keys)]);
-                        }
-                    }
-                } else {
-                    for (int i = 0; i < 2 && i < n; i++) {
-                        const uint32_t keys = base + place_of_keys(i);
-                        arrived(keys);
-                        if (!alive)
-                            continue;
-                        logits(i, 0, keys);
-                        tc_commit(&sh.logits[i]);
-                        tc_commit(&sh.empty[stage_of(keys)]);
-                    }
-                    for (int i = 0; i < n; i++) {
-                        const int w = i & 1;
-                        const uint32_t values = base + place_of_values(i, n);
-                        arrived(values);
+                /* logits run ahead of the weights by kBuffers tiles */
+#pragma unroll 1
+                for (int i = -kBuffers; i < n; i++) {
+                    if (i >= 0) {
+                        const uint32_t place = base + place_of_values(i, n), buffer = (tiles + i) % kBuffers;
                         if (alive)
-                            alive = await(&sh.weights[w], turns[w] & 1);
-                        turns[w]++;
+                            alive = await(&sh.full[stage_of(place)], parity_of(place)) &&
+                                    await(&sh.weights[buffer], (tiles + i) / kBuffers & 1);
                         if (alive) {
                             tc_after();
-                            outputs(w, values, i < 2);
-                            tc_commit(&sh.empty[stage_of(values)]);
-                            if (i + 2 >= n)
-                                tc_commit(&sh.outputs[w]);
-                        }
-                        if (i + 2 < n) {
-                            const uint32_t keys = base + place_of_keys(i + 2);
-                            arrived(keys);
-                            if (alive) {
-                                logits(w, 0, keys);
-                                tc_commit(&sh.logits[w]);
-                                tc_commit(&sh.empty[stage_of(keys)]);
-                            }
+                            const uint64_t v = matrix_at(ring_at + stage_of(place) * Plan::kStage, values_lead, 1024);
+                            const uint32_t weights = tmem + buffer * Plan::kLogits;
+#pragma unroll
+                            for (int t = 0; t < kTerms; t++)
+#pragma unroll
+                                for (int s = 0; s < kTile / 16; s++)
+                                    mma_ts(tmem + Plan::kOutputs, weights + t * (kTile / 2) + s * 8, v + s * (values_step >> 4),
+                                           kShapeO, i > 0 || t > 0 || s > 0);
+                            tc_commit(&sh.outputs);
+                            tc_commit(&sh.empty[stage_of(place)]);
                         }
                     }
+                    if (i + kBuffers < n)
+                        logits(i + kBuffers);
                 }
                 base += 2 * n;
+                tiles += n;
             }
             if (!alive) { /* products in flight end before tensor memory is given back */
                 tc_commit(&sh.drained);
@@ -486,90 +533,100 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
         }
         __syncwarp();
     } else {
-        const int w = warp >> 2, row = tid & 127; /* stream, row of the tile */
-        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t logits_at = tmem + lanes + w * Plan::kLogits, outputs_at = tmem + lanes + Plan::kOutputs + w * DP;
-        const auto everyone = [] { named_barrier(1, kStreams * 128); };
-        uint32_t turns = 0, ends = 0;
+        const uint32_t lanes = uint32_t(warp * 32) << 16, outputs_at = tmem + lanes + Plan::kOutputs;
+        const auto everyone = [] { named_barrier(1, kRows); };
+        uint32_t tiles = 0; /* of the items before */
         int4 join = make_int4(0, 0, 0, 0);
-        while (cursor.next(a, kTile, Plan::kBlockRows, x)) {
+        tree_blind_rows<R>(a, tid, kRows);
+        while (cursor.next(a, kTile, kRows, x)) {
             const int n = x.tile1 - x.tile0;
-            const bool both = x.rows > 128;
+            const bool counts = tid < x.rows;
+            const bool idle = warp * 32 >= x.rows; /* a warp without rows */
+            const uint32_t *seen = a.mask;
+            if (counts)
+                seen += (int64_t(x.span.row0) + tree_node(a, x.first_row + tid)) * a.mask_words;
+            const uint32_t seen0 = counts ? seen[0] : 0u; /* most trees have no more words */
 
-            /* the queries: a row's DP / 8 pieces of 8 dims by neighbouring lanes */
-            constexpr int kAcross = DP / 8;
-            const int query_rows = both ? kStreams * 128 : 128;
-            for (int i = tid; i < query_rows * kAcross; i += kStreams * 128) {
-                const int r = i / kAcross, c = i % kAcross;
-                const bool there = r < x.rows;
-                int64_t q_row = 0;
-                int h = 0;
-                if (there)
-                    tree_row(a, x.span.row0, x.head, x.first_row + r, q_row, h);
-                const R *q = static_cast<const R *>(a.q) + q_row * a.q_stride + int64_t(h) * D + c * 8;
-                char *to = smem + (r >> 7) * Plan::kQueryBytes + (c >> 3) * (128 * 128) + (r & 127) * 128 +
-                           (((c & 7) ^ (r & 7)) << 4);
-                if constexpr (kTerms == 1) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (there && c * 8 < D) {
-                        if (a.aligned) {
-                            v = *reinterpret_cast<const uint4 *>(q);
-                        } else {
-                            R *e = reinterpret_cast<R *>(&v);
+            /* the queries: a row's DP / 8 pieces of 8 dims by neighbouring lanes,
+             * kBatch of them in flight a thread */
+            constexpr int kAcross = DP / 8, kStep = kRows / kAcross, kBatch = 8;
+            constexpr int kLoads = sizeof(R) / 2; /* of 16 bytes a piece */
+            static_assert(kRows % (kBatch * kStep) == 0, "whole batches");
+            const int c = tid % kAcross;
+            /* a scale below 0 turns the queries round */
+            const uint32_t flip = a.scale < 0.0f ? (sizeof(R) == 4 ? 0x80000000u : 0x80008000u) : 0u;
+#pragma unroll 1
+            for (int r0 = tid / kAcross; r0 < (x.rows + kAcross - 1) / kAcross * kAcross; r0 += kBatch * kStep) {
+                uint4 pieces[kBatch][kLoads];
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                e[k] = q[k];
-                        }
+                for (int k = 0; k < kBatch; k++) {
+                    const int r = r0 + k * kStep;
+#pragma unroll
+                    for (int j = 0; j < kLoads; j++)
+                        pieces[k][j] = make_uint4(0, 0, 0, 0);
+                    if (r < x.rows && c * 8 < D) {
+                        int64_t q_row;
+                        int h;
+                        tree_row(a, x.span.row0, x.head, x.first_row + r, q_row, h);
+                        const R *q = static_cast<const R *>(a.q) + q_row * a.q_stride + h * D + c * 8;
+#pragma unroll
+                        for (int j = 0; j < kLoads; j++)
+                            pieces[k][j] = a.aligned ? *reinterpret_cast<const uint4 *>(q + j * (8 / kLoads))
+                                                     : load_elements(q + j * (8 / kLoads));
                     }
-                    *reinterpret_cast<uint4 *>(to) = v;
-                } else {
-                    float v[8];
+                }
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        v[k] = 0.0f;
-                    if (there && c * 8 < D) {
-                        if (a.aligned) {
-                            *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(q);
-                            *reinterpret_cast<float4 *>(v + 4) = *reinterpret_cast<const float4 *>(q + 4);
-                        } else {
+                for (int k = 0; k < kBatch; k++) {
+                    const int r = r0 + k * kStep;
+                    char *to = smem + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                v[k] = to_float(q[k]);
-                        }
+                    for (int j = 0; j < kLoads; j++) {
+                        pieces[k][j].x ^= flip;
+                        pieces[k][j].y ^= flip;
+                        pieces[k][j].z ^= flip;
+                        pieces[k][j].w ^= flip;
                     }
-                    float unit = a.scale * kTreeLog2e;
-                    if constexpr (kHalf) { /* greatest |q| to [2^10, 2^11) */
-                        float top = 0.0f;
+                    if constexpr (kTerms == 1) {
+                        *reinterpret_cast<uint4 *>(to) = pieces[k][0];
+                    } else {
+                        float v[8] = {
+                            __uint_as_float(pieces[k][0].x), __uint_as_float(pieces[k][0].y), __uint_as_float(pieces[k][0].z),
+                            __uint_as_float(pieces[k][0].w), __uint_as_float(pieces[k][kLoads - 1].x),
+                            __uint_as_float(pieces[k][kLoads - 1].y), __uint_as_float(pieces[k][kLoads - 1].z),
+                            __uint_as_float(pieces[k][kLoads - 1].w)};
+                        float unit = fabsf(a.scale) * kTreeLog2e;
+                        if constexpr (kHalf) { /* greatest |q| to [2^10, 2^11) */
+                            float top = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            top = fmaxf(top, fabsf(v[k]));
+                            for (int j = 0; j < 8; j++)
+                                top = fmaxf(top, fabsf(v[j]));
 #pragma unroll
-                        for (int e = kAcross / 2; e > 0; e >>= 1)
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
-                        const int e = int(__float_as_uint(top) >> 23);
-                        if (e > 0 && e < 255) {
-                            const int field = min(264 - e, 253);
-                            const float gain = __uint_as_float(uint32_t(field) << 23);
+                            for (int e = kAcross / 2; e > 0; e >>= 1)
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+                            const int e = int(__float_as_uint(top) >> 23);
+                            if (e > 0 && e < 255) {
+                                const int field = min(264 - e, 253);
+                                const float gain = __uint_as_float(uint32_t(field) << 23);
 #pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                v[k] *= gain;
-                            unit *= __uint_as_float(uint32_t(254 - field) << 23);
+                                for (int j = 0; j < 8; j++)
+                                    v[j] *= gain;
+                                unit *= __uint_as_float(uint32_t(254 - field) << 23);
+                            }
                         }
-                    }
-                    if (c == 0)
-                        sh.unit[r] = unit;
+                        if (c == 0)
+                            sh.unit[r] = unit;
 #pragma unroll
-                    for (int t = 0; t < kTerms; t++) {
-                        uint4 term;
-                        uint32_t *e = reinterpret_cast<uint32_t *>(&term);
+                        for (int t = 0; t < kTerms; t++) {
+                            uint32_t e[4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            e[k] = Pair<T>::pack(v[2 * k], v[2 * k + 1]);
-                            const float2 taken = Pair<T>::unpack(e[k]);
-                            v[2 * k] -= taken.x;
-                            v[2 * k + 1] -= taken.y;
+                            for (int j = 0; j < 4; j++) {
+                                e[j] = Pair<T>::pack(v[2 * j], v[2 * j + 1]);
+                                const float2 taken = Pair<T>::unpack(e[j]);
+                                v[2 * j] -= taken.x;
+                                v[2 * j + 1] -= taken.y;
+                            }
+                            *reinterpret_cast<uint4 *>(to + t * Plan::kQueryBytes) = make_uint4(e[0], e[1], e[2], e[3]);
                         }
-                        *reinterpret_cast<uint4 *>(to + t * Plan::kQueryBytes) = term;
                     }
                 }
             }
@@ -578,82 +635,38 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
             if constexpr (kTerms > 1)
                 everyone(); /* the units */
 
-            const int my_row = both ? w * 128 + row : row; /* of the item */
-            const bool counts = my_row < x.rows;
-            const bool idle = __all_sync(0xffffffffu, !counts); /* a warp without rows */
-            const float unit = kTerms > 1 ? sh.unit[row] : a.scale * kTreeLog2e;
-            const uint32_t *seen = a.mask;
-            if (counts)
-                seen += (int64_t(x.span.row0) + (x.first_row + my_row) / p.group) * a.mask_words;
+            const float unit = kTerms > 1 ? sh.unit[tid] : fabsf(a.scale) * kTreeLog2e;
             /* weights are 2^(logit - from), `from` kLift below a maximum */
             float from = -INFINITY, l = 0.0f;
-            const float unseen = unit < 0.0f ? INFINITY : -INFINITY;
-            int mine = 0; /* tiles of this stream */
-            for (int i = both ? 0 : w; i < n; i += both ? 1 : 2) {
-                const uint32_t values = base + place_of_values(i, n);
-                const int stage = stage_of(values), t0 = (x.tile0 + i) * kTile;
+#pragma unroll 1
+            for (int i = 0; i < n; i++, tiles++) {
+                const uint32_t logits_at = tmem + lanes + tiles % kBuffers * Plan::kLogits;
+                const int t0 = (x.tile0 + i) * kTile;
                 if (alive)
-                    alive = await(&sh.logits[w], turns & 1) && await(&sh.full[stage], parity_of(values));
+                    alive = await(&sh.logits[tiles % kBuffers], tiles / kBuffers & 1);
                 alive = __all_sync(0xffffffffu, alive);
-                turns++;
-                const bool first = mine++ == 0;
                 if (!alive)
                     continue;
                 tc_after();
-                uint32_t words[kTile / 32];
-                bool plain = t0 + kTile <= x.span.prefix;
-#pragma unroll
-                for (int k = 0; k < kTile / 32; k++) {
-                    words[k] = sh.valid[stage][k];
-                    plain &= words[k] == ~0u;
-                }
-                if (!plain && (!both || w == 0)) {
+                const volatile uint32_t *noted = sh.valid[(base / 2 + i) % kNoted];
+                uint32_t words[2] = {noted[0], noted[1]};
+                const bool plain = t0 + kTile <= x.span.prefix && (words[0] & words[1]) == ~0u;
+                if (!plain) {
                     /* values that must not meet weights of 0 */
-                    const int slot = row;
-                    if (slot < kTile) {
-                        const bool there = (sh.valid[stage][slot >> 5] >> (slot & 31)) & 1;
-                        if (!there || t0 + slot >= x.span.prefix) {
-                            bool odd = false;
-#pragma unroll
-                            for (int c = 0; c < DP / 8; c++) {
-                                const uint32_t at = ring_at + stage * Plan::kStage + (c >> 3) * (kTile * 128) + slot * 128 +
-                                                    (((c & 7) ^ (slot & 7)) << 4);
-                                uint4 v = make_uint4(0, 0, 0, 0);
-                                uint32_t *e = reinterpret_cast<uint32_t *>(&v);
-                                bool change = !there;
-                                if (there) {
-                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                                 : "r"(at));
-#pragma unroll
-                                    for (int k = 0; k < 4; k++) {
-                                        constexpr uint32_t kInf = Pair<T>::kInfinite;
-                                        if ((e[k] & kInf) == kInf) {
-                                            e[k] &= 0xffff0000u;
-                                            change = odd = true;
-                                        }
-                                        if ((e[k] & (kInf << 16)) == kInf << 16) {
-                                            e[k] &= 0x0000ffffu;
-                                            change = odd = true;
-                                        }
-                                    }
-                                }
-                                if (change)
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
-                                                 "r"(v.w)
-                                                 : "memory");
-                            }
-                            if (odd)
-                                sh.odd = 1;
-                        }
-                    }
+                    const uint32_t place = base + place_of_values(i, n);
+                    alive = __all_sync(0xffffffffu, await(&sh.full[stage_of(place)], parity_of(place)));
+                    static_assert(kRows == 2 * kTile, "two threads a slot");
+                    const int slot = tid >> 1;
+                    const bool there = (noted[slot >> 5] >> (slot & 31)) & 1;
+                    if (alive && (!there || t0 + slot >= x.span.prefix))
+                        clean_values<T, DP>(ring_at + stage_of(place) * Plan::kStage + (slot >> 4) * values_step + (slot & 15) * 128,
+                                            slot, tid & 1, values_lead, there, &sh.odd);
                     fence_async();
                 }
-                if (!idle) {
+                if (!idle && alive) {
                     float s[kTile];
-#pragma unroll
-                    for (int k = 0; k < kTile; k += 32)
-                        tmem_load32(logits_at + k, s + k);
+                    tmem_load32(logits_at, s);
+                    tmem_load32(logits_at + 32, s + 32);
                     tc_wait_ld();
                     if (!plain)
 #pragma unroll
@@ -661,37 +674,29 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                             uint32_t sees = words[k / 32];
                             const int node = t0 + k - x.span.prefix;
                             if (node > -32)
-                                sees &= counts ? tree_sees(seen, node, x.span.n) : 0u;
+                                sees &= x.span.n <= 32 ? tree_sees(&seen0, node, x.span.n) : tree_sees(seen, node, x.span.n);
 #pragma unroll
                             for (int j = 0; j < 32; j++)
-                                s[k + j] = (sees >> j) & 1 ? s[k + j] : unseen;
+                                s[k + j] = (sees >> j) & 1 ? s[k + j] : -INFINITY;
                         }
                     float top = s[0], other = s[1];
-                    if (unit >= 0.0f) {
 #pragma unroll
-                        for (int k = 2; k < kTile; k += 2) {
-                            top = fmaxf(top, s[k]);
-                            other = fmaxf(other, s[k + 1]);
-                        }
-                        top = fmaxf(top, other);
-                    } else {
-#pragma unroll
-                        for (int k = 2; k < kTile; k += 2) {
-                            top = fminf(top, s[k]);
-                            other = fminf(other, s[k + 1]);
-                        }
-                        top = fminf(top, other);
+                    for (int k = 2; k < kTile; k += 2) {
+                        top = fmaxf(top, s[k]);
+                        other = fmaxf(other, s[k + 1]);
                     }
                     /* rounded up, so that beside logits of 2^24 and more no weight passes 2^kLift either */
-                    const float to = __fsub_ru(__fmul_ru(top, unit), kLift);
+                    const float to = __fsub_ru(__fmul_ru(fmaxf(top, other), unit), kLift);
                     const float next = to - from > kSlack || from == -INFINITY ? fmaxf(from, to) : from;
                     if (__any_sync(0xffffffffu, next != from)) {
                         const float keep = from == next ? 1.0f : power2(from - next);
                         l *= keep;
                         from = next;
-                        if (!first) /* the products before this tile's logits are complete */
+                        if (i > 0) { /* once the products before are complete */
+                            alive = __all_sync(0xffffffffu, await(&sh.outputs, (tiles - 1) & 1));
+                            tc_after();
 #pragma unroll 1
-                            for (int c = 0; c < DP; c += 32) {
+                            for (int c = 0; c < DP && alive; c += 32) {
                                 float o[32];
                                 tmem_load32(outputs_at + c, o);
                                 tc_wait_ld();
@@ -700,6 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                                     o[j] *= keep;
                                 tmem_store32(outputs_at + c, o);
                             }
+                        }
                     }
                     const float less = from == -INFINITY ? 0.0f : -from;
                     float sum = 0.0f, sum1 = 0.0f;
@@ -709,18 +715,13 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             float w0 = power2(fmaf(s[k + 2 * j], unit, less)), w1 = power2(fmaf(s[k + 2 * j + 1], unit, less));
-                            if constexpr (kTerms > 1) {
-                                sum += w0;
-                                sum1 += w1;
-                            }
+                            sum += w0;
+                            sum1 += w1;
 #pragma unroll
                             for (int t = 0; t < kTerms; t++) {
                                 e[t][j] = Pair<T>::pack(w0, w1);
-                                const float2 taken = Pair<T>::unpack(e[t][j]);
-                                if constexpr (kTerms == 1) {
-                                    sum += taken.x;
-                                    sum1 += taken.y;
-                                } else {
+                                if (t + 1 < kTerms) {
+                                    const float2 taken = Pair<T>::unpack(e[t][j]);
                                     w0 -= taken.x;
                                     w1 -= taken.y;
                                 }
@@ -734,142 +735,98 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
                     tc_wait_st();
                 }
                 tc_before();
-                mbar_arrive(&sh.weights[w]);
+                mbar_arrive(&sh.weights[tiles % kBuffers]);
             }
             base += 2 * n;
 
             /* the end of the item, or of this block's part of it */
-            if (mine > 0) {
-                if (alive)
-                    alive = await(&sh.outputs[w], ends & 1);
-                ends++;
-            }
+            if (alive)
+                alive = await(&sh.outputs, (tiles - 1) & 1);
             alive = __all_sync(0xffffffffu, alive);
             tc_after();
-            sh.maxima[w][row] = from;
-            sh.sums[w][row] = l;
-            everyone(); /* and all products are done: the queries' place is free */
+            everyone(); /* all products are done: the queries' place is free */
             const bool odd = sh.odd != 0, whole = x.whole();
-            float factor = 1.0f, sum = l, top = from;
-            const bool paired = !both && n > 1;
-            if (paired) {
-                const float m1 = sh.maxima[1 - w][row], l1 = sh.sums[1 - w][row];
-                top = fmaxf(from, m1);
-                const float least = top == -INFINITY ? 0.0f : top;
-                const float f = exp2f(from - least), f1 = exp2f(m1 - least);
-                /* in the same order in both streams */
-                sum = w == 0 ? fmaf(l, f, l1 * f1) : fmaf(l1, f1, l * f);
-                factor = f;
-            }
-            if (whole)
-                factor *= sum == 0.0f ? 0.0f : 1.0f / sum;
-            if (paired) {
-                /* each stream hands the other the half of the dims that it does not finish */
-                if (!idle && alive) {
-#pragma unroll 1
-                    for (int c = 0; c < DP / 2; c += 32) {
-                        const int d0 = (w == 0 ? DP / 2 : 0) + c;
-                        float o[32];
-                        tmem_load32(outputs_at + d0, o);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const int piece = (d0 + j) / 4;
-                            float4 v = make_float4(o[j] * factor, o[j + 1] * factor, o[j + 2] * factor, o[j + 3] * factor);
-                            if (factor == 0.0f)
-                                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            *reinterpret_cast<float4 *>(smem + row * DP * 4 + ((piece ^ (row & 7)) << 4)) = v;
-                        }
-                    }
+            const float factor = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const TreePart part = tree_part(a, blockIdx.x, x.first <= start ? 0 : 1, x.rows);
+            if (counts && alive) {
+                if (!whole) {
+                    part.maxima[tid] = from;
+                    part.sums[tid] = l;
+                } else if (a.lse) {
+                    int64_t out_row;
+                    int h;
+                    tree_row(a, x.span.row0, x.head, x.first_row + tid, out_row, h);
+                    a.lse[out_row * p.heads + h] = l == 0.0f ? -INFINITY : (from + log2f(l)) * kTreeLn2;
                 }
-                everyone();
             }
-            if (!idle && alive && (both || paired || w == 0)) {
-                const TreePart part = tree_part(a, blockIdx.x, x.first <= start ? 0 : 1, x.rows);
-                int64_t out_row = 0;
-                int h = 0;
-                if (counts)
-                    tree_row(a, x.span.row0, x.head, x.first_row + my_row, out_row, h);
-                if (counts && (both || w == 0)) {
-                    if (whole) {
-                        if (a.lse)
-                            a.lse[out_row * p.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kTreeLn2;
-                    } else {
-                        part.maxima[my_row] = top;
-                        part.sums[my_row] = sum;
-                    }
+            /* 32 dims at a time leave through a warp's 4 KB of the queries'
+             * place, 128 bytes of a row by 8 lanes */
+            const int piece = lane & 7;
+            float4 *rows_at = reinterpret_cast<float4 *>(smem + warp * 32 * 128);
+            char *to[8]; /* row 4 i + lane / 8 of the warp, from this lane's dims on */
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = warp * 32 + i * 4 + (lane >> 3);
+                if (whole) {
+                    int64_t out_row;
+                    int h;
+                    tree_row(a, x.span.row0, x.head, x.first_row + r, out_row, h);
+                    to[i] = reinterpret_cast<char *>(static_cast<R *>(a.out) + out_row * a.out_stride + h * D + piece * 4);
+                } else {
+                    to[i] = reinterpret_cast<char *>(part.out + r * D + piece * 4);
                 }
-                const int d_from = paired && w == 1 ? DP / 2 : 0, d_to = paired && w == 0 ? DP / 2 : DP;
+            }
+            const int mine_from = warp * 32 + (lane >> 3);
 #pragma unroll 1
-                for (int d0 = d_from; d0 < d_to; d0 += 32) {
-                    float o[32];
-                    tmem_load32(outputs_at + d0, o);
-                    tc_wait_ld();
+            for (int d0 = 0; d0 < D && !idle && alive; d0 += 32) {
+                float o[32];
+                tmem_load32(outputs_at + d0, o);
+                tc_wait_ld();
+                __syncwarp();
+                float4 *mine = rows_at + lane * 8;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (paired)
-                            v = *reinterpret_cast<const float4 *>(smem + row * DP * 4 + ((((d0 + j) / 4) ^ (row & 7)) << 4));
-                        if (factor != 0.0f)
-                            v = make_float4(fmaf(o[j], factor, v.x), fmaf(o[j + 1], factor, v.y), fmaf(o[j + 2], factor, v.z),
-                                            fmaf(o[j + 3], factor, v.w));
-                        o[j] = v.x;
-                        o[j + 1] = v.y;
-                        o[j + 2] = v.z;
-                        o[j + 3] = v.w;
-                    }
-                    if (odd && counts) {
-                        /* infinities and NaN among the drafted tokens that the row sees */
-                        for (int t = max(x.span.prefix, x.tile0 * kTile); t < min(x.span.length, x.tile1 * kTile); t++) {
-                            const int node = t - x.span.prefix, page = lookup(p, x.sequence, t / p.page_size);
-                            if (page < 0 || !((seen[node >> 5] >> (node & 31)) & 1))
-                                continue;
-                            const T *v = static_cast<const T *>(p.values) + int64_t(page) * p.page_stride +
-                                         int64_t(x.head) * p.head_stride + int64_t(t % p.page_size) * p.slot_stride;
+                for (int j = 0; j < 8; j++)
+                    mine[j ^ (lane & 7)] = make_float4(o[4 * j] * factor, o[4 * j + 1] * factor, o[4 * j + 2] * factor,
+                                                       o[4 * j + 3] * factor);
+                if (odd && counts)
+                    add_odd_values<T>(a, x, seen, max(x.span.prefix, x.tile0 * kTile), min(x.span.length, x.tile1 * kTile), d0, mine,
+                                      lane);
+                __syncwarp();
+                float4 v[8];
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (d0 + j < D) {
-                                    const float e = to_float(v[d0 + j]);
-                                    o[j] += fabsf(e) <= 3.402823466e38f ? 0.0f : e;
-                                }
-                        }
-                    }
-                    if (!counts)
-                        continue;
-                    if (!whole) {
-                        float *to = part.out + int64_t(my_row) * D + d0;
+                for (int i = 0; i < 8; i++) {
+                    const int r = i * 4 + (lane >> 3);
+                    v[i] = rows_at[r * 8 + (piece ^ (r & 7))];
+                }
+                const int rows = d0 + piece * 4 < D ? x.rows : 0; /* that have these dims */
+                if (!whole || sizeof(R) == 4) {
+                    if (!whole || a.aligned) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            if (d0 + j < D)
-                                *reinterpret_cast<float4 *>(to + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int i = 0; i < 8; i++)
+                            if (mine_from + i * 4 < rows)
+                                *reinterpret_cast<float4 *>(to[i] + d0 * 4) = v[i];
                     } else {
-                        R *to = static_cast<R *>(a.out) + out_row * a.out_stride + int64_t(h) * D + d0;
-                        constexpr int kPer = 16 / sizeof(R);
 #pragma unroll
-                        for (int j = 0; j < 32; j += kPer)
-                            if (d0 + j < D) {
-                                uint4 v;
-                                R *e = reinterpret_cast<R *>(&v);
+                        for (int i = 0; i < 8; i++)
+                            store_elements(reinterpret_cast<float *>(to[i]) + d0, v[i], mine_from + i * 4 < rows);
+                    }
+                } else {
 #pragma unroll
-                                for (int k = 0; k < kPer; k++)
-                                    e[k] = output_of<R>(o[j + k]);
-                                if (a.aligned) {
-                                    *reinterpret_cast<uint4 *>(to + j) = v;
-                                } else {
-#pragma unroll
-                                    for (int k = 0; k < kPer; k++)
-                                        to[j + k] = e[k];
-                                }
-                            }
+                    for (int i = 0; i < 8; i++) {
+                        R *at = reinterpret_cast<R *>(to[i]) + d0;
+                        if (!a.aligned)
+                            store_elements(at, v[i], mine_from + i * 4 < rows);
+                        else if (mine_from + i * 4 < rows)
+                            *reinterpret_cast<uint2 *>(at) = make_uint2(pack_outputs<R>(v[i].x, v[i].y), pack_outputs<R>(v[i].z, v[i].w));
                     }
                 }
             }
             if (!whole && x.tile0 == 0)
                 join = tree_join(x, share);
-            everyone(); /* the statistics and the queries' place are free again */
+            tc_before();
+            everyone(); /* the queries' place is free again */
             if (tid == 0)
                 sh.odd = 0;
-            tc_before();
         }
         if (tid == 0)
             a.joins[blockIdx.x] = join;
@@ -878,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
     __syncthreads();
     if (warp == kIssuer) {
         tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(Plan::kMemory) : "memory");
     }
 }
 
@@ -896,22 +853,21 @@ template <typename T, typename R, int DP, int kTerms> cudaError_t launch(const P
             return e;
         set[device % kMaxDevices] = true;
     }
-    e = launch_kernel(kernel, dim3(a.sms), kThreads, Plan::kBytes, s, 1, a);
-    return e != cudaSuccess ? e : tree_join_parts(a, a.sms, Plan::kBlockRows, s);
+    const int ctas = a.sms * Plan::kPerSm;
+    e = launch_kernel(kernel, dim3(ctas), kThreads, Plan::kBytes, s, 1, a);
+    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, s);
+}
+
+template <typename T, int DP> cudaError_t launch(const PagedTree &a, cudaStream_t s) {
+    return a.type == 0 ? launch<T, float, DP, std::is_same<T, __half>::value ? 2 : 3>(a, s) : launch<T, T, DP, 1>(a, s);
 }
 
 } // namespace
 
 cudaError_t paged_tree_tc(const PagedTree &a, cudaStream_t s) {
-    const bool narrow = a.p.head_dim <= 64;
-    if (a.p.type == 1) {
-        if (a.type == 0)
-            return narrow ? launch<__half, float, 64, 2>(a, s) : launch<__half, float, 128, 2>(a, s);
-        return narrow ? launch<__half, __half, 64, 1>(a, s) : launch<__half, __half, 128, 1>(a, s);
-    }
-    if (a.type == 0)
-        return narrow ? launch<__nv_bfloat16, float, 64, 3>(a, s) : launch<__nv_bfloat16, float, 128, 3>(a, s);
-    return narrow ? launch<__nv_bfloat16, __nv_bfloat16, 64, 1>(a, s) : launch<__nv_bfloat16, __nv_bfloat16, 128, 1>(a, s);
+    if (a.p.type == 1)
+        return a.p.head_dim <= 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+    return a.p.head_dim <= 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
 }
 
 } // namespace nut
