@@ -307,27 +307,35 @@ template <typename R> __global__ void __launch_bounds__(kJoinThreads) join_kerne
     const float from = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    constexpr int kFlight = 16; /* loads of a lane */
     for (int c0 = 0; c0 < parts; c0 += 32) {
         const int c = c0 + lane, many = min(32, parts - c0);
         const float factor = c < parts ? exp2f(part(c).maxima[f] - from) : 0.0f;
         if (c < parts)
             sum = fmaf(part(c).sums[f], factor, sum);
-#pragma unroll 8
-        for (int i = 0; i < many; i++) {
-            const float w = __shfl_sync(0xffffffffu, factor, i);
-            const float *out = part(c0 + i).out + int64_t(f) * D;
+        for (int i0 = 0; i0 < many; i0 += kFlight)
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int d = k * 128 + lane * 4;
-                if (d < D && w != 0.0f) {
-                    const float4 v = *reinterpret_cast<const float4 *>(out + d);
-                    o[k].x = fmaf(v.x, w, o[k].x);
-                    o[k].y = fmaf(v.y, w, o[k].y);
-                    o[k].z = fmaf(v.z, w, o[k].z);
-                    o[k].w = fmaf(v.w, w, o[k].w);
+                if (k * 128 >= D)
+                    break;
+                float4 v[kFlight];
+#pragma unroll
+                for (int i = 0; i < kFlight; i++)
+                    v[i] = i0 + i < many && d < D
+                               ? __ldcg(reinterpret_cast<const float4 *>(part(c0 + i0 + i).out + int64_t(f) * D + d))
+                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < kFlight; i++) {
+                    const float w = __shfl_sync(0xffffffffu, factor, i0 + i);
+                    if (w != 0.0f) { /* a part in which the row saw nothing, or what underflows */
+                        o[k].x = fmaf(v[i].x, w, o[k].x);
+                        o[k].y = fmaf(v[i].y, w, o[k].y);
+                        o[k].z = fmaf(v[i].z, w, o[k].z);
+                        o[k].w = fmaf(v[i].w, w, o[k].w);
+                    }
                 }
             }
-        }
     }
     sum = warp_sum(sum);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;

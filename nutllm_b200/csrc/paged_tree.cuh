@@ -18,7 +18,14 @@ namespace nut {
 
 constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
 /* What an item costs besides its tiles, in tiles. */
-constexpr int kTreeItemCost = 2;
+#ifndef ITEM_COST
+#define ITEM_COST 4
+#endif
+#ifndef LEAST_SHARE
+#define LEAST_SHARE 4
+#endif
+constexpr int kTreeItemCost = ITEM_COST;
+constexpr int kTreeLeastShare = LEAST_SHARE;
 
 /* The drafted tokens of a sequence and what they see. */
 struct TreeSpan {
@@ -129,7 +136,7 @@ __device__ __forceinline__ TreeCursor tree_share(const PagedTree &a, int tile, i
         upto += w < warp ? sums[w] : 0;
         total += sums[w];
     }
-    share = (total + int(gridDim.x) - 1) / int(gridDim.x);
+    share = max((total + int(gridDim.x) - 1) / int(gridDim.x), kTreeLeastShare);
     const int start = min(int64_t(blockIdx.x) * share, int64_t(total));
     int at = upto - mine;
     if (start < total && start >= at && start < upto)

@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
 
             /* the queries: a row's DP / 8 pieces of 8 dims by neighbouring lanes,
              * kBatch of them in flight a thread */
-            constexpr int kAcross = DP / 8, kStep = kRows / kAcross, kBatch = 8;
+            constexpr int kAcross = DP / 8, kStep = kRows / kAcross, kBatch = kTerms == 1 ? kRows / kStep : 8;
             constexpr int kLoads = sizeof(R) / 2; /* of 16 bytes a piece */
             static_assert(kRows % (kBatch * kStep) == 0, "whole batches");
             const int c = tid % kAcross;
