@@ -31,13 +31,13 @@ struct PagesUpdate {
 };
 cudaError_t pages_update(const PagesUpdate &a, cudaStream_t s);
 
-constexpr int kBeamThreads = 256, kBeamEach = 32; /* logits a thread of a chunk */
-constexpr int kBeamChunk = kBeamThreads * kBeamEach;
+constexpr int kBeamTile = 1024; /* logits that a warp takes at a time */
 constexpr int kBeamMostOut = 64;
 
-/* A chunk's greatest logit and the sum of exp(logit - greatest). */
+/* A run's sum of exp(logit - top) and its greatest logit. */
 struct BeamPart {
-    float top, sum;
+    double sum;
+    float top;
 };
 
 struct BeamSelect {
@@ -49,9 +49,9 @@ struct BeamSelect {
     int32_t *out_rows, *out_tokens;
     uint8_t *out_finished;
     int sequences, beams, vocab, n_out, eos, type;
-    int chunks;               /* of a row */
-    BeamPart *parts;          /* [rows][chunks] */
-    unsigned long long *best; /* [rows][chunks][n_out], argmax keys, descending, 0 behind them */
+    int runs, run_tiles; /* runs of a row, tiles of a run */
+    BeamPart *parts;     /* [rows][runs] */
+    unsigned long long *best; /* [rows][runs][n_out], argmax keys, descending, 0 behind them */
 };
 cudaError_t beam_select(const BeamSelect &a, cudaStream_t s);
 

@@ -1,6 +1,7 @@
 /* C ABI of branching sequences' pages (nut_pages_*) and of beam selection
  * (nut_beam_*): argument checks, workspaces, and the calls into pages.cu and
  * beam.cu. */
+#include <algorithm>
 #include <climits>
 #include <memory>
 #include <string>
@@ -175,11 +176,16 @@ nut_status nut_beam_create(int64_t sequences, int64_t beams, int64_t vocab, int6
             refuse(NUT_LENGTH_ERROR, "beam", "n_out exceeds NUT_BEAM_MAX_OUT");
         if (sequences > kMostRows || beams > 1024 || sequences * beams > kMostRows || vocab > (1 << 28))
             refuse(NUT_LENGTH_ERROR, "beam", "dimensions exceed device limits");
-        /* a row's first chunk may begin up to 15 elements before it */
-        const int64_t chunks = (vocab + 15 + nut::kBeamChunk - 1) / nut::kBeamChunk;
-        if (beams * chunks * n_out > INT_MAX)
+        /* a row's first tile may begin up to 7 elements before it.  Runs for some 18
+         * warps on every SM: fewer leave its memory waiting, more list more */
+        const int64_t tiles = (vocab + 7 + nut::kBeamTile - 1) / nut::kBeamTile, rows = sequences * beams;
+        if (rows * tiles > INT_MAX / NUT_BEAM_MAX_OUT)
             refuse(NUT_LENGTH_ERROR, "beam", "dimensions exceed device limits");
         DeviceScope scope(device);
+        int sms = 0;
+        cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "count SMs");
+        const int64_t wanted = std::min(tiles, std::max<int64_t>(1, (18 * sms) / rows));
+        const int64_t run_tiles = (tiles + wanted - 1) / wanted, runs = (tiles + run_tiles - 1) / run_tiles;
         auto h = std::make_unique<nut_beam>();
         h->device = device;
         nut::BeamSelect &b = h->b;
@@ -187,10 +193,11 @@ nut_status nut_beam_create(int64_t sequences, int64_t beams, int64_t vocab, int6
         b.beams = int(beams);
         b.vocab = int(vocab);
         b.n_out = int(n_out);
-        b.chunks = int(chunks);
+        b.runs = int(runs);
+        b.run_tiles = int(run_tiles);
         Workspace &w = h->space;
-        const size_t blocks = size_t(sequences * beams * chunks);
-        const size_t parts = w.part(blocks, sizeof(nut::BeamPart)), best = w.part(blocks * size_t(n_out), 8);
+        const size_t all = size_t(rows * runs);
+        const size_t parts = w.part(all, sizeof(nut::BeamPart)), best = w.part(all * size_t(n_out), 8);
         w.make(device, 0);
         b.parts = reinterpret_cast<nut::BeamPart *>(w.block + parts);
         b.best = reinterpret_cast<unsigned long long *>(w.block + best);
