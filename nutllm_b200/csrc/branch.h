@@ -14,18 +14,18 @@ enum PagesError {
     kPagesNoneFree = 8
 };
 
-constexpr int kPagesCluster = 8, kPagesThreads = 512;
-constexpr int kPagesWarps = kPagesCluster * kPagesThreads / 32;
+constexpr int kPagesCluster = 8, kPagesMostWarps = kPagesCluster * 32;
 
 struct PagesUpdate {
     int32_t *table, *lengths, *refs, *free_pages, *free_count;
     const int32_t *parent, *keep, *add;
     int32_t *copy_from, *copy_to, *copy_slots;
     int sequences, max_pages, n_pages, page_size;
-    int32_t *staged;                  /* [sequences][max_pages]: the table to be */
+    int32_t *staged;                  /* [sequences][max_pages]: the table to be, */
+    int32_t *changes;                 /* from this entry of a sequence on; those before stay */
     int4 *plan;                       /* [sequences]: kept slots, new length, written tail page or -1, parent */
     int32_t *delta, *writers, *first; /* [n_pages], 0 between calls */
-    int32_t *freed;                   /* [kPagesWarps]: pages given back in each warp's run */
+    int32_t *freed;                   /* [kPagesMostWarps]: pages given back in each warp's run */
     int32_t *met;                     /* what this call met */
     int32_t *error;                   /* what the handle's calls met */
 };

@@ -92,8 +92,8 @@ nut_status nut_pages_create(const nut_pages_view *view, int device, nut_pages **
         const size_t words = w.part(2, 4), delta = w.part(pages, 4), writers = w.part(pages, 4),
                      first = w.part(pages, 4);
         const size_t zeroed = w.bytes;
-        const size_t plan = w.part(sequences, sizeof(int4)), freed = w.part(nut::kPagesWarps, 4),
-                     staged = w.part(sequences * size_t(v.max_pages), 4);
+        const size_t plan = w.part(sequences, sizeof(int4)), freed = w.part(nut::kPagesMostWarps, 4),
+                     staged = w.part(sequences * size_t(v.max_pages), 4), changes = w.part(sequences, 4);
         w.make(device, zeroed);
         const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w.block + at); };
         u.met = ints(words);
@@ -104,6 +104,7 @@ nut_status nut_pages_create(const nut_pages_view *view, int device, nut_pages **
         u.plan = reinterpret_cast<int4 *>(w.block + plan);
         u.freed = ints(freed);
         u.staged = ints(staged);
+        u.changes = ints(changes);
         *out = h.release();
     });
 }

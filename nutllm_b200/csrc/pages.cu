@@ -29,12 +29,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarpsABlock = kPagesThreads / 32;
+/* Loads that a lane has in flight: with one, a table of 512 rows of 1,000 pages
+ * took 125 us. */
+constexpr int kFlight = 8;
 
 __device__ __forceinline__ int pages_of(int slots, int page_size) { return int((unsigned(slots) + page_size - 1) / page_size); }
 
 /* Exclusive sum over the block's threads, and the total. */
-__device__ __forceinline__ int64_t before_in_block(int64_t v, int64_t *sums, int64_t &total) {
+template <int kWarpsABlock> __device__ __forceinline__ int64_t before_in_block(int64_t v, int64_t *sums, int64_t &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t upto = v;
 #pragma unroll
@@ -56,10 +58,11 @@ __device__ __forceinline__ int64_t before_in_block(int64_t v, int64_t *sums, int
     return before;
 }
 
-__global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_constant__ PagesUpdate a) {
+template <int kThreads> __global__ void __launch_bounds__(kThreads, 1) update_kernel(const __grid_constant__ PagesUpdate a) {
+    constexpr int kWarpsABlock = kThreads / 32, kWarps = kPagesCluster * kWarpsABlock;
     __shared__ int64_t sums[kWarpsABlock];
-    __shared__ int places[kPagesThreads];
-    __shared__ uint8_t copied[kPagesThreads];
+    __shared__ int places[kThreads];
+    __shared__ uint8_t copied[kThreads];
     begin_kernel();
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31;
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
     int met = 0;
 
     /* 1 */
-    for (int s = warp; s < S; s += kPagesWarps) {
+    for (int s = warp; s < S; s += kWarps) {
         const int p = a.parent ? a.parent[s] : s, length = a.lengths[s], more = a.add ? a.add[s] : 0;
         const int wish = a.keep ? a.keep[s] : INT_MAX;
         const bool fine = p >= -1 && p < S && more >= 0 && wish >= 0;
@@ -88,20 +91,38 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
         const int32_t *mine = a.table + int64_t(s) * a.max_pages, *its = a.table + int64_t(p) * a.max_pages;
         int32_t *to = a.staged + int64_t(s) * a.max_pages;
         /* a sequence that continues itself keeps its entries as they are */
-        for (int i = (p == s ? keeps : 0) + lane; i < max(had, keeps); i += 32) {
-            const int old = i < had ? mine[i] : -1, next = i < keeps ? its[i] : -1;
-            if ((i < had && unsigned(old) >= unsigned(P)) || (i < keeps && unsigned(next) >= unsigned(P))) {
-                met |= kPagesBadPage;
-                continue;
+        const int ends = max(had, keeps);
+        int changes = -1; /* entries from here on are staged: those before stay */
+        for (int i0 = (p == s ? keeps : 0) + lane; i0 - lane < ends; i0 += 32 * kFlight) {
+            int old[kFlight], next[kFlight];
+            bool differ = false;
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+                const int i = i0 + k * 32;
+                old[k] = i < had ? mine[i] : -1;
+                next[k] = i < keeps ? its[i] : -1;
+                differ |= old[k] != next[k];
             }
-            if (old != next) {
-                if (i < had)
-                    atomicAdd(a.delta + old, -1);
-                if (i < keeps)
-                    atomicAdd(a.delta + next, 1);
+            if (changes < 0 && __any_sync(0xffffffffu, differ))
+                changes = i0 - lane;
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+                const int i = i0 + k * 32;
+                if (i >= ends)
+                    break;
+                if ((i < had && unsigned(old[k]) >= unsigned(P)) || (i < keeps && unsigned(next[k]) >= unsigned(P))) {
+                    met |= kPagesBadPage;
+                    continue;
+                }
+                if (old[k] != next[k]) {
+                    if (i < had)
+                        atomicAdd(a.delta + old[k], -1);
+                    if (i < keeps)
+                        atomicAdd(a.delta + next[k], 1);
+                }
+                if (i < keeps && changes >= 0)
+                    to[i] = next[k];
             }
-            if (i < keeps)
-                to[i] = next;
         }
         if (lane == 0) {
             int tail = more > 0 && kept % ps != 0 ? its[keeps - 1] : -1;
@@ -112,6 +133,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
                 atomicMax(a.first + tail, S - s); /* the first writer has the greatest */
             }
             a.plan[s] = make_int4(kept, kept + more, tail, p);
+            a.changes[s] = changes < 0 ? keeps : min(changes, keeps);
         }
     }
     cluster.sync();
@@ -122,7 +144,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
     if (count < 0 || count > P)
         met |= kPagesBadPage;
     else
-        for (int s0 = 0; s0 < S; s0 += kPagesThreads) {
+        for (int s0 = 0; s0 < S; s0 += kThreads) {
             const int s = s0 + tid;
             int need = 0;
             bool copy = false;
@@ -136,7 +158,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
                 need = pages_of(plan.y, ps) - pages_of(plan.x, ps) + (copy ? 1 : 0);
             }
             int64_t all;
-            const int64_t before = total + before_in_block(need, sums, all);
+            const int64_t before = total + before_in_block<kWarpsABlock>(need, sums, all);
             total += all;
             if (total > count) /* the same in every block */
                 break;
@@ -144,7 +166,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
             copied[tid] = copy;
             __syncthreads();
             /* the block's warps stage the pages that the chunk's sequences take */
-            for (int i = warp; i < min(kPagesThreads, S - s0); i += kPagesWarps) {
+            for (int i = warp; i < min(kThreads, S - s0); i += kWarps) {
                 const int4 plan = __ldcg(a.plan + s0 + i);
                 const int keeps = pages_of(plan.x, ps), ends = pages_of(plan.y, ps), begin = keeps - copied[i];
                 int32_t *to = a.staged + int64_t(s0 + i) * a.max_pages;
@@ -171,7 +193,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
 
     /* 3 */
     const int wrong = __ldcg(a.met);
-    for (int s = warp; s < S; s += kPagesWarps) {
+    for (int s = warp; s < S; s += kWarps) {
         if (wrong) {
             if (lane == 0 && a.copy_from) {
                 a.copy_from[s] = a.copy_to[s] = -1;
@@ -182,15 +204,22 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
         const int4 plan = __ldcg(a.plan + s);
         const int keeps = pages_of(plan.x, ps), ends = pages_of(plan.y, ps);
         const bool copy = plan.w < -1;
-        const int parent = copy ? -2 - plan.w : plan.w;
         const int32_t *next = a.staged + int64_t(s) * a.max_pages;
         int32_t *row = a.table + int64_t(s) * a.max_pages;
         const int taken = keeps - (copy ? 1 : 0);
-        for (int i = (parent == s ? taken : 0) + lane; i < ends; i += 32) {
-            const int page = __ldcg(next + i);
-            row[i] = page;
-            if (i >= taken)
-                a.refs[page] = 1;
+        for (int i0 = min(__ldcg(a.changes + s), taken) + lane; i0 < ends; i0 += 32 * kFlight) {
+            int page[kFlight];
+#pragma unroll
+            for (int k = 0; k < kFlight; k++)
+                page[k] = i0 + k * 32 < ends ? __ldcg(next + i0 + k * 32) : -1;
+#pragma unroll
+            for (int k = 0; k < kFlight; k++) {
+                const int i = i0 + k * 32;
+                if (page[k] >= 0)
+                    row[i] = page[k];
+                if (page[k] >= 0 && i >= taken)
+                    a.refs[page[k]] = 1;
+            }
         }
         if (lane == 0) {
             a.lengths[s] = plan.y;
@@ -202,28 +231,38 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
         }
     }
     /* a run of pages for each warp: what their holders come to */
-    const int run = (P + kPagesWarps - 1) / kPagesWarps;
+    const int run = (P + kWarps - 1) / kWarps;
     const int p0 = min(int64_t(warp) * run, int64_t(P)), p1 = min(p0 + run, P);
     int gone = 0, late = 0;
-    for (int i = p0 + lane; i < p1; i += 32) {
-        const int d = __ldcg(a.delta + i), w = __ldcg(a.writers + i);
-        if (w) {
-            a.first[i] = 0;
-            a.writers[i] = 0;
+    for (int i0 = p0 + lane; i0 < p1; i0 += 32 * kFlight) {
+        int d[kFlight], w[kFlight], held[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; k++) {
+            const int i = i0 + k * 32;
+            d[k] = i < p1 ? __ldcg(a.delta + i) : 0;
+            w[k] = i < p1 ? __ldcg(a.writers + i) : 0;
+            held[k] = i < p1 ? __ldcg(a.refs + i) : 0;
         }
-        if (d || w) {
-            const int held = a.refs[i];
-            int next = held + d;
+#pragma unroll
+        for (int k = 0; k < kFlight; k++) {
+            const int i = i0 + k * 32;
+            if (!d[k] && !w[k])
+                continue;
+            if (w[k]) {
+                a.first[i] = 0;
+                a.writers[i] = 0;
+            }
+            int next = held[k] + d[k];
             /* copies take the place of writers, but where the first keeps the page; a page
              * taken from the list has one holder at most */
-            if (w && next > 1)
-                next -= w == next ? w - 1 : w;
+            if (w[k] && next > 1)
+                next -= w[k] == next ? w[k] - 1 : w[k];
             if (next < 0) { /* fewer holders than the table shows */
                 next = 0;
                 late |= kPagesBadPage;
             }
-            const bool freed = !wrong && held > 0 && next == 0;
-            if (!wrong && next != held)
+            const bool freed = !wrong && held[k] > 0 && next == 0;
+            if (!wrong && next != held[k])
                 a.refs[i] = next;
             a.delta[i] = freed ? INT_MIN : 0;
             gone += freed;
@@ -234,7 +273,7 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
         a.freed[warp] = gone;
     cluster.sync();
     int before = 0, all = 0;
-    for (int w = lane; w < kPagesWarps; w += 32) {
+    for (int w = lane; w < kWarps; w += 32) {
         const int n = __ldcg(a.freed + w);
         all += n;
         before += w < warp ? n : 0;
@@ -272,7 +311,11 @@ __global__ void __launch_bounds__(kPagesThreads, 1) update_kernel(const __grid_c
 } // namespace
 
 cudaError_t pages_update(const PagesUpdate &a, cudaStream_t s) {
-    return launch_kernel(update_kernel, dim3(kPagesCluster), kPagesThreads, 0, s, kPagesCluster, a);
+    /* a small book is a chain of round trips and barriers, which few threads pass sooner */
+    const bool small = a.sequences <= 128 && a.n_pages <= 16384 && int64_t(a.sequences) * a.max_pages <= 65536;
+    const int threads = small ? 256 : 1024;
+    return launch_kernel(small ? update_kernel<256> : update_kernel<1024>, dim3(kPagesCluster), threads, 0, s,
+                         kPagesCluster, a);
 }
 
 } // namespace nut
