@@ -8,12 +8,14 @@
  *
  * A tile is 64 slots, read once for all of an item's rows, in fp32 in shared
  * memory; 256 threads form the products as 4 rows by slots, then 4 rows by
- * dims.  FFMA and its operands' shared-memory reads bound it (16 products to
- * five 16-byte reads); 16-bit caches take it only where the tensor cores'
- * kernel has no form.
+ * dims.  The next tile's keys are on their way from when the logits are
+ * formed, its values from when the outputs are.  FFMA and its operands'
+ * shared-memory reads bound it; 16-bit caches take it only where the tensor
+ * cores' kernel has no form.
  */
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 #include <cuda_runtime.h>
 
 #include "paged_tree.cuh"
@@ -28,14 +30,28 @@ constexpr int kTile = 64;
 template <int kRows, int DP> struct WidePlan {
     static constexpr int kPitch = DP + 4; /* floats: rows begin 4 banks apart */
     static constexpr int kWeights = kTile + 4;
-    static constexpr int kFloats = kRows * kPitch + kTile * kPitch + kRows * kWeights;
+    static constexpr int kFloats = kRows * kPitch + 2 * kTile * kPitch + kRows * kWeights;
     static constexpr int kBytes = kFloats * 4;
     static constexpr int kAcross = kThreads / (kRows / 4); /* threads that share 4 rows */
     static constexpr int kSlots = kTile / kAcross;         /* slots of a thread */
-    static constexpr int kPieces = (DP / 4 + kAcross - 1) / kAcross; /* 4-dim pieces of a thread */
+    /* 4-dim pieces of a thread; or, with more threads than pieces, threads that
+     * share a piece, each over every kShares-th slot */
+    static constexpr int kPieces = DP / 4 > kAcross ? DP / 4 / kAcross : 1;
+    static constexpr int kShares = DP / 4 > kAcross ? 1 : kAcross / (DP / 4);
     static constexpr int kOfRow = kThreads / kRows;        /* threads of a row's softmax */
     static constexpr int kPerSm = kBytes <= 110 * 1024 ? 2 : 1;
+    static_assert(kShares * kRows * DP <= 2 * kTile * kPitch, "the shares' outputs meet in the tiles' place");
 };
+
+/* 16 bytes to shared memory, or zeros. */
+__device__ __forceinline__ void copy_piece(float *to, const void *from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(from),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+/* All but the newest group of copies. */
+__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group 1;\n" ::: "memory"); }
 
 template <typename T> __device__ __forceinline__ void load_four(const T *x, float *v) {
     if constexpr (sizeof(T) == 4) {
@@ -53,9 +69,9 @@ template <int kRows, int DP, typename T, typename R>
 __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_kernel(const __grid_constant__ PagedTree a) {
     using W = WidePlan<kRows, DP>;
     extern __shared__ float4 smem_raw[];
-    float *queries = reinterpret_cast<float *>(smem_raw), *cached = queries + kRows * W::kPitch,
-          *weights = cached + kTile * W::kPitch;
-    __shared__ int64_t places[kTile]; /* elements from the pool's start, -1: no such slot */
+    float *queries = reinterpret_cast<float *>(smem_raw), *keys = queries + kRows * W::kPitch,
+          *values = keys + kTile * W::kPitch, *weights = values + kTile * W::kPitch;
+    __shared__ int64_t places[2][kTile]; /* elements from the pool's start, -1: no such slot */
     __shared__ float maxima[kRows], sums[kRows], factors[kRows];
     const PagedPool &p = a.p;
     const int tid = threadIdx.x, D = p.head_dim;
@@ -65,6 +81,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
     tree_blind_rows<R>(a, tid, kThreads);
     const int start = cursor.pos;
     const int r0 = tid / W::kAcross * 4, c0 = tid % W::kAcross; /* of the products */
+    const int piece0 = c0 % (DP / 4), share0 = W::kShares > 1 ? c0 / (DP / 4) : 0;
     const int soft_row = tid / W::kOfRow, soft_at = tid % W::kOfRow;
     const float unit = a.scale * kTreeLog2e;
     int4 join = make_int4(0, 0, 0, 0);
@@ -99,30 +116,46 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 for (int j = 0; j < 4; j++)
                     o[r][k][j] = 0.0f;
 
-        for (int tile = x.tile0; tile < x.tile1; tile++) {
-            const int t0 = tile * kTile;
-            if (tid < kTile) {
-                const int t = t0 + tid;
+        const auto find = [&](int tile) { /* where a tile's slots lie */
+            if (tid < kTile && tile < x.tile1) {
+                const int t = tile * kTile + tid;
                 int64_t at = -1;
                 if (t < x.span.length) {
-                    const int j = t / p.page_size, page = checked_page(p, x.sequence, j);
+                    const int j = int((uint64_t(unsigned(t)) * a.page_magic) >> a.page_shift);
+                    const int page = checked_page(p, x.sequence, j);
                     if (page >= 0)
                         at = int64_t(page) * p.page_stride + int64_t(x.head) * p.head_stride +
                              int64_t(t - j * p.page_size) * p.slot_stride;
                 }
-                places[tid] = at;
+                places[tile & 1][tid] = at;
             }
-            __syncthreads();
-            const auto fetch = [&](const void *pool) {
+        };
+        const auto fetch = [&](int tile, const void *pool, float *to) {
+            if (tile < x.tile1)
                 for (int i = tid; i < kTile * (DP / 4); i += kThreads) {
                     const int t = i / (DP / 4), d = i % (DP / 4) * 4;
-                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (places[t] >= 0 && d < D)
-                        load_four(static_cast<const T *>(pool) + places[t] + d, v);
-                    *reinterpret_cast<float4 *>(cached + t * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    const int64_t at = places[tile & 1][t];
+                    const bool there = at >= 0 && d < D;
+                    const T *from = static_cast<const T *>(pool) + (there ? at + d : 0);
+                    if constexpr (sizeof(T) == 4) {
+                        copy_piece(to + t * W::kPitch + d, from, there);
+                    } else {
+                        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (there)
+                            load_four(from, v);
+                        *reinterpret_cast<float4 *>(to + t * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    }
                 }
-            };
-            fetch(p.keys);
+            copies_done();
+        };
+        find(x.tile0);
+        __syncthreads();
+        fetch(x.tile0, p.keys, keys);
+        fetch(x.tile0, p.values, values);
+        for (int tile = x.tile0; tile < x.tile1; tile++) {
+            const int t0 = tile * kTile;
+            find(tile + 1);
+            await_copies(); /* the keys */
             __syncthreads();
             float z[4][W::kSlots];
 #pragma unroll
@@ -138,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                     q[r] = *reinterpret_cast<const float4 *>(queries + (r0 + r) * W::kPitch + d);
 #pragma unroll
                 for (int k = 0; k < W::kSlots; k++) {
-                    const float4 c = *reinterpret_cast<const float4 *>(cached + (c0 + k * W::kAcross) * W::kPitch + d);
+                    const float4 c = *reinterpret_cast<const float4 *>(keys + (c0 + k * W::kAcross) * W::kPitch + d);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         z[r][k] = fmaf(q[r].x, c.x, z[r][k]);
@@ -154,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 for (int k = 0; k < W::kSlots; k++)
                     weights[(r0 + r) * W::kWeights + c0 + k * W::kAcross] = z[r][k] * unit;
             __syncthreads();
-            fetch(p.values); /* in flight during the softmax */
+            fetch(tile + 1, p.keys, keys);
 
             /* softmax: kOfRow threads a row, 64 / kOfRow neighbouring slots each */
             constexpr int kEach = kTile / W::kOfRow;
@@ -174,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 }
 #pragma unroll
                 for (int j = 0; j < kEach; j++) {
-                    v[j] = ((sees >> j) & 1) && places[s0 + j] >= 0 ? own[j] : -INFINITY;
+                    v[j] = ((sees >> j) & 1) && places[tile & 1][s0 + j] >= 0 ? own[j] : -INFINITY;
                     top = fmaxf(top, v[j]);
                 }
             }
@@ -199,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 maxima[soft_row] = next;
                 sums[soft_row] = sums[soft_row] * keep + sum;
             }
+            await_copies(); /* the values */
             __syncthreads();
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -210,28 +244,51 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                         o[r][k][j] *= keep;
             }
             /* values that a row does not see may be infinite or NaN: a weight of 0 takes no part */
-            const bool drafted = t0 + kTile > x.span.prefix;
+            const auto multiply = [&](auto drafted) {
 #pragma unroll 4
-            for (int t = 0; t < kTile; t++) {
-                float w[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    w[r] = weights[(r0 + r) * W::kWeights + t];
-#pragma unroll
-                for (int k = 0; k < W::kPieces; k++) {
-                    const int d = (c0 + k * W::kAcross) * 4;
-                    if (d >= DP)
-                        break;
-                    const float4 c = *reinterpret_cast<const float4 *>(cached + t * W::kPitch + d);
-                    const float e[4] = {c.x, c.y, c.z, c.w};
+                for (int t = share0; t < kTile; t += W::kShares) {
+                    float w[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++)
+                        w[r] = weights[(r0 + r) * W::kWeights + t];
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            o[r][k][j] = fmaf(w[r], drafted && w[r] == 0.0f ? 0.0f : e[j], o[r][k][j]);
+                    for (int k = 0; k < W::kPieces; k++) {
+                        const float4 c = *reinterpret_cast<const float4 *>(values + t * W::kPitch + (piece0 + k * W::kAcross) * 4);
+                        const float e[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                o[r][k][j] = fmaf(w[r], decltype(drafted)::value && w[r] == 0.0f ? 0.0f : e[j], o[r][k][j]);
+                    }
                 }
-            }
+            };
+            if (t0 + kTile > x.span.prefix)
+                multiply(std::true_type());
+            else
+                multiply(std::false_type());
             __syncthreads();
+            fetch(tile + 1, p.values, values);
+        }
+        if constexpr (W::kShares > 1) { /* the shares meet */
+            float *room = keys;
+            if (share0 > 0)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    *reinterpret_cast<float4 *>(room + (share0 * kRows + r0 + r) * DP + piece0 * 4) =
+                        make_float4(o[r][0][0], o[r][0][1], o[r][0][2], o[r][0][3]);
+            __syncthreads();
+            if (share0 == 0)
+#pragma unroll
+                for (int s = 1; s < W::kShares; s++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float4 v = *reinterpret_cast<const float4 *>(room + (s * kRows + r0 + r) * DP + piece0 * 4);
+                        o[r][0][0] += v.x;
+                        o[r][0][1] += v.y;
+                        o[r][0][2] += v.z;
+                        o[r][0][3] += v.w;
+                    }
         }
 
         const bool whole = x.whole();
@@ -252,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int f = r0 + r;
-            if (f >= x.rows)
+            if (f >= x.rows || share0 > 0)
                 break;
             int64_t row;
             int h;
@@ -260,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             const float inv = !whole ? 1.0f : sums[f] == 0.0f ? 0.0f : 1.0f / sums[f];
 #pragma unroll
             for (int k = 0; k < W::kPieces; k++) {
-                const int d = (c0 + k * W::kAcross) * 4;
+                const int d = (piece0 + k * W::kAcross) * 4;
                 if (d >= D)
                     break;
 #pragma unroll

@@ -740,6 +740,8 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
             base += 2 * n;
 
             /* the end of the item, or of this block's part of it */
+            if (alive && kBuffers > 1 && n > 1) /* the products may be two tiles behind */
+                alive = await(&sh.outputs, (tiles - 2) & 1);
             if (alive)
                 alive = await(&sh.outputs, (tiles - 1) & 1);
             alive = __all_sync(0xffffffffu, alive);

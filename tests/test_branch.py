@@ -165,6 +165,43 @@ def test_tree_attention_splits_long_caches(torch_cuda, cache, rows):
 
 
 @gpu
+@pytest.mark.parametrize("cache,rows", [("f32", "f32"), ("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("D,ps", [(64, 1), (64, 8), (128, 5), (128, 8), (128, 16), (128, 64), (256, 16)])
+def test_tree_long_runs_of_tiles(torch_cuda, D, ps, cache, rows):
+    """Many tiles for each block, arriving in few or in many copies: equal keys, and values that name their slots, so
+    that each output counts the slots of a class exactly."""
+    torch = torch_cuda
+    lens, heads, kv = [3000, 700, 3000, 1100, 2900, 64, 2300], 32, 8
+    pool = Pool(torch, lens, heads, kv, D, ps, cache, seed=2, fill=False)
+    classes = 40
+    for s, n in enumerate(lens):
+        v = torch.zeros(kv, n, D)
+        t = torch.arange(n)
+        v[:, t, (t // 64 + 7 * t) % classes] = 1.0  # by tile and by slot
+        k = torch.zeros(kv, n, D).to(dtypes(torch)[cache])
+        page = pool.table[s, (t // ps).cuda()].long()
+        pool.keys[page, :, (t % ps).cuda()] = k.transpose(0, 1).cuda()
+        pool.values[page, :, (t % ps).cuda()] = v.transpose(0, 1).to(pool.values.dtype).cuda()
+    pool.cache.reserve_tree(3)
+    nodes = [3, 1, 2, 3, 1, 2, 3]
+    tree = Tree(torch, pool, nodes, rows, masks=[[list(range(i + 1)) for i in range(n)] for n in nodes])
+    for _ in range(4):
+        tree.out.fill_(5.0)
+        tree.run()
+        pool.cache.check()
+        out, r = tree.out.reshape(-1, heads, D).float().cpu(), 0
+        for n, m in zip(lens, nodes):
+            for i in range(m):
+                seen = n - m + i + 1
+                t = torch.arange(seen)
+                want = torch.bincount((t // 64 + 7 * t) % classes, minlength=D).double() / seen
+                # equal weights: powers of two, their sum and the outputs are exact but for the division and the type
+                tol = want * (4 * EPS + (0.0 if rows == "f32" else torch.finfo(dtypes(torch)[rows]).eps / 2)) + 2.0 ** -25
+                assert bool(((out[r].double() - want).abs() <= tol).all()), (n, i)
+                r += 1
+
+
+@gpu
 @pytest.mark.parametrize("cache,rows", [("f32", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")])
 def test_tree_masks_that_are_no_trees(torch_cuda, cache, rows):
     """Rows that see nothing, only later tokens, or not themselves."""
