@@ -278,9 +278,11 @@ constexpr int kNoted = 8;
 template <int kStages> struct Shared {
     uint64_t full[kStages], empty[kStages];
     uint64_t queries;                      /* an item's are in shared memory */
+    /* of the tiles in each buffer: the softmax may be two tiles ahead of the
+     * products, and a barrier tells two phases apart, not three */
     uint64_t logits[2];                    /* a tile's are in tensor memory */
-    uint64_t weights[2];                   /* its weights are; the softmax may be a tile ahead of the products */
-    uint64_t outputs;                      /* its product with the values is done */
+    uint64_t weights[2];                   /* its weights are */
+    uint64_t outputs[2];                   /* its product with the values is done */
     uint64_t drained;                      /* products in flight after a wait ran out */
     uint32_t valid[kNoted][2];             /* slots there are of the tiles under way */
     float unit[kRows];                     /* of a row's logits (fp32 queries) */
@@ -320,7 +322,8 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
         mbar_init(&sh.logits[1], 1);
         mbar_init(&sh.weights[0], kRows);
         mbar_init(&sh.weights[1], kRows);
-        mbar_init(&sh.outputs, 1);
+        mbar_init(&sh.outputs[0], 1);
+        mbar_init(&sh.outputs[1], 1);
         mbar_init(&sh.drained, 1);
         sh.dead = sh.odd = 0;
         fence_barrier_init();
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                                 for (int s = 0; s < kTile / 16; s++)
                                     mma_ts(tmem + Plan::kOutputs, weights + t * (kTile / 2) + s * 8, v + s * (values_step >> 4),
                                            kShapeO, i > 0 || t > 0 || s > 0);
-                            tc_commit(&sh.outputs);
+                            tc_commit(&sh.outputs[buffer]);
                             tc_commit(&sh.empty[stage_of(place)]);
                         }
                     }
@@ -535,6 +538,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
     } else {
         const uint32_t lanes = uint32_t(warp * 32) << 16, outputs_at = tmem + lanes + Plan::kOutputs;
         const auto everyone = [] { named_barrier(1, kRows); };
+        /* A barrier for every buffer: no phase of one is waited for when the next may
+         * have ended too, or have not begun. */
+        const auto await_outputs = [&](uint32_t tile) { return await(&sh.outputs[tile % kBuffers], tile / kBuffers & 1); };
         uint32_t tiles = 0; /* of the items before */
         int4 join = make_int4(0, 0, 0, 0);
         tree_blind_rows<R>(a, tid, kRows);
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         l *= keep;
                         from = next;
                         if (i > 0) { /* once the products before are complete */
-                            alive = __all_sync(0xffffffffu, await(&sh.outputs, (tiles - 1) & 1));
+                            alive = __all_sync(0xffffffffu, await_outputs(tiles - 1));
                             tc_after();
 #pragma unroll 1
                             for (int c = 0; c < DP && alive; c += 32) {
@@ -741,9 +747,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
 
             /* the end of the item, or of this block's part of it */
             if (alive && kBuffers > 1 && n > 1) /* the products may be two tiles behind */
-                alive = await(&sh.outputs, (tiles - 2) & 1);
+                alive = await_outputs(tiles - 2);
             if (alive)
-                alive = await(&sh.outputs, (tiles - 1) & 1);
+                alive = await_outputs(tiles - 1);
             alive = __all_sync(0xffffffffu, alive);
             tc_after();
             everyone(); /* all products are done: the queries' place is free */
