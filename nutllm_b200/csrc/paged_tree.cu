@@ -24,7 +24,7 @@ namespace nut {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64;
+constexpr int kTile = kTreeTile;
 
 /* kRows: 16 or 64 rows of an item. */
 template <int kRows, int DP> struct WidePlan {
@@ -42,6 +42,22 @@ template <int kRows, int DP> struct WidePlan {
     static constexpr int kPerSm = kBytes <= 110 * 1024 ? 2 : 1;
     static_assert(kShares * kRows * DP <= 2 * kTile * kPitch, "the shares' outputs meet in the tiles' place");
 };
+
+/* Two fp32 numbers, and two products added to two sums in one instruction. */
+using Two = unsigned long long;
+__device__ __forceinline__ Two two_of(float a, float b) {
+    Two v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 parts_of(Two v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ void add_products(Two &sum, Two a, Two b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sum) : "l"(a), "l"(b));
+}
 
 /* 16 bytes to shared memory, or zeros. */
 __device__ __forceinline__ void copy_piece(float *to, const void *from, bool there) {
@@ -107,14 +123,12 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             maxima[tid] = -INFINITY;
             sums[tid] = 0.0f;
         }
-        float o[4][W::kPieces][4];
+        Two o2[4][W::kPieces][2];
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int k = 0; k < W::kPieces; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    o[r][k][j] = 0.0f;
+                o2[r][k][0] = o2[r][k][1] = 0;
 
         const auto find = [&](int tile) { /* where a tile's slots lie */
             if (tid < kTile && tile < x.tile1) {
@@ -157,35 +171,35 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             find(tile + 1);
             await_copies(); /* the keys */
             __syncthreads();
-            float z[4][W::kSlots];
+            Two z[4][W::kSlots];
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int k = 0; k < W::kSlots; k++)
-                    z[r][k] = 0.0f;
+                    z[r][k] = 0;
 #pragma unroll 4
             for (int d = 0; d < DP; d += 4) {
-                float4 q[4];
+                ulonglong2 q[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    q[r] = *reinterpret_cast<const float4 *>(queries + (r0 + r) * W::kPitch + d);
+                    q[r] = *reinterpret_cast<const ulonglong2 *>(queries + (r0 + r) * W::kPitch + d);
 #pragma unroll
                 for (int k = 0; k < W::kSlots; k++) {
-                    const float4 c = *reinterpret_cast<const float4 *>(keys + (c0 + k * W::kAcross) * W::kPitch + d);
+                    const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(keys + (c0 + k * W::kAcross) * W::kPitch + d);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        z[r][k] = fmaf(q[r].x, c.x, z[r][k]);
-                        z[r][k] = fmaf(q[r].y, c.y, z[r][k]);
-                        z[r][k] = fmaf(q[r].z, c.z, z[r][k]);
-                        z[r][k] = fmaf(q[r].w, c.w, z[r][k]);
+                        add_products(z[r][k], q[r].x, c.x);
+                        add_products(z[r][k], q[r].y, c.y);
                     }
                 }
             }
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int k = 0; k < W::kSlots; k++)
-                    weights[(r0 + r) * W::kWeights + c0 + k * W::kAcross] = z[r][k] * unit;
+                for (int k = 0; k < W::kSlots; k++) {
+                    const float2 v = parts_of(z[r][k]);
+                    weights[(r0 + r) * W::kWeights + c0 + k * W::kAcross] = (v.x + v.y) * unit;
+                }
             __syncthreads();
             fetch(tile + 1, p.keys, keys);
 
@@ -240,26 +254,31 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 #pragma unroll
                 for (int k = 0; k < W::kPieces; k++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        o[r][k][j] *= keep;
+                    for (int j = 0; j < 2; j++) {
+                        const float2 v = parts_of(o2[r][k][j]);
+                        o2[r][k][j] = two_of(v.x * keep, v.y * keep);
+                    }
             }
             /* values that a row does not see may be infinite or NaN: a weight of 0 takes no part */
             const auto multiply = [&](auto drafted) {
 #pragma unroll 4
                 for (int t = share0; t < kTile; t += W::kShares) {
-                    float w[4];
+                    Two w[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[r] = weights[(r0 + r) * W::kWeights + t];
+                    for (int r = 0; r < 4; r++) {
+                        const float v = weights[(r0 + r) * W::kWeights + t];
+                        w[r] = two_of(v, v);
+                    }
 #pragma unroll
                     for (int k = 0; k < W::kPieces; k++) {
-                        const float4 c = *reinterpret_cast<const float4 *>(values + t * W::kPitch + (piece0 + k * W::kAcross) * 4);
-                        const float e[4] = {c.x, c.y, c.z, c.w};
+                        const ulonglong2 c =
+                            *reinterpret_cast<const ulonglong2 *>(values + t * W::kPitch + (piece0 + k * W::kAcross) * 4);
 #pragma unroll
-                        for (int r = 0; r < 4; r++)
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                o[r][k][j] = fmaf(w[r], decltype(drafted)::value && w[r] == 0.0f ? 0.0f : e[j], o[r][k][j]);
+                        for (int r = 0; r < 4; r++) {
+                            const bool none = decltype(drafted)::value && w[r] == 0;
+                            add_products(o2[r][k][0], w[r], none ? 0 : c.x);
+                            add_products(o2[r][k][1], w[r], none ? 0 : c.y);
+                        }
                     }
                 }
             };
@@ -270,6 +289,17 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             __syncthreads();
             fetch(tile + 1, p.values, values);
         }
+        float o[4][W::kPieces][4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int k = 0; k < W::kPieces; k++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float2 v = parts_of(o2[r][k][j]);
+                    o[r][k][2 * j] = v.x;
+                    o[r][k][2 * j + 1] = v.y;
+                }
         if constexpr (W::kShares > 1) { /* the shares meet */
             float *room = keys;
             if (share0 > 0)
@@ -338,12 +368,13 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 
 /* ---- joining the parts of an item --------------------------------------- */
 
-constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 32;
+constexpr int kJoinWarps = 8, kJoinOwn = 2, kJoinRows = kJoinWarps * kJoinOwn;
 
-/* A warp joins a row: out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m).  Lanes
- * turn the parts' maxima and sums into factors, 32 parts at a time, then take
- * 4 dims each. */
-template <typename R> __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ PagedTree a, int block_rows) {
+/* out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) for two rows a warp, whose loads
+ * are in flight together.  Lanes turn the parts' maxima and sums into factors, 32 parts at a time,
+ * then take 4 dims each. */
+template <typename R>
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_constant__ PagedTree a, int block_rows) {
     begin_kernel();
     const int4 join = a.joins[blockIdx.x];
     const int parts = join.x, lane = threadIdx.x & 31;
@@ -353,63 +384,103 @@ template <typename R> __global__ void __launch_bounds__(kJoinThreads) join_kerne
     const int D = p.head_dim, first_row = join.w >> 1, inside = join.w & 1;
     const int row0 = a.starts[join.y], n = a.starts[join.y + 1] - row0;
     const int rows = min(block_rows, n * p.group - first_row);
-    const int f = int(blockIdx.y) * kJoinRows + int(threadIdx.x >> 5);
-    if (f >= rows)
+    const int f0 = int(blockIdx.y) * kJoinRows + int(threadIdx.x >> 5) * kJoinOwn;
+    if (f0 >= rows)
         return;
-    const auto part = [&](int c) { return tree_part(a, blockIdx.x + c, c == 0 ? inside : 0, rows); };
-    float top = -INFINITY;
+    const TreePart first = tree_part(a, blockIdx.x, inside, rows), second = tree_part(a, blockIdx.x + 1, 0, rows);
+    const int64_t step = 2 * a.part_floats;
+    const auto at = [&](const float *x, const float *y, int c, int f) { return (c == 0 ? x : y + (c - 1) * step) + min(f, rows - 1); };
+    float from[kJoinOwn], sum[kJoinOwn];
+#pragma unroll
+    for (int r = 0; r < kJoinOwn; r++) {
+        from[r] = -INFINITY;
+        sum[r] = 0.0f;
+    }
     for (int c = lane; c < parts; c += 32)
-        top = fmaxf(top, part(c).maxima[f]);
-    top = warp_max(top);
-    const float from = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    constexpr int kFlight = 16; /* loads of a lane */
+#pragma unroll
+        for (int r = 0; r < kJoinOwn; r++)
+            from[r] = fmaxf(from[r], *at(first.maxima, second.maxima, c, f0 + r));
+#pragma unroll
+    for (int r = 0; r < kJoinOwn; r++) {
+        from[r] = warp_max(from[r]);
+        from[r] = from[r] == -INFINITY ? 0.0f : from[r];
+    }
+    constexpr int kMost = 2; /* pieces of 4 dims a lane, 128 dims apart */
+    float4 o[kJoinOwn][kMost];
+#pragma unroll
+    for (int r = 0; r < kJoinOwn; r++)
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            o[r][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c0 = 0; c0 < parts; c0 += 32) {
         const int c = c0 + lane, many = min(32, parts - c0);
-        const float factor = c < parts ? exp2f(part(c).maxima[f] - from) : 0.0f;
-        if (c < parts)
-            sum = fmaf(part(c).sums[f], factor, sum);
-        for (int i0 = 0; i0 < many; i0 += kFlight)
+        float factor[kJoinOwn];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int d = k * 128 + lane * 4;
-                if (k * 128 >= D)
-                    break;
-                float4 v[kFlight];
+        for (int r = 0; r < kJoinOwn; r++) {
+            factor[r] = c < parts ? exp2f(*at(first.maxima, second.maxima, c, f0 + r) - from[r]) : 0.0f;
+            sum[r] += c < parts ? *at(first.sums, second.sums, c, f0 + r) * factor[r] : 0.0f;
+        }
 #pragma unroll
-                for (int i = 0; i < kFlight; i++)
-                    v[i] = i0 + i < many && d < D
-                               ? __ldcg(reinterpret_cast<const float4 *>(part(c0 + i0 + i).out + int64_t(f) * D + d))
-                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < kMost; k++) {
+            if (k * 128 >= D)
+                break;
+            const int d = k * 128 + lane * 4;
+            constexpr int kFlight = 4;
+            for (int i0 = 0; i0 < many; i0 += kFlight) {
+                float4 v[kFlight][kJoinOwn];
 #pragma unroll
                 for (int i = 0; i < kFlight; i++) {
-                    const float w = __shfl_sync(0xffffffffu, factor, i0 + i);
-                    if (w != 0.0f) { /* a part in which the row saw nothing, or what underflows */
-                        o[k].x = fmaf(v[i].x, w, o[k].x);
-                        o[k].y = fmaf(v[i].y, w, o[k].y);
-                        o[k].z = fmaf(v[i].z, w, o[k].z);
-                        o[k].w = fmaf(v[i].w, w, o[k].w);
+                    const int part = c0 + i0 + i;
+                    const float *x = (part == 0 ? first.out : second.out + (part - 1) * step) + d;
+#pragma unroll
+                    for (int r = 0; r < kJoinOwn; r++)
+                        v[i][r] = i0 + i < many && d < D
+                                      ? *reinterpret_cast<const float4 *>(x + min(f0 + r, rows - 1) * D)
+                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < kFlight; i++)
+#pragma unroll
+                    for (int r = 0; r < kJoinOwn; r++) {
+                        const float w = __shfl_sync(0xffffffffu, factor[r], i0 + i);
+                        if (w != 0.0f) { /* 0: a part in which the row saw nothing, or what underflows */
+                            o[r][k].x = fmaf(v[i][r].x, w, o[r][k].x);
+                            o[r][k].y = fmaf(v[i][r].y, w, o[r][k].y);
+                            o[r][k].z = fmaf(v[i][r].z, w, o[r][k].z);
+                            o[r][k].w = fmaf(v[i][r].w, w, o[r][k].w);
+                        }
                     }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kJoinOwn; r++) {
+        const float all = warp_sum(sum[r]), inv = all == 0.0f ? 0.0f : 1.0f / all;
+        if (f0 + r >= rows)
+            break;
+        int64_t row;
+        int h;
+        tree_row(a, row0, join.z, first_row + f0 + r, row, h);
+        if (a.lse && lane == 0)
+            a.lse[row * p.heads + h] = all == 0.0f ? -INFINITY : (from[r] + log2f(all)) * kTreeLn2;
+        R *to = static_cast<R *>(a.out) + row * a.out_stride + int64_t(h) * D;
+#pragma unroll
+        for (int k = 0; k < kMost; k++) {
+            const int d = k * 128 + lane * 4;
+            if (d < D) {
+                const R e[4] = {output_of<R>(o[r][k].x * inv), output_of<R>(o[r][k].y * inv), output_of<R>(o[r][k].z * inv),
+                                output_of<R>(o[r][k].w * inv)};
+                if (a.aligned) {
+                    if constexpr (sizeof(R) == 4)
+                        *reinterpret_cast<float4 *>(to + d) = make_float4(e[0], e[1], e[2], e[3]);
+                    else
+                        *reinterpret_cast<uint2 *>(to + d) = *reinterpret_cast<const uint2 *>(e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        to[d + j] = e[j];
                 }
             }
-    }
-    sum = warp_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    int64_t row;
-    int h;
-    tree_row(a, row0, join.z, first_row + f, row, h);
-    if (a.lse && lane == 0)
-        a.lse[row * p.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kTreeLn2;
-    R *to = static_cast<R *>(a.out) + row * a.out_stride + int64_t(h) * D;
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int d = k * 128 + lane * 4;
-        if (d < D) {
-            to[d] = output_of<R>(o[k].x * inv);
-            to[d + 1] = output_of<R>(o[k].y * inv);
-            to[d + 2] = output_of<R>(o[k].z * inv);
-            to[d + 3] = output_of<R>(o[k].w * inv);
         }
     }
 }
@@ -447,10 +518,12 @@ template <typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cu
 } // namespace
 
 cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaStream_t s) {
+    if (a.p.capacity <= kTreeTile) /* items of one tile lie in one block */
+        return cudaSuccess;
     const int rows = int(std::min<int64_t>(block_rows, int64_t(a.max_new) * a.p.group));
     const dim3 grid(ctas, (rows + kJoinRows - 1) / kJoinRows);
     const auto kernel = a.type == 0 ? join_kernel<float> : a.type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>;
-    return launch_kernel(kernel, grid, kJoinThreads, 0, s, 1, a, block_rows);
+    return launch_kernel(kernel, grid, kJoinWarps * 32, 0, s, 1, a, block_rows);
 }
 
 int64_t tree_part_floats(const PagedPool &p, int max_new) {

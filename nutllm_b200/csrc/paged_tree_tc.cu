@@ -38,7 +38,7 @@ namespace nut {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kTile = 64;
+constexpr int kTile = kTreeTile;
 constexpr int kProducer = 4, kIssuer = 5; /* warps */
 constexpr int kThreads = 192;
 constexpr uint64_t kTreeWaitNs = 2000000000ull;
