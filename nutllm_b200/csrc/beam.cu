@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kRunWarps * 32) runs_kernel(const __grid_const
             for (int i = 0; i < kEach; i++) {
                 const int e = at(i);
                 reinterpret_cast<T *>(now + i / kPer * 32 + lane)[i % kPer] =
-                    e >= 0 && e < a.vocab ? logits[e] : from_float<T>(-INFINITY);
+                    e >= 0 && e < a.vocab ? logits[e] : output_of<T>(-INFINITY);
             }
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {

@@ -288,6 +288,100 @@ def test_tree_rising_logits(torch_cuda, cache, rows):
         tree.check(scale=float(np.float32(0.4)))
 
 
+PAIRS = [("f32", "f32"), ("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")]
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("scale", [-0.25, 3.0, 1e-4])
+def test_tree_scales(torch_cuda, cache, rows, scale):
+    torch = torch_cuda
+    pool = Pool(torch, [300, 40], 8, 2, 64, 16, cache, seed=12)
+    pool.cache.reserve_tree(17)
+    tree = Tree(torch, pool, [17, 5], rows)
+    tree.run(scale=scale)
+    pool.cache.check()
+    tree.check(scale=float(np.float32(scale)))
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("power", [20, 24, 26])
+def test_tree_logits_far_from_zero(torch_cuda, cache, rows, power):
+    """Logits of 2^20 and more, all but a few of them equal: weights stay in their type's range, and the equal ones share
+    the output."""
+    torch = torch_cuda
+    L, D = 700, 64
+    pool = Pool(torch, [L + 1], 2, 1, D, 16, cache, seed=13)
+    k = torch.zeros(1, L + 1, D)
+    k[0, :, 0] = 2.0 ** 8
+    k[0, 5::97, 0] = 2.0 ** 7
+    v = torch.zeros(1, L + 1, D)
+    v[0, torch.arange(L + 1), torch.arange(L + 1) % D] = 1.0
+    k, v = k.to(dtypes(torch)[cache]), v.to(dtypes(torch)[cache])
+    pool.put(0, k, v, 0)
+    pool.k, pool.v = [k], [v]
+    pool.cache.reserve_tree(1)
+    tree = Tree(torch, pool, [1], rows)
+    tree.q_cpu.zero_()
+    tree.q_cpu[:, :, 0] = 2.0 ** 9
+    tree.q.copy_(tree.q_cpu.reshape(1, -1))
+    tree.run(scale=2.0 ** (power - 17))
+    pool.cache.check()
+    great = k[0, :, 0] == 2.0 ** 8
+    want = (v[0].double() * great[:, None]).sum(0) / int(great.sum())
+    err = (tree.out.reshape(2, D).cpu().double() - want).abs()
+    assert bool((err <= want * (8 * EPS + torch.finfo(dtypes(torch)[rows]).eps / 2 + UNIT[rows]) + 2.0 ** -25).all())
+    # log-sum-exp: the logit and the count, rounded a few times
+    lse = 2.0 ** power + math.log(int(great.sum()))
+    assert bool(((tree.lse.cpu().double() - lse).abs() <= 8 * EPS * lse).all())
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("D", [40, 128])
+def test_tree_rows_at_any_element(torch_cuda, cache, rows, D):
+    """q and out that begin and step at odd elements, and no lse."""
+    torch = torch_cuda
+    pool = Pool(torch, [600, 50], 6, 2, D, 16, cache, seed=14)
+    pool.cache.reserve_tree(12)
+    tree = Tree(torch, pool, [12, 7], rows, q_pad=3, out_pad=5)
+    dt, n, width = dtypes(torch)[rows], tree.rows, 6 * D
+    room = torch.full((n * tree.out_stride + 9,), 77.0, dtype=dt, device="cuda")
+    q = torch.zeros(n * tree.q_stride + 9, dtype=dt, device="cuda")
+    q[1:1 + n * tree.q_stride] = tree.q.reshape(-1)
+    pool.cache.tree_attention(q[1:].data_ptr(), room[3:].data_ptr(), tree.starts.data_ptr(), tree.mask.data_ptr(), n, 12, tree.words,
+                              dtype=KINDS[rows], q_stride=tree.q_stride, out_stride=tree.out_stride)
+    pool.cache.check()
+    tree.run()  # the same at even ones
+    got = room[3:3 + n * tree.out_stride].view(n, tree.out_stride)
+    assert torch.equal(got[:, :width], tree.out[:, :width]) and bool((got[:, width:] == 77).all())
+    assert bool((room[:3] == 77).all()) and bool((room[3 + n * tree.out_stride:] == 77).all())
+    tree.check()
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+def test_tree_many_sequences_and_one_kv_head(torch_cuda, cache, rows):
+    """More sequences than a block has threads; and a group of 48 heads, so that tokens lie across blocks of rows."""
+    torch = torch_cuda
+    r = random.Random(5)
+    lens = [r.choice([0, 1, 5, 40, 90]) for _ in range(420)]
+    nodes = [r.randrange(min(n, 4) + 1) for n in lens]
+    pool = Pool(torch, lens, 2, 1, 32, 8, cache, seed=15)
+    pool.cache.reserve_tree(4)
+    tree = Tree(torch, pool, nodes, rows)
+    tree.run()
+    pool.cache.check()
+    tree.check(only={(s, i, 0) for s in range(0, 420, 13) for i in range(4)})
+    pool = Pool(torch, [333, 20], 48, 1, 64, 16, cache, seed=16)
+    pool.cache.reserve_tree(9)
+    tree = Tree(torch, pool, [9, 5], rows)
+    tree.run()
+    pool.cache.check()
+    tree.check()
+
+
 @gpu
 def test_tree_many_small_weights_beside_a_great_one(torch_cuda):
     """2,047 weights 18 units below the greatest add up to a share of an fp32 row's output."""
@@ -903,6 +997,22 @@ def test_beam_select_ties_and_what_is_not_finite(torch_cuda, kind):
         logits = logits.to(dt)
         got = run_beams(torch, logits.cuda(), scores.cuda(), n)
         same_beams(got, plain_beams(torch, logits, scores, None, -1, n))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [3, 700, 1025, 9001])
+def test_beam_select_rows_of_the_lowest_value(torch_cuda, kind, V):
+    """Rows of the type's lowest value, alone or but for a few logits: places outside the row count for nothing."""
+    torch = torch_cuda
+    dt = dtypes(torch)[kind]
+    logits = torch.full((3, V), torch.finfo(dt).min, dtype=dt)
+    logits[1, V // 2] = 1.0
+    logits[2, :] = -math.inf
+    logits[2, V - 1] = torch.finfo(dt).min
+    scores = torch.tensor([[-1.0, -2.0, -0.5]])
+    n = min(5, V)
+    same_beams(run_beams(torch, logits.cuda(), scores.cuda(), n), plain_beams(torch, logits, scores, None, -1, n))
 
 
 @gpu
