@@ -533,9 +533,10 @@ nut_status nut_paged_append_at(nut_paged *paged, const nut_paged_append_args *ar
                                const int32_t *row_position, void *stream);
 
 /* Workspace for nut_paged_tree_attention calls of up to max_new (1 to
- * NUT_TREE_MAX) drafted tokens a sequence.  Allocates, so not within a
- * capture.  Called again with more it allocates anew; what earlier captures
- * use stays until the handle goes. */
+ * NUT_TREE_MAX) drafted tokens a sequence: on 148 SMs 592 parts of
+ * min(128, max_new * heads / kv_heads) rows of head_dim + 2 floats.
+ * Allocates, so not within a capture.  Called again with more it allocates
+ * anew; what earlier captures use stays until the handle goes. */
 #define NUT_TREE_MAX 1024
 nut_status nut_paged_reserve_tree(nut_paged *paged, int64_t max_new);
 
@@ -550,9 +551,9 @@ nut_status nut_paged_reserve_tree(nut_paged *paged, int64_t max_new);
  * nothing gives zeros and lse = -infinity.  Masks need not be those of a
  * tree.  Whatever is stored in slots that a row does not see, infinities and
  * NaN included, has no part in its outputs; an infinity or NaN among the
- * values it sees makes that dimension of its output infinite or NaN.  Sums,
- * the softmax and its statistics are fp32.  Products are formed from 16-bit
- * terms where the cache has 16 bits: fp32 queries and their weights in two
+ * values it sees makes that dimension of its output infinite or NaN, and an
+ * infinite key that it sees may make the row NaN.  Sums, the softmax and its
+ * statistics are fp32.  Products are formed from 16-bit terms where the cache has 16 bits: fp32 queries and their weights in two
  * (fp16) or three (bf16) of them, rows of the cache's type in one (weights
  * within 2^-8 of themselves on bf16, 2^-11 on fp16; the sum is taken before).
  * Rows behind starts[sequences] are left as they were.  A sequence whose
@@ -623,8 +624,8 @@ typedef struct nut_pages_view {
     int64_t sequences, max_pages, n_pages, page_size;
 } nut_pages_view;
 
-/* A handle on them with this library's workspace (8 to 12 bytes a page, 4 for
- * every entry of the table); as for nut_paged, calls of one handle are
+/* A handle on them with this library's workspace (12 bytes a page, 4 for every
+ * entry of the table); as for nut_paged, calls of one handle are
  * ordered by the caller, and none of them allocates. */
 typedef struct nut_pages nut_pages;
 
@@ -653,7 +654,10 @@ nut_status nut_pages_error(nut_pages *pages, void *stream);
  * Table entries behind a sequence's last page stay as they were.  If a
  * parent, keep, add, length or page is out of range, a sequence outgrows its
  * table, or the free pages do not suffice, nothing changes: the copy lists
- * are all -1 (and 0), and the error is kept for nut_pages_error. */
+ * are all -1 (and 0), and the error is kept for nut_pages_error.  (Pages of
+ * entries that stay are not looked at.  A book whose refs are fewer than the
+ * table shows, or which lists pages in use as free, is reported where an update
+ * meets it; what changed is then not undone.) */
 typedef struct nut_pages_update_args {
     const int32_t *parent; /* [sequences]; NULL: itself */
     const int32_t *keep;   /* [sequences], not negative; NULL: all */

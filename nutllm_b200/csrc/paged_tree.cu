@@ -26,7 +26,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = kTreeTile;
 
-/* kRows: 16 or 64 rows of an item. */
+/* kRows: 16, 32 or 64 rows of an item. */
 template <int kRows, int DP> struct WidePlan {
     static constexpr int kPitch = DP + 4; /* floats: rows begin 4 banks apart */
     static constexpr int kWeights = kTile + 4;
@@ -505,14 +505,29 @@ template <int kRows, int DP, typename T, typename R> cudaError_t launch_wide(con
     return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, s);
 }
 
+/* Rows of an item, by how many a sequence can have: few that fill them, two blocks an SM; or more of
+ * them, between which a tile is shared.  With 16, 32 and 64, us for fp32 caches of 24 sequences up
+ * to 2,000 slots, 32 kv heads of 128 dims:
+ *   rows    16   48   64   96  128   512
+ *   16     367  604  734 1019 1315  6135
+ *   32     514  609  685  878 1087  4722
+ *   64     914  924  943 1121 1275  4515
+ * (192 rows of 8 kv heads of 64: 306, 250, 240; of 4 of 256, bf16: 1318, 872, 748). */
+template <int DP, typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cudaStream_t s) {
+    const int64_t rows = int64_t(a.max_new) * a.p.group;
+    return rows <= 48    ? launch_wide<16, DP, T, R>(a, s)
+           : rows <= 128 ? launch_wide<32, DP, T, R>(a, s)
+                         : launch_wide<64, DP, T, R>(a, s);
+}
+
 template <typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cudaStream_t s) {
-    const int D = a.p.head_dim;
-    const bool few = int64_t(a.max_new) * a.p.group <= 16;
-    if (D <= 64)
-        return few ? launch_wide<16, 64, T, R>(a, s) : launch_wide<64, 64, T, R>(a, s);
-    if (D <= 128)
-        return few ? launch_wide<16, 128, T, R>(a, s) : launch_wide<64, 128, T, R>(a, s);
-    return few ? launch_wide<16, 256, T, R>(a, s) : launch_wide<64, 256, T, R>(a, s);
+    if constexpr (sizeof(T) == 4) {
+        if (a.p.head_dim <= 64)
+            return launch_wide<64, T, R>(a, s);
+        if (a.p.head_dim <= 128)
+            return launch_wide<128, T, R>(a, s);
+    }
+    return launch_wide<256, T, R>(a, s);
 }
 
 } // namespace

@@ -361,6 +361,21 @@ def test_tree_rows_at_any_element(torch_cuda, cache, rows, D):
 
 
 @gpu
+@pytest.mark.parametrize("D,cache,rows", [(40, "f32", "f32"), (128, "f32", "f32"), (256, "f32", "f32"), (256, "f16", "f32"),
+                                          (256, "f16", "f16"), (256, "bf16", "f32"), (256, "bf16", "bf16"), (64, "f16", "f16")])
+@pytest.mark.parametrize("most", [1, 6, 7, 16, 17, 45])
+def test_tree_any_number_of_rows(torch_cuda, D, cache, rows, most):
+    """8 query heads to a kv head: 8 to 360 rows of a sequence, in the items' every size and one beyond it."""
+    torch = torch_cuda
+    pool = Pool(torch, [260, most, 97], 8, 1, D, 16, cache, seed=17)
+    pool.cache.reserve_tree(most)
+    tree = Tree(torch, pool, [most, most, most // 2], rows)
+    tree.run()
+    pool.cache.check()
+    tree.check()
+
+
+@gpu
 @pytest.mark.parametrize("cache,rows", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
 def test_tree_many_sequences_and_one_kv_head(torch_cuda, cache, rows):
     """More sequences than a block has threads; and a group of 48 heads, so that tokens lie across blocks of rows."""
