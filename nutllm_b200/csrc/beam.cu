@@ -3,14 +3,20 @@
  *   score(b, t) = scores[b] + logit[b][t] - log sum_u exp(logit[b][u])
  * The logits are read once, by warps that need no one else: each takes a run
  * of a row, 1,024 logits at a time (while the next ones are on their way to
- * shared memory), and keeps a maximum and a sum
- * of exponentials for each lane and a list in shared memory of what can be
- * among the run's n_out greatest.  The first logits set an edge that n_out of
+ * shared memory), and keeps a maximum and a sum of exponentials for each lane
+ * and a list in shared memory of what can be among the run's n_out greatest.
+ * The first logits set an edge that n_out of
  * them reach; from then on only what reaches it is listed, and a full list is
  * reduced to its n_out greatest, the last of which is the new edge.  Then a
  * block for each request joins the runs' sums in fp64, turns what they listed
  * into scores and chooses among them: an edge from its threads' maxima, what
  * reaches it ranked by counting.
+ *
+ * Instructions bound the runs where there is much to read: 256 rows of 128,000
+ * fp32 logits (123 MB without the ended beams') 38 us, 3.2 TB/s, 18 million
+ * warp instructions at 0.55 a cycle and scheduler.  The choice is a chain of
+ * barriers and round trips, 9 to 12 us.  In a persistent grid whose last block
+ * of a request chose, the requests' choices came one behind another.
  *
  * Sums: exponentials and a lane's sum in fp32, all beyond it in fp64.  Scores
  * are compared in fp64: a logit is fp32, and in an fp32 sum neighbours of

@@ -14,7 +14,9 @@
  * Sums of whole numbers do not depend on the order of the atomics, and
  * places come from prefix sums, so results do not depend on timing.
  *
- * It is a chain of round trips to L2, not bytes.
+ * It is a chain of round trips to L2, not bytes: with the copies behind it 64
+ * sequences of 1,003 slots take 16 us, 512 of 16,000 slots, a table of half a
+ * million entries, 37 us.
  */
 #include <climits>
 #include <cooperative_groups.h>
@@ -311,7 +313,10 @@ template <int kThreads> __global__ void __launch_bounds__(kThreads, 1) update_ke
 } // namespace
 
 cudaError_t pages_update(const PagesUpdate &a, cudaStream_t s) {
-    /* a small book is a chain of round trips and barriers, which few threads pass sooner */
+    /* A small book is a chain of barriers, which few threads pass sooner; a large one needs loads in
+     * flight.  A pass with 256 and with 1,024 threads a block, us: 32 sequences of 1,000 slots 14.3 and
+     * 18.2, 128 of 1,000 19.4 and 19.7, 128 of 8,000 24.3 and 21.1, 256 of 1,000 27.5 and 20.8, 512 of
+     * 16,000 78 and 37. */
     const bool small = a.sequences <= 128 && a.n_pages <= 16384 && int64_t(a.sequences) * a.max_pages <= 65536;
     const int threads = small ? 256 : 1024;
     return launch_kernel(small ? update_kernel<256> : update_kernel<1024>, dim3(kPagesCluster), threads, 0, s,
