@@ -30,21 +30,26 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = kTreeTile;
 
-/* kRows: 16, 32 or 64 rows of an item. */
+/* kRows: 16, 32 or 64 rows of an item.  Of the logits a thread forms 4 rows by
+ * 4 slots over a part of the dims, of the outputs 4 rows by 2 (or more) 4-dim
+ * pieces over a part of the slots: fewer operands out of shared memory than
+ * smaller tiles over all of them.  Neighbouring lanes have the other parts. */
 template <int kRows, int DP> struct WidePlan {
-    static constexpr int kPitch = DP + 4; /* floats: rows begin 4 banks apart */
-    static constexpr int kWeights = kTile + 4;
-    static constexpr int kFloats = kRows * kPitch + 2 * kTile * kPitch + kRows * kWeights;
-    static constexpr int kBytes = kFloats * 4;
     static constexpr int kAcross = kThreads / (kRows / 4); /* threads that share 4 rows */
-    static constexpr int kSlots = kTile / kAcross;         /* slots of a thread */
-    /* 4-dim pieces of a thread; or, with more threads than pieces, threads that
-     * share a piece, each over every kShares-th slot */
-    static constexpr int kPieces = DP / 4 > kAcross ? DP / 4 / kAcross : 1;
-    static constexpr int kShares = DP / 4 > kAcross ? 1 : kAcross / (DP / 4);
-    static constexpr int kOfRow = kThreads / kRows;        /* threads of a row's softmax */
+    static constexpr int kSplits = kAcross / (kTile / 4);  /* of the dims */
+    static constexpr int kPieces = kRows * DP / 16 / kThreads > 2 ? kRows * DP / 16 / kThreads : 2;
+    static constexpr int kEvery = DP / 4 / kPieces;        /* pieces between a thread's */
+    static constexpr int kShares = kAcross / kEvery;       /* of the slots */
+    /* floats between rows, so that 8 neighbouring lanes meet no bank twice: they are kSplits pieces
+     * of 8 / kSplits keys, and 8 / kShares pieces of kShares values */
+    static constexpr int kKeyPitch = DP + 4 * kSplits, kValuePitch = DP + (kShares > 1 ? 32 / kShares : 4);
+    static constexpr int kWeights = kRows + 4; /* of a slot */
+    static constexpr int kFloats = (kRows + kTile) * kKeyPitch + kTile * (kValuePitch + kWeights);
+    static constexpr int kBytes = kFloats * 4;
+    static constexpr int kOfRow = kThreads / kRows; /* threads of a row's softmax */
     static constexpr int kPerSm = kBytes <= 110 * 1024 ? 2 : 1;
-    static_assert(kShares * kRows * DP <= 2 * kTile * kPitch, "the shares' outputs meet in the tiles' place");
+    static_assert(kSplits >= 1 && kSplits <= 4 && kShares >= 1 && kShares <= 8, "lanes of a part lie in a warp");
+    static_assert(kShares <= 4 || kShares == 4 * kPieces, "each lane writes a row, or a piece of it");
 };
 
 /* Two fp32 numbers, and two products added to two sums in one instruction. */
@@ -89,8 +94,8 @@ template <int kRows, int DP, typename T, typename R>
 __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_kernel(const __grid_constant__ PagedTree a) {
     using W = WidePlan<kRows, DP>;
     extern __shared__ float4 smem_raw[];
-    float *queries = reinterpret_cast<float *>(smem_raw), *keys = queries + kRows * W::kPitch,
-          *values = keys + kTile * W::kPitch, *weights = values + kTile * W::kPitch;
+    float *queries = reinterpret_cast<float *>(smem_raw), *keys = queries + kRows * W::kKeyPitch,
+          *values = keys + kTile * W::kKeyPitch, *weights = values + kTile * W::kValuePitch; /* [slot][row] */
     __shared__ int64_t places[2][kTile]; /* elements from the pool's start, -1: no such slot */
     __shared__ float maxima[kRows], sums[kRows], factors[kRows];
     const PagedPool &p = a.p;
@@ -101,8 +106,10 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
     tree_blind_rows<R>(a, tid, kThreads);
     const int start = cursor.pos;
     const int r0 = tid / W::kAcross * 4, c0 = tid % W::kAcross; /* of the products */
-    const int piece0 = c0 % (DP / 4), share0 = W::kShares > 1 ? c0 / (DP / 4) : 0;
-    const int soft_row = tid / W::kOfRow, soft_at = tid % W::kOfRow;
+    const int split = c0 % W::kSplits, slot0 = c0 / W::kSplits;
+    const int share0 = c0 % W::kShares, piece0 = c0 / W::kShares;
+    constexpr int kOfWarp = 32 / W::kOfRow; /* rows of a warp's softmax; rows of neighbouring lanes differ */
+    const int soft_row = tid / 32 * kOfWarp + tid % kOfWarp, soft_at = tid % 32 / kOfWarp;
     const float unit = a.scale * kTreeLog2e;
     int4 join = make_int4(0, 0, 0, 0);
 
@@ -121,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 for (int j = 0; j < 4; j++)
                     v[j] = to_float(q[j]);
             }
-            *reinterpret_cast<float4 *>(queries + r * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(queries + r * W::kKeyPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
         }
         if (tid < kRows) {
             maxima[tid] = -INFINITY;
@@ -148,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 places[tile & 1][tid] = at;
             }
         };
-        const auto fetch = [&](int tile, const void *pool, float *to) {
+        const auto fetch = [&](int tile, const void *pool, float *to, int pitch) {
             if (tile < x.tile1)
                 for (int i = tid; i < kTile * (DP / 4); i += kThreads) {
                     const int t = i / (DP / 4), d = i % (DP / 4) * 4;
@@ -156,81 +163,108 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                     const bool there = at >= 0 && d < D;
                     const T *from = static_cast<const T *>(pool) + (there ? at + d : 0);
                     if constexpr (sizeof(T) == 4) {
-                        copy_piece(to + t * W::kPitch + d, from, there);
+                        copy_piece(to + t * pitch + d, from, there);
                     } else {
                         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                         if (there)
                             load_four(from, v);
-                        *reinterpret_cast<float4 *>(to + t * W::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4 *>(to + t * pitch + d) = make_float4(v[0], v[1], v[2], v[3]);
                     }
                 }
             copies_done();
         };
         find(x.tile0);
         __syncthreads();
-        fetch(x.tile0, p.keys, keys);
-        fetch(x.tile0, p.values, values);
+        fetch(x.tile0, p.keys, keys, W::kKeyPitch);
+        fetch(x.tile0, p.values, values, W::kValuePitch);
         for (int tile = x.tile0; tile < x.tile1; tile++) {
             const int t0 = tile * kTile;
             find(tile + 1);
             await_copies(); /* the keys */
             __syncthreads();
-            Two z[4][W::kSlots];
+            Two z2[4][4];
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int k = 0; k < W::kSlots; k++)
-                    z[r][k] = 0;
-#pragma unroll 4
-            for (int d = 0; d < DP; d += 4) {
+                for (int k = 0; k < 4; k++)
+                    z2[r][k] = 0;
+#pragma unroll 2
+            for (int d = split * 4; d < DP; d += 4 * W::kSplits) {
                 ulonglong2 q[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    q[r] = *reinterpret_cast<const ulonglong2 *>(queries + (r0 + r) * W::kPitch + d);
+                    q[r] = *reinterpret_cast<const ulonglong2 *>(queries + (r0 + r) * W::kKeyPitch + d);
 #pragma unroll
-                for (int k = 0; k < W::kSlots; k++) {
-                    const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(keys + (c0 + k * W::kAcross) * W::kPitch + d);
+                for (int k = 0; k < 4; k++) {
+                    const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(keys + (slot0 + k * (kTile / 4)) * W::kKeyPitch + d);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        add_products(z[r][k], q[r].x, c.x);
-                        add_products(z[r][k], q[r].y, c.y);
+                        add_products(z2[r][k], q[r].x, c.x);
+                        add_products(z2[r][k], q[r].y, c.y);
                     }
                 }
             }
+            /* the dims' parts meet: of 4 rows a lane keeps 4 / kSplits */
+            constexpr int kKept = 4 / W::kSplits;
+            float z[4][4];
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int k = 0; k < W::kSlots; k++) {
-                    const float2 v = parts_of(z[r][k]);
-                    weights[(r0 + r) * W::kWeights + c0 + k * W::kAcross] = (v.x + v.y) * unit;
+                for (int k = 0; k < 4; k++) {
+                    const float2 v = parts_of(z2[r][k]);
+                    z[r][k] = (v.x + v.y) * unit;
                 }
+#pragma unroll
+            for (int e = W::kSplits / 2, left = 4; e > 0; e >>= 1) {
+                left /= 2;
+#pragma unroll
+                for (int r = 0; r < left; r++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const bool upper = split & e;
+                        const float kept = upper ? z[r + left][k] : z[r][k], sent = upper ? z[r][k] : z[r + left][k];
+                        z[r][k] = kept + __shfl_xor_sync(0xffffffffu, sent, e);
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float *to = weights + (slot0 + k * (kTile / 4)) * W::kWeights + r0 + split * kKept;
+                if constexpr (kKept == 4)
+                    *reinterpret_cast<float4 *>(to) = make_float4(z[0][k], z[1][k], z[2][k], z[3][k]);
+                else if constexpr (kKept == 2)
+                    *reinterpret_cast<float2 *>(to) = make_float2(z[0][k], z[1][k]);
+                else
+                    *to = z[0][k];
+            }
             __syncthreads();
-            fetch(tile + 1, p.keys, keys);
+            fetch(tile + 1, p.keys, keys, W::kKeyPitch);
 
-            /* softmax: kOfRow threads a row, 64 / kOfRow neighbouring slots each */
+            /* softmax: kOfRow lanes a row, every kOfRow-th slot each */
             constexpr int kEach = kTile / W::kOfRow;
-            const int s0 = soft_at * kEach;
-            float *own = weights + soft_row * W::kWeights + s0;
+            float *own = weights + soft_at * W::kWeights + soft_row;
             float v[kEach], top = -INFINITY;
             {
-                uint32_t sees = 0;
-                const int base = t0 + s0 - x.span.prefix;
+                uint32_t sees[2] = {0, 0}; /* of 32 slots from this thread's first on, and of 32 behind them */
+                const int base = t0 - x.span.prefix;
                 if (soft_row < x.rows) {
-                    if (base <= -kEach) {
-                        sees = ~0u;
+                    if (base <= -kTile) {
+                        sees[0] = sees[1] = ~0u;
                     } else {
                         const int node = tree_node(a, x.first_row + soft_row);
-                        sees = tree_sees(a.mask + (int64_t(x.span.row0) + node) * a.mask_words, base, x.span.n);
+                        const uint32_t *words = a.mask + (int64_t(x.span.row0) + node) * a.mask_words;
+                        sees[0] = tree_sees(words, base + soft_at, x.span.n);
+                        sees[1] = tree_sees(words, base + soft_at + 32, x.span.n);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < kEach; j++) {
-                    v[j] = ((sees >> j) & 1) && places[tile & 1][s0 + j] >= 0 ? own[j] : -INFINITY;
+                    const int t = j * W::kOfRow;
+                    v[j] = ((sees[t / 32] >> (t % 32)) & 1) && places[tile & 1][soft_at + t] >= 0 ? own[t * W::kWeights] : -INFINITY;
                     top = fmaxf(top, v[j]);
                 }
             }
 #pragma unroll
-            for (int e = W::kOfRow / 2; e > 0; e >>= 1)
+            for (int e = 16; e >= kOfWarp; e >>= 1)
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
             const float before = maxima[soft_row], next = fmaxf(before, top);
             const float from = next == -INFINITY ? 0.0f : next;
@@ -238,11 +272,11 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 #pragma unroll
             for (int j = 0; j < kEach; j++) {
                 const float w = exp2f(v[j] - from);
-                own[j] = w;
+                own[j * W::kOfRow * W::kWeights] = w;
                 sum += w;
             }
 #pragma unroll
-            for (int e = W::kOfRow / 2; e > 0; e >>= 1)
+            for (int e = 16; e >= kOfWarp; e >>= 1)
                 sum += __shfl_xor_sync(0xffffffffu, sum, e);
             if (soft_at == 0) {
                 const float keep = before == next ? 1.0f : exp2f(before - next);
@@ -267,16 +301,12 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             const auto multiply = [&](auto drafted) {
 #pragma unroll 4
                 for (int t = share0; t < kTile; t += W::kShares) {
-                    Two w[4];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float v = weights[(r0 + r) * W::kWeights + t];
-                        w[r] = two_of(v, v);
-                    }
+                    const float4 of = *reinterpret_cast<const float4 *>(weights + t * W::kWeights + r0);
+                    const Two w[4] = {two_of(of.x, of.x), two_of(of.y, of.y), two_of(of.z, of.z), two_of(of.w, of.w)};
 #pragma unroll
                     for (int k = 0; k < W::kPieces; k++) {
                         const ulonglong2 c =
-                            *reinterpret_cast<const ulonglong2 *>(values + t * W::kPitch + (piece0 + k * W::kAcross) * 4);
+                            *reinterpret_cast<const ulonglong2 *>(values + t * W::kValuePitch + (piece0 + k * W::kEvery) * 4);
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             const bool none = decltype(drafted)::value && w[r] == 0;
@@ -291,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             else
                 multiply(std::false_type());
             __syncthreads();
-            fetch(tile + 1, p.values, values);
+            fetch(tile + 1, p.values, values, W::kValuePitch);
         }
         float o[4][W::kPieces][4];
 #pragma unroll
@@ -304,26 +334,15 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                     o[r][k][2 * j] = v.x;
                     o[r][k][2 * j + 1] = v.y;
                 }
-        if constexpr (W::kShares > 1) { /* the shares meet */
-            float *room = keys;
-            if (share0 > 0)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    *reinterpret_cast<float4 *>(room + (share0 * kRows + r0 + r) * DP + piece0 * 4) =
-                        make_float4(o[r][0][0], o[r][0][1], o[r][0][2], o[r][0][3]);
-            __syncthreads();
-            if (share0 == 0)
+        for (int e = W::kShares / 2; e > 0; e >>= 1) /* the slots' parts meet */
 #pragma unroll
-                for (int s = 1; s < W::kShares; s++)
+            for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float4 v = *reinterpret_cast<const float4 *>(room + (s * kRows + r0 + r) * DP + piece0 * 4);
-                        o[r][0][0] += v.x;
-                        o[r][0][1] += v.y;
-                        o[r][0][2] += v.z;
-                        o[r][0][3] += v.w;
-                    }
-        }
+                for (int k = 0; k < W::kPieces; k++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[r][k][j] += __shfl_xor_sync(0xffffffffu, o[r][k][j], e);
 
         const bool whole = x.whole();
         const TreePart part = tree_part(a, blockIdx.x, x.first <= start ? 0 : 1, x.rows);
@@ -343,23 +362,27 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int f = r0 + r;
-            if (f >= x.rows || share0 > 0)
+            if (f >= x.rows)
                 break;
+            if ((r ^ share0) & ((W::kShares < 4 ? W::kShares : 4) - 1)) /* another lane's */
+                continue;
             int64_t row;
             int h;
             tree_row(a, x.span.row0, x.head, x.first_row + f, row, h);
             const float inv = !whole ? 1.0f : sums[f] == 0.0f ? 0.0f : 1.0f / sums[f];
 #pragma unroll
             for (int k = 0; k < W::kPieces; k++) {
-                const int d = (piece0 + k * W::kAcross) * 4;
+                const int d = (piece0 + k * W::kEvery) * 4;
                 if (d >= D)
                     break;
+                if (W::kShares > 4 && k != share0 / 4)
+                    continue;
+                if (whole) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (whole)
+                    for (int j = 0; j < 4; j++)
                         static_cast<R *>(a.out)[row * a.out_stride + int64_t(h) * D + d + j] = output_of<R>(o[r][k][j] * inv);
-                    else
-                        part.out[int64_t(f) * D + d + j] = o[r][k][j];
+                } else {
+                    *reinterpret_cast<float4 *>(part.out + int64_t(f) * D + d) = make_float4(o[r][k][0], o[r][k][1], o[r][k][2], o[r][k][3]);
                 }
             }
         }
