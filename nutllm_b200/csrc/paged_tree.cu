@@ -7,15 +7,18 @@
  * over the slots a row sees, in one pass with a running maximum and sum.
  *
  * A tile is 64 slots, read once for all of an item's rows, in fp32 in shared
- * memory; 256 threads form the products as 4 rows by slots, then 4 rows by
- * dims.  The next tile's keys are on their way from when the logits are
- * formed, its values from when the outputs are.  The operands' way out of
- * shared memory bounds it, and the four barriers of a tile with two blocks an
- * SM: 4 fp32 caches up to 1,000 slots, 32 kv heads of 128 dims, 12 tokens (84
- * MB) 60 us, 1.4 TB/s, 0.40 instructions a cycle and scheduler.  Without the
- * next tile's prefetch it was 108 us.  16-bit caches take it only where the
- * tensor cores' kernel has no form, head_dim above 128: the batch of that
- * kernel's comment was 865 us here.
+ * memory; 256 threads form the products, then the softmax, then the outputs.
+ * The next tile's keys are on their way from when the logits are formed, its
+ * values from when the outputs are, its pages' numbers a tile before that.
+ * What bounds it is that these steps follow one another behind barriers, with
+ * two blocks an SM to fill the gaps: of some 11,500 cycles a tile the logits
+ * take 3,500, the outputs 2,600 and the softmax 2,700, where FFMA alone would
+ * need 2,050.  4 fp32 caches up to 1,000 slots, 32 kv heads of 128 dims, 12
+ * tokens (84 MB) 56 us, 1.5 TB/s.  Without the prefetch it was 108 us; a bulk
+ * copy a row in place of 16 bytes a thread made no difference at 128 dims and
+ * took 29 us in place of 23 at 64.  16-bit caches take it only where the tensor
+ * cores' kernel has no form, head_dim above 128: the batch of that kernel's
+ * comment was 865 us in a first form of this one.
  */
 #include <algorithm>
 #include <cstdint>
@@ -141,16 +144,25 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
             for (int k = 0; k < W::kPieces; k++)
                 o2[r][k][0] = o2[r][k][1] = 0;
 
-        const auto find = [&](int tile) { /* where a tile's slots lie */
+        /* Threads 0 to 63 have a slot of a tile each: its page is looked up a tile before its place
+         * is needed. */
+        const auto look = [&](int tile) {
+            const int t = tile * kTile + tid;
+            return tid < kTile && tile < x.tile1 && t < x.span.length
+                       ? p.table[int64_t(x.sequence) * p.max_pages + int((uint64_t(unsigned(t)) * a.page_magic) >> a.page_shift)]
+                       : -1;
+        };
+        const auto place = [&](int tile, int page) {
             if (tid < kTile && tile < x.tile1) {
                 const int t = tile * kTile + tid;
                 int64_t at = -1;
                 if (t < x.span.length) {
                     const int j = int((uint64_t(unsigned(t)) * a.page_magic) >> a.page_shift);
-                    const int page = checked_page(p, x.sequence, j);
-                    if (page >= 0)
+                    if (unsigned(page) < unsigned(p.n_pages))
                         at = int64_t(page) * p.page_stride + int64_t(x.head) * p.head_stride +
                              int64_t(t - j * p.page_size) * p.slot_stride;
+                    else
+                        paged_fail(p, kPagedBadPage);
                 }
                 places[tile & 1][tid] = at;
             }
@@ -173,13 +185,15 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                 }
             copies_done();
         };
-        find(x.tile0);
+        place(x.tile0, look(x.tile0));
+        int page = look(x.tile0 + 1);
         __syncthreads();
         fetch(x.tile0, p.keys, keys, W::kKeyPitch);
         fetch(x.tile0, p.values, values, W::kValuePitch);
         for (int tile = x.tile0; tile < x.tile1; tile++) {
             const int t0 = tile * kTile;
-            find(tile + 1);
+            place(tile + 1, page);
+            page = look(tile + 2);
             await_copies(); /* the keys */
             __syncthreads();
             Two z2[4][4];
@@ -537,10 +551,10 @@ template <int kRows, int DP, typename T, typename R> cudaError_t launch_wide(con
  * them, between which a tile is shared.  With 16, 32 and 64, us for fp32 caches of 24 sequences up
  * to 2,000 slots, 32 kv heads of 128 dims:
  *   rows    16   48   64   96  128   512
- *   16     367  604  734 1019 1315  6135
- *   32     514  609  685  878 1087  4722
- *   64     914  924  943 1121 1275  4515
- * (192 rows of 8 kv heads of 64: 306, 250, 240; of 4 of 256, bf16: 1318, 872, 748). */
+ *   16     336  554  672  934 1203  5726
+ *   32     493  578  648  833 1029  4395
+ *   64     890  905  921 1095 1251  4384
+ * (512 rows of 8 kv heads of 64: 877, 659, 586; of 4 of 256, bf16: 3492, 2161, 1627). */
 template <int DP, typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cudaStream_t s) {
     const int64_t rows = int64_t(a.max_new) * a.p.group;
     return rows <= 48    ? launch_wide<16, DP, T, R>(a, s)
