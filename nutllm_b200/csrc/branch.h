@@ -14,7 +14,7 @@ enum PagesError {
     kPagesNoneFree = 8
 };
 
-constexpr int kPagesCluster = 8, kPagesMostWarps = kPagesCluster * 32;
+constexpr int kPagesMostWarps = 16 * 32; /* of an update */
 
 struct PagesUpdate {
     int32_t *table, *lengths, *refs, *free_pages, *free_count;

@@ -1,6 +1,6 @@
 /* Pages of branching sequences (nut_pages_update).
  *
- * One cluster of 8 blocks does all of an update in three steps, with a
+ * One cluster of blocks does all of an update in three steps, with a
  * barrier of the cluster between them:
  *   1  each sequence's kept pages are staged; every entry of the table that
  *      changes takes a holder from its old page and gives one to its new
@@ -16,7 +16,7 @@
  *
  * It is a chain of round trips to L2, not bytes: with the copies behind it 64
  * sequences of 1,003 slots take 16 us, 512 of 16,000 slots, a table of half a
- * million entries, 37 us.
+ * million entries, 27 us.
  */
 #include <climits>
 #include <cooperative_groups.h>
@@ -60,8 +60,8 @@ template <int kWarpsABlock> __device__ __forceinline__ int64_t before_in_block(i
     return before;
 }
 
-template <int kThreads> __global__ void __launch_bounds__(kThreads, 1) update_kernel(const __grid_constant__ PagesUpdate a) {
-    constexpr int kWarpsABlock = kThreads / 32, kWarps = kPagesCluster * kWarpsABlock;
+template <int kThreads, int kBlocks> __global__ void __launch_bounds__(kThreads, 1) update_kernel(const __grid_constant__ PagesUpdate a) {
+    constexpr int kWarpsABlock = kThreads / 32, kWarps = kBlocks * kWarpsABlock;
     __shared__ int64_t sums[kWarpsABlock];
     __shared__ int places[kThreads];
     __shared__ uint8_t copied[kThreads];
@@ -314,13 +314,25 @@ template <int kThreads> __global__ void __launch_bounds__(kThreads, 1) update_ke
 
 cudaError_t pages_update(const PagesUpdate &a, cudaStream_t s) {
     /* A small book is a chain of barriers, which few threads pass sooner; a large one needs loads in
-     * flight.  A pass with 256 and with 1,024 threads a block, us: 32 sequences of 1,000 slots 14.3 and
-     * 18.2, 128 of 1,000 19.4 and 19.7, 128 of 8,000 24.3 and 21.1, 256 of 1,000 27.5 and 20.8, 512 of
-     * 16,000 78 and 37. */
+     * flight, and takes the most blocks that a cluster can have.  A pass with 8 blocks of 256, 8 of 1,024 and
+     * 16 of 1,024 threads, us: 128 sequences of 1,000 slots 19.4, 19.7, -; 128 of 8,000 24.3, 21.1, 20.6; 256 of
+     * 1,000 27.5, 20.8, 19.8; 512 of 16,000 78, 37, 30; 32 of 1,000 14.3, 18.2, -. */
     const bool small = a.sequences <= 128 && a.n_pages <= 16384 && int64_t(a.sequences) * a.max_pages <= 65536;
-    const int threads = small ? 256 : 1024;
-    return launch_kernel(small ? update_kernel<256> : update_kernel<1024>, dim3(kPagesCluster), threads, 0, s,
-                         kPagesCluster, a);
+    if (small)
+        return launch_kernel(update_kernel<256, 8>, dim3(8), 256, 0, s, 8, a);
+    const auto kernel = update_kernel<1024, 16>;
+    static bool set[kMaxDevices] = {};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    if (!set[device % kMaxDevices]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess)
+            return e;
+        set[device % kMaxDevices] = true;
+    }
+    return launch_kernel(kernel, dim3(16), 1024, 0, s, 16, a);
 }
 
 } // namespace nut
