@@ -1,6 +1,7 @@
 #pragma once
 /* What the C ABI's entry points share (paged_host.cu, branch_host.cu): C++
  * failures as status codes, the handle's device, and workspaces. */
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <stdexcept>
@@ -81,6 +82,14 @@ inline cudaMemPool_t workspace_pool(int device) {
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+/* Arrays of 32-bit words; NULL is aligned. */
+inline bool aligned4(std::initializer_list<const void *> arrays) {
+    for (const void *p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) & 3)
+            return false;
+    return true;
+}
 
 } // namespace abi
 } // namespace nut

@@ -69,6 +69,8 @@ nut_status nut_pages_create(const nut_pages_view *view, int device, nut_pages **
         const nut_pages_view &v = *view;
         if (!v.table || !v.lengths || !v.refs || !v.free_pages || !v.free_count)
             refuse(NUT_INVALID_ARGUMENT, "pages", "null table, lengths, refs, free_pages or free_count");
+        if (!aligned4({v.table, v.lengths, v.refs, v.free_pages, v.free_count}))
+            refuse(NUT_INVALID_ARGUMENT, "pages", "arrays must be multiples of their elements");
         if (v.sequences <= 0 || v.max_pages <= 0 || v.n_pages <= 0 || v.page_size <= 0)
             refuse(NUT_INVALID_ARGUMENT, "pages", "invalid dimensions");
         if (v.sequences > kMostRows || v.n_pages > INT_MAX - 4096 || v.page_size > (1 << 24) ||
@@ -154,6 +156,8 @@ nut_status nut_pages_update(nut_pages *h, const nut_pages_update_args *args, voi
             refuse(NUT_INVALID_ARGUMENT, "pages", "copy_from, copy_to and copy_slots go together");
         if (!lists && g.add)
             refuse(NUT_INVALID_ARGUMENT, "pages", "add needs the copy lists");
+        if (!aligned4({g.parent, g.keep, g.add, g.copy_from, g.copy_to, g.copy_slots}))
+            refuse(NUT_INVALID_ARGUMENT, "pages", "arrays must be multiples of their elements");
         nut::PagesUpdate u = h->u;
         u.parent = g.parent;
         u.keep = g.keep;
@@ -239,8 +243,13 @@ nut_status nut_beam_select(nut_beam *h, const nut_beam_select_args *args, void *
             refuse(NUT_INVALID_ARGUMENT, "beam", "eos outside the vocabulary");
         if (g.finished && g.eos < 0)
             refuse(NUT_INVALID_ARGUMENT, "beam", "finished beams need eos");
+        if (!aligned4({g.scores, g.out_scores, g.out_rows, g.out_tokens}))
+            refuse(NUT_INVALID_ARGUMENT, "beam", "arrays must be multiples of their elements");
         if (g.sequences == 0)
             return;
+        /* a request's outputs are written while others' beams are still read */
+        if (b.n_out != b.beams && (g.out_scores == g.scores || (g.finished && g.out_finished == g.finished)))
+            refuse(NUT_INVALID_ARGUMENT, "beam", "outputs in the inputs' place need n_out to be beams");
         b.logits = g.logits;
         b.stride = g.logits_stride ? g.logits_stride : b.vocab;
         b.scores = g.scores;

@@ -350,6 +350,8 @@ nut_status nut_paged_append_at(nut_paged *h, const nut_paged_append_args *args, 
     return guarded([&] {
                if (!row_position)
                    raise(NUT_INVALID_ARGUMENT, "null row_position");
+               if (!aligned4({row_position}))
+                   raise(NUT_INVALID_ARGUMENT, "row_position must be a multiple of its elements");
            }) == NUT_OK
                ? append(h, args, row_position, stream)
                : NUT_INVALID_ARGUMENT;
@@ -546,6 +548,12 @@ nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *arg
         if (!g.q || !g.out || !g.starts || !g.mask)
             raise(NUT_INVALID_ARGUMENT, "null q, out, starts or mask");
         check_row_type(*h, g.type);
+        const int64_t element = g.type == NUT_F32 ? 4 : 2;
+        if (!aligned4({g.starts, g.mask, g.lse}) || reinterpret_cast<uintptr_t>(g.q) % element != 0 ||
+            reinterpret_cast<uintptr_t>(g.out) % element != 0)
+            raise(NUT_INVALID_ARGUMENT, "arrays must be multiples of their elements");
+        if (g.q == g.out)
+            raise(NUT_INVALID_ARGUMENT, "out must not be q: rows are read again while others are written");
         if (g.rows < 0 || g.max_new < 0)
             raise(NUT_INVALID_ARGUMENT, "negative row count");
         if (g.max_new > h->tree_max)
@@ -583,7 +591,6 @@ nut_status nut_paged_tree_attention(nut_paged *h, const nut_paged_tree_args *arg
         a.rows = int(g.rows);
         a.max_new = int(g.max_new);
         a.type = g.type;
-        const int64_t element = g.type == NUT_F32 ? 4 : 2;
         a.aligned = aligned16(g.q) && aligned16(g.out) && a.q_stride * element % 16 == 0 && a.out_stride * element % 16 == 0;
         a.scale = g.scale != 0.0f ? g.scale : float(1.0 / std::sqrt(double(p.head_dim)));
         a.partial = h->tree_partial;
@@ -602,6 +609,8 @@ nut_status nut_paged_compact(nut_paged *h, const nut_paged_compact_args *args, v
         const nut_paged_compact_args &g = *args;
         if (!g.starts || !g.new_lengths || (!g.accepted && g.n_accepted != 0))
             raise(NUT_INVALID_ARGUMENT, "null starts, accepted or new_lengths");
+        if (!aligned4({g.starts, g.accepted, g.new_lengths, g.positions, g.weights}))
+            raise(NUT_INVALID_ARGUMENT, "arrays must be multiples of their elements");
         if (g.n_accepted < 0)
             raise(NUT_INVALID_ARGUMENT, "negative n_accepted");
         if (g.n_accepted > NUT_TREE_MAX)
@@ -631,6 +640,8 @@ nut_status nut_paged_copy(nut_paged *h, const nut_paged_copy_args *args, void *s
             return;
         if (!g.source || !g.target)
             raise(NUT_INVALID_ARGUMENT, "null source or target");
+        if (!aligned4({g.source, g.target, g.slots}))
+            raise(NUT_INVALID_ARGUMENT, "arrays must be multiples of their elements");
         if (g.count > INT_MAX)
             raise(NUT_LENGTH_ERROR, "too many pages");
         nut::PagedCopy a{};

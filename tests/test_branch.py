@@ -1094,6 +1094,41 @@ def test_beam_select_refusals(torch_cuda):
     beam.select(**(good | dict(sequences=0)))
 
 
+@gpu
+def test_arrays_in_the_wrong_place_are_refused(torch_cuda):
+    """Between elements, or where a call would write what it still reads."""
+    torch = torch_cuda
+    buf = torch.zeros(8192, device="cuda")
+    at = buf.data_ptr()
+    pool = Pool(torch, [50], 4, 2, 64, 16, "f16")
+    pool.cache.reserve_tree(8)
+    tree = dict(q=at, out=at + 16384, starts=at, mask=at, rows=5, max_new=5, mask_words=1, dtype=nb.F16, lse=at + 8192)
+    for more in (dict(q=at + 1), dict(out=at + 1), dict(starts=at + 2), dict(mask=at + 1), dict(lse=at + 2), dict(out=at),
+                 dict(dtype=nb.F32, q=at + 2), dict(dtype=nb.F32, out=at + 2)):
+        with pytest.raises(ValueError):
+            pool.cache.tree_attention(**(tree | more))
+    for name in ("source", "target", "slots"):
+        with pytest.raises(ValueError, match="multiples"):
+            pool.cache.copy_pages(count=1, **(dict(source=at, target=at) | {name: at + 2}))
+    for name in ("starts", "accepted", "new_lengths", "positions", "weights"):
+        with pytest.raises(ValueError, match="multiples"):
+            pool.cache.compact(n_accepted=1, **(dict(starts=at, accepted=at, new_lengths=at) | {name: at + 2}))
+    book = nb.PageBook(at, at + 4096, at + 8192, at + 12288, at + 16384, sequences=4, max_pages=8, n_pages=30, page_size=16)
+    for name in ("parent", "keep", "add", "copy_from", "copy_to", "copy_slots"):
+        with pytest.raises(ValueError, match="multiples"):
+            book.update(**(dict(copy_from=at, copy_to=at, copy_slots=at) | {name: at + 2}))
+    with pytest.raises(ValueError, match="multiples"):
+        nb.PageBook(at + 2, at, at, at, at, sequences=4, max_pages=8, n_pages=30, page_size=16)
+    beam = nb.BeamSearch(2, 2, 100, 4)
+    good = dict(logits=at, scores=at, out_scores=at + 4096, out_rows=at + 8192, out_tokens=at + 12288)
+    for more in (dict(scores=at + 2), dict(out_scores=at + 1), dict(out_rows=at + 2), dict(out_tokens=at + 3), dict(out_scores=at),
+                 dict(finished=at, out_finished=at, eos=1)):
+        with pytest.raises(ValueError):
+            beam.select(**(good | more))
+    torch.cuda.synchronize()
+    assert not bool(buf.any())
+
+
 # ---------------------------------------------------------------------------
 # argument checks that need no GPU
 
