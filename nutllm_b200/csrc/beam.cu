@@ -205,11 +205,18 @@ __global__ void __launch_bounds__(kRunWarps * 32) runs_kernel(const __grid_const
             top = most;
         }
         const float from = top == -INFINITY ? 0.0f : top;
-        float more[2] = {0.0f, 0.0f};
+        Two more2 = two_of(0.0f, 0.0f);
+        const Two less = two_of(-from, -from), scale = two_of(kLog2e, kLog2e);
 #pragma unroll
-        for (int i = 0; i < kEach; i++)
-            more[i & 1] += power2((v[i] - from) * kLog2e);
-        sum += more[0] + more[1];
+        for (int i = 0; i < kEach; i += 2) { /* (v - from) log2 e */
+            Two x = two_of(v[i], v[i + 1]);
+            asm("add.rn.f32x2 %0, %0, %1;\n" : "+l"(x) : "l"(less));
+            asm("mul.rn.f32x2 %0, %0, %1;\n" : "+l"(x) : "l"(scale));
+            const float2 z = parts_of(x);
+            asm("add.rn.f32x2 %0, %0, %1;\n" : "+l"(more2) : "l"(two_of(power2(z.x), power2(z.y))));
+        }
+        const float2 more = parts_of(more2);
+        sum += more.x + more.y;
 
         /* what reaches the edge, by value first */
         const uint32_t edge_bits = uint32_t(edge >> 32);

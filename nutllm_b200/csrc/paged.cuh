@@ -118,4 +118,17 @@ __device__ __forceinline__ float finite_key(float v) {
     return v != v ? 0.0f : fminf(fmaxf(v, -3.402823466e38f), 3.402823466e38f);
 }
 
+/* Two fp32 numbers for instructions that take both. */
+using Two = unsigned long long;
+__device__ __forceinline__ Two two_of(float a, float b) {
+    Two v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 parts_of(Two v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+
 } // namespace nut

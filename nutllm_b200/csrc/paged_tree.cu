@@ -55,18 +55,7 @@ template <int kRows, int DP> struct WidePlan {
     static_assert(kShares <= 4 || kShares == 4 * kPieces, "each lane writes a row, or a piece of it");
 };
 
-/* Two fp32 numbers, and two products added to two sums in one instruction. */
-using Two = unsigned long long;
-__device__ __forceinline__ Two two_of(float a, float b) {
-    Two v;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-__device__ __forceinline__ float2 parts_of(Two v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
+/* Two products added to two sums in one instruction. */
 __device__ __forceinline__ void add_products(Two &sum, Two a, Two b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(sum) : "l"(a), "l"(b));
 }
