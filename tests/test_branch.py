@@ -1031,6 +1031,22 @@ def test_beam_select_rows_of_the_lowest_value(torch_cuda, kind, V):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [3, 40])
+def test_beam_select_nan_among_ordinary_logits(torch_cuda, kind, n):
+    """NaN counts as -infinity in the sums too, a logit here and there, and beside +infinity."""
+    torch = torch_cuda
+    g = torch.Generator().manual_seed(21)
+    logits = (torch.randn(4, 5003, generator=g) * 3).to(dtypes(torch)[kind])
+    logits[0, 5::97] = math.nan
+    logits[1, 4099] = math.nan
+    logits[2, 17], logits[2, 18], logits[2, 4999] = math.inf, math.nan, math.nan
+    logits[3, :5000] = math.nan
+    scores = torch.tensor([[-1.0, -1.5, -0.5, -2.0]])
+    same_beams(run_beams(torch, logits.cuda(), scores.cuda(), n), plain_beams(torch, logits, scores, None, -1, n))
+
+
+@gpu
 def test_beam_select_finished_beams_and_too_few_candidates(torch_cuda):
     torch = torch_cuda
     g = torch.Generator().manual_seed(3)
