@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(kRunWarps * 32) runs_kernel(const __grid_const
             continue;
         const float edge_value = edge_bits < 0x007fffffu ? -INFINITY : float_of(edge_bits);
         uint32_t hits = 0;
-        if (any)
+        if (any && edge_value == -INFINITY)
+            hits = ~0u; /* every logit reaches it, NaN too, which counts as -infinity */
+        else if (any)
 #pragma unroll
             for (int i = 0; i < kEach; i++)
                 hits |= uint32_t(v[i] >= edge_value) << i;
