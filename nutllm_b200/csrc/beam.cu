@@ -306,15 +306,22 @@ struct Beam {
     int ended;
 };
 
-/* Entry i of what beam b's runs listed, as a candidate; false: there is none. */
-__device__ __forceinline__ bool candidate(const BeamSelect &a, const Beam *beams, int b, int i, Key key, Candidate &c) {
+/* Entry `rank` of what run `run` of beam b listed, as a candidate; false: there is none.
+ * An ended beam has one.  All tokens of a beam whose score is -infinity (or NaN)
+ * tie, and the lowest are first: those, not the greatest logits that its runs
+ * listed. */
+__device__ __forceinline__ bool candidate(const BeamSelect &a, const Beam *beams, int b, int run, int rank, Key key,
+                                          Candidate &c) {
     const Beam beam = beams[b];
-    if (beam.ended ? i != 0 : key == 0)
+    const bool none = !(beam.score > -INFINITY);
+    if (beam.ended ? run != 0 || rank != 0 : none ? run != 0 || rank >= a.vocab : key == 0)
         return false;
-    double score = beam.score;
+    double score = none ? double(-INFINITY) : double(beam.score);
     c.place = static_cast<unsigned long long>(b) << 32;
     if (beam.ended) {
         c.place += a.eos;
+    } else if (none) {
+        c.place += rank;
     } else {
         score += double(float_of(uint32_t(key >> 32))) - beam.lse;
         c.place += argmax_index(key);
@@ -369,7 +376,7 @@ __device__ __forceinline__ void for_candidates(const BeamSelect &a, const Beam *
             for (int k = 0; k < kBatch; k++) {
                 const int list = l0 + k * step, b = list / a.runs;
                 Candidate c;
-                if (list < lists && candidate(a, beams, b, (list - b * a.runs) | rank, keys[k], c))
+                if (list < lists && candidate(a, beams, b, list - b * a.runs, rank, keys[k], c))
                     f(c);
             }
         }

@@ -48,3 +48,18 @@ def test_beam_select_nan_are_candidates(torch_cuda, kind, V, n, case):
     got = run_beams(torch, logits.cuda(), scores.cuda(), n, ended.to(torch.uint8).cuda() if ended is not None else None,
                     1 if ended is not None else -1)
     same_beams(got, plain_beams(torch, logits, scores, ended, 1 if ended is not None else -1, n))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("low", [-math.inf, math.nan])
+@pytest.mark.parametrize("V", [5, 3000, 70000])
+def test_beam_select_ties_of_beams_without_a_score(torch_cuda, kind, low, V):
+    """All tokens of a beam whose score is -infinity tie, whatever their logits: the lowest ones are chosen."""
+    torch = torch_cuda
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(8, V, generator=g).to(dtypes(torch)[kind])
+    scores = torch.tensor([[-1.0, low, -2.0, low], [low, low, low, low]])
+    ended = torch.tensor([[1, 0, 1, 0], [0, 1, 0, 0]])
+    got = run_beams(torch, logits.cuda(), scores.cuda(), 12, ended.to(torch.uint8).cuda(), 4)
+    same_beams(got, plain_beams(torch, logits, scores, ended, 4, 12))
