@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 #pragma unroll
             for (int j = 0; j < kEach; j++) {
                 const float w = exp2f(v[j] - from);
-                own[j * W::kOfRow * W::kWeights] = w;
+                own[j * W::kOfRow * W::kWeights] = v[j] == -INFINITY ? -0.0f : w;
                 sum += w;
             }
 #pragma unroll
@@ -300,7 +300,9 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                         o2[r][k][j] = two_of(v.x * keep, v.y * keep);
                     }
             }
-            /* values that a row does not see may be infinite or NaN: a weight of 0 takes no part */
+            /* values that a row does not see may be infinite or NaN: a weight of -0 takes no part.  (One
+             * that is seen and weighs 0 beside a much greater one does: 0 times it is NaN.) */
+            constexpr Two kUnseen = 0x8000000080000000ull; /* two of -0 */
             const auto multiply = [&](auto drafted) {
 #pragma unroll 4
                 for (int t = share0; t < kTile; t += W::kShares) {
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                             *reinterpret_cast<const ulonglong2 *>(values + t * W::kValuePitch + (piece0 + k * W::kEvery) * 4);
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const bool none = decltype(drafted)::value && w[r] == 0;
+                            const bool none = decltype(drafted)::value && w[r] == kUnseen;
                             add_products(o2[r][k][0], w[r], none ? 0 : c.x);
                             add_products(o2[r][k][1], w[r], none ? 0 : c.y);
                         }
@@ -398,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 
 /* ---- joining the parts of an item --------------------------------------- */
 
+constexpr float kNothing = -1.0f; /* the factor of a part in which the row saw nothing */
 constexpr int kJoinWarps = 8, kJoinOwn = 2, kJoinRows = kJoinWarps * kJoinOwn;
 
 /* out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) for two rows a warp, whose loads
@@ -448,8 +451,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
         float factor[kJoinOwn];
 #pragma unroll
         for (int r = 0; r < kJoinOwn; r++) {
-            factor[r] = c < parts ? exp2f(*at(first.maxima, second.maxima, c, f0 + r) - from[r]) : 0.0f;
+            const float most = c < parts ? *at(first.maxima, second.maxima, c, f0 + r) : -INFINITY;
+            factor[r] = exp2f(most - from[r]);
             sum[r] += c < parts ? *at(first.sums, second.sums, c, f0 + r) * factor[r] : 0.0f;
+            if (most == -INFINITY)
+                factor[r] = kNothing;
         }
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
@@ -474,7 +480,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
 #pragma unroll
                     for (int r = 0; r < kJoinOwn; r++) {
                         const float w = __shfl_sync(0xffffffffu, factor[r], i0 + i);
-                        if (w != 0.0f) { /* 0: a part in which the row saw nothing, or what underflows */
+                        /* (0, beside a much greater maximum: infinities and NaN of that part become NaN) */
+                        if (w != kNothing) {
                             o[r][k].x = fmaf(v[i][r].x, w, o[r][k].x);
                             o[r][k].y = fmaf(v[i][r].y, w, o[r][k].y);
                             o[r][k].z = fmaf(v[i][r].z, w, o[r][k].z);

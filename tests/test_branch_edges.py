@@ -6,8 +6,8 @@ import math
 
 import pytest
 
-from test_branch import plain_beams, run_beams, same_beams
-from test_paged import dtypes
+from test_branch import PAIRS, Tree, plain_beams, run_beams, same_beams
+from test_paged import Pool, dtypes
 
 gpu = pytest.mark.gpu
 
@@ -63,3 +63,49 @@ def test_beam_select_ties_of_beams_without_a_score(torch_cuda, kind, low, V):
     ended = torch.tensor([[1, 0, 1, 0], [0, 1, 0, 0]])
     got = run_beams(torch, logits.cuda(), scores.cuda(), 12, ended.to(torch.uint8).cuda(), 4)
     same_beams(got, plain_beams(torch, logits, scores, ended, 4, 12))
+
+
+# ---------------------------------------------------------------------------
+# tree attention
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("length,low", [(70, "first"), (70, "last"), (5000, "first"), (5000, "last")])
+def test_tree_values_that_are_no_numbers_and_hardly_weigh(torch_cuda, cache, rows, D, length, low):
+    """An infinity or NaN among the values that a row sees shows in that dimension, also where its slot's weight, beside
+    others 256 nats greater, is 0 in any format; in one block, and in a part of several blocks that weighs nothing."""
+    torch = torch_cuda
+    n, H, KV = 9, 4, 2
+    pool = Pool(torch, [length], H, KV, D, 16, cache, seed=6)
+    k = torch.zeros(KV, length, D)
+    few = length // 2 if low == "first" else length - length // 2
+    if low == "first":
+        k[:, :few, 0] = -256.0
+        odd = few // 4  # in the prefix
+    else:
+        k[:, few:, 0] = -256.0
+        odd = length - n + 4  # a drafted token
+    v = pool.v[0].float().clone()
+    v[:, odd, 3], v[:, odd, 5], v[:, odd, 7] = math.nan, math.inf, -math.inf
+    dt = dtypes(torch)[cache]
+    pool.put(0, k.to(dt), v.to(dt), 0)
+    pool.k[0], pool.v[0] = k.to(dt), v.to(dt)
+    pool.cache.reserve_tree(n)
+    seen = [[j for j in range(i + 1) if j != 4 or i % 2] for i in range(n)]
+    tree = Tree(torch, pool, [n], rows, masks=[seen])
+    tree.q_cpu.zero_()
+    tree.q_cpu[:, :, 0] = 1.0
+    tree.q.copy_(tree.q_cpu.reshape(n, -1))
+    tree.run(scale=1.0)
+    pool.cache.check()
+    out = tree.out.reshape(n, H, D).float().cpu()
+    rest = [d for d in range(D) if d not in (3, 5, 7)]
+    for i in range(n):
+        shows = low == "first" or 4 in seen[i]
+        assert bool(out[i, :, 3].isnan().all()) == shows, i
+        assert bool((~out[i][:, [5, 7]].isfinite()).all()) == shows, i
+        assert bool(out[i][:, rest].isfinite().all()), i
+        if not shows:
+            assert bool(out[i].isfinite().all()), i
