@@ -61,6 +61,12 @@ def depths(parents: list) -> list:
     return got
 
 
+def _check_prompts(prompts: list) -> None:
+    """A prompt's last row gives the first token: there has to be one."""
+    if not all(len(p) > 0 for p in prompts):
+        raise ValueError("branch session: empty prompt")
+
+
 class Model:
     """Embedding, attention layers and a head, with random weights."""
 
@@ -158,6 +164,7 @@ def beam_search(model: Model, prompts: list, steps: int, beams: int, eos: int, d
                 page_size: int = 16) -> list:
     """The `beams` best continuations of each prompt as (score, tokens), best first.  The loop over the steps never waits
     for the device."""
+    _check_prompts(prompts)
     requests = len(prompts)
     most, S = max(map(len, prompts)), requests * beams
     max_pages = -(-(most + steps) // page_size)
@@ -220,6 +227,7 @@ def tree_greedy(model: Model, prompts: list, steps: int, widths: list, dtype: to
                 page_size: int = 16) -> tuple:
     """Greedy continuations of `steps` tokens, verified a drafted tree at a time (widths []: a token at a time), and the
     number of passes over the caches."""
+    _check_prompts(prompts)
     S, size = len(prompts), 1
     for w in reversed(widths):
         size = 1 + w * size

@@ -109,3 +109,17 @@ def test_tree_values_that_are_no_numbers_and_hardly_weigh(torch_cuda, cache, row
         assert bool(out[i][:, rest].isfinite().all()), i
         if not shows:
             assert bool(out[i].isfinite().all()), i
+
+
+# ---------------------------------------------------------------------------
+# the loops of branch_demo
+
+
+def test_empty_prompts_are_refused(torch_cuda):
+    """Their first token was taken from the row of the prompt before."""
+    from nutllm_b200 import branch_demo as demo
+    for prompts in ([[]], [[1, 2], []], [[], [3]]):
+        with pytest.raises(ValueError, match="empty prompt"):
+            demo.beam_search(None, prompts, 4, 2, 0)
+        with pytest.raises(ValueError, match="empty prompt"):
+            demo.tree_greedy(None, prompts, 4, [2])
