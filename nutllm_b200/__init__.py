@@ -1028,6 +1028,15 @@ def _misfit(e: Exception, part: str = "paged") -> ValueError:
     return ValueError(f"{part}: an argument does not fit its field ({e})")
 
 
+def _check_fields(part: str, addresses=(), numbers=(), words=()) -> None:
+    """ctypes keeps the low bits of an int beyond its field: it is refused instead."""
+    for what, values, low, high in (("address", addresses, -1 << 63, 1 << 64),
+                                    ("number", numbers, -1 << 63, 1 << 63),
+                                    ("number", words, -1 << 31, 1 << 31)):
+        if not all(low <= v < high for v in values if isinstance(v, int)):
+            raise _misfit(OverflowError(what), part)
+
+
 def _packed(lib: C.CDLL, name: str):
     """An entry point that takes (handle, arguments as bytes, stream)."""
     return C.CFUNCTYPE(C.c_int, _P, _P, _P)(C.cast(getattr(lib, name), _P).value)
@@ -1058,6 +1067,9 @@ class PagedCache:
                  slot_stride: int = 0, bounds: int = 0, bound_scales: int = 0, max_rows: int = 0,
                  track_weights: bool = False, device: int = 0):
         self.handle = None
+        _check_fields("paged", (keys, values, table, lengths, bounds, bound_scales),
+                      (page_stride, head_stride, slot_stride, sequences, max_pages, n_pages, page_size,
+                       heads, kv_heads, head_dim, max_rows), (dtype, device))
         view = PagedView(keys, values, table, lengths, bounds, bound_scales, page_stride,
                          head_stride, slot_stride, sequences, max_pages, n_pages, page_size,
                          heads, kv_heads, head_dim, max_rows, dtype, int(track_weights))
@@ -1086,6 +1098,7 @@ class PagedCache:
         except _MISFIT as e:
             raise _misfit(e) from None
         if row_position:
+            _check_fields("paged", (row_position,))
             status = self._append_at(self.handle, args, row_position, stream)
         else:
             status = self._append(self.handle, args, stream)
@@ -1139,8 +1152,7 @@ class PagedCache:
     def reserve_tree(self, max_new: int) -> None:
         """Workspace for tree_attention() of up to max_new drafted tokens a
         sequence (nut_paged_reserve_tree); not within a capture."""
-        if not -1 << 63 <= max_new < 1 << 63:
-            raise _misfit(OverflowError("max_new"))
+        _check_fields("paged", numbers=(max_new,))
         _check(cuda_lib().nut_paged_reserve_tree(self.handle, max_new))
 
     def tree_attention(self, q: int, out: int, starts: int, mask: int, rows: int, max_new: int,
@@ -1218,6 +1230,8 @@ class PageBook:
     def __init__(self, table: int, lengths: int, refs: int, free_pages: int, free_count: int, *,
                  sequences: int, max_pages: int, n_pages: int, page_size: int, device: int = 0):
         self.handle = None
+        _check_fields("pages", (table, lengths, refs, free_pages, free_count),
+                      (sequences, max_pages, n_pages, page_size), (device,))
         view = PagesView(table, lengths, refs, free_pages, free_count, sequences, max_pages,
                          n_pages, page_size)
         h = C.c_void_p()
@@ -1264,8 +1278,7 @@ class BeamSearch:
 
     def __init__(self, sequences: int, beams: int, vocab: int, n_out: int, *, device: int = 0):
         self.handle = None
-        if not all(-1 << 63 <= n < 1 << 63 for n in (sequences, beams, vocab, n_out)):
-            raise _misfit(OverflowError("dimension"), "beam")
+        _check_fields("beam", (), (sequences, beams, vocab, n_out), (device,))
         h = C.c_void_p()
         lib = cuda_lib()
         _check(lib.nut_beam_create(sequences, beams, vocab, n_out, device, C.byref(h)))

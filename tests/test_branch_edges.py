@@ -6,6 +6,7 @@ import math
 
 import pytest
 
+import nutllm_b200 as nb
 from test_branch import PAIRS, Tree, plain_beams, run_beams, same_beams
 from test_paged import Pool, dtypes
 
@@ -123,3 +124,48 @@ def test_empty_prompts_are_refused(torch_cuda):
             demo.beam_search(None, prompts, 4, 2, 0)
         with pytest.raises(ValueError, match="empty prompt"):
             demo.tree_greedy(None, prompts, 4, [2])
+
+
+# ---------------------------------------------------------------------------
+# numbers beyond their fields
+
+
+def test_numbers_beyond_their_fields_are_refused():
+    """ctypes would keep their low 64 bits."""
+    book = dict(sequences=4, max_pages=8, n_pages=30, page_size=16)
+    for name in book:
+        for wrap in (1 << 64, 3 << 64, -1 << 64):
+            with pytest.raises(ValueError, match="field"):
+                nb.PageBook(16, 16, 16, 16, 16, **(book | {name: book[name] + wrap}))
+    for k in range(5):
+        for at in ((1 << 64) + 16, (-1 << 64) + 16):
+            with pytest.raises(ValueError, match="field"):
+                nb.PageBook(*(at if i == k else 16 for i in range(5)), **book)
+    cache = dict(sequences=4, max_pages=8, n_pages=30, page_size=16, heads=8, kv_heads=2, head_dim=64, max_rows=0, page_stride=0,
+                 head_stride=0, slot_stride=0)
+    for name in cache:
+        with pytest.raises(ValueError, match="field"):
+            nb.PagedCache(16, 16, 16, 16, **(cache | {name: cache[name] + (1 << 64)}))
+    for more in (dict(dtype=1 << 32), dict(device=1 << 32)):
+        with pytest.raises(ValueError, match="field"):
+            nb.PagedCache(16, 16, 16, 16, **cache, **more)
+    with pytest.raises(ValueError, match="field"):
+        nb.PageBook(16, 16, 16, 16, 16, **book, device=1 << 32)
+    for name in ("bounds", "bound_scales"):
+        with pytest.raises(ValueError, match="field"):
+            nb.PagedCache(16, 16, 16, 16, **cache, **{name: (1 << 64) + 16})
+    for name in ("sequences", "beams", "vocab", "n_out"):
+        with pytest.raises(ValueError, match="field"):
+            nb.BeamSearch(**(dict(sequences=1, beams=1, vocab=10, n_out=1) | {name: (1 << 64) + 1}))
+
+
+@gpu
+def test_row_positions_beyond_an_address_are_refused(torch_cuda):
+    torch = torch_cuda
+    pool = Pool(torch, [30], 4, 2, 64, 16, "f16")
+    x = torch.zeros(1, 256, dtype=torch.float16, device="cuda")
+    starts = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for at in ((1 << 64) + starts.data_ptr(), (-1 << 64) + starts.data_ptr()):
+        with pytest.raises(ValueError, match="field"):
+            pool.cache.append(0, x.data_ptr(), x.data_ptr(), starts.data_ptr(), 1, 1, dtype=nb.F16, row_position=at)
+    pool.cache.check()
