@@ -583,7 +583,11 @@ nut_status nut_paged_tree_attention(nut_paged *paged, const nut_paged_tree_args 
  * numbers below n, then -1.  positions and weights (each or NULL) move with
  * them.  A sequence with a bad length, starts, list or page is left as it is
  * (new_lengths[s] = lengths[s]) and reported.  new_lengths may be the view's
- * lengths.  Key bounds are not recomputed (nut_paged_summarise). */
+ * lengths where nothing else goes by them.  Handles that share lengths (a
+ * model's layers) are all compacted from the lengths as they were, and a book
+ * of pages (nut_pages) counts holders by them: there new_lengths is an array
+ * of its own, the `keep` of the next nut_pages_update.  Key bounds are not
+ * recomputed (nut_paged_summarise). */
 typedef struct nut_paged_compact_args {
     const int32_t *starts;   /* [sequences + 1] */
     const int32_t *accepted; /* [sequences][n_accepted] */
@@ -614,7 +618,12 @@ nut_status nut_paged_copy(nut_paged *paged, const nut_paged_copy_args *args, voi
  *               for later, say)
  *   free_pages  its first free_count[0] entries are the pages without a
  *               holder; pages are taken from the end of them and given back
- *               there */
+ *               there
+ * A sequence may write to the slots that its newest update gave it room for:
+ * no one else holds their pages.  Others may be shared and are only read
+ * (nut_paged_evict, which moves slots anywhere, is not for sequences of a
+ * book).  Positions and weights of slots belong to a sequence, not to its
+ * pages: they do not follow `parent`. */
 typedef struct nut_pages_view {
     int32_t *table;      /* [sequences][max_pages] */
     int32_t *lengths;    /* [sequences] */
@@ -654,10 +663,12 @@ nut_status nut_pages_error(nut_pages *pages, void *stream);
  * Table entries behind a sequence's last page stay as they were.  If a
  * parent, keep, add, length or page is out of range, a sequence outgrows its
  * table, or the free pages do not suffice, nothing changes: the copy lists
- * are all -1 (and 0), and the error is kept for nut_pages_error.  (Pages of
- * entries that stay are not looked at.  A book whose refs are fewer than the
- * table shows, or which lists pages in use as free, is reported where an update
- * meets it; what changed is then not undone.) */
+ * are all -1 (and 0), and the error is kept for nut_pages_error.  (Lengths are
+ * the old ones then: a loop that appends without having asked writes over its
+ * sequences' newest slots.  Pages of entries that stay are not looked at.  A
+ * book whose refs are fewer than the table shows, or which lists pages in use
+ * as free, is reported where an update meets it; what changed is then not
+ * undone.) */
 typedef struct nut_pages_update_args {
     const int32_t *parent; /* [sequences]; NULL: itself */
     const int32_t *keep;   /* [sequences], not negative; NULL: all */

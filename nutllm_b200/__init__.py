@@ -1174,7 +1174,8 @@ class PagedCache:
                 positions: int = 0, weights: int = 0, stream: int = 0) -> None:
         """Moves the accepted ones of each sequence's drafted tokens (ascending
         numbers in int32 [sequences][n_accepted], -1 behind) to where the
-        drafted tokens begin (nut_paged_compact)."""
+        drafted tokens begin (nut_paged_compact).  new_lengths is the cache's
+        own lengths only where no other cache and no PageBook goes by them."""
         try:
             args = _COMPACT.pack(starts, accepted, n_accepted, new_lengths, positions, weights)
         except _MISFIT as e:

@@ -3,11 +3,12 @@ short cuts could part: logits and scores that are no numbers, values that are
 none and hardly weigh, starts that contradict themselves, lists and books
 across layers, and numbers beyond their fields."""
 import math
+import random
 
 import pytest
 
 import nutllm_b200 as nb
-from test_branch import PAIRS, Tree, plain_beams, run_beams, same_beams
+from test_branch import PAIRS, Book, Tree, paths, plain_beams, run_beams, same_beams
 from test_paged import Pool, dtypes
 
 gpu = pytest.mark.gpu
@@ -169,3 +170,48 @@ def test_row_positions_beyond_an_address_are_refused(torch_cuda):
         with pytest.raises(ValueError, match="field"):
             pool.cache.append(0, x.data_ptr(), x.data_ptr(), starts.data_ptr(), 1, 1, dtype=nb.F16, row_position=at)
     pool.cache.check()
+
+
+# ---------------------------------------------------------------------------
+# caches of several layers, and their book
+
+
+@gpu
+def test_compact_of_every_layer_then_the_book(torch_cuda):
+    """Layers share table and lengths: each is compacted from the lengths as they were, into an array that the next
+    update keeps; in place for the last alone."""
+    torch = torch_cuda
+    S, M, P, ps, KV, D, n = 3, 8, 40, 4, 2, 64, 7
+    lens = [9, 17, 12]
+    book = Book(torch, S, M, P, ps)
+    book.plain(None, None, [a + n for a in lens])
+    book.update(None, None, [a + n for a in lens])
+    g = torch.Generator().manual_seed(3)
+    layers = [torch.randn(2, P, KV, ps, D, generator=g).half().cuda() for _ in range(3)]
+    caches = [nb.PagedCache(x[0].data_ptr(), x[1].data_ptr(), book.dev["table"].data_ptr(), book.dev["lengths"].data_ptr(), sequences=S,
+                            max_pages=M, n_pages=P, page_size=ps, heads=4, kv_heads=KV, head_dim=D, dtype=nb.F16) for x in layers]
+    lists = [[0, 3, 6], [2], []]
+    starts = torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32, device="cuda")
+    accepted = paths(torch, lists, 4)
+    left = torch.zeros(S, dtype=torch.int32, device="cuda")
+
+    def rows(x, s, slots):
+        pages = torch.tensor([book.table[s][t // ps] for t in slots], device="cuda").long()
+        return x[:, pages, :, torch.tensor([t % ps for t in slots], device="cuda")]
+
+    want = [[rows(x, s, list(range(lens[s])) + [lens[s] + j for j in lists[s]]).clone() for s in range(S)] for x in layers]
+    for cache in caches:
+        cache.compact(starts.data_ptr(), accepted.data_ptr(), 4, new_lengths=left.data_ptr())
+        cache.check()
+        assert left.tolist() == [a + len(x) for a, x in zip(lens, lists)]
+        assert book.dev["lengths"].tolist() == [a + n for a in lens]
+    for x, kept in zip(layers, want):
+        for s in range(S):
+            assert torch.equal(rows(x, s, range(lens[s] + len(lists[s]))), kept[s])
+    # the update gives back the pages behind what is kept
+    keep = [a + len(x) for a, x in zip(lens, lists)]
+    copies = book.plain(None, keep, [1] * S)
+    book.update(None, keep, [1] * S)
+    book.same(copies)
+    assert book.count == P - sum(book.pages(k + 1) for k in keep)
+    book.book.check()
