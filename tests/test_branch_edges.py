@@ -215,3 +215,73 @@ def test_compact_of_every_layer_then_the_book(torch_cuda):
     book.same(copies)
     assert book.count == P - sum(book.pages(k + 1) for k in keep)
     book.book.check()
+
+
+@gpu
+@pytest.mark.parametrize("seed", [0, 1, 2, 3])
+def test_refused_updates_say_why(torch_cuda, seed):
+    """LengthError where the free pages do not suffice, IndexError where a sequence outgrows its table (or both)."""
+    torch = torch_cuda
+    S, M, P, ps = 9, 6, 30, 4
+    book, r, met = Book(torch, S, M, P, ps, seed), random.Random(seed), set()
+    for _ in range(40):
+        parent = [r.randrange(S) for _ in range(S)] if r.random() < 0.5 else list(range(S))
+        keep = [r.randrange(M * ps + 1) for _ in range(S)]
+        add = [r.choice([0, 1, 2, 5, 9, 20]) for _ in range(S)]
+        outgrown = any(min(w, book.lengths[p]) + a > M * ps for p, w, a in zip(parent, keep, add))
+        want = book.plain(parent, keep, add)
+        book.update(parent, keep, add)
+        book.same(want)
+        if want is None:
+            met.add(outgrown)
+            with pytest.raises(IndexError if outgrown else nb.LengthError):
+                book.book.check()
+        book.book.check()
+    assert met == {False, True}
+
+
+@gpu
+@pytest.mark.parametrize("beams,eos,seed", [(1, 3, 3), (1, 0, 8), (3, 5, 3), (4, 0, 9)])
+def test_beam_search_paths(torch_cuda, beams, eos, seed):
+    """Paths and not scores alone: equal to those of the search by the definition wherever every choice of it was clear,
+    that is, no two neighbours among a step's beams + 1 best within 1e-3 of one another (scores are within 1e-4)."""
+    torch = torch_cuda
+    from nutllm_b200 import branch_demo as demo
+    from test_branch_demo import plain_hidden
+    model = demo.Model(vocab=60, layers=2, heads=4, kv_heads=2, head_dim=32, seed=seed)
+    prompts = [[5, 9, 31, 7, 22, 50, 1, 2, 40], [11], list(range(17)), [3, 3], [59, 0, 1, 30]]
+    got = demo.beam_search(model, prompts, 6, beams, eos, dtype=torch.float32, page_size=4)
+    clear = 0
+    for prompt, best in zip(prompts, got):
+        kept, gap = [(0.0, [], False)], math.inf
+        for _ in range(6):
+            found = []
+            for i, (score, path, done) in enumerate(kept):
+                if done:
+                    found.append((-score, i, eos, path, True))
+                    continue
+                logits = plain_hidden(torch, model, torch.tensor([prompt + path], device="cuda"))[0, -1]
+                top = torch.topk(torch.log_softmax(logits, -1), beams + 1)
+                found += [(-(score + v), i, t, path + [t], t == eos) for v, t in zip(top.values.tolist(), top.indices.tolist())]
+            found.sort(key=lambda c: c[:3])
+            gap = min([gap] + [b[0] - a[0] for a, b in zip(found[:beams], found[1:])])
+            kept = [(-f[0], f[3], f[4]) for f in found[:beams]]
+        for (score, _), (b, _, _) in zip(best, kept):
+            assert abs(score - b) <= 1e-4 * (1 + abs(b))
+        if gap > 1e-3:
+            clear += 1
+            assert [path for _, path in best] == [k[1] for k in kept]
+    assert clear >= 1
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("D", [8, 16, 24, 72, 120, 136])
+def test_tree_heads_of_odd_widths(torch_cuda, D, cache, rows):
+    torch = torch_cuda
+    pool = Pool(torch, [150, 31, 70], 6, 2, D, 12, cache, seed=D)
+    pool.cache.reserve_tree(31)
+    tree = Tree(torch, pool, [9, 31, 1], rows, seed=D)
+    tree.run()
+    pool.cache.check()
+    tree.check()
