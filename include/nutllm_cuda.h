@@ -534,7 +534,7 @@ nut_status nut_paged_append_at(nut_paged *paged, const nut_paged_append_args *ar
 
 /* Workspace for nut_paged_tree_attention calls of up to max_new (1 to
  * NUT_TREE_MAX) drafted tokens a sequence: on 148 SMs 592 parts of
- * min(128, max_new * heads / kv_heads) rows of head_dim + 2 floats.
+ * min(128, max_new * heads / kv_heads) rows of head_dim + 3 floats.
  * Allocates, so not within a capture.  Called again with more it allocates
  * anew; what earlier captures use stays until the handle goes. */
 #define NUT_TREE_MAX 1024

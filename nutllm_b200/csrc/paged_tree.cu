@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
                     a.lse[row * p.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kTreeLn2;
             } else {
                 part.maxima[tid] = m;
+                part.rests[tid] = 0.0f;
                 part.sums[tid] = l;
             }
         }
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, (WidePlan<kRows, DP>::kPerSm)) wide_
 constexpr float kNothing = -1.0f; /* the factor of a part in which the row saw nothing */
 constexpr int kJoinWarps = 8, kJoinOwn = 2, kJoinRows = kJoinWarps * kJoinOwn;
 
-/* out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m) for two rows a warp, whose loads
+/* out = sum_c O_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), m_c a maximum and its rest, for two rows a warp, whose loads
  * are in flight together.  Lanes turn the parts' maxima and sums into factors, 32 parts at a time,
  * then take 4 dims each.  It is round trips: which item, its span, maxima, outputs; 8.4 us after 32
  * caches of up to 4,096 slots, 10 with a row a warp, whose blocks came in two waves. */
@@ -424,20 +425,26 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
     const TreePart first = tree_part(a, blockIdx.x, inside, rows), second = tree_part(a, blockIdx.x + 1, 0, rows);
     const int64_t step = 2 * a.part_floats;
     const auto at = [&](const float *x, const float *y, int c, int f) { return (c == 0 ? x : y + (c - 1) * step) + min(f, rows - 1); };
-    float from[kJoinOwn], sum[kJoinOwn];
+    float from[kJoinOwn], rest[kJoinOwn], sum[kJoinOwn]; /* the greatest maximum, and its greatest rest */
 #pragma unroll
     for (int r = 0; r < kJoinOwn; r++) {
-        from[r] = -INFINITY;
+        from[r] = rest[r] = -INFINITY;
         sum[r] = 0.0f;
     }
     for (int c = lane; c < parts; c += 32)
 #pragma unroll
-        for (int r = 0; r < kJoinOwn; r++)
-            from[r] = fmaxf(from[r], *at(first.maxima, second.maxima, c, f0 + r));
+        for (int r = 0; r < kJoinOwn; r++) {
+            const float most = *at(first.maxima, second.maxima, c, f0 + r), more = *at(first.rests, second.rests, c, f0 + r);
+            rest[r] = most > from[r] ? more : most == from[r] ? fmaxf(rest[r], more) : rest[r];
+            from[r] = fmaxf(from[r], most);
+        }
 #pragma unroll
     for (int r = 0; r < kJoinOwn; r++) {
-        from[r] = warp_max(from[r]);
-        from[r] = from[r] == -INFINITY ? 0.0f : from[r];
+        const float most = warp_max(from[r]);
+        rest[r] = warp_max(from[r] == most ? rest[r] : -INFINITY);
+        from[r] = most;
+        if (most == -INFINITY)
+            from[r] = rest[r] = 0.0f;
     }
     constexpr int kMost = 2; /* pieces of 4 dims a lane, 128 dims apart */
     float4 o[kJoinOwn][kMost];
@@ -452,7 +459,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
 #pragma unroll
         for (int r = 0; r < kJoinOwn; r++) {
             const float most = c < parts ? *at(first.maxima, second.maxima, c, f0 + r) : -INFINITY;
-            factor[r] = exp2f(most - from[r]);
+            const float more = c < parts ? *at(first.rests, second.rests, c, f0 + r) : 0.0f;
+            factor[r] = exp2f((most - from[r]) + (more - rest[r]));
             sum[r] += c < parts ? *at(first.sums, second.sums, c, f0 + r) * factor[r] : 0.0f;
             if (most == -INFINITY)
                 factor[r] = kNothing;
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
         int h;
         tree_row(a, row0, join.z, first_row + f0 + r, row, h);
         if (a.lse && lane == 0)
-            a.lse[row * p.heads + h] = all == 0.0f ? -INFINITY : (from[r] + log2f(all)) * kTreeLn2;
+            a.lse[row * p.heads + h] = all == 0.0f ? -INFINITY : (from[r] + (rest[r] + log2f(all))) * kTreeLn2;
         R *to = static_cast<R *>(a.out) + row * a.out_stride + int64_t(h) * D;
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
@@ -581,7 +589,7 @@ cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaSt
 
 int64_t tree_part_floats(const PagedPool &p, int max_new) {
     const int64_t rows = std::min<int64_t>(128, int64_t(max_new) * p.group);
-    return (rows * 2 + 3) / 4 * 4 + rows * p.head_dim;
+    return (rows * 3 + 3) / 4 * 4 + rows * p.head_dim;
 }
 
 int64_t tree_most_places(const PagedPool &p, int max_new, int64_t rows) {

@@ -182,15 +182,16 @@ __device__ __forceinline__ void tree_row(const PagedTree &a, int row0, int head,
     query_head = head * a.p.group + f - node * a.p.group;
 }
 
-/* A CTA's part of an item: maxima and sums of its rows, then outputs.  The item
- * that a CTA's share begins within lies in its first place, another in the
- * second. */
+/* A CTA's part of an item: maxima and sums of its rows, then outputs.  Sums and
+ * outputs are those of weights 2^(logit - maximum - rest): a rest holds what
+ * rounding took from a great maximum.  The item that a CTA's share begins
+ * within lies in its first place, another in the second. */
 struct TreePart {
-    float *maxima, *sums, *out;
+    float *maxima, *rests, *sums, *out;
 };
 __device__ __forceinline__ TreePart tree_part(const PagedTree &a, int cta, int second, int rows) {
     float *at = a.partial + (int64_t(cta) * 2 + second) * a.part_floats;
-    return {at, at + rows, at + (rows * 2 + 3) / 4 * 4};
+    return {at, at + rows, at + rows * 2, at + (rows * 3 + 3) / 4 * 4};
 }
 
 /* What join_kernel has to know of the item that begins in this CTA and goes on

@@ -652,8 +652,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                 everyone(); /* the units */
 
             const float unit = kTerms > 1 ? sh.unit[tid] : fabsf(a.scale) * kTreeLog2e;
-            /* weights are 2^(logit - from), `from` kLift below a maximum */
-            float from = -INFINITY, l = 0.0f;
+            /* weights are 2^((s - m) unit + kLift), m a maximum of s.  (Differences of s: beside products
+             * s unit of 2^27 and more, rounded, the greatest weight would be off by their last place.) */
+            float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
             for (int i = 0; i < n; i++, tiles++) {
                 const uint32_t logits_at = tmem + lanes + tiles % kBuffers * Plan::kLogits;
@@ -701,13 +702,12 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         top = fmaxf(top, s[k]);
                         other = fmaxf(other, s[k + 1]);
                     }
-                    /* rounded up, so that beside logits of 2^24 and more no weight passes 2^kLift either */
-                    const float to = __fsub_ru(__fmul_ru(fmaxf(top, other), unit), kLift);
-                    const float next = to - from > kSlack || from == -INFINITY ? fmaxf(from, to) : from;
-                    if (__any_sync(0xffffffffu, next != from)) {
-                        const float keep = from == next ? 1.0f : power2(from - next);
+                    top = fmaxf(top, other);
+                    const float next = (top - m) * unit > kSlack ? top : m; /* (NaN: both are -infinity) */
+                    if (__any_sync(0xffffffffu, next != m)) {
+                        const float keep = m == next ? 1.0f : power2((m - next) * unit);
                         l *= keep;
-                        from = next;
+                        m = next;
                         if (i > 0) { /* once the products before are complete */
                             alive = __all_sync(0xffffffffu, await_outputs(tiles - 1));
                             tc_after();
@@ -723,14 +723,19 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                             }
                         }
                     }
-                    const float less = from == -INFINITY ? 0.0f : -from;
+                    const float none = m == -INFINITY ? 0.0f : -m;
+                    const Two less = two_of(none, none), units = two_of(unit, unit), lift = two_of(kLift, kLift);
                     float sum = 0.0f, sum1 = 0.0f;
 #pragma unroll
                     for (int k = 0; k < kTile; k += 32) {
                         uint32_t e[kTerms][16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            float w0 = power2(fmaf(s[k + 2 * j], unit, less)), w1 = power2(fmaf(s[k + 2 * j + 1], unit, less));
+                            Two z = two_of(s[k + 2 * j], s[k + 2 * j + 1]);
+                            asm("add.rn.f32x2 %0, %0, %1;\n" : "+l"(z) : "l"(less));
+                            asm("fma.rn.f32x2 %0, %0, %1, %2;\n" : "+l"(z) : "l"(units), "l"(lift));
+                            const float2 of = parts_of(z);
+                            float w0 = power2(of.x), w1 = power2(of.y);
                             sum += w0;
                             sum1 += w1;
 #pragma unroll
@@ -768,13 +773,15 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
             const TreePart part = tree_part(a, blockIdx.x, x.first <= start ? 0 : 1, x.rows);
             if (counts && alive) {
                 if (!whole) {
-                    part.maxima[tid] = from;
+                    const float most = m * unit;
+                    part.maxima[tid] = most;
+                    part.rests[tid] = (fabsf(most) < INFINITY ? fmaf(m, unit, -most) : 0.0f) - kLift;
                     part.sums[tid] = l;
                 } else if (a.lse) {
                     int64_t out_row;
                     int h;
                     tree_row(a, x.span.row0, x.head, x.first_row + tid, out_row, h);
-                    a.lse[out_row * p.heads + h] = l == 0.0f ? -INFINITY : (from + log2f(l)) * kTreeLn2;
+                    a.lse[out_row * p.heads + h] = l == 0.0f ? -INFINITY : fmaf(m, unit, log2f(l) - kLift) * kTreeLn2;
                 }
             }
             /* 32 dims at a time leave through a warp's 4 KB of the queries'

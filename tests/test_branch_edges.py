@@ -5,11 +5,12 @@ across layers, and numbers beyond their fields."""
 import math
 import random
 
+import numpy as np
 import pytest
 
 import nutllm_b200 as nb
-from test_branch import PAIRS, Book, Tree, paths, plain_beams, run_beams, same_beams
-from test_paged import Pool, dtypes
+from test_branch import PAIRS, UNIT, Book, Tree, paths, plain_beams, run_beams, same_beams
+from test_paged import EPS, Pool, dtypes
 
 gpu = pytest.mark.gpu
 
@@ -285,3 +286,38 @@ def test_tree_heads_of_odd_widths(torch_cuda, D, cache, rows):
     tree.run()
     pool.cache.check()
     tree.check()
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("length", [40, 3000])
+@pytest.mark.parametrize("scale", [2.0 ** 27, 3e10, -7e15, 1e30])
+def test_tree_logits_beyond_every_difference(torch_cuda, cache, rows, D, length, scale):
+    """Logits so great that their last places are many units: the greatest ones, a few equal ones across the cache, share
+    the output, and the others (1/64 of the greatest below it or more) have no part."""
+    torch = torch_cuda
+    dt = dtypes(torch)[cache]
+    pool = Pool(torch, [length], 2, 1, D, 16, cache, seed=18)
+    k = torch.zeros(1, length, D)
+    k[0, :, 0] = 1.0 + torch.arange(length).remainder(32) / 64
+    best = [3, length // 2, length - 7]
+    k[0, best, 0] = 1.703125
+    k = k.to(dt) * (1.0 if scale > 0 else -1.0)
+    pool.put(0, k, pool.v[0], 0)
+    pool.k[0] = k
+    pool.cache.reserve_tree(4)
+    tree = Tree(torch, pool, [4], rows, masks=[[list(range(i + 1)) for i in range(4)]])
+    tree.q_cpu.zero_()
+    tree.q_cpu[:, :, 0] = torch.tensor([1.37, 0.8125]).to(tree.q_cpu.dtype)
+    tree.q.copy_(tree.q_cpu.reshape(4, -1))
+    tree.run(scale=scale)
+    pool.cache.check()
+    out, lse = tree.out.reshape(4, 2, D).cpu().double(), tree.lse.cpu().double()
+    v = pool.v[0][0][best].double()
+    half = 0.0 if rows == "f32" else torch.finfo(dtypes(torch)[rows]).eps / 2
+    # three equal weights, each within 2^-24 (fp32), 2^-11 (fp16) or 2^-8 (bf16) of itself; a division; the output's type
+    tol = v.abs().mean(0) * (16 * EPS + 2 * UNIT[rows] + half) + 2.0 ** -25
+    assert bool(((out - v.mean(0)).abs() <= tol).all())
+    top = abs(float(np.float32(scale))) * 1.703125 * tree.q_cpu[:, :, 0].double()
+    assert bool(((lse - top - math.log(3)).abs() <= 8 * EPS * top).all())
