@@ -626,7 +626,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
 #pragma unroll
                                 for (int j = 0; j < 8; j++)
                                     v[j] *= gain;
-                                unit *= __uint_as_float(uint32_t(254 - field) << 23);
+                                /* not 0, which would make NaN of a masked -infinity; at 2^-126 no
+                                 * logit is above 2^-90, and weights are as at any unit below */
+                                unit = fmaxf(unit * __uint_as_float(uint32_t(254 - field) << 23), 1.17549435e-38f);
                             }
                         }
                         if (c == 0)

@@ -321,3 +321,19 @@ def test_tree_logits_beyond_every_difference(torch_cuda, cache, rows, D, length,
     assert bool(((out - v.mean(0)).abs() <= tol).all())
     top = abs(float(np.float32(scale))) * 1.703125 * tree.q_cpu[:, :, 0].double()
     assert bool(((lse - top - math.log(3)).abs() <= 8 * EPS * top).all())
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("q,scale", [(2e-38, 1e-9), (3e-38, -1e-30), (1e-30, 1e-38), (1.0, 1e-42)])
+def test_tree_logits_next_to_nothing(torch_cuda, cache, q, scale):
+    """Queries and scales whose product no float holds: every slot that is seen weighs the same."""
+    torch = torch_cuda
+    pool = Pool(torch, [90], 2, 1, 64, 16, cache, seed=19)
+    pool.cache.reserve_tree(5)
+    tree = Tree(torch, pool, [5], "f32")
+    tree.q_cpu.mul_(q)
+    tree.q.copy_(tree.q_cpu.reshape(5, -1))
+    tree.run(scale=scale)
+    pool.cache.check()
+    tree.check(scale=scale)
