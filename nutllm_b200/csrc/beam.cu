@@ -65,10 +65,10 @@ __device__ __forceinline__ uint32_t warp_nth(uint32_t key, int want) {
 
 /* ---- a run of a row --------------------------------------------------- */
 
-constexpr int kListed = 256; /* keys of a warp */
-constexpr int kFull = 96;    /* where there are more, they are reduced */
+constexpr int kFull = 96;    /* keys of a warp's list; where there are more, they are reduced */
+constexpr int kListed = 128; /* and room for one more of each lane */
 constexpr int kRunWarps = 4;
-static_assert(kListed >= kFull + 5 * 32 && kFull >= kBeamMostOut, "room for more logits of each lane");
+static_assert(kListed >= kFull + 32 && kFull >= kBeamMostOut, "a logit of each lane at a time");
 
 /* Leaves the `want` greatest of a warp's n keys, in descending order, and
  * returns how many there are. */
