@@ -181,17 +181,23 @@ nut_status nut_beam_create(int64_t sequences, int64_t beams, int64_t vocab, int6
             refuse(NUT_LENGTH_ERROR, "beam", "n_out exceeds NUT_BEAM_MAX_OUT");
         if (sequences > kMostRows || beams > 1024 || sequences * beams > kMostRows || vocab > (1 << 28))
             refuse(NUT_LENGTH_ERROR, "beam", "dimensions exceed device limits");
-        /* a row's first tile may begin up to 7 elements before it.  Runs for some 18
-         * warps on every SM: fewer leave its memory waiting, more list more.  With 12, 16,
-         * 20, 28 and 40: 256 rows of 128,000 42.9, 44.6, 44.6, 47.7 and 49.9 us, 256 rows
-         * of 32,000 (bf16) 22.8, 22.3, 20.9, 22.1 and 22.1 */
+        /* a row's first tile may begin up to 7 elements before it.  Runs for some 16
+         * warps on every SM: with fewer its memory waits, more warps list and reduce more, of which n_out
+         * is the measure.  With 12, 14, 16, 18, 20, 24 and 28, us in a graph:
+         *   64 rows of 128,000, fp32, of 16    25.7   26.4   26.4   26.4   28.1   28.2   32.8
+         *   256 of 128,000, fp32, of 16        45.5   44.7   43.3   44.5   44.0   44.0   49.4
+         *   256 of 128,000, fp32, of 64        98.9  110.8  106.2  118.5  117.5  128.3  145.8
+         *   1,024 of 32,000, fp32, of 16       54.0   45.8   45.8   45.8   45.8   43.5   49.0
+         *   256 of 32,000, bf16, of 16         24.1   23.3   23.3   23.3   22.3   22.3   23.3
+         *   512 of 128,000, bf16, of 16        68.4   64.8   64.8   63.7   63.7   62.2   58.4
+         * (up to 32 rows are a run a tile: no difference) */
         const int64_t tiles = (vocab + 7 + nut::kBeamTile - 1) / nut::kBeamTile, rows = sequences * beams;
         if (rows * tiles > INT_MAX / NUT_BEAM_MAX_OUT)
             refuse(NUT_LENGTH_ERROR, "beam", "dimensions exceed device limits");
         DeviceScope scope(device);
         int sms = 0;
         cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "count SMs");
-        const int64_t wanted = std::min(tiles, std::max<int64_t>(1, (18 * sms) / rows));
+        const int64_t wanted = std::min(tiles, std::max<int64_t>(1, (16 * sms) / rows));
         const int64_t run_tiles = (tiles + wanted - 1) / wanted, runs = (tiles + run_tiles - 1) / run_tiles;
         auto h = std::make_unique<nut_beam>();
         h->device = device;
