@@ -19,12 +19,21 @@ namespace nut {
 constexpr float kTreeLog2e = 1.4426950408889634f, kTreeLn2 = 0.6931471805599453f;
 constexpr int kTreeTile = 64; /* slots of a tile */
 /* What an item costs besides its tiles, in tiles: its queries' way in and its
- * outputs' way out.  With 2, 4 and 6 a batch of 32 caches of up to 4,096 slots
- * took 75, 66 and 69 us. */
+ * outputs' way out.  With 2, 4 and 6, us in a graph:
+ *   32 bf16 caches of 1,024 to 4,096 slots, 16 tokens, 32/8 heads of 128   81.0   78.3   79.7
+ *   16 fp16 of 500 to 2,000, 64 tokens, 32/4 of 128                        68.4   63.8   62.7
+ *   256 fp16 of 125 to 500, 4 tokens, 32/8 of 64                            152    145    145
+ *   4 fp32 of 250 to 1,000, 12 tokens, 32/32 of 128                         45.2   51.2   50.4
+ *   24 bf16 of 500 to 2,000, 16 tokens, 4/4 of 256 (fp32 arithmetic)        324    342    363 */
 constexpr int kTreeItemCost = 4;
 /* The least share of a CTA: each part of an item is written and read again.
- * With 1, 2, 4 and 8 one cache of 2,000 slots took 22, 19, 20 and 25 us. */
-constexpr int kTreeLeastShare = 4;
+ * With 1, 2, 3, 4 and 8, us in a graph:
+ *   one bf16 cache of 300 slots, 8 tokens, 32/8 heads of 128   15.1   15.1   15.6   16.6   20.2
+ *   2,000 slots, 25 tokens                                     24.8   20.4   20.5   21.3   26.2
+ *   4 fp16 of 250 to 1,000, 8 fp32 rows, 32/4 of 64            18.7   18.7   19.3   20.2   24.8
+ *   one fp32 of 1,000, 8 tokens, 32/4 of 64                    19.6   19.5   22.5   26.1   40.4
+ * (16,000 slots and more, or 32 sequences: no difference) */
+constexpr int kTreeLeastShare = 2;
 
 /* The drafted tokens of a sequence and what they see. */
 struct TreeSpan {
