@@ -553,9 +553,10 @@ nut_status nut_paged_reserve_tree(nut_paged *paged, int64_t max_new);
  * NaN included, has no part in its outputs; an infinity or NaN among the
  * values it sees makes that dimension of its output infinite or NaN, and an
  * infinite key that it sees may make the row NaN.  Sums, the softmax and its
- * statistics are fp32.  Products are formed from 16-bit terms where the cache has 16 bits: fp32 queries and their weights in two
- * (fp16) or three (bf16) of them, rows of the cache's type in one (weights
- * within 2^-8 of themselves on bf16, 2^-11 on fp16; the sum is taken before).
+ * statistics are fp32.  Products are formed from 16-bit terms where the cache
+ * has 16 bits: fp32 queries and their weights in two (fp16) or three (bf16)
+ * of them, rows of the cache's type in one (weights within 2^-8 of themselves
+ * on bf16, 2^-11 on fp16; the sum is taken before).
  * Rows behind starts[sequences] are left as they were; out is no part of q.
  * A sequence whose `starts` do not ascend within `rows` is skipped (its rows stay); where its
  * length is bad or n exceeds it or max_new, its rows see nothing; slots of a

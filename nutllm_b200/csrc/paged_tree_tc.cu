@@ -23,6 +23,20 @@
  * greatest overflows.  A row's maximum may lag behind by kSlack: its outputs
  * are rescaled only when it rises by more.
  *
+ * Sums in tensor memory are cut off, not rounded: over a thousand products a
+ * row of outputs comes out short by 4 to 8 parts in 10^5, less than a 16-bit
+ * output's rounding, but not an fp32 one's.  fp32 rows therefore take a tile's
+ * product at a time, which the softmax of the next tile adds, rounded to
+ * nearest, to what it has put aside (kAside), and small terms are multiplied
+ * first.  With and without: 32 caches of up to 4,096 slots, 32/8 heads, 16
+ * tokens, fp16 of 64 dims 77.5 and 79.7 us, of 128 dims 135 and 128.5, bf16 of
+ * 64 dims 99 and 94.5, of 128 dims 163 and 160.5.
+ *
+ * Rows of the cache's type have weights in one term.  Two would bring the error
+ * down to that of rounding the outputs (bf16: 2.2 in place of 3.0 x 10^-4, root
+ * mean square), and take 85 us where the batch below takes 72 after a flush of
+ * L2.  A caller who wants them passes fp32 rows.
+ *
  * Values of slots that some rows do not see would meet weights of 0 in the
  * product: among the drafted tokens infinities and NaN are taken out of the
  * tile, and added at the end to the rows that see them.
@@ -49,6 +63,7 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kTile = kTreeTile;
+constexpr int kBuffers = 2; /* of logits */
 constexpr int kProducer = 4, kIssuer = 5; /* warps */
 constexpr int kThreads = 192;
 constexpr uint64_t kTreeWaitNs = 2000000000ull;
@@ -65,12 +80,13 @@ template <int DP_, int kTerms_> struct TcPlan {
     static constexpr int kFit = ((kPerSm == 2 ? 114 : 227) * 1024 - kSpare - kQueries) / kStage;
     static constexpr int kStages = kFit < 12 ? kFit : 12;
     static constexpr int kBytes = 1024 + kQueries + kStages * kStage;
-    /* tensor memory: S, with P in its place, once or twice; then O */
-    static constexpr int kLogits = kTerms * kTile / 2 > kTile ? kTerms * kTile / 2 : kTile;
+    /* tensor memory: S twice, two terms of P in its place; the third; O; what earlier tiles added to O.
+     * Of that, dims that find no room are in registers */
     static constexpr int kMemory = kPerSm == 2 ? 256 : 512;
-    static constexpr int kBuffers = 2 * kLogits + DP <= kMemory ? 2 : 1;
-    static constexpr int kOutputs = kBuffers * kLogits;
-    static_assert(kOutputs + DP <= kMemory, "columns of tensor memory");
+    static constexpr int kThird = 2 * kTile, kOutputs = kThird + (kTerms > 2 ? kTile / 2 : 0), kSums = kOutputs + DP;
+    static constexpr bool kAside = kTerms > 1;
+    static constexpr int kHeld = !kAside || kSums + DP <= kMemory ? 0 : kSums + DP - kMemory;
+    static_assert(kSums + (kAside ? DP - kHeld : 0) <= kMemory && kHeld % 32 == 0 && kHeld < DP, "columns of tensor memory");
     static_assert(kQueries >= kRows * 128, "the outputs leave through there, 32 dims at a time");
     static_assert(kStages >= 4, "keys of two tiles and values of one are in use at a time");
     static_assert(kStages / 2 + 2 < 8, "tiles under way: Shared::valid");
@@ -308,7 +324,8 @@ __device__ __forceinline__ int place_of_values(int i, int n) { return i == n - 1
 template <typename T, typename R, typename Plan>
 __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid_constant__ PagedTree a) {
     constexpr int DP = Plan::DP, kStages = Plan::kStages, kTerms = Plan::kTerms, kColumns = Plan::kColumns,
-                  kBuffers = Plan::kBuffers;
+                  kHeld = Plan::kHeld;
+    constexpr bool kAside = Plan::kAside;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr float kSlack = kTerms > 1 ? 0.0f : kHalf ? 7.0f : 8.0f;
     constexpr float kLift = !kHalf ? -38.0f : kTerms > 1 ? 15.0f : 8.0f; /* log2 of the greatest weight */
@@ -495,12 +512,12 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                 const uint64_t k = matrix_at(ring_at + stage_of(place) * Plan::kStage, 16, 1024);
                 const uint64_t q = matrix_at(queries_at, 16, 1024);
 #pragma unroll
-                for (int t = 0; t < kTerms; t++)
+                for (int t = kTerms - 1; t >= 0; t--) /* the small ones first */
 #pragma unroll
                     for (int s = 0; s < DP / 16; s++)
-                        mma_ss(tmem + buffer * Plan::kLogits,
+                        mma_ss(tmem + buffer * kTile,
                                q + ((t * Plan::kQueryBytes + s / 4 * (kRows * 128) + s % 4 * 32) >> 4),
-                               k + ((s / 4 * (kTile * 128) + s % 4 * 32) >> 4), kShapeS, t > 0 || s > 0);
+                               k + ((s / 4 * (kTile * 128) + s % 4 * 32) >> 4), kShapeS, t < kTerms - 1 || s > 0);
                 tc_commit(&sh.logits[buffer]);
                 tc_commit(&sh.empty[stage_of(place)]);
             };
@@ -520,13 +537,13 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         if (alive) {
                             tc_after();
                             const uint64_t v = matrix_at(ring_at + stage_of(place) * Plan::kStage, values_lead, 1024);
-                            const uint32_t weights = tmem + buffer * Plan::kLogits;
+                            const uint32_t weights = tmem + buffer * kTile;
 #pragma unroll
-                            for (int t = 0; t < kTerms; t++)
+                            for (int t = kTerms - 1; t >= 0; t--)
 #pragma unroll
                                 for (int s = 0; s < kTile / 16; s++)
-                                    mma_ts(tmem + Plan::kOutputs, weights + t * (kTile / 2) + s * 8, v + s * (values_step >> 4),
-                                           kShapeO, i > 0 || t > 0 || s > 0);
+                                    mma_ts(tmem + Plan::kOutputs, (t < 2 ? weights + t * (kTile / 2) : tmem + Plan::kThird) + s * 8,
+                                           v + s * (values_step >> 4), kShapeO, (!kAside && i > 0) || t < kTerms - 1 || s > 0);
                             tc_commit(&sh.outputs[buffer]);
                             tc_commit(&sh.empty[stage_of(place)]);
                         }
@@ -546,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
         }
         __syncwarp();
     } else {
-        const uint32_t lanes = uint32_t(warp * 32) << 16, outputs_at = tmem + lanes + Plan::kOutputs;
+        const uint32_t lanes = uint32_t(warp * 32) << 16, outputs_at = tmem + lanes + Plan::kOutputs,
+                       sums_at = tmem + lanes + Plan::kSums;
         const auto everyone = [] { named_barrier(1, kRows); };
         /* A barrier for every buffer: no phase of one is waited for when the next may
          * have ended too, or have not begun. */
@@ -657,9 +675,28 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
             /* weights are 2^((s - m) unit + kLift), m a maximum of s.  (Differences of s: beside products
              * s unit of 2^27 and more, rounded, the greatest weight would be off by their last place.) */
             float m = -INFINITY, l = 0.0f;
+            /* kAside: O is a tile's own; earlier tiles' sum is put aside, to be multiplied by `ratio` */
+            float ratio = 1.0f, held[kHeld > 0 ? kHeld : 1];
+#pragma unroll
+            for (int j = 0; j < kHeld; j++)
+                held[j] = 0.0f;
+            const auto add_sums = [&](int c, float *o, bool there) {
+                if (c >= DP - kHeld) {
+#pragma unroll
+                    for (int j = 0; j < kHeld; j++)
+                        o[j] = fmaf(held[j], ratio, o[j]);
+                } else if (there) {
+                    float sums[32];
+                    tmem_load32(sums_at + c, sums);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        o[j] = fmaf(sums[j], ratio, o[j]);
+                }
+            };
 #pragma unroll 1
             for (int i = 0; i < n; i++, tiles++) {
-                const uint32_t logits_at = tmem + lanes + tiles % kBuffers * Plan::kLogits;
+                const uint32_t logits_at = tmem + lanes + tiles % kBuffers * kTile;
                 const int t0 = (x.tile0 + i) * kTile;
                 if (alive)
                     alive = await(&sh.logits[tiles % kBuffers], tiles / kBuffers & 1);
@@ -681,6 +718,31 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         clean_values<T, DP>(ring_at + stage_of(place) * Plan::kStage + (slot >> 4) * values_step + (slot & 15) * 128,
                                             slot, tid & 1, values_lead, there, &sh.odd);
                     fence_async();
+                }
+                if (kAside && i > 0 && !idle && alive) {
+                    alive = __all_sync(0xffffffffu, await_outputs(tiles - 1));
+                    tc_after();
+                    if (alive) {
+#pragma unroll 1
+                        for (int c = 0; c < DP - kHeld; c += 32) {
+                            float o[32];
+                            tmem_load32(outputs_at + c, o);
+                            tc_wait_ld();
+                            add_sums(c, o, i > 1);
+                            tmem_store32(sums_at + c, o);
+                        }
+                        if constexpr (kHeld > 0) {
+                            static_assert(kHeld <= 32, "one piece");
+                            float o[32];
+                            tmem_load32(outputs_at + DP - kHeld, o);
+                            tc_wait_ld();
+                            add_sums(DP - kHeld, o, true);
+#pragma unroll
+                            for (int j = 0; j < kHeld; j++)
+                                held[j] = o[j];
+                        }
+                        ratio = 1.0f;
+                    }
                 }
                 if (!idle && alive) {
                     float s[kTile];
@@ -710,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         const float keep = m == next ? 1.0f : power2((m - next) * unit);
                         l *= keep;
                         m = next;
-                        if (i > 0) { /* once the products before are complete */
+                        ratio *= keep;
+                        if (!kAside && i > 0) { /* once the products before are complete */
                             alive = __all_sync(0xffffffffu, await_outputs(tiles - 1));
                             tc_after();
 #pragma unroll 1
@@ -752,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         }
 #pragma unroll
                         for (int t = 0; t < kTerms; t++)
-                            tmem_store16(logits_at + t * (kTile / 2) + k / 2, e[t]);
+                            tmem_store16((t < 2 ? logits_at + t * (kTile / 2) : tmem + lanes + Plan::kThird) + k / 2, e[t]);
                     }
                     l += sum + sum1;
                     tc_wait_st();
@@ -763,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
             base += 2 * n;
 
             /* the end of the item, or of this block's part of it */
-            if (alive && kBuffers > 1 && n > 1) /* the products may be two tiles behind */
+            if (alive && n > 1) /* the products may be two tiles behind */
                 alive = await_outputs(tiles - 2);
             if (alive)
                 alive = await_outputs(tiles - 1);
@@ -809,6 +872,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                 float o[32];
                 tmem_load32(outputs_at + d0, o);
                 tc_wait_ld();
+                if constexpr (kAside)
+                    if (n > 1)
+                        add_sums(d0, o, true);
                 __syncwarp();
                 float4 *mine = rows_at + lane * 8;
 #pragma unroll

@@ -10,7 +10,7 @@ import pytest
 
 import nutllm_b200 as nb
 from test_branch import PAIRS, UNIT, Book, Tree, paths, plain_beams, run_beams, same_beams
-from test_paged import EPS, Pool, dtypes
+from test_paged import EPS, KINDS, Pool, dtypes
 
 gpu = pytest.mark.gpu
 
@@ -337,3 +337,37 @@ def test_tree_logits_next_to_nothing(torch_cuda, cache, q, scale):
     tree.run(scale=scale)
     pool.cache.check()
     tree.check(scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_long_sums_have_no_drift(torch_cuda, cache, D):
+    """fp32 rows, positive values, and over a hundred tiles to a block: rounding to nearest leaves errors of either sign, a
+    sum that cuts off what it cannot hold is short by up to 2^-23 of itself every time.  Within a tile of 64 slots that
+    happens 4 times for each of 3 terms of the weights; were it the whole way, a thousand times.  (Errors of the weights
+    have either sign, and are in numerator and denominator.)"""
+    torch = torch_cuda
+    S, KV, L, ps, n = 10, 16, 16000, 16, 3
+    dt, pages = dtypes(torch)[cache], S * (L // ps)
+    g = torch.Generator(device="cuda").manual_seed(20)
+    keys = torch.randn(pages, KV, ps, D, generator=g, device="cuda").to(dt)
+    values = (1 + torch.rand(pages, KV, ps, D, generator=g, device="cuda")).to(dt)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").reshape(S, L // ps)
+    lengths = torch.full((S,), L, dtype=torch.int32, device="cuda")
+    pool = nb.PagedCache(keys.data_ptr(), values.data_ptr(), table.data_ptr(), lengths.data_ptr(), sequences=S, max_pages=L // ps,
+                         n_pages=pages, page_size=ps, heads=KV, kv_heads=KV, head_dim=D, dtype=KINDS[cache])
+    pool.reserve_tree(n)
+    q = torch.randn(S * n, KV * D, generator=g, device="cuda")
+    out = torch.empty_like(q)
+    starts = torch.arange(S + 1, dtype=torch.int32, device="cuda") * n
+    mask = torch.full((S * n, 1), 7, dtype=torch.int32, device="cuda")
+    pool.tree_attention(q.data_ptr(), out.data_ptr(), starts.data_ptr(), mask.data_ptr(), S * n, n, 1, scale=0.125)
+    pool.check()
+    errors = []
+    for s in range(S):
+        k, v = (x[s * (L // ps):(s + 1) * (L // ps)].transpose(1, 2).reshape(L, KV, D).double() for x in (keys, values))
+        z = 0.125 * torch.einsum("ihd,thd->iht", q[s * n:(s + 1) * n].reshape(n, KV, D).double(), k)
+        want = torch.einsum("iht,thd->ihd", torch.softmax(z, -1), v)
+        errors.append(out[s * n:(s + 1) * n].reshape(n, KV, D).double() / want - 1)
+    assert abs(float(torch.stack(errors).mean())) <= 12 * 2.0 ** -23
