@@ -225,19 +225,21 @@ __global__ void __launch_bounds__(kRunWarps * 32) runs_kernel(const __grid_const
         }
         sum += more;
 
-        /* what reaches the edge, by value first */
-        const uint32_t edge_bits = uint32_t(edge >> 32);
-        const bool any = ordered_bits(most) >= edge_bits;
+        /* what is above the edge, by value first: its key is that of an earlier token, which
+         * wins a tie, or the one below n_out equal ones */
+        const uint32_t edge_bits = uint32_t(edge >> 32), lowest = 0x007fffffu; /* of -infinity */
+        const bool any = edge_bits < lowest || ordered_bits(most) > edge_bits;
         if (!__any_sync(0xffffffffu, any))
             continue;
-        const float edge_value = edge_bits < 0x007fffffu ? -INFINITY : float_of(edge_bits);
         uint32_t hits = 0;
-        if (any && edge_value == -INFINITY)
-            hits = ~0u; /* every logit reaches it, NaN too, which counts as -infinity */
-        else if (any)
+        if (edge_bits < lowest) {
+            hits = ~0u; /* every logit, NaN too, which counts as -infinity */
+        } else if (any) {
+            const float edge_value = float_of(edge_bits);
 #pragma unroll
             for (int i = 0; i < kEach; i++)
-                hits |= uint32_t(v[i] >= edge_value) << i;
+                hits |= uint32_t(v[i] > edge_value) << i;
+        }
         /* a logit of each lane at a time, from where it lies: registers have no index */
         while (__any_sync(0xffffffffu, hits != 0)) {
             Key key = 0;
