@@ -695,9 +695,10 @@ nut_status nut_beam_destroy(nut_beam *beam);
  * token.  A finished beam has one candidate, (b, eos) with score scores[s][b],
  * and its logits are not read.  NaN counts as -infinity in logits and scores,
  * a logit of +infinity as the greatest finite float; candidates of
- * score -infinity rank last.  (Beside scores of 2^40 and more, whose sums with
- * logits round to ties in fp64, which of a beam's tokens go first is not
- * specified.)  Where there are fewer candidates than n_out,
+ * score -infinity rank last.  (Where different logits of a beam round to equal
+ * scores in fp64, beside scores of 2^40 and more or because they are next to
+ * nothing themselves, which of their tokens go first is not specified.)
+ * Where there are fewer candidates than n_out,
  * rows and tokens are -1 and scores -infinity behind them.  The choice does
  * not depend on timing.  out_scores and out_finished may be scores and finished
  * where n_out is beams. */

@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(kRunWarps * 32) runs_kernel(const __grid_const
         if (edge_bits < lowest) {
             hits = ~0u; /* every logit, NaN too, which counts as -infinity */
         } else if (any) {
-            const float edge_value = float_of(edge_bits);
+            /* (below +0, which -0 counts as too, comes the least negative number) */
+            const float edge_value = float_of(edge_bits == 0x7fffffffu ? 0x7ffffffeu : edge_bits);
 #pragma unroll
             for (int i = 0; i < kEach; i++)
                 hits |= uint32_t(v[i] > edge_value) << i;

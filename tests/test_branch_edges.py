@@ -68,6 +68,33 @@ def test_beam_select_ties_of_beams_without_a_score(torch_cuda, kind, low, V):
     same_beams(got, plain_beams(torch, logits, scores, ended, 4, 12))
 
 
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [31, 1023, 5000])
+@pytest.mark.parametrize("n", [1, 8, 31, 64])
+def test_beam_select_equal_logits_around_zero(torch_cuda, kind, V, n):
+    """+0 and -0 are equal logits, next to the least numbers of either sign and to a few levels."""
+    torch = torch_cuda
+    g = torch.Generator().manual_seed(V + n)
+    dt = dtypes(torch)[kind]
+    least = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps  # the least subnormal
+    scores = torch.tensor([[-1.0, -1.0], [-3.0, -0.25]])
+    for levels in ([0.0, -0.0], [-0.0, -least], [0.0, -0.0, -least, least], [-1.0, -0.0, 0.0], [-1.0, -2.0, -0.0]):
+        logits = torch.tensor(levels, dtype=dt)[torch.randint(len(levels), (4, V), generator=g)]
+        got, want = run_beams(torch, logits.cuda(), scores.cuda(), n), plain_beams(torch, logits, scores, None, -1, n)
+        if least not in (abs(v) for v in levels):
+            same_beams(got, want)
+            continue
+        # What is less than 2^-100 rounds to nothing beside a score of 1/4 or more, so that all tokens of a beam tie in 64
+        # bits, and the interface leaves open which go first; fp16's 2^-24 is less than what separates two beams' sums
+        # (40 roundings of 2^-24).  So: different candidates, with the scores as defined
+        for r, row in enumerate(want):
+            chosen = [c for c in zip(got[1][r].tolist(), got[2][r].tolist()) if c[0] >= 0]
+            assert len(set(chosen)) == len(chosen) and all(0 <= t < V for _, t in chosen)
+            for x, c in zip(got[0][r].tolist(), row):
+                assert x == c[0] or abs(x - c[0]) <= 40 * EPS + abs(c[0]) * EPS
+
+
 # ---------------------------------------------------------------------------
 # tree attention
 
