@@ -409,7 +409,7 @@ constexpr int kJoinWarps = 8, kJoinOwn = 2, kJoinRows = kJoinWarps * kJoinOwn;
  * then take 4 dims each.  It is round trips: which item, its span, maxima, outputs; 8.4 us after 32
  * caches of up to 4,096 slots, 10 with a row a warp, whose blocks came in two waves. */
 template <typename R>
-__global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_constant__ PagedTree a, int block_rows) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_constant__ PagedTree a, int block_rows, float drop) {
     begin_kernel();
     const int4 join = a.joins[blockIdx.x];
     const int parts = join.x, lane = threadIdx.x & 31;
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) join_kernel(const __grid_c
         int h;
         tree_row(a, row0, join.z, first_row + f0 + r, row, h);
         if (a.lse && lane == 0)
-            a.lse[row * p.heads + h] = all == 0.0f ? -INFINITY : (from[r] + (rest[r] + log2f(all))) * kTreeLn2;
+            a.lse[row * p.heads + h] = all == 0.0f ? -INFINITY : (from[r] + (rest[r] + log2f(all * drop))) * kTreeLn2;
         R *to = static_cast<R *>(a.out) + row * a.out_stride + int64_t(h) * D;
 #pragma unroll
         for (int k = 0; k < kMost; k++) {
@@ -548,7 +548,7 @@ template <int kRows, int DP, typename T, typename R> cudaError_t launch_wide(con
     static_assert(W::kPerSm <= kTreeCtasPerSm, "the workspace has room for as many");
     const int ctas = a.sms * W::kPerSm;
     e = launch_kernel(kernel, dim3(ctas), kThreads, W::kBytes, s, 1, a);
-    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, s);
+    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, 1.0f, s);
 }
 
 /* Rows of an item, by how many a sequence can have: few that fill them, two blocks an SM; or more of
@@ -578,13 +578,13 @@ template <typename T, typename R> cudaError_t launch_wide(const PagedTree &a, cu
 
 } // namespace
 
-cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaStream_t s) {
+cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, float drop, cudaStream_t s) {
     if (a.p.capacity <= kTreeTile) /* items of one tile lie in one block */
         return cudaSuccess;
     const int rows = int(std::min<int64_t>(block_rows, int64_t(a.max_new) * a.p.group));
     const dim3 grid(ctas, (rows + kJoinRows - 1) / kJoinRows);
     const auto kernel = a.type == 0 ? join_kernel<float> : a.type == 1 ? join_kernel<__half> : join_kernel<__nv_bfloat16>;
-    return launch_kernel(kernel, grid, kJoinWarps * 32, 0, s, 1, a, block_rows);
+    return launch_kernel(kernel, grid, kJoinWarps * 32, 0, s, 1, a, block_rows, drop);
 }
 
 int64_t tree_part_floats(const PagedPool &p, int max_new) {

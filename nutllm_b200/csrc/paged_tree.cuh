@@ -192,8 +192,8 @@ __device__ __forceinline__ void tree_row(const PagedTree &a, int row0, int head,
 }
 
 /* A CTA's part of an item: maxima and sums of its rows, then outputs.  Sums and
- * outputs are those of weights 2^(logit - maximum - rest): a rest holds what
- * rounding took from a great maximum.  The item that a CTA's share begins
+ * outputs are those of weights 2^(logit - maximum - rest), times a power of two
+ * that all parts share: a rest holds what rounding took from a great maximum.  The item that a CTA's share begins
  * within lies in its first place, another in the second. */
 struct TreePart {
     float *maxima, *rests, *sums, *out;
@@ -231,6 +231,7 @@ __device__ __forceinline__ uint32_t tree_sees(const uint32_t *words, int base, i
     return bits;
 }
 
-cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, cudaStream_t s);
+/* drop: the inverse of the power of two in the parts' sums. */
+cudaError_t tree_join_parts(const PagedTree &a, int ctas, int block_rows, float drop, cudaStream_t s);
 
 } // namespace nut

@@ -91,7 +91,12 @@ template <int DP_, int kTerms_> struct TcPlan {
     static_assert(kStages >= 4, "keys of two tiles and values of one are in use at a time");
     static_assert(kStages / 2 + 2 < 8, "tiles under way: Shared::valid");
     static_assert(kPerSm <= kTreeCtasPerSm, "the workspace has room for as many");
+    template <typename T> static constexpr float lift() {
+        return !std::is_same<T, __half>::value ? -38.0f : kTerms > 1 ? 15.0f : 8.0f;
+    }
 };
+
+__host__ __device__ constexpr float power_of_two(int e) { return e == 0 ? 1.0f : e > 0 ? 2.0f * power_of_two(e - 1) : 0.5f * power_of_two(e + 1); }
 
 /* ---- PTX --------------------------------------------------------------- */
 
@@ -328,7 +333,9 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
     constexpr bool kAside = Plan::kAside;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr float kSlack = kTerms > 1 ? 0.0f : kHalf ? 7.0f : 8.0f;
-    constexpr float kLift = !kHalf ? -38.0f : kTerms > 1 ? 15.0f : 8.0f; /* log2 of the greatest weight */
+    constexpr float kLift = Plan::template lift<T>(); /* log2 of the greatest weight */
+    /* sums are freed of it before their logarithm is taken: beside -38 it would lose its last places */
+    constexpr float kDrop = power_of_two(-int(kLift));
     extern __shared__ char smem_raw[];
     char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ Shared<kStages> sh;
@@ -789,7 +796,8 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         }
                     }
                     const float none = m == -INFINITY ? 0.0f : -m;
-                    const Two less = two_of(none, none), units = two_of(unit, unit), lift = two_of(kLift, kLift);
+                    const Two less = two_of(none, none), units = two_of(unit, unit),
+                              lift = kHalf ? two_of(kLift, kLift) : two_of(1.0f / kDrop, 1.0f / kDrop);
                     float sum = 0.0f, sum1 = 0.0f;
 #pragma unroll
                     for (int k = 0; k < kTile; k += 32) {
@@ -798,9 +806,18 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                         for (int j = 0; j < 16; j++) {
                             Two z = two_of(s[k + 2 * j], s[k + 2 * j + 1]);
                             asm("add.rn.f32x2 %0, %0, %1;\n" : "+l"(z) : "l"(less));
-                            asm("fma.rn.f32x2 %0, %0, %1, %2;\n" : "+l"(z) : "l"(units), "l"(lift));
-                            const float2 of = parts_of(z);
-                            float w0 = power2(of.x), w1 = power2(of.y);
+                            float w0, w1;
+                            if constexpr (kHalf) {
+                                asm("fma.rn.f32x2 %0, %0, %1, %2;\n" : "+l"(z) : "l"(units), "l"(lift));
+                                w0 = power2(parts_of(z).x);
+                                w1 = power2(parts_of(z).y);
+                            } else { /* beside -38 the exponent would lose its last 5 bits */
+                                asm("mul.rn.f32x2 %0, %0, %1;\n" : "+l"(z) : "l"(units));
+                                z = two_of(power2(parts_of(z).x), power2(parts_of(z).y));
+                                asm("mul.rn.f32x2 %0, %0, %1;\n" : "+l"(z) : "l"(lift));
+                                w0 = parts_of(z).x;
+                                w1 = parts_of(z).y;
+                            }
                             sum += w0;
                             sum1 += w1;
 #pragma unroll
@@ -840,13 +857,13 @@ __global__ void __launch_bounds__(kThreads, Plan::kPerSm) tc_kernel(const __grid
                 if (!whole) {
                     const float most = m * unit;
                     part.maxima[tid] = most;
-                    part.rests[tid] = (fabsf(most) < INFINITY ? fmaf(m, unit, -most) : 0.0f) - kLift;
+                    part.rests[tid] = fabsf(most) < INFINITY ? fmaf(m, unit, -most) : 0.0f;
                     part.sums[tid] = l;
                 } else if (a.lse) {
                     int64_t out_row;
                     int h;
                     tree_row(a, x.span.row0, x.head, x.first_row + tid, out_row, h);
-                    a.lse[out_row * p.heads + h] = l == 0.0f ? -INFINITY : fmaf(m, unit, log2f(l) - kLift) * kTreeLn2;
+                    a.lse[out_row * p.heads + h] = l == 0.0f ? -INFINITY : fmaf(m, unit, log2f(l * kDrop)) * kTreeLn2;
                 }
             }
             /* 32 dims at a time leave through a warp's 4 KB of the queries'
@@ -948,7 +965,7 @@ template <typename T, typename R, int DP, int kTerms> cudaError_t launch(const P
     }
     const int ctas = a.sms * Plan::kPerSm;
     e = launch_kernel(kernel, dim3(ctas), kThreads, Plan::kBytes, s, 1, a);
-    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, s);
+    return e != cudaSuccess ? e : tree_join_parts(a, ctas, kRows, power_of_two(-int(Plan::template lift<T>())), s);
 }
 
 template <typename T, int DP> cudaError_t launch(const PagedTree &a, cudaStream_t s) {

@@ -398,3 +398,25 @@ def test_tree_long_sums_have_no_drift(torch_cuda, cache, D):
         want = torch.einsum("iht,thd->ihd", torch.softmax(z, -1), v)
         errors.append(out[s * n:(s + 1) * n].reshape(n, KV, D).double() / want - 1)
     assert abs(float(torch.stack(errors).mean())) <= 12 * 2.0 ** -23
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", PAIRS)
+@pytest.mark.parametrize("length", [3, 15, 60, 2500])
+def test_tree_lse_of_small_logits(torch_cuda, cache, rows, length):
+    """Logits next to 0: the log-sum-exp is the logarithm of a count, to a few parts of its own last place."""
+    torch = torch_cuda
+    n = min(length, 28)
+    pool = Pool(torch, [length], 8, 2, 40, 16, cache, seed=length)
+    pool.cache.reserve_tree(n)
+    tree = Tree(torch, pool, [n], rows, masks=[[list(range(i + 1)) for i in range(n)]])
+    tree.run(scale=2.0 ** -20)
+    pool.cache.check()
+    # |logits| <= 2^-20 sqrt(40) 5^2 or so, known to (40 + 8) roundings; the sum rounded for every slot, a logarithm, a product
+    for i in range(n):
+        m = length - n + i + 1
+        z = 2.0 ** -20 * torch.einsum("hgd,htd->hgt", tree.q_cpu[i].double().reshape(2, 4, 40), pool.k[0][:, :m].double())
+        want = torch.logsumexp(z, -1).reshape(8)
+        err = (tree.lse[i].cpu().double() - want).abs()
+        tol = 48 * EPS * z.abs().amax(-1).reshape(8) + (4 + 2 * math.sqrt(m)) * EPS + 4 * EPS * want.abs()
+        assert bool((err <= tol).all()), (i, float(err.max()))
