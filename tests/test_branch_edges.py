@@ -420,3 +420,25 @@ def test_tree_lse_of_small_logits(torch_cuda, cache, rows, length):
         err = (tree.lse[i].cpu().double() - want).abs()
         tol = 48 * EPS * z.abs().amax(-1).reshape(8) + (4 + 2 * math.sqrt(m)) * EPS + 4 * EPS * want.abs()
         assert bool((err <= tol).all()), (i, float(err.max()))
+
+
+@gpu
+@pytest.mark.parametrize("cache,rows", [p for p in PAIRS if p[0] != "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("length", [40, 3000])
+def test_tree_values_near_the_greatest(torch_cuda, cache, rows, D, length):
+    """A mean of values near a 16-bit type's greatest is one of them: no sum on the way passes fp32's range."""
+    torch = torch_cuda
+    dt = dtypes(torch)[cache]
+    pool = Pool(torch, [length], 4, 2, D, 16, cache, seed=1)
+    v = torch.full((2, length, D), 0.9 * torch.finfo(dt).max).to(dt)
+    v[:, :, 1::2] *= -1
+    pool.put(0, pool.k[0], v, 0)
+    pool.cache.reserve_tree(3)
+    tree = Tree(torch, pool, [3], rows)
+    tree.run()
+    pool.cache.check()
+    # weights and their sum as in the other tests, relative to the one value that there is
+    tol = (2 * length + 64) * EPS + UNIT[rows] + (0.0 if rows == "f32" else torch.finfo(dt).eps / 2)
+    error = tree.out.reshape(3, 2, 2, D).double().cpu() / v[None, :, None, 0].double() - 1
+    assert bool((error.abs() <= tol).all())
