@@ -5,16 +5,15 @@
  * of a row, 1,024 logits at a time (while the next ones are on their way to
  * shared memory), and keeps a maximum and a sum of exponentials for each lane
  * and a list in shared memory of what can be among the run's n_out greatest.
- * The first logits set an edge that n_out of
- * them reach; from then on only what reaches it is listed, and a full list is
- * reduced to its n_out greatest, the last of which is the new edge.  Then a
- * block for each request joins the runs' sums in fp64, turns what they listed
+ * The first logits set an edge that n_out of them reach; from then on only what
+ * is above it is listed, and a full list is reduced to its n_out greatest, the
+ * last of which is the new edge.  Then a block for each request joins the runs' sums in fp64, turns what they listed
  * into scores and chooses among them: an edge from its threads' maxima, what
  * reaches it ranked by counting.
  *
  * Instructions bound the runs where there is much to read: 256 rows of 128,000
- * fp32 logits (123 MB without the ended beams') 36.7 us, 3.35 TB/s, 15.5
- * million warp instructions at 0.50 a cycle and scheduler.  The choice is a chain of
+ * fp32 logits (123 MB without the ended beams') 33.8 us, 3.6 TB/s, 14.7
+ * million warp instructions at 0.47 a cycle and scheduler.  The choice is a chain of
  * barriers and round trips, 9 to 12 us.  In a persistent grid whose last block
  * of a request chose, the requests' choices came one behind another.
  *

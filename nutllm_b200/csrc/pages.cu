@@ -14,9 +14,9 @@
  * Sums of whole numbers do not depend on the order of the atomics, and
  * places come from prefix sums, so results do not depend on timing.
  *
- * It is a chain of round trips to L2, not bytes: with the copies behind it 64
- * sequences of 1,003 slots take 16 us, 512 of 16,000 slots, a table of half a
- * million entries, 27 us.
+ * It is a chain of round trips to L2, not bytes: in a graph, with the copies
+ * behind it, 64 sequences of 1,003 slots take 16 us, 512 of 16,000 slots, a
+ * table of half a million entries, 27 us.
  */
 #include <climits>
 #include <cooperative_groups.h>
@@ -314,9 +314,10 @@ template <int kThreads, int kBlocks> __global__ void __launch_bounds__(kThreads,
 
 cudaError_t pages_update(const PagesUpdate &a, cudaStream_t s) {
     /* A small book is a chain of barriers, which few threads pass sooner; a large one needs loads in
-     * flight, and takes the most blocks that a cluster can have.  A pass with 8 blocks of 256, 8 of 1,024 and
-     * 16 of 1,024 threads, us: 128 sequences of 1,000 slots 19.4, 19.7, -; 128 of 8,000 24.3, 21.1, 20.6; 256 of
-     * 1,000 27.5, 20.8, 19.8; 512 of 16,000 78, 37, 30; 32 of 1,000 14.3, 18.2, -. */
+     * flight, and takes the most blocks that a cluster can have.  With 8 blocks of 256, 8 of 1,024 and
+     * 16 of 1,024 threads, us in a graph, with copies of one small head behind it: 32 sequences of 1,000 slots
+     * 13.3, 17.5, 19.8; 64 of 1,003 14.2, 19.1, 21.8; 128 of 1,000 17.5, 18.1, 19.7; 128 of 8,000 20.9, 19.3,
+     * 20.6; 256 of 1,000 23.9, 18.4, 20.2; 1,024 of 2,000 67, 31.1, 24.6; 512 of 16,000 72, 34.9, 26.2. */
     const bool small = a.sequences <= 128 && a.n_pages <= 16384 && int64_t(a.sequences) * a.max_pages <= 65536;
     if (small)
         return launch_kernel(update_kernel<256, 8>, dim3(8), 256, 0, s, 8, a);
