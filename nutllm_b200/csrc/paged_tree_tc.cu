@@ -25,7 +25,8 @@
  *
  * Sums in tensor memory are cut off, not rounded: over a thousand products a
  * row of outputs comes out short by 4 to 8 parts in 10^5, less than a 16-bit
- * output's rounding, but not an fp32 one's.  fp32 rows therefore take a tile's
+ * output's rounding (200,000 slots in one block would reach fp16's half step),
+ * but not an fp32 one's.  fp32 rows therefore take a tile's
  * product at a time, which the softmax of the next tile adds, rounded to
  * nearest, to what it has put aside (kAside), and small terms are multiplied
  * first.  With and without: 32 caches of up to 4,096 slots, 32/8 heads, 16
