@@ -1,7 +1,7 @@
 """Branching decode (test_branch.py) where its definitions and its kernels'
-short cuts could part: logits and scores that are no numbers, values that are
-none and hardly weigh, starts that contradict themselves, lists and books
-across layers, and numbers beyond their fields."""
+short cuts could part: logits and scores that are no numbers or tie, values
+that are none and hardly weigh, logits far from zero and next to it, long sums,
+books and caches of several layers, and numbers beyond their fields."""
 import math
 import random
 
